@@ -260,13 +260,22 @@ def prepare(case, seed):
     return st
 
 
+# 2^e for whole e, from the number's bits (a device's pow may be a step off).
+def _pow2(e):
+    return ((e.to(torch.int32) + 127) << 23).view(torch.float32)
+
+
+def _pow2_64(e):
+    return ((e.to(torch.int64) + 1023) << 52).view(torch.float64)
+
+
 # ---- the plain forms ------------------------------------------------------------------
 def _plain_codes(x):
     """Codes [..., D] and biased exponents [..., D / 32] of x's groups."""
     g = x.float().unflatten(-1, (-1, 32))
     m, k = torch.frexp(g.abs().amax(-1))           # largest = m 2^k, m in [0.5, 1)
     e = (k - 3 + (m > 0.875).to(k.dtype)).clamp(-125, 125)
-    y = torch.ldexp(g, -e[..., None])
+    y = g * _pow2(-e)[..., None]
     a = y.abs()
     code = ((a > 0.25).to(torch.uint8) + (a >= 0.75).to(torch.uint8) + (a > 1.25).to(torch.uint8)
             + (a >= 1.75).to(torch.uint8) + (a > 2.5).to(torch.uint8) + (a >= 3.5).to(torch.uint8)
@@ -287,7 +296,7 @@ def _plain_read(st, slots):
     code = torch.stack([p & 15, p >> 4], -1).flatten(-2).long()
     grid = torch.tensor(GRID + tuple(-v for v in GRID), device=p.device)
     val = grid[code].unflatten(-1, (-1, 32))
-    return torch.ldexp(val, st["exps"][slots].int()[..., None] - 127).flatten(-2)
+    return (val * _pow2(st["exps"][slots].int() - 127)[..., None]).flatten(-2)
 
 
 def _softmax(x):
@@ -437,9 +446,9 @@ def _stored64(x):
     g = x.double().unflatten(-1, (-1, 32))
     a = g.abs().amax(-1)
     e = torch.ceil(torch.log2(a.clamp_min(1e-300) / 7))
-    e = torch.where(a > 7 * 2.0 ** e, e + 1, e)
-    e = torch.where(a <= 7 * 2.0 ** (e - 1), e - 1, e).clamp(-125, 125)
-    step = (2.0 ** e)[..., None]
+    e = torch.where(a > 7 * _pow2_64(e), e + 1, e)
+    e = torch.where(a <= 7 * _pow2_64(e - 1), e - 1, e).clamp(-125, 125)
+    step = _pow2_64(e)[..., None]
     best = torch.full_like(g, math.inf)
     val = torch.zeros_like(g)
     for i in (0, 2, 4, 6, 1, 3, 5, 7):              # even codes first: they keep ties
