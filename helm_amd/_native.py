@@ -100,6 +100,26 @@ SIGNATURES = {
         _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _c_void_p, ctypes.c_int, _f32,
         _c_void_p, _c_void_p, _i64, ctypes.c_int, _c_void_p, _c_void_p, ctypes.c_int,
         ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, _c_void_p]),
+    "helm_batch_tables": (ctypes.c_int, [
+        _c_void_p, _c_void_p, ctypes.c_int, _c_void_p, _i64, ctypes.c_int, _c_void_p,
+        ctypes.c_int, ctypes.c_int, ctypes.c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
+        _c_void_p, _c_void_p]),
+    "helm_pool4_write": (ctypes.c_int, [
+        _c_void_p, _i64, ctypes.c_int, ctypes.c_int, ctypes.c_int, _c_void_p, ctypes.c_int,
+        _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, ctypes.c_int, _c_void_p]),
+    "helm_pool4_read": (ctypes.c_int, [
+        _c_void_p, _i64, ctypes.c_int, ctypes.c_int, ctypes.c_int, _c_void_p, ctypes.c_int,
+        _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, ctypes.c_int, _c_void_p]),
+    "helm_pool4_workspace_bytes": (_sz, [ctypes.c_int] * 7),
+    "helm_pool4_decode_attn": (ctypes.c_int, [
+        _c_void_p, _c_void_p, _c_void_p, _i64, ctypes.c_int, _c_void_p, _i64, ctypes.c_int,
+        _c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, _f32,
+        _f32, _c_void_p, _i64, _i64, _i64, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+        ctypes.c_int, _c_void_p, _sz, _c_void_p]),
+    "helm_prompt_attn": (ctypes.c_int, [
+        _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p, _i64,
+        _i64, _c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+        _f32, _f32, ctypes.c_int, ctypes.c_int, ctypes.c_int, _c_void_p]),
     "helm_profile_split_kernels": (ctypes.c_int, [ctypes.c_int]),
     "helm_profile_split_read": (ctypes.c_int, [_c_void_p, ctypes.c_int]),
     "helm_profile_workgroup_stamps": (ctypes.c_int, [_c_void_p, ctypes.c_int]),

@@ -1,0 +1,372 @@
+// Causal attention of packed whole prompts on 32 x 32 matrix-core tiles
+// (helm_prompt_attn): row i of a sequence gets softmax(cap(q . K^T scale)) . V
+// over the sequence's rows j <= i (and j > i - window).
+//
+// Bound by the matrix cores: 4 D operations a visible (row, head) pair against
+// 8 bytes a row and head dim.  A workgroup owns 128 rows of one query head, a wave
+// 32 of them; it walks the keys in stages of 64 tokens, whose K and V go straight
+// from memory into LDS (two stage buffers, one barrier a stage), and computes 32
+// tokens a step.  Lane l = 32 hh + jr owns query row jr:
+//   S^T = K Q^T  (v_mfma_f32_32x32x16): A is K of token tau(jr), B query row jr; with
+//         tau(8g + 4h + t) = 16 (g >> 1) + 8h + 4 (g & 1) + t the lane gets row jr's
+//         scores of tokens 8 hh .. 8 hh + 7 of both 16-token blocks of the step,
+//   O^T += V^T P^T: which are the tokens that B wants of it; A is V by LDS
+//         transpose reads.  O register 4g + t of dim group e is dim
+//         32 e + 8 g + 4 hh + t of row jr.
+// So a row's scores, maximum, sum and output sit in the two lanes (*, jr).  The
+// running maximum is refreshed only when a score passes it by 2^8 (base-2 units).
+// Weights are rounded once to the 16-bit type (half a step, 2^-9 or 2^-12 of the
+// weight, at random: below the output's own rounding) and the row's sum adds the
+// rounded ones; f16 weights are taken times 2^9 (weight_shift: nothing above 2^-34
+// of the largest is lost).
+//
+// Hidden tokens take no part whatever they hold: their scores are overwritten,
+// and an infinity or NaN in V (which would turn a weight of zero into NaN) shows
+// as NaN in an output, upon which the workgroup walks again with V's infinities
+// and NaN taken out of the products and added where a row weighs them (careful).
+#pragma once
+
+#include <type_traits>
+
+#include "attn_chunk32.h"
+
+namespace helm {
+
+constexpr int kPromptWaves = 4;
+constexpr int kPromptRows = 32 * kPromptWaves;   // query rows of a workgroup
+constexpr int kPromptTok = 64;                   // tokens of a stage
+
+struct PromptParams {
+  const char *q, *k, *v;
+  char* out;
+  int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head, o_tok, o_head;   // bytes
+  const int32_t* cu;
+  int B, N, Hq, Hkv, G;
+  int tiles;           // grid's row tiles: at least the sequences' together
+  float scale;         // >= 0 (a negative one's sign is taken into q)
+  uint32_t q_sign;     // xor on packed q pairs
+  float softcap;
+  int window;          // <= 0: off
+  int zero_rest;
+};
+
+// Sequence b's rows, clamped to the tensors.
+struct PromptSeq {
+  int first, len;
+};
+__device__ __forceinline__ PromptSeq prompt_seq(const PromptParams& p, int b) {
+  const int s = min(max(p.cu[b], 0), p.N);
+  const int e = min(max(p.cu[b + 1], s), p.N);
+  return {s, e - s};
+}
+
+// Row tile j of the packed batch: its sequence (lanes take 64 sequences at a time)
+// and its first row in it, the later rows of a sequence (the longer walks) first.
+// b < 0: past the last tile, row = its number there.
+struct PromptTile {
+  int b, first, len, row;
+};
+__device__ __forceinline__ PromptTile prompt_tile(const PromptParams& p, int j, int lane) {
+  int base = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 64) {
+    PromptSeq s{0, 0};
+    if (b0 + lane < p.B) s = prompt_seq(p, b0 + lane);
+    const int nt = (s.len + kPromptRows - 1) / kPromptRows;
+    int incl = nt;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int t = __shfl_up(incl, d, 64);
+      if (lane >= d) incl += t;
+    }
+    const uint64_t past = __builtin_amdgcn_ballot_w64(base + incl > j);
+    if (past) {
+      const int at = __builtin_ctzll(past);
+      const int first = __builtin_amdgcn_readlane(s.first, at);
+      const int len = __builtin_amdgcn_readlane(s.len, at);
+      const int t = __builtin_amdgcn_readlane(base + incl, at) - 1 - j;   // from the last
+      return {b0 + at, first, len, t * kPromptRows};
+    }
+    base += __builtin_amdgcn_readlane(incl, 63);
+  }
+  return {-1, 0, 0, j - base};
+}
+
+template <typename T> __device__ __forceinline__ uint32_t nonfinite_halves(uint32_t w) {
+  constexpr uint32_t kExp = std::is_same<T, bf16_t>::value ? 0x7f80u : 0x7c00u;
+  uint32_t r = 0;
+  if ((w & kExp) == kExp) r |= 0xffffu;
+  if ((w >> 16 & kExp) == kExp) r |= 0xffff0000u;
+  return r;
+}
+
+template <typename T, int D, bool kCap, bool kWindow>
+__device__ __forceinline__ void prompt_body(const PromptParams& p) {
+  constexpr int NW = kPromptWaves;
+  constexpr int SB = kPromptTok / kBlockTok;
+  constexpr int NK = D / 16, NE = D / 32, CPR = D / 8;
+  constexpr int kRow = 2 * D, kBlk = kBlockTok * kRow;
+  constexpr int kShift = std::is_same<T, f16_t>::value ? 9 : 0;
+  constexpr float kSlack = chunk_slack(kShift);
+  constexpr int kBlkLoads = kBlk / 1024;
+  static_assert(SB == NW, "a wave loads one block of K and of V");
+  using Ops = MfmaOps<T>;
+  using M32 = Mfma32<T>;
+  typedef mf_u32x4 StageBuf[2][SB][kBlk / 16];
+  __shared__ StageBuf lds0, lds1;
+
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = tid & 63, jr = lane & 31, hh = lane >> 5;
+  const int hq = blockIdx.x % p.Hq, hk = hq / p.G;
+  const PromptTile tl = prompt_tile(p, blockIdx.x / p.Hq, lane);
+  if (tl.b < 0) {
+    if (!p.zero_rest) return;
+    // (the workgroups past the last tile share out the rows outside every sequence)
+    const int r0 = min(max(p.cu[0], 0), p.N), r1 = min(max(p.cu[p.B], r0), p.N);
+    const int spare = p.tiles - (blockIdx.x / p.Hq - tl.row);
+    for (int64_t i = (int64_t)tl.row * NW + wave; i < p.N - (r1 - r0); i += (int64_t)spare * NW) {
+      const int64_t r = i < r0 ? i : i + (r1 - r0);
+      if (lane < CPR)
+        *reinterpret_cast<mf_u32x4*>(p.out + r * p.o_tok + hq * p.o_head + 16 * lane) =
+            mf_u32x4{0u, 0u, 0u, 0u};
+    }
+    return;
+  }
+  const int row_w = tl.row + 32 * wave;                  // the wave's first row
+  const int row = row_w + jr;
+  const bool row_ok = row < tl.len;
+  const bool wave_rows = row_w < tl.len;
+  const int row_last = min(row_w + 31, tl.len - 1);
+  const int end = min(tl.row + kPromptRows, tl.len);     // keys: [0, end)
+  const int win = kWindow ? p.window : 0;
+  const int st0 = kWindow ? max(0, tl.row - win + 1) / kPromptTok : 0;
+  const int st1 = (end + kPromptTok - 1) / kPromptTok;
+
+  mf_u32x4 qop[NK];
+  {
+    const char* qp = p.q + (int64_t)(tl.first + (row_ok ? row : 0)) * p.q_tok + hq * p.q_head;
+#pragma unroll
+    for (int i = 0; i < NK; ++i) {
+      const mf_u32x4 w = *reinterpret_cast<const mf_u32x4*>(qp + 16 * (2 * i + hh));
+      qop[i] = row_ok ? w ^ p.q_sign : mf_u32x4{0u, 0u, 0u, 0u};
+    }
+  }
+  const float scale2 = p.scale * kLog2E;
+  const float inv_cap = kCap ? 1.f / p.softcap : 0.f, cap2 = p.softcap * kLog2E;
+
+  const char* kb = p.k + tl.first * p.k_tok + hk * p.k_head;
+  const char* vb = p.v + tl.first * p.v_tok + hk * p.v_head;
+  // this wave's block of a stage, K and V, straight into LDS; lane i of load u fetches
+  // the chunk that the swizzle (attn_chunk32.h) keeps in slot 64 u + i; tokens past
+  // the sequence's end come in as zeros
+  auto dma_stage = [&](int st, StageBuf& dst) {
+    const int tok0 = st * kPromptTok + wave * kBlockTok;
+    const int nt = min(max(tl.len - tok0, 0), kBlockTok);
+    const auto rk = make_rsrc(kb + tok0 * p.k_tok, nt ? (nt - 1) * (int)p.k_tok + kRow : 0);
+    const auto rv = make_rsrc(vb + tok0 * p.v_tok, nt ? (nt - 1) * (int)p.v_tok + kRow : 0);
+#pragma unroll
+    for (int u = 0; u < kBlkLoads; ++u) {
+      const int t = (64 / CPR) * u + lane / CPR;
+      const int c = 16 * ((lane % CPR) ^ swz<D>(t));
+      buf_load16_lds(rk, &dst[0][wave][64 * u], t * (int)p.k_tok + c);
+      buf_load16_lds(rv, &dst[1][wave][64 * u], t * (int)p.v_tok + c);
+    }
+  };
+
+  const int g_a = jr >> 3, h_a = (jr >> 2) & 1, t_a = jr & 3;
+  const int tau = 16 * (g_a >> 1) + 8 * h_a + 4 * (g_a & 1) + t_a;
+  const int kblk = tau >> 4, ktok = tau & 15;
+  const int nl = lane & 15;
+  auto vaddr = [&](const StageBuf& cur, int blk, int z, int e) -> const char* {
+    const int vtok = 8 * hh + 4 * z + (nl >> 2);
+    const int chunk = 4 * e + 2 * (jr >> 4) + ((nl & 3) >> 1);
+    return reinterpret_cast<const char*>(&cur[1][blk][vtok * CPR + (chunk ^ swz<D>(vtok))]) +
+           8 * (nl & 1);
+  };
+
+  float m, lsum;
+  mf_f32x16 o[NE];
+
+  auto step = [&](auto careful, int tok0, int bp, const StageBuf& cur) {
+    mf_f32x16 sc;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sc[r] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NK; ++i)
+      sc = M32::mma(cur[0][bp + kblk][ktok * CPR + ((2 * i + hh) ^ swz<D>(ktok))], qop[i], sc);
+    float x[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] = sc[r];
+    if constexpr (kCap) softcap_scores<16>(x, p.scale * inv_cap, cap2);
+    const float mul = kCap ? 1.f : scale2;     // logits in base-2 units
+    const bool limit = tok0 + 31 > row_w || (kWindow && tok0 <= row_last - win);
+    if (limit) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int t = tok0 + 16 * (r >> 3) + 8 * hh + (r & 7);
+        if (t > row || (kWindow && t <= row - win)) x[r] = -INFINITY;
+      }
+    }
+    float top = x[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) top = fmaxf(top, x[r]);
+    top *= mul;
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(top > m + kSlack) != 0, 0)) {
+      float mn = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)));
+      if constexpr (kShift) mn = ceilf(mn);    // (so that m - kShift is exact)
+      const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      lsum *= f;
+#pragma unroll
+      for (int e = 0; e < NE; ++e) o[e] *= f;
+    }
+    const float base = m == -INFINITY ? 0.f : m - kShift;
+    uint32_t w[8];
+    uint32_t some[8];                          // careful: 1 where a weight is not zero
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float w0 = __builtin_amdgcn_exp2f(fmaf(x[2 * i], mul, -base));
+      const float w1 = __builtin_amdgcn_exp2f(fmaf(x[2 * i + 1], mul, -base));
+      w[i] = Ops::pk(w0, w1);
+      lsum = dot2<T>(w[i], Ops::ones8()[0], lsum);
+      if constexpr (careful.value) {
+        const uint32_t one = Ops::ones8()[0];
+        some[i] = (w0 != 0.f ? one & 0xffffu : 0u) | (w1 != 0.f ? one & 0xffff0000u : 0u);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const mf_u32x4 pop{w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]};
+#pragma unroll
+      for (int e = 0; e < NE; ++e) {
+        const uint2 a0 = ld_tr16(vaddr(cur, bp + u, 0, e));
+        const uint2 a1 = ld_tr16(vaddr(cur, bp + u, 1, e));
+        mf_u32x4 vop{a0.x, a0.y, a1.x, a1.y};
+        if constexpr (careful.value) {
+          mf_u32x4 bad;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) bad[i] = nonfinite_halves<T>(vop[i]);
+          if (__builtin_amdgcn_ballot_w64((bad[0] | bad[1] | bad[2] | bad[3]) != 0u)) {
+            const mf_u32x4 sop{some[4 * u], some[4 * u + 1], some[4 * u + 2], some[4 * u + 3]};
+            constexpr uint32_t kMant = std::is_same<T, bf16_t>::value ? 0x7fu : 0x3ffu;
+            const uint32_t one = Ops::ones8()[0];
+            mf_u32x4 pos, neg, nan;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t is_nan = 0, is_neg = 0;
+              if (vop[i] & kMant) is_nan |= 0xffffu;
+              if (vop[i] >> 16 & kMant) is_nan |= 0xffff0000u;
+              if (vop[i] & 0x8000u) is_neg |= 0xffffu;
+              if (vop[i] & 0x80000000u) is_neg |= 0xffff0000u;
+              nan[i] = one & bad[i] & is_nan;
+              neg[i] = one & bad[i] & ~is_nan & is_neg;
+              pos[i] = one & bad[i] & ~is_nan & ~is_neg;
+              vop[i] &= ~bad[i];
+            }
+            mf_f32x16 zero;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) zero[r] = 0.f;
+            const mf_f32x16 hp = M32::mma(pos, sop, zero), hn = M32::mma(neg, sop, zero),
+                            hx = M32::mma(nan, sop, zero);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              if (hp[r] != 0.f) o[e][r] += INFINITY;
+              if (hn[r] != 0.f) o[e][r] -= INFINITY;
+              if (hx[r] != 0.f) o[e][r] = __builtin_nanf("");
+            }
+          }
+        }
+        o[e] = M32::mma(vop, pop, o[e]);
+      }
+    }
+  };
+  auto walk = [&](auto careful) {
+    m = -INFINITY;
+    lsum = 0.f;
+#pragma unroll
+    for (int e = 0; e < NE; ++e)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[e][r] = 0.f;
+    // a step none of whose tokens any row of the wave sees is left out (uniform)
+    auto part = [&](int st, int bp, const StageBuf& cur) {
+      const int tok0 = st * kPromptTok + bp * kBlockTok;
+      if (wave_rows && tok0 <= row_last && !(kWindow && tok0 + 31 <= row_w - win))
+        step(careful, tok0, bp, cur);
+    };
+    if constexpr (careful.value) {
+      for (int st = st0; st < st1; ++st) {
+        __syncthreads();                    // (every wave is done with the stage before)
+        dma_stage(st, lds0);
+        __builtin_amdgcn_s_waitcnt(0x0F70);
+        __syncthreads();
+#pragma unroll 1
+        for (int bp = 0; bp < SB; bp += 2) part(st, bp, lds0);
+      }
+    } else {
+      auto stage = [&](int st, const StageBuf& cur, StageBuf& nxt) {
+        // stage st is in LDS (this wave's loads done, then everyone's), and every wave
+        // is done with the other buffer, which the next stage's loads fill
+        __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0)
+        __syncthreads();
+        if (st + 1 < st1) dma_stage(st + 1, nxt);
+        part(st, 0, cur);
+        part(st, 2, cur);
+      };
+      dma_stage(st0, lds0);
+      for (int st = st0; st < st1; st += 2) {
+        stage(st, lds0, lds1);
+        if (st + 1 < st1) stage(st + 1, lds1, lds0);
+      }
+    }
+  };
+  walk(std::false_type{});
+  bool odd = false;
+#pragma unroll
+  for (int e = 0; e < NE; ++e)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) odd = odd || o[e][r] != o[e][r];
+  // (the barrier also ends every wave's reads of the buffers that a second walk fills)
+  if (__syncthreads_or(odd && row_ok)) walk(std::true_type{});
+
+  if (!row_ok) return;
+  const float l = lsum + __shfl_xor(lsum, 32, 64);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  char* op = p.out + (int64_t)(tl.first + row) * p.o_tok + hq * p.o_head;
+#pragma unroll
+  for (int e = 0; e < NE; ++e)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<uint2*>(op + 2 * (32 * e + 8 * g + 4 * hh)) =
+          make_uint2(Ops::pk(o[e][4 * g] * inv, o[e][4 * g + 1] * inv),
+                     Ops::pk(o[e][4 * g + 2] * inv, o[e][4 * g + 3] * inv));
+}
+
+template <typename T, int D, bool kCap, bool kWindow>
+__global__ __launch_bounds__(64 * kPromptWaves, D == 256 ? 1 : 2) void prompt_attn_kernel(
+    PromptParams p) {
+  prompt_body<T, D, kCap, kWindow>(p);
+}
+
+template <typename T, int D>
+hipError_t launch_prompt_dim(const PromptParams& p, hipStream_t st) {
+  const dim3 grid((uint32_t)p.tiles * p.Hq), block(64 * kPromptWaves);
+  const bool cap = p.softcap > 0.f, win = p.window > 0;
+  if (cap && win) hipLaunchKernelGGL((prompt_attn_kernel<T, D, true, true>), grid, block, 0, st, p);
+  else if (cap) hipLaunchKernelGGL((prompt_attn_kernel<T, D, true, false>), grid, block, 0, st, p);
+  else if (win) hipLaunchKernelGGL((prompt_attn_kernel<T, D, false, true>), grid, block, 0, st, p);
+  else hipLaunchKernelGGL((prompt_attn_kernel<T, D, false, false>), grid, block, 0, st, p);
+  return hipGetLastError();
+}
+
+// One per element type, each in a source of its own (prompt_bf16.hip, prompt_f16.hip).
+hipError_t launch_prompt_bf16(const PromptParams& p, int D, hipStream_t st);
+hipError_t launch_prompt_f16(const PromptParams& p, int D, hipStream_t st);
+
+template <typename T>
+hipError_t launch_prompt_type(const PromptParams& p, int D, hipStream_t st) {
+  if (D == 64) return launch_prompt_dim<T, 64>(p, st);
+  if (D == 128) return launch_prompt_dim<T, 128>(p, st);
+  return launch_prompt_dim<T, 256>(p, st);
+}
+
+}  // namespace helm

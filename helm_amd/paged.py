@@ -10,7 +10,7 @@ the slot stride is ``2*Hkv*page*D`` elements and one page's head tile is
 from __future__ import annotations
 
 import math
-from typing import Dict, Optional, Sequence
+from typing import Dict, NamedTuple, Optional, Sequence
 
 import numpy as np
 import torch
@@ -157,3 +157,73 @@ def _decode_args(q, k_pool, v_pool, page_table, seq_lens, max_pages, total_pages
     keep = {"q": q, "out": out, "mask": m, "ws": ws, "table": page_table, "lens": seq_lens,
             "host_lens": hl}
     return args, keep
+
+
+class BatchTables(NamedTuple):
+    """A step's offsets and slots (``batch_tables``), all on the device."""
+    cu_seqlens: torch.Tensor    # int32 [B + 1], running sums of the new lengths
+    positions: torch.Tensor     # int64 [max_tokens], each packed token's position
+    slot_map: torch.Tensor      # int64 [max_tokens], its row of the pool, -1 for padding
+    seq_lens: torch.Tensor      # int32 [B], tokens with this step's
+    pages_taken: torch.Tensor   # int32 [1], pages taken from the free list
+
+
+def batch_tables(new_lens: torch.Tensor, cached_lens: torch.Tensor, page_table: torch.Tensor,
+                 free_slots: torch.Tensor, page_size: int, max_tokens: int,
+                 out: Optional[BatchTables] = None) -> BatchTables:
+    """A serving step's request lengths into block tables, slots, positions and
+    offsets, in one launch and without reading anything back.
+
+    new_lens / cached_lens: int32 [B], tokens that each sequence gets and has;
+    page_table: int32 [B, width], updated in place: the pages that the new tokens
+    need come from free_slots (int32, in order) and are written behind the pages
+    the sequence has, ceil(cached / page_size).  max_tokens: rows of the packed
+    step, at least the sum of new_lens (a captured step keeps it fixed).  out: a
+    former result of the same sizes, written instead of new tensors.
+
+    Token i of the step, of sequence b, has position cached + i - cu_seqlens[b]
+    and row page_table[b, position // page_size] * page_size + position %
+    page_size of the pool; rows past the last token get position 0 and slot -1,
+    which the pool's write skips.  A step that needs more pages than free_slots
+    holds (pages_taken says how many) or than the table is wide gets slot -1 for
+    their tokens, and -1 in the table.  At most 4096 sequences."""
+    for name, t in (("new_lens", new_lens), ("cached_lens", cached_lens),
+                    ("page_table", page_table), ("free_slots", free_slots)):
+        if t.dtype != torch.int32:
+            raise TypeError(f"{name} must be int32")
+    B = new_lens.numel()
+    if new_lens.dim() != 1 or cached_lens.shape != new_lens.shape or free_slots.dim() != 1:
+        raise ValueError("new_lens and cached_lens must be [B], free_slots [n]")
+    if page_table.dim() != 2 or page_table.size(0) != B:
+        raise ValueError("page_table must be [B, width]")
+    if page_table.stride(1) != 1 and page_table.size(1) > 1:
+        raise ValueError("page_table rows must be dense")
+    if B > 1 and page_table.stride(0) < page_table.size(1):
+        raise ValueError("page_table rows overlap")
+    for name, t in (("new_lens", new_lens), ("cached_lens", cached_lens),
+                    ("free_slots", free_slots)):
+        if not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+    if B < 1 or B > 4096 or page_size < 1 or max_tokens < 0:
+        raise ValueError("batch_tables takes 1 to 4096 sequences, page_size >= 1, max_tokens >= 0")
+    dev = new_lens.device
+    if out is None:
+        _engine.check_operands("batch_tables", dev, new_lens, cached_lens, page_table, free_slots)
+        ints = torch.empty(2 * B + 2, dtype=torch.int32, device=dev)
+        longs = torch.empty((2, max_tokens), dtype=torch.int64, device=dev)
+        out = BatchTables(ints[:B + 1], longs[0], longs[1], ints[B + 1:2 * B + 1], ints[2 * B + 1:])
+    else:
+        shapes = ((B + 1, torch.int32), (max_tokens, torch.int64), (max_tokens, torch.int64),
+                  (B, torch.int32), (1, torch.int32))
+        for name, t, (n, dt) in zip(BatchTables._fields, out, shapes):
+            if t.shape != (n,) or t.dtype != dt or not t.is_contiguous():
+                raise ValueError(f"out.{name} must be contiguous {dt} [{n}]")
+        _engine.check_operands("batch_tables", dev, new_lens, cached_lens, page_table, free_slots,
+                               *out)
+    _engine.call_on(dev, "helm_batch_tables", new_lens.data_ptr(), cached_lens.data_ptr(), B,
+                    page_table.data_ptr(), max(page_table.stride(0), page_table.size(1)),
+                    page_table.size(1), free_slots.data_ptr(), free_slots.numel(), page_size,
+                    max_tokens, out.cu_seqlens.data_ptr(), out.positions.data_ptr(),
+                    out.slot_map.data_ptr(), out.seq_lens.data_ptr(),
+                    out.pages_taken.data_ptr(), _engine.stream_ptr(dev))
+    return out

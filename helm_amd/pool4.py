@@ -1,0 +1,214 @@
+"""A slot pool whose pages hold K and V in 4 bits, and decode attention over it.
+
+``Pool4`` is the 4-bit counterpart of the slot pools that ``helm_amd.paged`` reads
+(same slots, page tables and lengths, 3.76 times as many tokens in the same memory);
+``Pool4.write`` puts a step's K and V rows into it, ``Pool4.read`` gets their values
+back, ``pool4_decode_attention`` attends over its pages.
+
+A value is held as an E2M1 code (0, .5, 1, 1.5, 2, 3, 4, 6 and their negatives) times
+its group's power of two, a group being 32 dims of one token and head: the smallest
+2^e, -125 <= e <= 125, that brings the group's largest magnitude to 7 or less; values go
+to the nearest code (ties to the even one), those above 6 to 6.  A group that holds an
+infinity or NaN stands for NaN.
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional, Tuple
+
+import torch
+
+from helm_amd import _native
+from helm_amd.runtime import engine as _engine
+
+_DIMS = (64, 128, 256)
+_MASKS = (torch.float32, torch.bfloat16, torch.float16)
+
+
+class Pool4:
+    """`n_slots` pages of `page_size` tokens (a multiple of 16) of `num_kv_heads` heads
+    of `head_dim` 64, 128 or 256, in 4 bits.  ``data`` is the storage, uint8
+    ``[n_slots, Hkv, page_size / 16, 17 * head_dim]``; what its bytes mean is the
+    library's affair."""
+
+    def __init__(self, n_slots: int, num_kv_heads: int, head_dim: int, page_size: int = 16,
+                 device="cuda"):
+        if head_dim not in _DIMS:
+            raise NotImplementedError(f"a 4-bit pool has head_dim 64, 128 or 256, not {head_dim}")
+        if n_slots < 0 or n_slots > 0x7fffffff or num_kv_heads < 1:
+            raise ValueError("n_slots must be 0 to 2^31 - 1 and num_kv_heads at least 1")
+        if page_size < 16 or page_size % 16:
+            raise ValueError("page_size must be a multiple of 16")
+        self.n_slots, self.num_kv_heads = n_slots, num_kv_heads
+        self.head_dim, self.page_size = head_dim, page_size
+        self.data = torch.zeros((n_slots, num_kv_heads, page_size // 16, 17 * head_dim),
+                                dtype=torch.uint8, device=device)
+
+    def _rows(self, what: str, k: torch.Tensor, v: torch.Tensor, slot_map: torch.Tensor) -> None:
+        want = (slot_map.numel(), self.num_kv_heads, self.head_dim)
+        if slot_map.dtype != torch.int64:
+            raise TypeError("slot_map must be int64")
+        if slot_map.dim() != 1 or not slot_map.is_contiguous():
+            raise ValueError("slot_map must be a contiguous [n]")
+        if tuple(k.shape) != want or tuple(v.shape) != want:
+            raise ValueError(f"{what}: k and v must be {list(want)}, one row a slot")
+        if k.dtype != v.dtype:
+            raise TypeError("k and v must share a dtype")
+
+    def write(self, k: torch.Tensor, v: torch.Tensor, slot_map: torch.Tensor) -> None:
+        """Rows n of k and v ([n, Hkv, D] float16, bfloat16 or float32, any strides) into
+        row slot_map[n] (int64, slot * page_size + token; outside the pool, -1 for
+        instance: skipped).  Rows of one call that share a slot leave either's values,
+        group by group: give each its own."""
+        self._rows("Pool4.write", k, v, slot_map)
+        code = _native.dtype_code(k.dtype)
+        _engine.check_operands("Pool4.write", self.data.device, k, v, slot_map)
+        k, v = _aligned_rows(k), _aligned_rows(v)
+        _engine.call_on(self.data.device, "helm_pool4_write", self.data.data_ptr(), self.n_slots,
+                        self.page_size, self.num_kv_heads, self.head_dim, slot_map.data_ptr(),
+                        slot_map.numel(), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
+                        v.stride(0), v.stride(1), code, _engine.stream_ptr(self.data.device))
+
+    def read(self, slot_map: torch.Tensor, dtype: torch.dtype = torch.bfloat16
+             ) -> Tuple[torch.Tensor, torch.Tensor]:
+        """The values held in rows slot_map, (k, v) [n, Hkv, D] of `dtype` (exact but for
+        its rounding); zeros for rows outside the pool."""
+        code = _native.dtype_code(dtype)
+        kv = torch.empty((2, slot_map.numel(), self.num_kv_heads, self.head_dim), dtype=dtype,
+                         device=self.data.device)
+        k, v = kv[0], kv[1]
+        self._rows("Pool4.read", k, v, slot_map)
+        _engine.check_operands("Pool4.read", self.data.device, slot_map)
+        _engine.call_on(self.data.device, "helm_pool4_read", self.data.data_ptr(), self.n_slots,
+                        self.page_size, self.num_kv_heads, self.head_dim, slot_map.data_ptr(),
+                        slot_map.numel(), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
+                        v.stride(0), v.stride(1), code, _engine.stream_ptr(self.data.device))
+        return k, v
+
+
+def _aligned_rows(x: torch.Tensor) -> torch.Tensor:
+    """x [n, H, D] itself where its rows are dense and 16-byte aligned, else a copy."""
+    unit = 16 // x.element_size()
+    if (x.stride(2) != 1 or x.stride(0) % unit or x.stride(1) % unit or x.data_ptr() % 16):
+        x = torch.empty(x.shape, dtype=x.dtype, device=x.device).copy_(x)
+    return x
+
+
+class PreparedPool4Decode:
+    """``pool4_decode_attention`` with its arguments checked and its workspace taken
+    once, for loops that issue the same shape every step.  ``run`` reads q, page table,
+    lengths, mask and pool as they are then, on torch's current stream; runs of one
+    object (its replays in graphs among them) share its workspace and `out` and must
+    not overlap."""
+
+    def __init__(self, device, args, out, keep):
+        self._device, self._args, self.out, self._keep = device, args, out, keep
+
+    def run(self) -> torch.Tensor:
+        _engine.call_on(self._device, "helm_pool4_decode_attn", *self._args,
+                        _engine.stream_ptr(self._device))
+        return self.out
+
+
+def prepare_pool4_decode(q: torch.Tensor, pool: Pool4, page_table: torch.Tensor,
+                         seq_lens: torch.Tensor, max_pages: Optional[int] = None,
+                         scale: Optional[float] = None, softcap: Optional[float] = None,
+                         attention_mask: Optional[torch.Tensor] = None, causal: bool = False,
+                         out: Optional[torch.Tensor] = None) -> PreparedPool4Decode:
+    """Arguments as ``pool4_decode_attention``; q must be contiguous and the mask one that
+    is read as given (float32, bfloat16 or float16, dense rows), so that later runs
+    see what is written to them."""
+    if not q.is_contiguous():
+        raise ValueError("a prepared call reads q in place: it must be contiguous")
+    m = attention_mask
+    if m is not None and (m.dtype not in _MASKS or m.stride(-1) != 1):
+        raise ValueError("a prepared call reads the mask in place: float32, bfloat16 or "
+                         "float16 with dense rows")
+    args, out, keep = _decode_args(q, pool, page_table, seq_lens, max_pages, scale, softcap,
+                                   attention_mask, causal, out)
+    return PreparedPool4Decode(q.device, args, out, keep)
+
+
+def pool4_decode_attention(q: torch.Tensor, pool: Pool4, page_table: torch.Tensor,
+                           seq_lens: torch.Tensor, max_pages: Optional[int] = None,
+                           scale: Optional[float] = None, softcap: Optional[float] = None,
+                           attention_mask: Optional[torch.Tensor] = None, causal: bool = False,
+                           out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of q [B, Hq, q_len, D] (float16 or bfloat16) over 4-bit pages, the
+    arguments of ``paged.paged_decode_attention``.
+
+    page_table: int32 [B, >= max_pages] slots of the pool (others count as hidden
+    pages); seq_lens: int32 [B] tokens, on the device; attention_mask: additive
+    [B|1, Hq|1, q_len|1, T], tokens from T on are hidden; causal: the q_len rows are
+    the sequence's last tokens, each sees those up to its own.  Hidden tokens (-inf in
+    the mask among them) take no part whatever they hold, and a row that sees nothing
+    is zeros.  Returns out [B, Hq, q_len, D] in q's dtype."""
+    args, out, _ = _decode_args(q, pool, page_table, seq_lens, max_pages, scale, softcap,
+                                attention_mask, causal, out)
+    _engine.call_on(q.device, "helm_pool4_decode_attn", *args, _engine.stream_ptr(q.device))
+    return out
+
+
+def check_scores(scale: Optional[float], softcap: Optional[float], D: int) -> Tuple[float, float]:
+    """(scale, softcap or 0) of an attention call."""
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    cap = 0.0 if softcap is None else float(softcap)
+    if not math.isfinite(scale):
+        raise ValueError("scale must be finite")
+    if not (0.0 <= cap < math.inf):
+        raise ValueError("softcap must be a positive number (None or 0: off)")
+    return scale, cap
+
+
+def _decode_args(q, pool, page_table, seq_lens, max_pages, scale, softcap, mask, causal, out):
+    """Checks the operands; (C-ABI arguments up to the stream, out, tensors to keep)."""
+    if q.dim() != 4:
+        raise ValueError("q must be [B, Hq, q_len, D]")
+    B, Hq, S, D = q.shape
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError("queries over a 4-bit pool are float16 or bfloat16")
+    if D != pool.head_dim or Hq < 1 or Hq % pool.num_kv_heads or S < 1:
+        raise ValueError("q does not match the pool's heads")
+    if page_table.dtype != torch.int32 or seq_lens.dtype != torch.int32:
+        raise TypeError("page_table and seq_lens must be int32")
+    if page_table.dim() != 2 or page_table.size(0) != B or seq_lens.shape != (B,):
+        raise ValueError("page_table must be [B, >=max_pages] and seq_lens [B]")
+    if (page_table.stride(1) != 1 and page_table.size(1) > 1) or not seq_lens.is_contiguous():
+        raise ValueError("page_table rows and seq_lens must be dense")
+    if max_pages is None:
+        max_pages = page_table.size(1)
+    if not 0 <= max_pages <= page_table.size(1):
+        raise ValueError("max_pages must be 0 to the table's width")
+    scale, cap = check_scores(scale, softcap, D)
+    m, ms, width = None, (0, 0, 0), 0
+    if mask is not None:
+        if mask.dim() != 4 or mask.size(0) not in (1, B) or mask.size(1) not in (1, Hq) or \
+                mask.size(2) not in (1, S) or mask.size(3) < 1:
+            raise ValueError("attention_mask must be [B|1, Hq|1, q_len|1, T]")
+        if not mask.is_floating_point():
+            raise TypeError("attention_mask is additive: a floating-point tensor")
+        m = mask if mask.dtype in _MASKS else mask.float()
+        if m.stride(3) != 1:
+            m = m.contiguous()
+        ms = tuple(m.stride(i) if m.size(i) > 1 else 0 for i in range(3))
+        width = m.size(3)
+    if out is None:
+        out = torch.empty((B, Hq, S, D), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+        raise ValueError("out must be contiguous, of q's shape and dtype")
+    _engine.check_operands("pool4_decode_attention", q.device, q, pool.data, page_table, seq_lens, m,
+                           out)
+    q = q.contiguous()
+    if q.data_ptr() % 16:
+        q = q.clone()
+    lib = _native.load()
+    need = lib.helm_pool4_workspace_bytes(B, Hq, pool.num_kv_heads, S, D, max_pages,
+                                          pool.page_size)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    args = (q.data_ptr(), out.data_ptr(), pool.data.data_ptr(), pool.n_slots, pool.page_size,
+            page_table.data_ptr(), max(page_table.stride(0), max_pages), max_pages,
+            seq_lens.data_ptr(), B, Hq, pool.num_kv_heads, S, D, scale, cap,
+            m.data_ptr() if m is not None else None, *ms, width,
+            _native.dtype_code(m.dtype) if m is not None else _native.HELM_F32, int(bool(causal)),
+            _native.dtype_code(q.dtype), ws.data_ptr() if ws is not None else None, need)
+    return args, out, (q, pool, page_table, seq_lens, m, ws)

@@ -62,6 +62,33 @@ def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(idx).cuda_stream
 
 
+def call_on(device: torch.device, fn: str, *args) -> None:
+    """One native call that launches on `device`: the device is current for it
+    (and the one before is again afterwards); raises as ``_native.call`` does."""
+    f = _native.entry(fn)
+    if device.index is None or device.index == torch.cuda.current_device():
+        rc = f(*args)
+    else:
+        with torch.cuda.device(device):
+            rc = f(*args)
+    if rc:
+        _native.check(fn, rc)
+
+
+def check_operands(what: str, device: torch.device, *tensors) -> None:
+    """The operands of a call sit on one HIP device and ask for no gradient
+    (None is skipped)."""
+    for t in tensors:
+        if t is None:
+            continue
+        if t.device != device:
+            raise ValueError(f"{what}: operands on {device} and {t.device}")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{what} records no gradient: call it under torch.no_grad()")
+    if device.type != "cuda":
+        raise RuntimeError(f"{what} needs HIP tensors")
+
+
 @atexit.register
 def _destroy_engines() -> None:
     if not _engines:

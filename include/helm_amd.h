@@ -361,6 +361,99 @@ int helm_prefetch_pages(helm_engine* eng, int n, const uint64_t* src_host,
                         const uint64_t* dst_dev, const uint64_t* bytes,
                         int sync, void* stream);
 
+/* ---- a step's tables ------------------------------------------------------- */
+
+/* Request lengths into a step's block tables, slots, positions and offsets, on
+ * the device, in one launch; no counterpart in the reference (its pages are
+ * Python lists, helm/runtime/kv_cache.py:113-171).  Sequence b (of B) holds
+ * cached_lens[b] tokens and gets new_lens[b] more (device int32; negative
+ * ones count as 0).  It owns ceil(cached / page_size) pages, the first entries
+ * of its row of page_table (table_stride elements apart, table_width entries
+ * used), and takes ceil((cached + new) / page_size) less those from
+ * free_slots[0 .. n_free), sequences in order, written to its next entries.
+ * Out: cu_seqlens[B + 1] running sums of new; for each i < max_tokens the
+ * position of packed token i in its sequence (positions, 0 past the last
+ * token) and its row page_table[..] * page_size + position % page_size
+ * (slot_map, -1 past the last token); seq_lens[b] = cached + new; pages_taken
+ * (one int) = pages needed by all.  Where pages_taken > n_free, or a sequence
+ * needs more than table_width pages, the missing pages' tokens get slot -1 and
+ * their entries inside the table -1.  Entries that the call does not take are
+ * not written; tokens past max_tokens are left out.  Sums stop at 2^31 - 1.
+ * B <= HELM_TABLES_MAX_SEQS. */
+#define HELM_TABLES_MAX_SEQS 4096
+int helm_batch_tables(const int32_t* new_lens, const int32_t* cached_lens, int B,
+                      int32_t* page_table, int64_t table_stride, int table_width,
+                      const int32_t* free_slots, int n_free, int page_size, int max_tokens,
+                      int32_t* cu_seqlens, int64_t* positions, int64_t* slot_map,
+                      int32_t* seq_lens, int32_t* pages_taken, void* stream);
+
+/* ---- a pool of 4-bit pages --------------------------------------------------- */
+
+/* K and V held in 4 bits: E2M1 codes (0, .5, 1, 1.5, 2, 3, 4, 6 and negatives)
+ * in groups of 32 dims of one token and head under one power of two 2^e, the
+ * smallest with |largest| <= 7 * 2^e, -125 <= e <= 125; a value goes to the
+ * nearest code (ties to the even one), above 6 to 6.  A group that holds an
+ * infinity or NaN stands for NaN.  17 D / 32 bytes a row of D dims.
+ * The pool is [n_slots][Hkv][page_size / 16][17 D] bytes, 16-byte aligned: per
+ * tile of 16 tokens K codes, V codes, K exponents, V exponents (the layout is
+ * the library's; read it with helm_pool4_read).  head_dim 64, 128 or 256
+ * (HELM_E_UNSUPPORTED otherwise), page_size a multiple of 16.
+ *
+ * helm_pool4_write: row n of k and v ([n_tok, Hkv, D], strides in elements, D
+ * contiguous, rows 16-byte aligned, HELM_F16 / BF16 / F32) into row
+ * slot_map[n] = slot * page_size + token of the pool; rows outside
+ * [0, n_slots * page_size) are skipped.  Two rows of one call with the same
+ * slot leave either's values, group by group.
+ * helm_pool4_read: the values of those rows, exact but for the rounding to
+ * the output type; zeros for rows outside the pool. */
+int helm_pool4_write(void* pool, int64_t n_slots, int page_size, int Hkv, int D,
+                     const int64_t* slot_map, int n_tok, const void* k, int64_t k_tok_stride,
+                     int64_t k_head_stride, const void* v, int64_t v_tok_stride,
+                     int64_t v_head_stride, int dtype, void* stream);
+int helm_pool4_read(const void* pool, int64_t n_slots, int page_size, int Hkv, int D,
+                    const int64_t* slot_map, int n_tok, void* k, int64_t k_tok_stride,
+                    int64_t k_head_stride, void* v, int64_t v_tok_stride,
+                    int64_t v_head_stride, int dtype, void* stream);
+
+/* helm_paged_decode_attn over a 4-bit pool.  q and out [B, Hq, q_len, D] dense,
+ * HELM_F16 or HELM_BF16; page_table, seq_lens and mask as there.  causal != 0:
+ * the q_len rows are the sequence's last tokens, row s sees tokens
+ * 0 .. len - q_len + s.  mask_len: columns of the mask; tokens from there on are
+ * hidden.  Hidden tokens (those, past the limit, or under -inf) take no part
+ * whatever they hold; a row that sees nothing is zeros.  Pages whose slot is
+ * outside [0, n_slots), and tokens past max_pages, count as hidden.  The
+ * workspace (helm_pool4_workspace_bytes; 0: none needed, 16-byte aligned)
+ * needs no contents before or after a call; calls that may overlap need one
+ * each. */
+size_t helm_pool4_workspace_bytes(int B, int Hq, int Hkv, int q_len, int D, int max_pages,
+                                  int page_size);
+int helm_pool4_decode_attn(const void* q, void* out, const void* pool, int64_t n_slots,
+                           int page_size, const int32_t* page_table, int64_t table_stride,
+                           int max_pages, const int32_t* seq_lens, int B, int Hq, int Hkv,
+                           int q_len, int D, float scale, float softcap, const void* mask,
+                           int64_t mask_bstride, int64_t mask_hstride, int64_t mask_qstride,
+                           int mask_len, int mask_dtype, int causal, int q_dtype,
+                           void* workspace, size_t ws_bytes, void* stream);
+
+/* ---- whole prompts ------------------------------------------------------------- */
+
+/* Causal attention of packed whole prompts: the keys and values are the prompts'
+ * own tokens (the first-chunk attention of _stream_prefill_batched,
+ * helm/runtime/kv_cache.py:562-568, of sequences of different lengths in one
+ * call).  q [N, Hq, D], k and v [N, Hkv, D], out [N, Hq, D]: strides in elements,
+ * D contiguous, rows 16-byte aligned, HELM_F16 or HELM_BF16.  Sequence b is
+ * rows cu_seqlens[b] .. cu_seqlens[b + 1] (device int32, ascending; clamped to
+ * [0, N]); row i of it sees rows j <= i, with window > 0 only j > i - window.
+ * softcap <= 0: off.  Rows before cu_seqlens[0] and from cu_seqlens[B] on: left
+ * as they are, or zeros with zero_rest != 0.  head_dim 64, 128 or 256. */
+int helm_prompt_attn(const void* q, int64_t q_tok_stride, int64_t q_head_stride, const void* k,
+                     int64_t k_tok_stride, int64_t k_head_stride, const void* v,
+                     int64_t v_tok_stride, int64_t v_head_stride, void* out,
+                     int64_t out_tok_stride, int64_t out_head_stride,
+                     const int32_t* cu_seqlens, int B, int N, int Hq, int Hkv, int D,
+                     float scale, float softcap, int window, int zero_rest, int dtype,
+                     void* stream);
+
 /* ---- device profile ------------------------------------------------------- */
 
 /* Bandwidths of one device, as HELM's device profiler measures them for its

@@ -1,0 +1,220 @@
+"""What the serving operators refuse, and what they do not need a GPU for: argument
+checks of the Python entry points and of the C-ABI (which return before any device
+work), the oracle's own properties."""
+import math
+
+import pytest
+import torch
+
+from helm_amd import _native, paged, pool4, prompt
+from oracle import serving as R
+
+I32, I64 = torch.int32, torch.int64
+
+
+def _tables(B=2, width=4, **kw):
+    a = dict(new_lens=torch.ones(B, dtype=I32), cached_lens=torch.zeros(B, dtype=I32),
+             page_table=torch.zeros((B, width), dtype=I32), free_slots=torch.arange(8, dtype=I32),
+             page_size=16, max_tokens=4)
+    a.update(kw)
+    return a
+
+
+@pytest.mark.parametrize("bad,err", [
+    (dict(new_lens=torch.ones(2, dtype=I64)), TypeError),
+    (dict(free_slots=torch.arange(8, dtype=I64)), TypeError),
+    (dict(cached_lens=torch.zeros(3, dtype=I32)), ValueError),
+    (dict(page_table=torch.zeros((3, 4), dtype=I32)), ValueError),
+    (dict(page_table=torch.zeros((4, 2), dtype=I32).t()), ValueError),
+    (dict(page_table=torch.zeros((1, 4), dtype=I32).expand(2, 4)), ValueError),
+    (dict(new_lens=torch.ones(4, dtype=I32)[::2]), ValueError),
+    (dict(page_size=0), ValueError),
+    (dict(max_tokens=-1), ValueError),
+    (dict(new_lens=torch.ones(4097, dtype=I32), cached_lens=torch.zeros(4097, dtype=I32),
+          page_table=torch.zeros((4097, 1), dtype=I32)), ValueError),
+    ({}, RuntimeError),            # CPU tensors
+])
+def test_batch_tables_refusals(bad, err):
+    with pytest.raises(err):
+        paged.batch_tables(**_tables(**bad))
+
+
+def test_batch_tables_out_refusals():
+    good = paged.BatchTables(torch.zeros(3, dtype=I32), torch.zeros(4, dtype=I64),
+                             torch.zeros(4, dtype=I64), torch.zeros(2, dtype=I32),
+                             torch.zeros(1, dtype=I32))
+    with pytest.raises(ValueError):
+        paged.batch_tables(**_tables(), out=good._replace(slot_map=torch.zeros(5, dtype=I64)))
+    with pytest.raises(ValueError):
+        paged.batch_tables(**_tables(), out=good._replace(positions=torch.zeros(4, dtype=I32)))
+
+
+@pytest.mark.parametrize("kw,err", [
+    (dict(head_dim=96), NotImplementedError), (dict(page_size=24), ValueError),
+    (dict(page_size=0), ValueError), (dict(n_slots=-1), ValueError),
+    (dict(num_kv_heads=0), ValueError)])
+def test_pool4_refusals(kw, err):
+    a = dict(n_slots=4, num_kv_heads=2, head_dim=64, page_size=16, device="cpu")
+    a.update(kw)
+    with pytest.raises(err):
+        pool4.Pool4(**a)
+
+
+@pytest.mark.parametrize("k,v,slots,err", [
+    (torch.zeros(3, 2, 64), torch.zeros(3, 2, 64), torch.zeros(3, dtype=I32), TypeError),
+    (torch.zeros(3, 2, 64), torch.zeros(3, 2, 64), torch.zeros(4, dtype=I64), ValueError),
+    (torch.zeros(3, 1, 64), torch.zeros(3, 2, 64), torch.zeros(3, dtype=I64), ValueError),
+    (torch.zeros(3, 2, 128), torch.zeros(3, 2, 128), torch.zeros(3, dtype=I64), ValueError),
+    (torch.zeros(3, 2, 64), torch.zeros(3, 2, 64).half(), torch.zeros(3, dtype=I64), TypeError),
+    (torch.zeros(3, 2, 64).double(), torch.zeros(3, 2, 64).double(), torch.zeros(3, dtype=I64),
+     TypeError),
+    (torch.zeros(3, 2, 64), torch.zeros(3, 2, 64), torch.zeros(6, dtype=I64)[::2], ValueError),
+    (torch.zeros(3, 2, 64), torch.zeros(3, 2, 64), torch.zeros(3, dtype=I64), RuntimeError),
+])
+def test_pool4_write_refusals(k, v, slots, err):
+    pool = pool4.Pool4(2, 2, 64, device="cpu")
+    with pytest.raises(err):
+        pool.write(k, v, slots)
+    if err is RuntimeError:
+        with pytest.raises(err):
+            pool.read(slots)
+
+
+def _decode(**kw):
+    a = dict(q=torch.zeros(2, 4, 1, 64, dtype=torch.bfloat16),
+             pool=pool4.Pool4(4, 2, 64, device="cpu"), page_table=torch.zeros((2, 2), dtype=I32),
+             seq_lens=torch.ones(2, dtype=I32))
+    a.update(kw)
+    return a
+
+
+@pytest.mark.parametrize("bad,err", [
+    (dict(q=torch.zeros(2, 4, 1, 64)), TypeError),
+    (dict(q=torch.zeros(2, 3, 1, 64).bfloat16()), ValueError),
+    (dict(q=torch.zeros(2, 4, 0, 64).bfloat16()), ValueError),
+    (dict(q=torch.zeros(2, 4, 64).bfloat16()), ValueError),
+    (dict(q=torch.zeros(2, 4, 1, 128).bfloat16()), ValueError),
+    (dict(page_table=torch.zeros((2, 2), dtype=I64)), TypeError),
+    (dict(page_table=torch.zeros((3, 2), dtype=I32)), ValueError),
+    (dict(seq_lens=torch.ones(3, dtype=I32)), ValueError),
+    (dict(max_pages=3), ValueError), (dict(max_pages=-1), ValueError),
+    (dict(softcap=-1.0), ValueError), (dict(softcap=math.inf), ValueError),
+    (dict(scale=math.nan), ValueError),
+    (dict(attention_mask=torch.zeros(2, 4, 1, 32, dtype=torch.bool)), TypeError),
+    (dict(attention_mask=torch.zeros(2, 3, 1, 32)), ValueError),
+    (dict(attention_mask=torch.zeros(1, 32)), ValueError),
+    (dict(attention_mask=torch.zeros(2, 1, 1, 0)), ValueError),
+    (dict(out=torch.zeros(2, 4, 1, 64)), ValueError),
+    ({}, RuntimeError)])
+def test_pool4_decode_refusals(bad, err):
+    with pytest.raises(err):
+        pool4.pool4_decode_attention(**_decode(**bad))
+
+
+def test_prepared_pool4_decode_reads_in_place():
+    q = torch.zeros(2, 1, 4, 64, dtype=torch.bfloat16).transpose(1, 2)
+    assert not q.is_contiguous() or q.shape[2] == 1
+    q = torch.zeros(2, 4, 2, 128, dtype=torch.bfloat16)[..., :64]
+    with pytest.raises(ValueError, match="in place"):
+        pool4.prepare_pool4_decode(**_decode(q=q))
+    with pytest.raises(ValueError, match="in place"):
+        pool4.prepare_pool4_decode(**_decode(attention_mask=torch.zeros(2, 1, 1, 32).double()))
+
+
+def _prompt(**kw):
+    a = dict(q=torch.zeros(5, 4, 64).half(), k=torch.zeros(5, 2, 64).half(),
+             v=torch.zeros(5, 2, 64).half(), cu_seqlens=torch.tensor([0, 5], dtype=I32))
+    a.update(kw)
+    return a
+
+
+@pytest.mark.parametrize("bad,err", [
+    (dict(q=torch.zeros(5, 4, 64)), TypeError),
+    (dict(v=torch.zeros(5, 2, 64).bfloat16()), TypeError),
+    (dict(q=torch.zeros(5, 3, 64).half()), ValueError),
+    (dict(q=torch.zeros(6, 4, 64).half()), ValueError),
+    (dict(v=torch.zeros(5, 1, 64).half()), ValueError),
+    (dict(q=torch.zeros(5, 4, 80).half(), k=torch.zeros(5, 2, 80).half(),
+          v=torch.zeros(5, 2, 80).half()), NotImplementedError),
+    (dict(cu_seqlens=torch.tensor([0, 5])), TypeError),
+    (dict(cu_seqlens=torch.zeros((1, 2), dtype=I32)), ValueError),
+    (dict(window=-1), ValueError), (dict(softcap=-2.0), ValueError),
+    (dict(scale=math.inf), ValueError),
+    (dict(out=torch.zeros(5, 4, 64)), ValueError),
+    ({}, RuntimeError)])
+def test_prompt_refusals(bad, err):
+    with pytest.raises(err):
+        prompt.prompt_attention(**_prompt(**bad))
+
+
+def test_operands_that_ask_for_a_gradient_are_refused():
+    a = _prompt()
+    a["q"].requires_grad_()
+    with pytest.raises(RuntimeError, match="no gradient"):
+        prompt.prompt_attention(**a)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="HIP tensors"):
+        prompt.prompt_attention(**a)
+
+
+def test_c_entries_refuse_before_device_work():
+    lib = _native.load()
+    E, U, W = _native.HELM_E_INVALID, _native.HELM_E_UNSUPPORTED, _native.HELM_E_WORKSPACE
+    BF, F32 = _native.HELM_BF16, _native.HELM_F32
+
+    def tables(B=1, page=16, width=1, stride=1, n=0, p=1):
+        return lib.helm_batch_tables(p, p, B, p, stride, width, p, n, page, 1, p, p, p, p, p, None)
+    assert tables(B=0) == E and tables(B=4097) == E and tables(page=0) == E
+    assert tables(stride=0) == E and tables(n=-1) == E and tables(p=None) == E
+
+    def write(D=64, page=16, n=1, dt=BF, p=16, ts=64):
+        return lib.helm_pool4_write(p, 1, page, 1, D, p, n, p, ts, 64, p, ts, 64, dt, None)
+    assert write(D=96) == U and write(page=8) == E and write(dt=9) == E and write(n=-1) == E
+    assert write(p=None) == E and write(p=8) == E and write(ts=65) == E
+    assert write(n=0) == 0
+
+    def attn(D=64, page=16, dt=BF, p=16, B=1, Hq=2, Hkv=1, S=1, mp=1, ts=1, mask=None, ml=0, mdt=F32,
+             ws=None, wb=0, q=16):
+        return lib.helm_pool4_decode_attn(q, p, p, 1, page, p, ts, mp, p, B, Hq, Hkv, S, D, 1.0, 0.0,
+                                          mask, 0, 0, 0, ml, mdt, 0, dt, ws, wb, None)
+    assert attn(D=80) == U and attn(dt=F32) == U and attn(page=20) == E and attn(Hq=3, Hkv=2) == E
+    assert attn(S=0) == E and attn(mp=2) == E and attn(p=None) == E and attn(q=8) == E
+    assert attn(mask=16, ml=0) == E and attn(mask=16, ml=4, mdt=7) == E
+    assert attn(mp=4096, ts=4096) == W and attn(B=0) == 0
+    assert lib.helm_pool4_workspace_bytes(1, 2, 1, 1, 64, 4096, 16) > 0
+    assert lib.helm_pool4_workspace_bytes(1, 3, 2, 1, 64, 16, 16) == 0
+
+    def prom(D=64, dt=BF, p=16, B=1, N=1, Hq=2, Hkv=1, scale=1.0, ts=64, kt=64):
+        return lib.helm_prompt_attn(p, ts, 64, p, kt, 64, p, kt, 64, p, 128, 64, p, B, N, Hq, Hkv, D,
+                                    scale, 0.0, 0, 0, dt, None)
+    assert prom(D=96) == U and prom(dt=F32) == U and prom(Hq=3, Hkv=2) == E and prom(N=-1) == E
+    assert prom(scale=math.nan) == E and prom(p=None) == E and prom(p=8) == E and prom(ts=4) == E
+    assert prom(kt=1 << 26) == E and prom(N=0) == 0
+    assert prom(N=0x7fffffff, Hq=64) == E
+
+
+# ---- the oracle ------------------------------------------------------------------------
+def test_stored_values_are_nearest_within_half_a_step():
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(64, 64, generator=g) * torch.exp(4 * torch.randn(64, 1, generator=g))
+    y = R.stored4(x)
+    top = x.double().unflatten(-1, (-1, 32)).abs().amax(-1, keepdim=True)
+    e = torch.ceil(torch.log2(top / 7))
+    r = x.double().unflatten(-1, (-1, 32)).abs() / 2 ** e
+    half = torch.where(r < 2, 0.25, torch.where(r < 4, 0.5, 1.0))
+    err = (y.unflatten(-1, (-1, 32)) - x.double().unflatten(-1, (-1, 32))).abs() / 2 ** e
+    assert (err <= half).all()
+    assert (R.stored4(y) == y).all()           # what is held stays
+
+
+def test_stored_edges():
+    x = torch.zeros(8, 32)
+    x[1, 3] = 7.0
+    x[2, 3] = 7.0000005
+    x[3, :2] = torch.tensor([6.0, 0.25])
+    x[4, :3] = torch.tensor([6.0, 0.75, -2.5])
+    x[5, 0], x[6, 0] = math.inf, math.nan
+    x[7, 0] = 1e-45
+    y = R.stored4(x)
+    assert y[1, 3] == 6.0 and y[2, 3] == 8.0 and y[3, 1] == 0.0
+    assert y[4, 1] == 1.0 and y[4, 2] == -2.0
+    assert torch.isnan(y[5]).all() and torch.isnan(y[6]).all() and (y[7] == 0).all()
