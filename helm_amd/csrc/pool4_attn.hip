@@ -6,11 +6,13 @@
 // once.  The codes become bf16 matrix-core operands in registers (two values an
 // instruction, exact), so nothing but the 4-bit page crosses memory.
 //
-// Work: grid.x = split of the sequence's tiles, grid.y = KV head * row tiles of
-// 16 query rows, grid.z = sequence; four waves, wave w takes blocks w, w + 4, ..
-// of 32 tokens (two tiles) of the split.  A split's length comes from the
-// sequence's own length, read on the device: ceil(tiles / splits), so that one
-// launch shape serves any lengths.  Lane (n, h) = (lane % 16, lane / 16):
+// Work: grid.x = split, grid.y = KV head * row tiles of 16 query rows, grid.z =
+// sequence; four waves.  The sequence's blocks of 32 tokens (two tiles) go round
+// the waves of all splits: wave w of split s takes blocks 4 s + w + 4 splits * j.  A
+// wave's first blocks so follow from the launch alone (their table entries are
+// read beside the sequence's length, not after it), a sequence of any length is
+// spread evenly, and a short one uses few splits.
+// Lane (n, h) = (lane % 16, lane / 16):
 //   S^T = K Q^T  (16 x 16 x 32, one product per tile and 32 dims): A is token n's
 //         dims D/4 h + 8i .. + 7, which is word i of the lane's D/8 contiguous code
 //         bytes; B is query row n at the same dims.  The lane gets row n's scores
@@ -44,7 +46,8 @@ namespace {
 
 constexpr int kP4Waves = 4;
 constexpr int kP4Rows = 16;
-constexpr int kP4MaxTiles = 2048;    // of a split (their slots sit in LDS)
+// blocks of a wave in registers, all but one in flight; D = 256's are twice as large
+constexpr int p4_bufs(int D) { return D == 256 ? 2 : 3; }
 constexpr float kP4Slack = 8.f;      // base-2 units
 constexpr float kP4Log2E = 1.4426950408889634f;
 
@@ -61,28 +64,26 @@ struct P4Attn {
   int B, Hq, Hkv, G, S, row_tiles;
   int q16;                           // 1: q and out are f16, else bf16
   int splits;
-  int min_tiles;                     // a split's least tiles (whole waves' blocks)
   int causal;
   float scale, softcap;
   const char* mask;
   int64_t mask_b, mask_h, mask_q;    // elements
   int mask_dt, mask_len;             // tokens from mask_len on are hidden
-  float* part_o;                     // [B][Hq * S][splits][D]
-  float* part_ml;                    // [B][Hq * S][splits][2]
+  float* part_o;                     // [tile][splits][16 rows][D], tile = (b, KV head, row tile)
+  float* part_ml;                    // [tile][splits][16 rows][2]
 };
 
-// Tiles of sequence b, and how its splits share them.
-struct P4Split {
-  int len, tiles, per, n;            // tokens; tiles; tiles a split; splits in use
+// Sequence b's tokens, tiles, blocks, and the splits that have any of them.
+struct P4Seq {
+  int len, tiles, blocks, splits;
 };
-__device__ __forceinline__ P4Split p4_split(const P4Attn& a, int b) {
-  P4Split s;
+__device__ __forceinline__ P4Seq p4_seq(const P4Attn& a, int b) {
+  P4Seq s;
   const int64_t room = (int64_t)a.max_pages * a.tpp * kP4Tok;
   s.len = (int)min((int64_t)max(0, a.seq_lens[b]), room);
-  s.tiles = (s.len + kP4Tok - 1) / kP4Tok;
-  s.per = max(a.min_tiles, (s.tiles + a.splits - 1) / a.splits);
-  s.per = (s.per + 1) & ~1;          // whole blocks
-  s.n = (s.tiles + s.per - 1) / s.per;
+  s.tiles = (int)(((int64_t)s.len + kP4Tok - 1) / kP4Tok);
+  s.blocks = (s.tiles + 1) / 2;
+  s.splits = min(a.splits, (s.blocks + kP4Waves - 1) / kP4Waves);
   return s;
 }
 
@@ -144,19 +145,51 @@ __device__ __forceinline__ uint32_t p4_v_pair(const P4Raw<D>& r, int j, int c, f
   }
 }
 
+__device__ __forceinline__ mf_u32x2 load8_any(const char* p) {
+  struct __attribute__((packed)) Any { mf_u32x2 v; };
+  return reinterpret_cast<const Any*>(p)->v;
+}
+
 // Any byte of x equal to 255.
 __device__ __forceinline__ bool any_ff(uint32_t x) {
   return ((~x - 0x01010101u) & x & 0x80808080u) != 0u;
 }
 
-template <int D, int QP, bool kMask, bool kCap>
+__device__ __forceinline__ void add_scaled(float4& acc, float f, const float4 v) {
+  acc.x += f * v.x;
+  acc.y += f * v.y;
+  acc.z += f * v.z;
+  acc.w += f * v.w;
+}
+
+// Dims 4 col .. of query row `row` (of the head's G * S) of the output: acc / sum.
+template <int D>
+__device__ __forceinline__ void store_row(const P4Attn& a, int b, int hk, int row, int col,
+                                          const float4 acc, float sum) {
+  const RowCoord c = row_coord(row, a.G);
+  const int64_t r = (int64_t)(b * a.Hq + hk * a.G + c.g) * a.S + c.s;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  uint2 w;
+  if (a.q16)
+    w = make_uint2(MfmaOps<f16_t>::pk(acc.x * inv, acc.y * inv),
+                   MfmaOps<f16_t>::pk(acc.z * inv, acc.w * inv));
+  else
+    w = make_uint2(MfmaOps<bf16_t>::pk(acc.x * inv, acc.y * inv),
+                   MfmaOps<bf16_t>::pk(acc.z * inv, acc.w * inv));
+  // (out is 8-byte aligned or better: checked on the host)
+  *reinterpret_cast<uint2*>(reinterpret_cast<char*>(a.out) + 2 * (r * D + 4 * col)) = w;
+}
+
+// MB: bytes of a mask element (0: no mask).
+template <int D, int QP, int MB, bool kCap>
 __global__ __launch_bounds__(64 * kP4Waves) void pool4_attn_kernel(P4Attn a) {
+  constexpr bool kMask = MB != 0;
+  constexpr int NB = p4_bufs(D);
   constexpr int NS = D / 32;                 // 32-dim steps of q . k
   constexpr int NE = D / 16;                 // dims of a V chunk: products of P . V
   using Ops = MfmaOps<bf16_t>;
-  __shared__ int slots[kP4MaxTiles];
   __shared__ float sh_o[kP4Waves][kP4Rows][D + 4];
-  __shared__ float sh_m[kP4Waves][kP4Rows], sh_l[kP4Waves][kP4Rows];
+  __shared__ float2 sh_ml[kP4Waves][kP4Rows];
 
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -164,18 +197,29 @@ __global__ __launch_bounds__(64 * kP4Waves) void pool4_attn_kernel(P4Attn a) {
   const int split = blockIdx.x;
   const int hk = blockIdx.y % a.Hkv, rt = blockIdx.y / a.Hkv;
   const int b = blockIdx.z;
-  const P4Split sp = p4_split(a, b);
   const int rows_all = a.G * a.S;
   const int row0 = rt * kP4Rows, nrows = min(kP4Rows, rows_all - row0);
-  if (split >= max(1, sp.n)) return;
-  const int t_lo = split * sp.per, t_n = min(sp.per, sp.tiles - t_lo);   // (0 tiles: n = 0)
 
-  for (int i = tid; i < t_n; i += 64 * kP4Waves) {
-    const int t = t_lo + i;
-    const int page = a.tpp_log2 >= 0 ? t >> a.tpp_log2 : t / a.tpp;
-    const int s = a.table[(int64_t)b * a.table_stride + page];
-    slots[i] = s >= 0 && s < a.n_slots ? s : -1;
-  }
+  // Lane i holds the slot of tile i % 2 of the wave's block win0 + i / 2, a window of
+  // blocks read before the first and then ahead of the next (scalar loads a block
+  // ahead came too late: 64 k tokens x 4 at 256 workgroups 56 -> 64 us); a tile's place
+  // in its page is stepped without a division.
+  const char* head_base = a.pool + hk * a.head_bytes;
+  const int blk0 = split * kP4Waves + wave, hop = a.splits * kP4Waves;
+  auto slots_from = [&](int j0) -> int {
+    const int64_t t = 2 * (blk0 + (int64_t)hop * (j0 + (lane >> 1))) + (lane & 1);
+    const int64_t page = a.tpp_log2 >= 0 ? t >> a.tpp_log2 : t / a.tpp;
+    return page < a.max_pages ? a.table[(int64_t)b * a.table_stride + page] : -1;
+  };
+  constexpr int kWin = 30;                 // blocks of a later window: whole rounds
+  int slots = slots_from(0), win0 = 0;
+  int refill = NB - 1 + (32 - (NB - 1)) / NB * NB;
+  int slots_next = slots_from(refill);
+  const int hop_in = a.tpp_log2 >= 0 ? (2 * hop) & (a.tpp - 1) : 2 * hop % a.tpp;
+  int in_page = a.tpp_log2 >= 0 ? (2 * blk0) & (a.tpp - 1) : 2 * blk0 % a.tpp;
+  const P4Seq sq = p4_seq(a, b);
+  if (split >= max(1, sq.splits)) return;
+  const int mine = blk0 < sq.blocks ? (sq.blocks - 1 - blk0) / hop + 1 : 0;
 
   // query row n of the tile: position and head of its group
   const bool row_ok = n < nrows;
@@ -205,11 +249,13 @@ __global__ __launch_bounds__(64 * kP4Waves) void pool4_attn_kernel(P4Attn a) {
       }
     }
   }
-  MaskRow mrow{nullptr, HELM_F32};
-  if constexpr (kMask) {
-    const int64_t e = b * a.mask_b + head * a.mask_h + rc.s * a.mask_q;
-    mrow = MaskRow{a.mask, a.mask_dt} + e;
-  }
+  // row n of the mask; a block's elements are loaded with its K and V (a load behind
+  // the next blocks' would have to wait for those too), four at a time at the mask's
+  // own alignment, pulled back into the row where they would pass its end
+  const char* mrow = nullptr;
+  const bool mwide = a.mask_len >= 4;
+  if constexpr (kMask)
+    mrow = a.mask + MB * (b * a.mask_b + head * a.mask_h + rc.s * a.mask_q);
   // with a mask the logits stay in natural units (finfo.min would leave fp32's
   // range in base 2), the weight's exponent is scaled instead
   const float unit = kMask ? 1.f : kP4Log2E, to2 = kMask ? kP4Log2E : 1.f;
@@ -217,48 +263,71 @@ __global__ __launch_bounds__(64 * kP4Waves) void pool4_attn_kernel(P4Attn a) {
   const float qscale = a.scale * unit;
   const float inv_cap = kCap ? 1.f / a.softcap : 0.f, cap = a.softcap * unit;
   // row n's last visible token
-  const int last_vis = a.causal ? min(sp.len - 1, sp.len - a.S + rc.s) : sp.len - 1;
+  const int last_vis = a.causal ? min(sq.len - 1, sq.len - a.S + rc.s) : sq.len - 1;
   // the block's tokens all lie at or before every row's last visible one
-  const int all_vis = a.causal ? sp.len - a.S + row0 / a.G : sp.len - 1;
+  const int all_vis = a.causal ? sq.len - a.S + row0 / a.G : sq.len - 1;
 
   float m = -INFINITY, l = 0.f;
   mf_f32x4 o[NE];
 #pragma unroll
   for (int e = 0; e < NE; ++e) o[e] = mf_f32x4{0.f, 0.f, 0.f, 0.f};
 
-  __syncthreads();
-  const char* head_base = a.pool + hk * a.head_bytes;
-  auto load = [&](int blk, P4Raw<D> (&r)[2]) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const int i = 2 * blk + s;
-      const int slot = __builtin_amdgcn_readfirstlane(i < t_n ? slots[i] : -1);
-      const int t = t_lo + i;
-      const int in_page = a.tpp_log2 >= 0 ? t & (a.tpp - 1) : t % a.tpp;
-      r[s] = p4_load<D>(head_base + max(slot, 0) * a.slot_bytes +
-                            (int64_t)in_page * P4<D>::kBytes,
-                        slot >= 0, n, h);
-    }
+  struct Block {
+    P4Raw<D> r[2];
+    uint32_t mk[kMask ? 2 * MB : 1];       // eight mask elements
+    int gone;                              // bit s: tile s is not there
   };
-  auto step = [&](int blk, P4Raw<D> (&r)[2]) {
-    const int tok0 = (t_lo + 2 * blk) * kP4Tok;
-    // a slot that the pool does not have hides its tile
-    const bool gone0 = __builtin_amdgcn_readfirstlane(slots[2 * blk]) < 0;
-    const bool gone1 =
-        2 * blk + 1 >= t_n || __builtin_amdgcn_readfirstlane(slots[2 * blk + 1]) < 0;
-    float x[8];
+  // the wave's block j (past its last: zeros, nothing read)
+  auto load = [&](int j, Block& k) {
+    if constexpr (kMask) {
+      const int64_t tok = 32 * (blk0 + (int64_t)hop * j) + 4 * h;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const char* src = mwide ? mrow + MB * min(tok + 16 * s, (int64_t)a.mask_len - 4)
+                                : reinterpret_cast<const char*>(a.q);
+        if constexpr (MB == 2) {
+          const mf_u32x2 w = load8_any(src);
+          k.mk[2 * s] = w[0];
+          k.mk[2 * s + 1] = w[1];
+        } else {
+          const mf_u32x4 w = load16_any(src);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) k.mk[4 * s + i] = w[i];
+        }
+      }
+    }
+    k.gone = 0;
+    const int in[2] = {in_page, in_page + 1 == a.tpp ? 0 : in_page + 1};
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      mf_f32x4 sc{0.f, 0.f, 0.f, 0.f};
+      const int slot = __builtin_amdgcn_readlane(slots, 2 * (j - win0) + s);
+      // (a slot that the pool does not have hides its tile)
+      const bool there = (j < mine) & (2 * (blk0 + hop * j) + s < sq.tiles) &
+                         ((uint32_t)slot < (uint32_t)a.n_slots);
+      const char* tile = head_base + (there ? slot : 0) * a.slot_bytes + in[s] * P4<D>::kBytes;
+      k.r[s] = p4_load<D>(tile, there, n, h);
+      if (!there) k.gone |= 1 << s;
+    }
+    in_page += hop_in;
+    if (in_page >= a.tpp) in_page -= a.tpp;
+  };
+  auto step = [&](int j, Block& k) {
+    P4Raw<D> (&r)[2] = k.r;
+    const int tok0 = 32 * (blk0 + hop * j);
+    float x[8];
+    {
+      mf_f32x4 sc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-      for (int i = 0; i < NS; ++i) {
-        const uint32_t e = D == 256 && i >= NS / 2 ? r[s].ke >> 8 : r[s].ke & 255u;
-        const mf_u32x4 kop = p4_decode8(r[s].k[i], p4_scale(e));
+      for (int i = 0; i < NS; ++i)
 #pragma unroll
-        for (int p = 0; p < QP; ++p) sc = Ops::mma(kop, qop[p][i], sc);
-      }
+        for (int s = 0; s < 2; ++s) {      // (the two tiles' sums side by side)
+          const uint32_t e = D == 256 && i >= NS / 2 ? r[s].ke >> 8 : r[s].ke & 255u;
+          const mf_u32x4 kop = p4_decode8(r[s].k[i], p4_scale(e));
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[4 * s + j] = sc[j];
+          for (int p = 0; p < QP; ++p) sc[s] = Ops::mma(kop, qop[p][i], sc[s]);
+        }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = sc[j >> 2][j & 3];
     }
     if constexpr (kCap) {
       softcap_scores<8>(x, a.scale * inv_cap, cap);
@@ -270,19 +339,31 @@ __global__ __launch_bounds__(64 * kP4Waves) void pool4_attn_kernel(P4Attn a) {
     if constexpr (kMask) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float mk = mrow[min(tok(j), a.mask_len - 1)];
-        x[j] = mk == -INFINITY || tok(j) >= a.mask_len ? -INFINITY : x[j] + mk;
+        float mk;
+        if constexpr (MB == 2) {
+          const uint32_t w = k.mk[j >> 1] >> (16 * (j & 1)) & 0xffffu;
+          mk = a.mask_dt == HELM_BF16
+                   ? __uint_as_float(w << 16)
+                   : static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w)));
+        } else {
+          mk = __uint_as_float(k.mk[j]);
+        }
+        if (tok0 + 31 >= a.mask_len) {       // (uniform: the mask's last block)
+          mk = -INFINITY;
+          if (tok(j) < a.mask_len) mk = (MaskRow{mrow, a.mask_dt})[tok(j)];
+        }
+        x[j] = mk == -INFINITY ? -INFINITY : x[j] + mk;
       }
     }
-    const bool limits = gone0 || gone1 || tok0 + 31 > all_vis;      // uniform
+    const bool limits = k.gone || tok0 + 31 > all_vis;      // uniform
     if (limits) {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (tok(j) > last_vis || (j < 4 ? gone0 : gone1)) x[j] = -INFINITY;
+        if (tok(j) > last_vis || (k.gone >> (j >> 2) & 1)) x[j] = -INFINITY;
       // exponents of tokens past the sequence are whatever the page held
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (tok(j) >= sp.len) r[j >> 2].ve &= ~(255u << (8 * (j & 3)));
+        if (tok(j) >= sq.len) r[j >> 2].ve &= ~(255u << (8 * (j & 3)));
     }
     float top = x[0];
 #pragma unroll
@@ -335,8 +416,8 @@ __global__ __launch_bounds__(64 * kP4Waves) void pool4_attn_kernel(P4Attn a) {
       const mf_u32x4 odd{pack_hi(d[0], d[1]), pack_hi(d[2], d[3]), pack_hi(d[4], d[5]),
                          pack_hi(d[6], d[7])};
       o[2 * c] = Ops::mma(even, hi, o[2 * c]);
-      o[2 * c] = Ops::mma(even, lo, o[2 * c]);
       o[2 * c + 1] = Ops::mma(odd, hi, o[2 * c + 1]);
+      o[2 * c] = Ops::mma(even, lo, o[2 * c]);
       o[2 * c + 1] = Ops::mma(odd, lo, o[2 * c + 1]);
     }
     if (__builtin_expect(nan, 0)) {
@@ -355,110 +436,172 @@ __global__ __launch_bounds__(64 * kP4Waves) void pool4_attn_kernel(P4Attn a) {
           for (int e = 0; e < NE; ++e) o[e][r4] = __builtin_nanf("");
     }
   };
-  const int nblk = (t_n + 1) / 2;
-  for (int blk = wave; blk < nblk; blk += kP4Waves) {
-    P4Raw<D> r[2];
-    load(blk, r);
-    step(blk, r);
+  // block j is computed while the next NB - 1 are on their way; loads past the
+  // last block read nothing, so that every round issues the same
+  Block buf[NB];
+#pragma unroll
+  for (int i = 0; i < NB - 1; ++i) load(i, buf[i]);
+  for (int j = 0; j < mine; j += NB) {
+    if (j + NB - 1 == refill) {
+      slots = slots_next;
+      win0 = refill;
+      refill += kWin;
+      slots_next = slots_from(refill);
+    }
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      load(j + i + NB - 1, buf[(i + NB - 1) % NB]);
+      __builtin_amdgcn_sched_barrier(0);
+      if (j + i < mine) step(j + i, buf[i]);
+    }
   }
 
-  // the split's rows: the waves' states joined in LDS
+  // the split's rows: the waves' states joined in LDS, four dims a thread
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
-  if (h == 0) {
-    sh_m[wave][n] = m;
-    sh_l[wave][n] = l;
-  }
+  if (h == 0) sh_ml[wave][n] = make_float2(m, l);
 #pragma unroll
   for (int r4 = 0; r4 < 4; ++r4)
 #pragma unroll
     for (int e = 0; e < NE; ++e) sh_o[wave][n][(4 * h + r4) * NE + e] = o[e][r4];
   __syncthreads();
-  for (int i = tid; i < nrows * D; i += 64 * kP4Waves) {
-    const int row = i / D, d = i % D;
-    float mx = sh_m[0][row];
+  constexpr int C = D / 4, R = 64 * kP4Waves / C;     // columns of a row; rows at a time
+  const int col = tid % C;
+  const int tile = (b * a.Hkv + hk) * a.row_tiles + rt;
+  const bool alone = sq.splits <= 1;
+  for (int row = tid / C; row < nrows; row += R) {
+    float mx = -INFINITY, sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 1; w < kP4Waves; ++w) mx = fmaxf(mx, sh_m[w][row]);
+    for (int w = 0; w < kP4Waves; ++w) mx = fmaxf(mx, sh_ml[w][row].x);
     const float base = mx == -INFINITY ? 0.f : mx;
-    float sum = 0.f, acc = 0.f;
 #pragma unroll
     for (int w = 0; w < kP4Waves; ++w) {
-      const float f = __builtin_amdgcn_exp2f((sh_m[w][row] - base) * to2);
-      sum += f * sh_l[w][row];
-      acc += f * sh_o[w][row][d];
+      const float2 ml = sh_ml[w][row];
+      const float f = __builtin_amdgcn_exp2f((ml.x - base) * to2);
+      sum += f * ml.y;
+      add_scaled(acc, f, *reinterpret_cast<const float4*>(&sh_o[w][row][4 * col]));
     }
-    const RowCoord c = row_coord(row0 + row, a.G);
-    const int64_t r = (int64_t)(b * a.Hq + hk * a.G + c.g) * a.S + c.s;
-    if (sp.n <= 1) {
-      char* dst = reinterpret_cast<char*>(a.out) + 2 * (r * D + d);
-      const float v = sum == 0.f ? 0.f : acc / sum;
-      if (a.q16) store_elem<f16_t>(dst, v);
-      else store_elem<bf16_t>(dst, v);
+    if (alone) {
+      store_row<D>(a, b, hk, row0 + row, col, acc, sum);
     } else {
-      const int64_t p = r * a.splits + split;
-      a.part_o[p * D + d] = acc;
-      if (d == 0) {
-        a.part_ml[2 * p] = mx;
-        a.part_ml[2 * p + 1] = sum;
-      }
+      const int64_t p = ((int64_t)tile * a.splits + split) * kP4Rows + row;
+      reinterpret_cast<float4*>(a.part_o)[p * C + col] = acc;
+      if (col == 0) reinterpret_cast<float2*>(a.part_ml)[p] = make_float2(mx, sum);
     }
   }
 }
 
-// Row blockIdx.x of the output from its splits' partials; a thread a dim.
+// Row blockIdx.y of tile blockIdx.x from its splits' partials: a thread holds four dims
+// and every (256 / (D / 4))th split, eight of them in flight; the threads of one column
+// meet in LDS.  (3.4 us at 32 splits.  Joined by the last split of a tile to arrive, one
+// launch less but coherent accesses and a ticket: 32 k tokens 16.2 us against 15.9 for
+// both kernels, 64 k x 4 54.7 against 55.)
 template <int D>
-__global__ __launch_bounds__(D) void pool4_join_kernel(P4Attn a) {
-  const int64_t r = blockIdx.x;
-  const int b = (int)(r / ((int64_t)a.Hq * a.S));
-  const P4Split sp = p4_split(a, b);
-  if (sp.n <= 1) return;                     // written by its only split
-  const float* ml = a.part_ml + 2 * r * a.splits;
-  const float* po = a.part_o + r * a.splits * D + threadIdx.x;
-  const float to2 = a.mask ? kP4Log2E : 1.f;   // (the units of the partials' maxima)
-  float mx = -INFINITY;
-  for (int s = 0; s < sp.n; ++s) mx = fmaxf(mx, ml[2 * s]);
-  const float base = mx == -INFINITY ? 0.f : mx;
-  float sum = 0.f, acc = 0.f;
-  for (int s = 0; s < sp.n; ++s) {
-    const float f = __builtin_amdgcn_exp2f((ml[2 * s] - base) * to2);
-    sum += f * ml[2 * s + 1];
-    acc += f * po[(int64_t)s * D];
+__global__ __launch_bounds__(256) void pool4_join_kernel(P4Attn a) {
+  constexpr int C = D / 4, R = 256 / C, U = 8;
+  __shared__ float4 sh_o[R][C];
+  __shared__ float2 sh_ml[R];
+  const int tile = blockIdx.x, row = blockIdx.y;
+  const int rt = tile % a.row_tiles, hk = tile / a.row_tiles % a.Hkv;
+  const int b = tile / a.row_tiles / a.Hkv;
+  if (rt * kP4Rows + row >= a.G * a.S) return;
+  const int n = p4_seq(a, b).splits;
+  if (n <= 1) return;                              // written by its only split
+  const float to2 = a.mask ? kP4Log2E : 1.f;       // (the units of the partials' maxima)
+  const int c = threadIdx.x % C, g = threadIdx.x / C;
+  const int64_t p0 = (int64_t)tile * a.splits * kP4Rows + row;
+  const float2* part_ml = reinterpret_cast<const float2*>(a.part_ml) + p0;
+  const float4* part_o = reinterpret_cast<const float4*>(a.part_o) + p0 * C + c;
+  float m = -INFINITY, l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s0 = g; s0 < n; s0 += U * R) {
+    float2 ml[U];
+    float4 v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t i = (int64_t)min(s0 + u * R, n - 1) * kP4Rows;
+      ml[u] = part_ml[i];
+      v[u] = part_o[i * C];
+    }
+    float mn = m;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (s0 + u * R < n) mn = fmaxf(mn, ml[u].x);
+    const float base = mn == -INFINITY ? 0.f : mn;
+    const float f = __builtin_amdgcn_exp2f((m - base) * to2);
+    l *= f;
+    acc.x *= f;
+    acc.y *= f;
+    acc.z *= f;
+    acc.w *= f;
+    m = mn;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (s0 + u * R < n) {
+        const float w = __builtin_amdgcn_exp2f((ml[u].x - base) * to2);
+        l += w * ml[u].y;
+        add_scaled(acc, w, v[u]);
+      }
   }
-  char* dst = reinterpret_cast<char*>(a.out) + 2 * (r * D + threadIdx.x);
-  const float v = sum == 0.f ? 0.f : acc / sum;
-  if (a.q16) store_elem<f16_t>(dst, v);
-  else store_elem<bf16_t>(dst, v);
+  sh_o[g][c] = acc;
+  if (c == 0) sh_ml[g] = make_float2(m, l);
+  __syncthreads();
+  if (g > 0) return;
+  float mx = -INFINITY, sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < R; ++i) mx = fmaxf(mx, sh_ml[i].x);
+  const float base = mx == -INFINITY ? 0.f : mx;
+  acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const float2 p = sh_ml[i];
+    const float f = __builtin_amdgcn_exp2f((p.x - base) * to2);
+    sum += f * p.y;
+    add_scaled(acc, f, sh_o[i][c]);
+  }
+  store_row<D>(a, b, hk, rt * kP4Rows + row, c, acc, sum);
+}
+
+template <int D, int QP, int MB>
+void launch_mask(const P4Attn& a, dim3 grid, dim3 block, bool cap, hipStream_t st) {
+  if (cap) hipLaunchKernelGGL((pool4_attn_kernel<D, QP, MB, true>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((pool4_attn_kernel<D, QP, MB, false>), grid, block, 0, st, a);
 }
 
 template <int D, int QP>
 void launch_attn(const P4Attn& a, hipStream_t st) {
   const dim3 grid(a.splits, a.Hkv * a.row_tiles, a.B), block(64 * kP4Waves);
   const bool cap = a.softcap > 0.f;
-  if (a.mask && cap) hipLaunchKernelGGL((pool4_attn_kernel<D, QP, true, true>), grid, block, 0, st, a);
-  else if (a.mask) hipLaunchKernelGGL((pool4_attn_kernel<D, QP, true, false>), grid, block, 0, st, a);
-  else if (cap) hipLaunchKernelGGL((pool4_attn_kernel<D, QP, false, true>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((pool4_attn_kernel<D, QP, false, false>), grid, block, 0, st, a);
+  const int mb = !a.mask ? 0 : a.mask_dt == HELM_F32 ? 4 : 2;
+  if (mb == 0) launch_mask<D, QP, 0>(a, grid, block, cap, st);
+  else if (mb == 2) launch_mask<D, QP, 2>(a, grid, block, cap, st);
+  else launch_mask<D, QP, 4>(a, grid, block, cap, st);
   if (a.splits > 1)
-    hipLaunchKernelGGL((pool4_join_kernel<D>), dim3((uint32_t)(a.B * a.Hq * a.S)), dim3(D), 0, st, a);
+    hipLaunchKernelGGL((pool4_join_kernel<D>),
+                       dim3((uint32_t)(a.B * a.Hkv * a.row_tiles), std::min(kP4Rows, a.G * a.S)),
+                       dim3(256), 0, st, a);
 }
 
 struct P4Plan {
-  int splits, min_tiles, row_tiles;
-  size_t bytes;
+  int splits, row_tiles;
+  size_t parts, bytes;
 };
-// Splits: enough workgroups for every CU several times over, none with less than
-// one block a wave; at most kP4MaxTiles tiles each.
+// Splits (grid.x) from the widest table: two workgroups a CU over the whole launch
+// (64 k x 4: 53.2 us, one a CU 55.8; 32 k: 14.6, 14.1), at least one per 128 blocks, so
+// that a long sequence of a ragged batch does not trail behind, and no more workgroups
+// than that gains from (their partials are 16 rows each).  A split has a block a wave.
 P4Plan p4_plan(int B, int Hq, int Hkv, int S, int D, int max_pages, int page_size) {
   P4Plan p{};
-  const int64_t tiles = (int64_t)max_pages * (page_size / kP4Tok);
+  const int64_t blocks = ((int64_t)max_pages * (page_size / kP4Tok) + 1) / 2;
   p.row_tiles = ((int64_t)(Hq / Hkv) * S + kP4Rows - 1) / kP4Rows;
-  p.min_tiles = 2 * kP4Waves;
   const int64_t wgs = (int64_t)B * Hkv * p.row_tiles;
-  int64_t n = std::max<int64_t>(1, (1024 + wgs - 1) / wgs);
-  n = std::min<int64_t>(n, (tiles + p.min_tiles - 1) / p.min_tiles);
-  n = std::max<int64_t>(n, (tiles + kP4MaxTiles - 1) / kP4MaxTiles);
+  int64_t n = std::max<int64_t>(512 / wgs, (blocks + 127) / 128);
+  n = std::min<int64_t>(n, 16384 / wgs);
+  n = std::min<int64_t>(n, (blocks + kP4Waves - 1) / kP4Waves);
   p.splits = (int)std::max<int64_t>(1, n);
-  p.bytes = p.splits > 1 ? (size_t)B * Hq * S * p.splits * (D + 2) * sizeof(float) : 0;
+  p.parts = p.splits > 1 ? (size_t)wgs * p.splits * kP4Rows : 0;
+  p.bytes = p.parts * (D + 2) * sizeof(float);
   return p;
 }
 
@@ -501,8 +644,9 @@ extern "C" int helm_pool4_decode_attn(const void* q, void* out, const void* pool
   if (B == 0) return HELM_OK;
   if (!q || !out || (!pool && n_slots) || (!page_table && max_pages) || !seq_lens)
     return report_error(HELM_E_INVALID, "null pointer argument");
-  if ((reinterpret_cast<uint64_t>(q) | reinterpret_cast<uint64_t>(pool)) & 15)
-    return report_error(HELM_E_INVALID, "q and the pool must be 16-byte aligned");
+  if ((reinterpret_cast<uint64_t>(q) | reinterpret_cast<uint64_t>(pool) |
+       reinterpret_cast<uint64_t>(out) | reinterpret_cast<uint64_t>(workspace)) & 15)
+    return report_error(HELM_E_INVALID, "q, out, the pool and the workspace must be 16-byte aligned");
   const P4Plan pl = p4_plan(B, Hq, Hkv, q_len, D, max_pages, page_size);
   if (pl.bytes && (!workspace || ws_bytes < pl.bytes))
     return report_error(HELM_E_WORKSPACE, "workspace too small: need " + std::to_string(pl.bytes));
@@ -527,7 +671,6 @@ extern "C" int helm_pool4_decode_attn(const void* q, void* out, const void* pool
   a.row_tiles = pl.row_tiles;
   a.q16 = q_dtype == HELM_F16;
   a.splits = pl.splits;
-  a.min_tiles = pl.min_tiles;
   a.causal = causal;
   a.scale = scale;
   a.softcap = softcap;
@@ -538,7 +681,7 @@ extern "C" int helm_pool4_decode_attn(const void* q, void* out, const void* pool
   a.mask_dt = mask_dtype;
   a.mask_len = mask_len;
   a.part_o = static_cast<float*>(workspace);
-  a.part_ml = a.part_o + (pl.splits > 1 ? (int64_t)B * Hq * q_len * pl.splits * D : 0);
+  a.part_ml = a.part_o + pl.parts * D;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (q_dtype == HELM_BF16) {
     if (D == 64) launch_attn<64, 1>(a, st);

@@ -125,7 +125,7 @@ def prepare_pool4_decode(q: torch.Tensor, pool: Pool4, page_table: torch.Tensor,
         raise ValueError("a prepared call reads the mask in place: float32, bfloat16 or "
                          "float16 with dense rows")
     args, out, keep = _decode_args(q, pool, page_table, seq_lens, max_pages, scale, softcap,
-                                   attention_mask, causal, out)
+                                   attention_mask, causal, out, in_place=True)
     return PreparedPool4Decode(q.device, args, out, keep)
 
 
@@ -160,7 +160,8 @@ def check_scores(scale: Optional[float], softcap: Optional[float], D: int) -> Tu
     return scale, cap
 
 
-def _decode_args(q, pool, page_table, seq_lens, max_pages, scale, softcap, mask, causal, out):
+def _decode_args(q, pool, page_table, seq_lens, max_pages, scale, softcap, mask, causal, out,
+                 in_place=False):
     """Checks the operands; (C-ABI arguments up to the stream, out, tensors to keep)."""
     if q.dim() != 4:
         raise ValueError("q must be [B, Hq, q_len, D]")
@@ -200,15 +201,18 @@ def _decode_args(q, pool, page_table, seq_lens, max_pages, scale, softcap, mask,
                            out)
     q = q.contiguous()
     if q.data_ptr() % 16:
+        if in_place:
+            raise ValueError("a prepared call reads q in place: it must be 16-byte aligned")
         q = q.clone()
     lib = _native.load()
     need = lib.helm_pool4_workspace_bytes(B, Hq, pool.num_kv_heads, S, D, max_pages,
                                           pool.page_size)
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    # (a call of its own takes a workspace of its own: calls on other streams, captured ones)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device)
     args = (q.data_ptr(), out.data_ptr(), pool.data.data_ptr(), pool.n_slots, pool.page_size,
             page_table.data_ptr(), max(page_table.stride(0), max_pages), max_pages,
             seq_lens.data_ptr(), B, Hq, pool.num_kv_heads, S, D, scale, cap,
             m.data_ptr() if m is not None else None, *ms, width,
             _native.dtype_code(m.dtype) if m is not None else _native.HELM_F32, int(bool(causal)),
-            _native.dtype_code(q.dtype), ws.data_ptr() if ws is not None else None, need)
+            _native.dtype_code(q.dtype), ws.data_ptr(), need)
     return args, out, (q, pool, page_table, seq_lens, m, ws)

@@ -421,10 +421,10 @@ int helm_pool4_read(const void* pool, int64_t n_slots, int page_size, int Hkv, i
  * 0 .. len - q_len + s.  mask_len: columns of the mask; tokens from there on are
  * hidden.  Hidden tokens (those, past the limit, or under -inf) take no part
  * whatever they hold; a row that sees nothing is zeros.  Pages whose slot is
- * outside [0, n_slots), and tokens past max_pages, count as hidden.  The
- * workspace (helm_pool4_workspace_bytes; 0: none needed, 16-byte aligned)
- * needs no contents before or after a call; calls that may overlap need one
- * each. */
+ * outside [0, n_slots), and tokens past max_pages, count as hidden.  q, out,
+ * the pool and the workspace are 16-byte aligned.  The workspace
+ * (helm_pool4_workspace_bytes; 0: none needed) needs no contents before or
+ * after a call; calls that may overlap need one each. */
 size_t helm_pool4_workspace_bytes(int B, int Hq, int Hkv, int q_len, int D, int max_pages,
                                   int page_size);
 int helm_pool4_decode_attn(const void* q, void* out, const void* pool, int64_t n_slots,
