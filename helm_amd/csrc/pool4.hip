@@ -2,11 +2,14 @@
 // back out (helm_pool4_write, helm_pool4_read).  Layout and rounding: pool4.h.
 //
 // Both are bound by memory: a bf16 row of D dims is 2 D bytes on one side and
-// 17 D / 32 on the other.  A lane owns eight dims of one row (one 16-byte load of
-// 16-bit values), four lanes a group, whose largest magnitude they share by two
-// quad moves; the matrix-core conversions of gfx950 encode and decode two
-// values an instruction (exact, ties to even, as checked over every code and
-// exponent).
+// 17 D / 32 on the other.  A thread owns eight dims of K or V of one head (16 bytes of a
+// 16-bit row; four lanes are a group, whose largest magnitude they share by two quad
+// moves) and takes them of four consecutive rows, whose loads are all in flight at
+// once: where its place in a row is worked out once for the four.  (A thread a row and
+// place spent half its time on divisions: 16,384 rows of 8 heads of 128, bf16, write
+// 31 us and read 28.5, now WRITE_US and READ_US.)  The conversions of gfx950 encode and
+// decode two values an instruction, exactly and with ties to the even code (checked
+// over every code and exponent).
 #include "pool4.h"
 
 #include <algorithm>
@@ -23,42 +26,44 @@ namespace {
 
 constexpr int kThreads4 = 256;
 
+constexpr int kRowsPer = 4;         // consecutive rows of a thread
+
 struct P4Rows {
   char* pool;
   int64_t slot_bytes;        // of one slot (page), all heads
   int64_t head_bytes;        // of one head of a page
   int64_t n_rows;            // slots * page tokens
-  int page;
+  int page, page_log2;       // its log2 or -1
   const int64_t* slots;
   int n_tok;
-  int Hkv;
+  int items;                 // places of a row: K's, then V's, D / 8 a head each
+  int abreast;               // rows that a workgroup's threads hold side by side
   char* k;
   char* v;
   int64_t k_tok, k_head, v_tok, v_head;   // elements
 };
 
-// Row `slot` of the pool, head h: its tile and its token in it.
+// Row `slot` of the pool (inside it): its tile of head 0, and its token in the tile.
 struct P4Place {
   char* tile;
   int t;
 };
 template <int D>
-__device__ __forceinline__ P4Place p4_place(const P4Rows& a, int64_t slot, int h) {
+__device__ __forceinline__ P4Place p4_place(const P4Rows& a, int64_t slot) {
   int64_t s;
   int r;
-  if (a.n_rows <= 0x7fffffff) {     // (uniform; a 64-bit division is ~100 instructions)
-    s = (uint32_t)slot / (uint32_t)a.page;
-    r = (int)((uint32_t)slot % (uint32_t)a.page);
+  if (a.page_log2 >= 0) {
+    s = slot >> a.page_log2;
+    r = (int)slot & (a.page - 1);
   } else {
     s = slot / a.page;
-    r = (int)(slot % a.page);
+    r = (int)(slot - s * a.page);
   }
-  return {a.pool + s * a.slot_bytes + h * a.head_bytes + (r / kP4Tok) * P4<D>::kBytes,
-          r % kP4Tok};
+  return {a.pool + s * a.slot_bytes + (r / kP4Tok) * P4<D>::kBytes, r % kP4Tok};
 }
 
-// Byte of the codes of dims 8c .. 8c + 7 of token t (V: D = 64 two chunks of two
-// bytes, 32 apart; see p4_v_store)
+// Byte of the codes of dims 8c .. 8c + 7 of token t (V at D = 64: the first of its two
+// chunks; see p4_v_store)
 template <int D> __device__ __forceinline__ int p4_k_byte(int t, int c) {
   return t * (D / 2) + 4 * c;
 }
@@ -103,98 +108,128 @@ template <typename T> __device__ __forceinline__ void store8(char* p, int64_t el
   }
 }
 
-// Item i of the launch: eight dims (chunk c) of K or V of head h of row n.
+// A thread's place in a row (eight dims, chunk c of head h of K or V) and its rows
+// n .. n + kRowsPer - 1; place < 0: none.  All four lanes of a group share all but c.
 template <int D> struct P4Item {
-  int n, h, c;
-  bool is_v;
-  __device__ __forceinline__ P4Item(int64_t i, int Hkv) {
-    c = (int)(i % (D / 8));
-    const int64_t j = i / (D / 8);
-    is_v = j & 1;
-    const uint32_t r = (uint32_t)(j >> 1);       // n * Hkv + h < 2^31 (checked on the host)
-    h = (int)(r % (uint32_t)Hkv);
-    n = (int)(r / (uint32_t)Hkv);
+  int64_t n;
+  int h, c;
+  bool some, is_v;
+  __device__ __forceinline__ explicit P4Item(const P4Rows& a) {
+    const int tid = threadIdx.x;
+    const int sub = a.abreast > 1 ? tid / a.items : 0;
+    int i = a.abreast > 1 ? tid - sub * a.items : (int)blockIdx.y * kThreads4 + tid;
+    some = sub < a.abreast && i < a.items;
+    n = ((int64_t)blockIdx.x * a.abreast + sub) * kRowsPer;
+    is_v = i >= a.items / 2;
+    if (is_v) i -= a.items / 2;
+    h = i / (D / 8);
+    c = i % (D / 8);
   }
 };
 
+// Eight dims of V codes go to one word, or two chunks' half words (D = 64).
+template <int D> __device__ __forceinline__ void p4_v_store(char* tile, int t, int c, uint32_t w) {
+  char* dst = tile + p4_v_byte<D>(t, c);
+  if constexpr (D == 64) {
+    *reinterpret_cast<uint16_t*>(dst) = (uint16_t)w;
+    *reinterpret_cast<uint16_t*>(dst + 2 * kP4Tok) = (uint16_t)(w >> 16);
+  } else {
+    *reinterpret_cast<uint32_t*>(dst) = w;
+  }
+}
+
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads4) void pool4_write_kernel(P4Rows a) {
-  const int64_t i = (int64_t)blockIdx.x * kThreads4 + threadIdx.x;
-  if (i >= (int64_t)a.n_tok * a.Hkv * (D / 4)) return;      // (whole groups of four lanes)
-  const P4Item<D> it(i, a.Hkv);
-  const int64_t slot = a.slots[it.n];
-  if (slot < 0 || slot >= a.n_rows) return;                 // (one row: whole groups again)
-  float x[8];
-  if (it.is_v) load8<T>(a.v, it.n * a.v_tok + it.h * a.v_head + 8 * it.c, x);
-  else load8<T>(a.k, it.n * a.k_tok + it.h * a.k_head + 8 * it.c, x);
-  uint32_t top = 0;                        // largest magnitude's bits (NaN above infinity)
+  const P4Item<D> it(a);
+  if (!it.some || it.n >= a.n_tok) return;                // (whole groups of four lanes)
+  const int m = min(kRowsPer, (int)(a.n_tok - it.n));
+  const char* src = it.is_v ? a.v : a.k;
+  const int64_t tok = it.is_v ? a.v_tok : a.k_tok;
+  const int64_t at = (it.is_v ? a.v_head : a.k_head) * it.h + 8 * it.c;
+  int64_t slot[kRowsPer];
+  float x[kRowsPer][8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(x[j]) & 0x7fffffffu);
-  top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0xB1, 0xf, 0xf, true));
-  top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x4E, 0xf, 0xf, true));
-  const uint32_t e = p4_exponent(top);
-  uint32_t w = 0;
-  if (e != 255u) {
-    const float s = p4_scale(e);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[0], x[1], s, 0);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2], x[3], s, 1);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[4], x[5], s, 2);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], s, 3);
+  for (int i = 0; i < kRowsPer; ++i) {
+    const int64_t n = it.n + min(i, m - 1);
+    slot[i] = i < m ? a.slots[n] : -1;
+    load8<T>(src, n * tok + at, x[i]);
   }
-  const P4Place p = p4_place<D>(a, slot, it.h);
-  if (it.is_v) {
-    if constexpr (D == 64) {               // two chunks of four dims
-      char* dst = p.tile + p4_v_byte<D>(p.t, it.c);
-      *reinterpret_cast<uint16_t*>(dst) = (uint16_t)w;
-      *reinterpret_cast<uint16_t*>(dst + 2 * kP4Tok) = (uint16_t)(w >> 16);
-    } else {
-      *reinterpret_cast<uint32_t*>(p.tile + p4_v_byte<D>(p.t, it.c)) = w;
+#pragma unroll
+  for (int i = 0; i < kRowsPer; ++i) {
+    uint32_t top = 0;                      // largest magnitude's bits (NaN above infinity)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(x[i][j]) & 0x7fffffffu);
+    top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0xB1, 0xf, 0xf, true));
+    top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x4E, 0xf, 0xf, true));
+    const uint32_t e = p4_exponent(top);
+    uint32_t w = 0;
+    if (e != 255u) {
+      const float s = p4_scale(e);
+      w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[i][0], x[i][1], s, 0);
+      w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[i][2], x[i][3], s, 1);
+      w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[i][4], x[i][5], s, 2);
+      w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[i][6], x[i][7], s, 3);
     }
-    if ((it.c & 3) == 0) p.tile[P4<D>::kVe + (it.c >> 2) * kP4Tok + p.t] = (char)e;
-  } else {
-    *reinterpret_cast<uint32_t*>(p.tile + p4_k_byte<D>(p.t, it.c)) = w;
-    if ((it.c & 3) == 0) p.tile[P4<D>::kKe + p.t * P4<D>::kGroups + (it.c >> 2)] = (char)e;
+    if (slot[i] < 0 || slot[i] >= a.n_rows) continue;
+    const P4Place p = p4_place<D>(a, slot[i]);
+    char* tile = p.tile + it.h * a.head_bytes;
+    if (it.is_v) {
+      p4_v_store<D>(tile, p.t, it.c, w);
+      if ((it.c & 3) == 0) tile[P4<D>::kVe + (it.c >> 2) * kP4Tok + p.t] = (char)e;
+    } else {
+      *reinterpret_cast<uint32_t*>(tile + p4_k_byte<D>(p.t, it.c)) = w;
+      if ((it.c & 3) == 0) tile[P4<D>::kKe + p.t * P4<D>::kGroups + (it.c >> 2)] = (char)e;
+    }
   }
 }
 
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads4) void pool4_read_kernel(P4Rows a) {
-  const int64_t i = (int64_t)blockIdx.x * kThreads4 + threadIdx.x;
-  if (i >= (int64_t)a.n_tok * a.Hkv * (D / 4)) return;
-  const P4Item<D> it(i, a.Hkv);
-  const int64_t slot = a.slots[it.n];
-  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (slot >= 0 && slot < a.n_rows) {
-    const P4Place p = p4_place<D>(a, slot, it.h);
-    uint32_t w, e;
+  const P4Item<D> it(a);
+  if (!it.some || it.n >= a.n_tok) return;
+  const int m = min(kRowsPer, (int)(a.n_tok - it.n));
+  uint32_t w[kRowsPer], e[kRowsPer];
+#pragma unroll
+  for (int i = 0; i < kRowsPer; ++i) {
+    const int64_t slot = a.slots[it.n + min(i, m - 1)];
+    w[i] = e[i] = 0u;                      // (a row outside the pool: zeros)
+    if (slot < 0 || slot >= a.n_rows) continue;
+    const P4Place p = p4_place<D>(a, slot);
+    const char* tile = p.tile + it.h * a.head_bytes;
     if (it.is_v) {
-      const char* src = p.tile + p4_v_byte<D>(p.t, it.c);
+      const char* src = tile + p4_v_byte<D>(p.t, it.c);
       if constexpr (D == 64)
-        w = *reinterpret_cast<const uint16_t*>(src) |
-            (uint32_t)*reinterpret_cast<const uint16_t*>(src + 2 * kP4Tok) << 16;
+        w[i] = *reinterpret_cast<const uint16_t*>(src) |
+               (uint32_t)*reinterpret_cast<const uint16_t*>(src + 2 * kP4Tok) << 16;
       else
-        w = *reinterpret_cast<const uint32_t*>(src);
-      e = (uint8_t)p.tile[P4<D>::kVe + (it.c >> 2) * kP4Tok + p.t];
+        w[i] = *reinterpret_cast<const uint32_t*>(src);
+      e[i] = (uint8_t)tile[P4<D>::kVe + (it.c >> 2) * kP4Tok + p.t];
     } else {
-      w = *reinterpret_cast<const uint32_t*>(p.tile + p4_k_byte<D>(p.t, it.c));
-      e = (uint8_t)p.tile[P4<D>::kKe + p.t * P4<D>::kGroups + (it.c >> 2)];
+      w[i] = *reinterpret_cast<const uint32_t*>(tile + p4_k_byte<D>(p.t, it.c));
+      e[i] = (uint8_t)tile[P4<D>::kKe + p.t * P4<D>::kGroups + (it.c >> 2)];
     }
-    const float s = p4_scale(e);           // (e = 255: NaN, and so is every product)
-    const auto a0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 0);
-    const auto a1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 1);
-    const auto a2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 2);
-    const auto a3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 3);
-    x[0] = a0[0]; x[1] = a0[1]; x[2] = a1[0]; x[3] = a1[1];
-    x[4] = a2[0]; x[5] = a2[1]; x[6] = a3[0]; x[7] = a3[1];
   }
-  if (it.is_v) store8<T>(a.v, it.n * a.v_tok + it.h * a.v_head + 8 * it.c, x);
-  else store8<T>(a.k, it.n * a.k_tok + it.h * a.k_head + 8 * it.c, x);
+  char* dst = it.is_v ? a.v : a.k;
+  const int64_t tok = it.is_v ? a.v_tok : a.k_tok;
+  const int64_t at = (it.is_v ? a.v_head : a.k_head) * it.h + 8 * it.c;
+#pragma unroll
+  for (int i = 0; i < kRowsPer; ++i) {
+    if (i >= m) break;
+    const float s = p4_scale(e[i]);        // (e = 255: NaN, and so is every product)
+    const auto a0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], s, 0);
+    const auto a1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], s, 1);
+    const auto a2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], s, 2);
+    const auto a3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], s, 3);
+    const float x[8] = {a0[0], a0[1], a1[0], a1[1], a2[0], a2[1], a3[0], a3[1]};
+    store8<T>(dst, (it.n + i) * tok + at, x);
+  }
 }
 
 template <typename T, int D>
 void launch_rows(bool write, const P4Rows& a, hipStream_t st) {
-  const int64_t items = (int64_t)a.n_tok * a.Hkv * (D / 4);
-  const dim3 grid((uint32_t)((items + kThreads4 - 1) / kThreads4));
+  const int64_t rows = (int64_t)a.abreast * kRowsPer;
+  const dim3 grid((uint32_t)((a.n_tok + rows - 1) / rows),
+                  (uint32_t)((a.items + kThreads4 - 1) / kThreads4));
   if (write) hipLaunchKernelGGL((pool4_write_kernel<T, D>), grid, dim3(kThreads4), 0, st, a);
   else hipLaunchKernelGGL((pool4_read_kernel<T, D>), grid, dim3(kThreads4), 0, st, a);
 }
@@ -212,10 +247,9 @@ int rows_call(bool write, const char* name, void* pool, int64_t n_slots, int pag
     return report_error(HELM_E_INVALID, "unknown dtype");
   if (D != 64 && D != 128 && D != 256)
     return report_error(HELM_E_UNSUPPORTED, "a 4-bit pool has head_dim 64, 128 or 256");
-  if (n_slots < 0 || page_size < kP4Tok || page_size % kP4Tok || Hkv < 1 || n_tok < 0 ||
-      (int64_t)n_tok * Hkv > 0x7fffffff)
+  if (n_slots < 0 || page_size < kP4Tok || page_size % kP4Tok || Hkv < 1 || Hkv > 65535 || n_tok < 0)
     return report_error(HELM_E_INVALID,
-                        "bad 4-bit pool shape (page_size a multiple of 16, rows * heads < 2^31)");
+                        "bad 4-bit pool shape (page_size a multiple of 16, 1 to 65535 heads)");
   if (n_tok == 0) return HELM_OK;
   const int eb = dtype == HELM_F32 ? 4 : 2;
   if (!slots || !k || !v || (!pool && n_slots))
@@ -230,9 +264,11 @@ int rows_call(bool write, const char* name, void* pool, int64_t n_slots, int pag
   a.slot_bytes = a.head_bytes * Hkv;
   a.n_rows = n_slots * page_size;
   a.page = page_size;
+  a.page_log2 = (page_size & (page_size - 1)) ? -1 : __builtin_ctz(page_size);
   a.slots = slots;
   a.n_tok = n_tok;
-  a.Hkv = Hkv;
+  a.items = Hkv * (D / 4);
+  a.abreast = std::max(1, kThreads4 / a.items);
   a.k = static_cast<char*>(k);
   a.v = static_cast<char*>(v);
   a.k_tok = k_tok;

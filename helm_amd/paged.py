@@ -187,43 +187,39 @@ def batch_tables(new_lens: torch.Tensor, cached_lens: torch.Tensor, page_table: 
     which the pool's write skips.  A step that needs more pages than free_slots
     holds (pages_taken says how many) or than the table is wide gets slot -1 for
     their tokens, and -1 in the table.  At most 4096 sequences."""
-    for name, t in (("new_lens", new_lens), ("cached_lens", cached_lens),
-                    ("page_table", page_table), ("free_slots", free_slots)):
-        if t.dtype != torch.int32:
-            raise TypeError(f"{name} must be int32")
-    B = new_lens.numel()
-    if new_lens.dim() != 1 or cached_lens.shape != new_lens.shape or free_slots.dim() != 1:
+    i32 = torch.int32
+    if new_lens.dtype != i32 or cached_lens.dtype != i32 or page_table.dtype != i32 or \
+            free_slots.dtype != i32:
+        raise TypeError("new_lens, cached_lens, page_table and free_slots must be int32")
+    lens, rows = new_lens.shape, page_table.shape
+    if len(lens) != 1 or cached_lens.shape != lens or free_slots.dim() != 1:
         raise ValueError("new_lens and cached_lens must be [B], free_slots [n]")
-    if page_table.dim() != 2 or page_table.size(0) != B:
+    B = lens[0]
+    if len(rows) != 2 or rows[0] != B:
         raise ValueError("page_table must be [B, width]")
-    if page_table.stride(1) != 1 and page_table.size(1) > 1:
-        raise ValueError("page_table rows must be dense")
-    if B > 1 and page_table.stride(0) < page_table.size(1):
-        raise ValueError("page_table rows overlap")
-    for name, t in (("new_lens", new_lens), ("cached_lens", cached_lens),
-                    ("free_slots", free_slots)):
-        if not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous")
+    stride, width = page_table.stride(), rows[1]
+    if (stride[1] != 1 and width > 1) or (stride[0] < width and B > 1):
+        raise ValueError("page_table rows must be dense and apart")
+    if not (new_lens.is_contiguous() and cached_lens.is_contiguous()
+            and free_slots.is_contiguous()):
+        raise ValueError("new_lens, cached_lens and free_slots must be contiguous")
     if B < 1 or B > 4096 or page_size < 1 or max_tokens < 0:
         raise ValueError("batch_tables takes 1 to 4096 sequences, page_size >= 1, max_tokens >= 0")
-    dev = new_lens.device
     if out is None:
-        _engine.check_operands("batch_tables", dev, new_lens, cached_lens, page_table, free_slots)
-        ints = torch.empty(2 * B + 2, dtype=torch.int32, device=dev)
-        longs = torch.empty((2, max_tokens), dtype=torch.int64, device=dev)
-        out = BatchTables(ints[:B + 1], longs[0], longs[1], ints[B + 1:2 * B + 1], ints[2 * B + 1:])
+        idx = _engine.common_device("batch_tables", new_lens, cached_lens, page_table, free_slots)
+        cu, seq, taken = new_lens.new_empty(2 * B + 2).split((B + 1, B, 1))
+        pos, slot = new_lens.new_empty((2, max_tokens), dtype=torch.int64).unbind(0)
+        out = BatchTables(cu, pos, slot, seq, taken)
     else:
-        shapes = ((B + 1, torch.int32), (max_tokens, torch.int64), (max_tokens, torch.int64),
-                  (B, torch.int32), (1, torch.int32))
-        for name, t, (n, dt) in zip(BatchTables._fields, out, shapes):
+        cu, pos, slot, seq, taken = out
+        for name, t, n, dt in zip(BatchTables._fields, out, (B + 1, max_tokens, max_tokens, B, 1),
+                                  (i32, torch.int64, torch.int64, i32, i32)):
             if t.shape != (n,) or t.dtype != dt or not t.is_contiguous():
                 raise ValueError(f"out.{name} must be contiguous {dt} [{n}]")
-        _engine.check_operands("batch_tables", dev, new_lens, cached_lens, page_table, free_slots,
-                               *out)
-    _engine.call_on(dev, "helm_batch_tables", new_lens.data_ptr(), cached_lens.data_ptr(), B,
-                    page_table.data_ptr(), max(page_table.stride(0), page_table.size(1)),
-                    page_table.size(1), free_slots.data_ptr(), free_slots.numel(), page_size,
-                    max_tokens, out.cu_seqlens.data_ptr(), out.positions.data_ptr(),
-                    out.slot_map.data_ptr(), out.seq_lens.data_ptr(),
-                    out.pages_taken.data_ptr(), _engine.stream_ptr(dev))
+        idx = _engine.common_device("batch_tables", new_lens, cached_lens, page_table, free_slots,
+                                    *out)
+    _engine.launch_on(idx, "helm_batch_tables", new_lens.data_ptr(), cached_lens.data_ptr(), B,
+                      page_table.data_ptr(), max(stride[0], width), width, free_slots.data_ptr(),
+                      free_slots.numel(), page_size, max_tokens, cu.data_ptr(), pos.data_ptr(),
+                      slot.data_ptr(), seq.data_ptr(), taken.data_ptr())
     return out

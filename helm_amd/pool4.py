@@ -22,7 +22,8 @@ from helm_amd import _native
 from helm_amd.runtime import engine as _engine
 
 _DIMS = (64, 128, 256)
-_MASKS = (torch.float32, torch.bfloat16, torch.float16)
+_CODES = {torch.float16: _native.HELM_F16, torch.bfloat16: _native.HELM_BF16,
+          torch.float32: _native.HELM_F32}
 
 
 class Pool4:
@@ -44,52 +45,56 @@ class Pool4:
         self.data = torch.zeros((n_slots, num_kv_heads, page_size // 16, 17 * head_dim),
                                 dtype=torch.uint8, device=device)
 
-    def _rows(self, what: str, k: torch.Tensor, v: torch.Tensor, slot_map: torch.Tensor) -> None:
-        want = (slot_map.numel(), self.num_kv_heads, self.head_dim)
+        self._idx = self.data.get_device()
+        # the C-ABI's leading arguments of a write or read
+        self._shape = (self.data.data_ptr(), n_slots, page_size, num_kv_heads, head_dim)
+
+    def _slots(self, slot_map: torch.Tensor) -> int:
         if slot_map.dtype != torch.int64:
             raise TypeError("slot_map must be int64")
         if slot_map.dim() != 1 or not slot_map.is_contiguous():
             raise ValueError("slot_map must be a contiguous [n]")
-        if tuple(k.shape) != want or tuple(v.shape) != want:
-            raise ValueError(f"{what}: k and v must be {list(want)}, one row a slot")
-        if k.dtype != v.dtype:
-            raise TypeError("k and v must share a dtype")
+        return slot_map.numel()
 
     def write(self, k: torch.Tensor, v: torch.Tensor, slot_map: torch.Tensor) -> None:
         """Rows n of k and v ([n, Hkv, D] float16, bfloat16 or float32, any strides) into
         row slot_map[n] (int64, slot * page_size + token; outside the pool, -1 for
         instance: skipped).  Rows of one call that share a slot leave either's values,
         group by group: give each its own."""
-        self._rows("Pool4.write", k, v, slot_map)
-        code = _native.dtype_code(k.dtype)
-        _engine.check_operands("Pool4.write", self.data.device, k, v, slot_map)
+        n = self._slots(slot_map)
+        want = (n, self.num_kv_heads, self.head_dim)
+        if k.shape != want or v.shape != want:
+            raise ValueError(f"Pool4.write: k and v must be {list(want)}, one row a slot")
+        code = _CODES.get(k.dtype)
+        if code is None or v.dtype != k.dtype:
+            raise TypeError("k and v must share float16, bfloat16 or float32")
+        _engine.refuse_grad("Pool4.write", k, v)
+        idx = _engine.common_device("Pool4.write", self.data, k, v, slot_map)
         k, v = _aligned_rows(k), _aligned_rows(v)
-        _engine.call_on(self.data.device, "helm_pool4_write", self.data.data_ptr(), self.n_slots,
-                        self.page_size, self.num_kv_heads, self.head_dim, slot_map.data_ptr(),
-                        slot_map.numel(), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
-                        v.stride(0), v.stride(1), code, _engine.stream_ptr(self.data.device))
+        ks, vs = k.stride(), v.stride()
+        _engine.launch_on(idx, "helm_pool4_write", *self._shape, slot_map.data_ptr(), n,
+                          k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], code)
 
     def read(self, slot_map: torch.Tensor, dtype: torch.dtype = torch.bfloat16
              ) -> Tuple[torch.Tensor, torch.Tensor]:
         """The values held in rows slot_map, (k, v) [n, Hkv, D] of `dtype` (exact but for
         its rounding); zeros for rows outside the pool."""
-        code = _native.dtype_code(dtype)
-        kv = torch.empty((2, slot_map.numel(), self.num_kv_heads, self.head_dim), dtype=dtype,
-                         device=self.data.device)
-        k, v = kv[0], kv[1]
-        self._rows("Pool4.read", k, v, slot_map)
-        _engine.check_operands("Pool4.read", self.data.device, slot_map)
-        _engine.call_on(self.data.device, "helm_pool4_read", self.data.data_ptr(), self.n_slots,
-                        self.page_size, self.num_kv_heads, self.head_dim, slot_map.data_ptr(),
-                        slot_map.numel(), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
-                        v.stride(0), v.stride(1), code, _engine.stream_ptr(self.data.device))
+        n = self._slots(slot_map)
+        code = _CODES.get(dtype)
+        if code is None:
+            raise TypeError("values are read as float16, bfloat16 or float32")
+        idx = _engine.common_device("Pool4.read", self.data, slot_map)
+        H, D = self.num_kv_heads, self.head_dim
+        k, v = slot_map.new_empty((2, n, H, D), dtype=dtype).unbind(0)
+        _engine.launch_on(idx, "helm_pool4_read", *self._shape, slot_map.data_ptr(), n,
+                          k.data_ptr(), H * D, D, v.data_ptr(), H * D, D, code)
         return k, v
 
 
 def _aligned_rows(x: torch.Tensor) -> torch.Tensor:
     """x [n, H, D] itself where its rows are dense and 16-byte aligned, else a copy."""
-    unit = 16 // x.element_size()
-    if (x.stride(2) != 1 or x.stride(0) % unit or x.stride(1) % unit or x.data_ptr() % 16):
+    s, unit = x.stride(), 16 // x.element_size()
+    if s[2] != 1 or s[0] % unit or s[1] % unit or x.data_ptr() % 16:
         x = torch.empty(x.shape, dtype=x.dtype, device=x.device).copy_(x)
     return x
 
@@ -101,12 +106,11 @@ class PreparedPool4Decode:
     object (its replays in graphs among them) share its workspace and `out` and must
     not overlap."""
 
-    def __init__(self, device, args, out, keep):
-        self._device, self._args, self.out, self._keep = device, args, out, keep
+    def __init__(self, idx, args, out, keep):
+        self._idx, self._args, self.out, self._keep = idx, args, out, keep
 
     def run(self) -> torch.Tensor:
-        _engine.call_on(self._device, "helm_pool4_decode_attn", *self._args,
-                        _engine.stream_ptr(self._device))
+        _engine.launch_on(self._idx, "helm_pool4_decode_attn", *self._args)
         return self.out
 
 
@@ -121,12 +125,11 @@ def prepare_pool4_decode(q: torch.Tensor, pool: Pool4, page_table: torch.Tensor,
     if not q.is_contiguous():
         raise ValueError("a prepared call reads q in place: it must be contiguous")
     m = attention_mask
-    if m is not None and (m.dtype not in _MASKS or m.stride(-1) != 1):
+    if m is not None and (m.dtype not in _CODES or m.stride(-1) != 1):
         raise ValueError("a prepared call reads the mask in place: float32, bfloat16 or "
                          "float16 with dense rows")
-    args, out, keep = _decode_args(q, pool, page_table, seq_lens, max_pages, scale, softcap,
-                                   attention_mask, causal, out, in_place=True)
-    return PreparedPool4Decode(q.device, args, out, keep)
+    return PreparedPool4Decode(*_decode_args(q, pool, page_table, seq_lens, max_pages, scale, softcap,
+                                             attention_mask, causal, out, in_place=True))
 
 
 def pool4_decode_attention(q: torch.Tensor, pool: Pool4, page_table: torch.Tensor,
@@ -143,9 +146,9 @@ def pool4_decode_attention(q: torch.Tensor, pool: Pool4, page_table: torch.Tenso
     the sequence's last tokens, each sees those up to its own.  Hidden tokens (-inf in
     the mask among them) take no part whatever they hold, and a row that sees nothing
     is zeros.  Returns out [B, Hq, q_len, D] in q's dtype."""
-    args, out, _ = _decode_args(q, pool, page_table, seq_lens, max_pages, scale, softcap,
-                                attention_mask, causal, out)
-    _engine.call_on(q.device, "helm_pool4_decode_attn", *args, _engine.stream_ptr(q.device))
+    idx, args, out, _ = _decode_args(q, pool, page_table, seq_lens, max_pages, scale, softcap,
+                                     attention_mask, causal, out)
+    _engine.launch_on(idx, "helm_pool4_decode_attn", *args)
     return out
 
 
@@ -162,7 +165,7 @@ def check_scores(scale: Optional[float], softcap: Optional[float], D: int) -> Tu
 
 def _decode_args(q, pool, page_table, seq_lens, max_pages, scale, softcap, mask, causal, out,
                  in_place=False):
-    """Checks the operands; (C-ABI arguments up to the stream, out, tensors to keep)."""
+    """Checks the operands; (device, C-ABI arguments up to the stream, out, tensors to keep)."""
     if q.dim() != 4:
         raise ValueError("q must be [B, Hq, q_len, D]")
     B, Hq, S, D = q.shape
@@ -188,7 +191,7 @@ def _decode_args(q, pool, page_table, seq_lens, max_pages, scale, softcap, mask,
             raise ValueError("attention_mask must be [B|1, Hq|1, q_len|1, T]")
         if not mask.is_floating_point():
             raise TypeError("attention_mask is additive: a floating-point tensor")
-        m = mask if mask.dtype in _MASKS else mask.float()
+        m = mask if mask.dtype in _CODES else mask.float()
         if m.stride(3) != 1:
             m = m.contiguous()
         ms = tuple(m.stride(i) if m.size(i) > 1 else 0 for i in range(3))
@@ -197,8 +200,10 @@ def _decode_args(q, pool, page_table, seq_lens, max_pages, scale, softcap, mask,
         out = torch.empty((B, Hq, S, D), dtype=q.dtype, device=q.device)
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
         raise ValueError("out must be contiguous, of q's shape and dtype")
-    _engine.check_operands("pool4_decode_attention", q.device, q, pool.data, page_table, seq_lens, m,
-                           out)
+    masks = () if m is None else (m,)
+    _engine.refuse_grad("pool4_decode_attention", q, *masks)
+    idx = _engine.common_device("pool4_decode_attention", q, pool.data, page_table, seq_lens, out,
+                                *masks)
     q = q.contiguous()
     if q.data_ptr() % 16:
         if in_place:
@@ -213,6 +218,6 @@ def _decode_args(q, pool, page_table, seq_lens, max_pages, scale, softcap, mask,
             page_table.data_ptr(), max(page_table.stride(0), max_pages), max_pages,
             seq_lens.data_ptr(), B, Hq, pool.num_kv_heads, S, D, scale, cap,
             m.data_ptr() if m is not None else None, *ms, width,
-            _native.dtype_code(m.dtype) if m is not None else _native.HELM_F32, int(bool(causal)),
-            _native.dtype_code(q.dtype), ws.data_ptr(), need)
-    return args, out, (q, pool, page_table, seq_lens, m, ws)
+            _CODES[m.dtype] if m is not None else _native.HELM_F32, int(bool(causal)),
+            _CODES[q.dtype], ws.data_ptr(), need)
+    return idx, args, out, (q, pool, page_table, seq_lens, m, ws)

@@ -62,31 +62,42 @@ def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(idx).cuda_stream
 
 
-def call_on(device: torch.device, fn: str, *args) -> None:
-    """One native call that launches on `device`: the device is current for it
-    (and the one before is again afterwards); raises as ``_native.call`` does."""
+_get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def launch_on(idx: int, fn: str, *args) -> None:
+    """One native call that launches on HIP device `idx`, on torch's current stream
+    there (its last argument): the device is current for it (and the one before is
+    again afterwards); raises as ``_native.call`` does."""
     f = _native.entry(fn)
-    if device.index is None or device.index == torch.cuda.current_device():
-        rc = f(*args)
+    stream = _raw_stream(idx) if _raw_stream is not None else \
+        torch.cuda.current_stream(idx).cuda_stream
+    if idx == _get_device():
+        rc = f(*args, stream)
     else:
-        with torch.cuda.device(device):
-            rc = f(*args)
+        with torch.cuda.device(idx):
+            rc = f(*args, stream)
     if rc:
         _native.check(fn, rc)
 
 
-def check_operands(what: str, device: torch.device, *tensors) -> None:
-    """The operands of a call sit on one HIP device and ask for no gradient
-    (None is skipped)."""
+def common_device(what: str, *tensors: torch.Tensor) -> int:
+    """The index of the one HIP device that a call's operands sit on."""
+    idx = tensors[0].get_device()
     for t in tensors:
-        if t is None:
-            continue
-        if t.device != device:
-            raise ValueError(f"{what}: operands on {device} and {t.device}")
-        if t.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError(f"{what} records no gradient: call it under torch.no_grad()")
-    if device.type != "cuda":
+        if t.get_device() != idx:
+            raise ValueError(f"{what}: operands on {tensors[0].device} and {t.device}")
+    if idx < 0:
         raise RuntimeError(f"{what} needs HIP tensors")
+    return idx
+
+
+def refuse_grad(what: str, *tensors: torch.Tensor) -> None:
+    """The package serves models: its attention records nothing for a backward pass."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                raise RuntimeError(f"{what} records no gradient: call it under torch.no_grad()")
 
 
 @atexit.register
