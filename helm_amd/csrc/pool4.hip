@@ -4,12 +4,14 @@
 // Both are bound by memory: a bf16 row of D dims is 2 D bytes on one side and
 // 17 D / 32 on the other.  A thread owns eight dims of K or V of one head (16 bytes of a
 // 16-bit row; four lanes are a group, whose largest magnitude they share by two quad
-// moves) and takes them of four consecutive rows, whose loads are all in flight at
-// once: where its place in a row is worked out once for the four.  (A thread a row and
-// place spent half its time on divisions: 16,384 rows of 8 heads of 128, bf16, write
-// 31 us and read 28.5, now WRITE_US and READ_US.)  The conversions of gfx950 encode and
-// decode two values an instruction, exactly and with ties to the even code (checked
-// over every code and exponent).
+// moves) and takes them of two consecutive rows: where its place in a row is worked out
+// once for both.  The workgroups of neighbouring rows run on one XCD, so that the 16
+// rows of a tile, which share cache lines, meet in one L2 instead of leaving it in
+// parts.  16,384 rows of 8 heads of 128, bf16, write / read: a thread a row and place
+// 31 / 28.5 us (half of it divisions), four rows 26 / 22, on one XCD 18.8 / 18.9, two
+// rows 18.1 / 17.5 (8: 21 / 24); 85 MB each, 16.7 us at a large copy's rate.
+// The conversions of gfx950 encode and decode two values an instruction, exactly and
+// with ties to the even code (checked over every code and exponent).
 #include "pool4.h"
 
 #include <algorithm>
@@ -26,7 +28,7 @@ namespace {
 
 constexpr int kThreads4 = 256;
 
-constexpr int kRowsPer = 4;         // consecutive rows of a thread
+constexpr int kRowsPer = 2;         // consecutive rows of a thread
 
 struct P4Rows {
   char* pool;
@@ -119,7 +121,9 @@ template <int D> struct P4Item {
     const int sub = a.abreast > 1 ? tid / a.items : 0;
     int i = a.abreast > 1 ? tid - sub * a.items : (int)blockIdx.y * kThreads4 + tid;
     some = sub < a.abreast && i < a.items;
-    n = ((int64_t)blockIdx.x * a.abreast + sub) * kRowsPer;
+    // neighbouring rows stay on one XCD (workgroups go round the eight of them)
+    const int64_t wg = (int64_t)(blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8;
+    n = (wg * a.abreast + sub) * kRowsPer;
     is_v = i >= a.items / 2;
     if (is_v) i -= a.items / 2;
     h = i / (D / 8);
@@ -228,7 +232,7 @@ __global__ __launch_bounds__(kThreads4) void pool4_read_kernel(P4Rows a) {
 template <typename T, int D>
 void launch_rows(bool write, const P4Rows& a, hipStream_t st) {
   const int64_t rows = (int64_t)a.abreast * kRowsPer;
-  const dim3 grid((uint32_t)((a.n_tok + rows - 1) / rows),
+  const dim3 grid((uint32_t)((a.n_tok + 8 * rows - 1) / (8 * rows) * 8),
                   (uint32_t)((a.items + kThreads4 - 1) / kThreads4));
   if (write) hipLaunchKernelGGL((pool4_write_kernel<T, D>), grid, dim3(kThreads4), 0, st, a);
   else hipLaunchKernelGGL((pool4_read_kernel<T, D>), grid, dim3(kThreads4), 0, st, a);
