@@ -32,8 +32,6 @@
 
 namespace helm {
 
-constexpr int kPromptWaves = 4;
-constexpr int kPromptRows = 32 * kPromptWaves;   // query rows of a workgroup
 constexpr int kPromptTok = 64;                   // tokens of a stage
 
 struct PromptParams {
@@ -60,18 +58,87 @@ __device__ __forceinline__ PromptSeq prompt_seq(const PromptParams& p, int b) {
   return {s, e - s};
 }
 
-// Row tile j of the packed batch: its sequence (lanes take 64 sequences at a time)
-// and its first row in it, the later rows of a sequence (the longer walks) first.
+__device__ __forceinline__ int wave_sum(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);   // row_shr 1, 2, 4, 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);   // row_bcast 15, 31
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+  return __builtin_amdgcn_readlane(x, 63);
+}
+
+// Row tile j (of `rows` rows) of the packed batch: its sequence and its first row in it.
 // b < 0: past the last tile, row = its number there.
 struct PromptTile {
   int b, first, len, row;
 };
-__device__ __forceinline__ PromptTile prompt_tile(const PromptParams& p, int j, int lane) {
+// Up to 256 sequences: the tiles that lie furthest into their sequences, whose walks are
+// the longest, come first over the whole batch, so that the last workgroups to run
+// are short ones.  F(l) = sum of max(0, tiles_b - l) counts the tiles at l or further;
+// tile j is at the l with F(l + 1) <= j < F(l), in the (j - F(l + 1))th sequence that
+// has one there.
+__device__ __forceinline__ PromptTile prompt_tile_longest(const PromptParams& p, int j, int rows,
+                                                          int lane) {
+  constexpr int K = 4;
+  PromptSeq s[K];
+  int nt[K], top = 0;
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    s[i] = {0, 0};
+    if (64 * i + lane < p.B) s[i] = prompt_seq(p, 64 * i + lane);
+    nt[i] = (s[i].len + rows - 1) / rows;
+    top = max(top, nt[i]);
+  }
+  auto from = [&](int l) {
+    int x = 0;
+#pragma unroll
+    for (int i = 0; i < K; ++i) x += max(0, nt[i] - l);
+    return wave_sum(x);
+  };
+  const int all = from(0);
+  if (j >= all) return {-1, 0, 0, j - all};
+  int lo = 0, hi = 1;                       // F(lo) > j >= F(hi), once hi is doubled up to it
+  int below = from(1);
+  while (below > j) {
+    lo = hi;
+    hi *= 2;
+    below = from(hi);
+  }
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1, f = from(mid);
+    if (f > j) {
+      lo = mid;
+    } else {
+      hi = mid;
+      below = f;
+    }
+  }
+  int nth = j - below;
+  PromptTile t{-1, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    const uint64_t has = __builtin_amdgcn_ballot_w64(nt[i] > lo);
+    const int n = __builtin_popcountll(has);
+    if (t.b < 0 && nth < n) {
+      const int rank = __builtin_popcountll(has & ((1ull << lane) - 1));
+      const uint64_t hit = __builtin_amdgcn_ballot_w64(nt[i] > lo && rank == nth);
+      const int at = __builtin_ctzll(hit);
+      t = {64 * i + at, __builtin_amdgcn_readlane(s[i].first, at),
+           __builtin_amdgcn_readlane(s[i].len, at), lo * rows};
+    }
+    nth -= n;
+  }
+  return t;
+}
+// Any number: sequence by sequence, the later rows of each first.
+__device__ __forceinline__ PromptTile prompt_tile_in_order(const PromptParams& p, int j, int rows,
+                                                           int lane) {
   int base = 0;
   for (int b0 = 0; b0 < p.B; b0 += 64) {
     PromptSeq s{0, 0};
     if (b0 + lane < p.B) s = prompt_seq(p, b0 + lane);
-    const int nt = (s.len + kPromptRows - 1) / kPromptRows;
+    const int nt = (s.len + rows - 1) / rows;
     int incl = nt;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -83,8 +150,8 @@ __device__ __forceinline__ PromptTile prompt_tile(const PromptParams& p, int j, 
       const int at = __builtin_ctzll(past);
       const int first = __builtin_amdgcn_readlane(s.first, at);
       const int len = __builtin_amdgcn_readlane(s.len, at);
-      const int t = __builtin_amdgcn_readlane(base + incl, at) - 1 - j;   // from the last
-      return {b0 + at, first, len, t * kPromptRows};
+      const int t = base + __builtin_amdgcn_readlane(incl, at) - 1 - j;   // from the last
+      return {b0 + at, first, len, t * rows};
     }
     base += __builtin_amdgcn_readlane(incl, 63);
   }
@@ -99,16 +166,16 @@ template <typename T> __device__ __forceinline__ uint32_t nonfinite_halves(uint3
   return r;
 }
 
-template <typename T, int D, bool kCap, bool kWindow>
+template <typename T, int D, int NW, bool kCap, bool kWindow>
 __device__ __forceinline__ void prompt_body(const PromptParams& p) {
-  constexpr int NW = kPromptWaves;
+  constexpr int kRows = 32 * NW;             // query rows of the workgroup
   constexpr int SB = kPromptTok / kBlockTok;
   constexpr int NK = D / 16, NE = D / 32, CPR = D / 8;
   constexpr int kRow = 2 * D, kBlk = kBlockTok * kRow;
   constexpr int kShift = std::is_same<T, f16_t>::value ? 9 : 0;
   constexpr float kSlack = chunk_slack(kShift);
   constexpr int kBlkLoads = kBlk / 1024;
-  static_assert(SB == NW, "a wave loads one block of K and of V");
+  static_assert(NW == SB || NW == 2 * SB, "a wave loads a block of K and of V, or of one");
   using Ops = MfmaOps<T>;
   using M32 = Mfma32<T>;
   typedef mf_u32x4 StageBuf[2][SB][kBlk / 16];
@@ -117,8 +184,11 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63, jr = lane & 31, hh = lane >> 5;
-  const int hq = blockIdx.x % p.Hq, hk = hq / p.G;
-  const PromptTile tl = prompt_tile(p, blockIdx.x / p.Hq, lane);
+  // the query heads of a KV head lie Hkv apart, which for 8 KV heads (2, 4) keeps each on
+  // one XCD (its share), whose L2 then reads its K and V once for all of them
+  const int hk = blockIdx.x % p.Hq % p.Hkv, hq = hk * p.G + blockIdx.x % p.Hq / p.Hkv;
+  const PromptTile tl = p.B <= 256 ? prompt_tile_longest(p, blockIdx.x / p.Hq, kRows, lane)
+                                   : prompt_tile_in_order(p, blockIdx.x / p.Hq, kRows, lane);
   if (tl.b < 0) {
     if (!p.zero_rest) return;
     // (the workgroups past the last tile share out the rows outside every sequence)
@@ -137,11 +207,35 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
   const bool row_ok = row < tl.len;
   const bool wave_rows = row_w < tl.len;
   const int row_last = min(row_w + 31, tl.len - 1);
-  const int end = min(tl.row + kPromptRows, tl.len);     // keys: [0, end)
+  const int end = min(tl.row + kRows, tl.len);     // keys: [0, end)
   const int win = kWindow ? p.window : 0;
   const int st0 = kWindow ? max(0, tl.row - win + 1) / kPromptTok : 0;
   const int st1 = (end + kPromptTok - 1) / kPromptTok;
 
+  const float scale2 = p.scale * kLog2E;
+  const float inv_cap = kCap ? 1.f / p.softcap : 0.f, cap2 = p.softcap * kLog2E;
+
+  const char* kb = p.k + tl.first * p.k_tok + hk * p.k_head;
+  const char* vb = p.v + tl.first * p.v_tok + hk * p.v_head;
+  // this wave's block of a stage, K and V, straight into LDS; lane i of load u fetches
+  // the chunk that the swizzle (attn_chunk32.h) keeps in slot 64 u + i; tokens past
+  // the sequence's end come in as zeros
+  const int own = NW == SB ? wave : wave % SB;
+  auto dma_stage = [&](int st, StageBuf& dst) {
+    const int tok0 = st * kPromptTok + own * kBlockTok;
+    const int nt = min(max(tl.len - tok0, 0), kBlockTok);
+    const auto rk = make_rsrc(kb + tok0 * p.k_tok, nt ? (nt - 1) * (int)p.k_tok + kRow : 0);
+    const auto rv = make_rsrc(vb + tok0 * p.v_tok, nt ? (nt - 1) * (int)p.v_tok + kRow : 0);
+#pragma unroll
+    for (int u = 0; u < kBlkLoads; ++u) {
+      const int t = (64 / CPR) * u + lane / CPR;
+      const int c = 16 * ((lane % CPR) ^ swz<D>(t));
+      if (NW == SB || wave < SB) buf_load16_lds(rk, &dst[0][own][64 * u], t * (int)p.k_tok + c);
+      if (NW == SB || wave >= SB) buf_load16_lds(rv, &dst[1][own][64 * u], t * (int)p.v_tok + c);
+    }
+  };
+
+  dma_stage(st0, lds0);                     // (on its way before the query rows)
   mf_u32x4 qop[NK];
   {
     const char* qp = p.q + (int64_t)(tl.first + (row_ok ? row : 0)) * p.q_tok + hq * p.q_head;
@@ -151,28 +245,6 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
       qop[i] = row_ok ? w ^ p.q_sign : mf_u32x4{0u, 0u, 0u, 0u};
     }
   }
-  const float scale2 = p.scale * kLog2E;
-  const float inv_cap = kCap ? 1.f / p.softcap : 0.f, cap2 = p.softcap * kLog2E;
-
-  const char* kb = p.k + tl.first * p.k_tok + hk * p.k_head;
-  const char* vb = p.v + tl.first * p.v_tok + hk * p.v_head;
-  // this wave's block of a stage, K and V, straight into LDS; lane i of load u fetches
-  // the chunk that the swizzle (attn_chunk32.h) keeps in slot 64 u + i; tokens past
-  // the sequence's end come in as zeros
-  auto dma_stage = [&](int st, StageBuf& dst) {
-    const int tok0 = st * kPromptTok + wave * kBlockTok;
-    const int nt = min(max(tl.len - tok0, 0), kBlockTok);
-    const auto rk = make_rsrc(kb + tok0 * p.k_tok, nt ? (nt - 1) * (int)p.k_tok + kRow : 0);
-    const auto rv = make_rsrc(vb + tok0 * p.v_tok, nt ? (nt - 1) * (int)p.v_tok + kRow : 0);
-#pragma unroll
-    for (int u = 0; u < kBlkLoads; ++u) {
-      const int t = (64 / CPR) * u + lane / CPR;
-      const int c = 16 * ((lane % CPR) ^ swz<D>(t));
-      buf_load16_lds(rk, &dst[0][wave][64 * u], t * (int)p.k_tok + c);
-      buf_load16_lds(rv, &dst[1][wave][64 * u], t * (int)p.v_tok + c);
-    }
-  };
-
   const int g_a = jr >> 3, h_a = (jr >> 2) & 1, t_a = jr & 3;
   const int tau = 16 * (g_a >> 1) + 8 * h_a + 4 * (g_a & 1) + t_a;
   const int kblk = tau >> 4, ktok = tau & 15;
@@ -312,7 +384,6 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
         part(st, 0, cur);
         part(st, 2, cur);
       };
-      dma_stage(st0, lds0);
       for (int st = st0; st < st1; st += 2) {
         stage(st, lds0, lds1);
         if (st + 1 < st1) stage(st + 1, lds1, lds0);
@@ -326,36 +397,55 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) odd = odd || o[e][r] != o[e][r];
   // (the barrier also ends every wave's reads of the buffers that a second walk fills)
-  if (__syncthreads_or(odd && row_ok)) walk(std::true_type{});
+  if (__syncthreads_or(odd && row_ok)) {
+    walk(std::true_type{});
+    __syncthreads();
+  }
 
-  if (!row_ok) return;
+  // The rows leave through LDS, each wave's in a part of its own (chunk c of row r at
+  // slot c ^ r, so that neither side meets bank conflicts): 16 bytes a lane, whole rows
+  // a store.  (Straight from the registers a row's lines went out in 16-byte pieces, which
+  // bound short prompts: EPILOGUE.)
   const float l = lsum + __shfl_xor(lsum, 32, 64);
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  char* op = p.out + (int64_t)(tl.first + row) * p.o_tok + hq * p.o_head;
+  char* rows = reinterpret_cast<char*>(&lds0[0][0][0]) + wave * (32 * kRow);
 #pragma unroll
   for (int e = 0; e < NE; ++e)
 #pragma unroll
     for (int g = 0; g < 4; ++g)
-      *reinterpret_cast<uint2*>(op + 2 * (32 * e + 8 * g + 4 * hh)) =
+      *reinterpret_cast<uint2*>(rows + jr * kRow + 16 * ((4 * e + g) ^ (jr % CPR)) + 8 * hh) =
           make_uint2(Ops::pk(o[e][4 * g] * inv, o[e][4 * g + 1] * inv),
                      Ops::pk(o[e][4 * g + 2] * inv, o[e][4 * g + 3] * inv));
+  char* op = p.out + (int64_t)(tl.first + row_w) * p.o_tok + hq * p.o_head + 16 * (lane % CPR);
+#pragma unroll
+  for (int i = 0; i < 32 * CPR / 64; ++i) {
+    const int r = (64 / CPR) * i + lane / CPR;
+    const mf_u32x4 w =
+        *reinterpret_cast<const mf_u32x4*>(rows + r * kRow + 16 * ((lane % CPR) ^ (r % CPR)));
+    if (row_w + r < tl.len) *reinterpret_cast<mf_u32x4*>(op + r * p.o_tok) = w;
+  }
 }
 
-template <typename T, int D, bool kCap, bool kWindow>
-__global__ __launch_bounds__(64 * kPromptWaves, D == 256 ? 1 : 2) void prompt_attn_kernel(
-    PromptParams p) {
-  prompt_body<T, D, kCap, kWindow>(p);
+template <typename T, int D, int NW, bool kCap, bool kWindow>
+__global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void prompt_attn_kernel(PromptParams p) {
+  prompt_body<T, D, NW, kCap, kWindow>(p);
 }
 
+template <typename T, int D, int NW>
+hipError_t launch_prompt_waves(PromptParams p, hipStream_t st) {
+  p.tiles = (p.N + 32 * NW - 1) / (32 * NW) + p.B;
+  const dim3 grid((uint32_t)p.tiles * p.Hq), block(64 * NW);
+  const bool cap = p.softcap > 0.f, win = p.window > 0;
+  if (cap && win) hipLaunchKernelGGL((prompt_attn_kernel<T, D, NW, true, true>), grid, block, 0, st, p);
+  else if (cap) hipLaunchKernelGGL((prompt_attn_kernel<T, D, NW, true, false>), grid, block, 0, st, p);
+  else if (win) hipLaunchKernelGGL((prompt_attn_kernel<T, D, NW, false, true>), grid, block, 0, st, p);
+  else hipLaunchKernelGGL((prompt_attn_kernel<T, D, NW, false, false>), grid, block, 0, st, p);
+  return hipGetLastError();
+}
 template <typename T, int D>
 hipError_t launch_prompt_dim(const PromptParams& p, hipStream_t st) {
-  const dim3 grid((uint32_t)p.tiles * p.Hq), block(64 * kPromptWaves);
-  const bool cap = p.softcap > 0.f, win = p.window > 0;
-  if (cap && win) hipLaunchKernelGGL((prompt_attn_kernel<T, D, true, true>), grid, block, 0, st, p);
-  else if (cap) hipLaunchKernelGGL((prompt_attn_kernel<T, D, true, false>), grid, block, 0, st, p);
-  else if (win) hipLaunchKernelGGL((prompt_attn_kernel<T, D, false, true>), grid, block, 0, st, p);
-  else hipLaunchKernelGGL((prompt_attn_kernel<T, D, false, false>), grid, block, 0, st, p);
-  return hipGetLastError();
+  if (D == 128 && getenv("PNW8")) return launch_prompt_waves<T, D, D == 256 ? 4 : 8>(p, st);
+  return launch_prompt_waves<T, D, 4>(p, st);
 }
 
 // One per element type, each in a source of its own (prompt_bf16.hip, prompt_f16.hip).

@@ -58,10 +58,8 @@ extern "C" int helm_prompt_attn(const void* q, int64_t q_tok_stride, int64_t q_h
   p.Hq = Hq;
   p.Hkv = Hkv;
   p.G = Hq / Hkv;
-  const int64_t tiles = ((int64_t)N + kPromptRows - 1) / kPromptRows + B;
-  if (tiles * Hq > 0x7fffffff / (64 * kPromptWaves))
+  if (((int64_t)N / 128 + 1 + B) * Hq > 0x7fffffff / 512)     // (tiles * heads * threads)
     return report_error(HELM_E_INVALID, "too many rows and heads for one launch");
-  p.tiles = (int)tiles;
   // the kernel takes the row's maximum before it scales
   p.q_sign = scale < 0.f ? 0x80008000u : 0u;
   p.scale = std::max(scale < 0.f ? -scale : scale, FLT_MIN);
