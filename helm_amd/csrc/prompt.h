@@ -32,7 +32,13 @@
 
 namespace helm {
 
-constexpr int kPromptTok = 64;                   // tokens of a stage
+// Tokens of a stage, waves of a workgroup: D = 256 would need 64 + 128 registers for a
+// wave's query operand and output alone, which left one wave a SIMD and its products
+// waiting for its softmax.  There half of the query operand stays in LDS (8 of the 40
+// KiB a step reads), eight waves share stages of 32 tokens, and each SIMD has two.
+template <int D> struct PromptShape {
+  static constexpr int kTok = D == 256 ? 32 : 64, kWaves = D == 256 ? 8 : 4;
+};
 
 struct PromptParams {
   const char *q, *k, *v;
@@ -166,20 +172,25 @@ template <typename T> __device__ __forceinline__ uint32_t nonfinite_halves(uint3
   return r;
 }
 
-template <typename T, int D, int NW, bool kCap, bool kWindow>
+template <typename T, int D, bool kCap, bool kWindow>
 __device__ __forceinline__ void prompt_body(const PromptParams& p) {
+  constexpr int NW = PromptShape<D>::kWaves;
   constexpr int kRows = 32 * NW;             // query rows of the workgroup
-  constexpr int SB = kPromptTok / kBlockTok;
+  constexpr int kTok = PromptShape<D>::kTok, SB = kTok / kBlockTok;
   constexpr int NK = D / 16, NE = D / 32, CPR = D / 8;
   constexpr int kRow = 2 * D, kBlk = kBlockTok * kRow;
   constexpr int kShift = std::is_same<T, f16_t>::value ? 9 : 0;
   constexpr float kSlack = chunk_slack(kShift);
   constexpr int kBlkLoads = kBlk / 1024;
-  static_assert(NW == SB || NW == 2 * SB, "a wave loads a block of K and of V, or of one");
+  // 16-byte-a-lane loads of a wave and stage: neighbours of one block of K or V, or two
+  constexpr int kLoads = 2 * SB * kBlkLoads / NW;
+  constexpr bool kQLds = D == 256;           // query dims 128 .. 255 in LDS
+  constexpr int NQ = kQLds ? NK / 2 : NK;
   using Ops = MfmaOps<T>;
   using M32 = Mfma32<T>;
   typedef mf_u32x4 StageBuf[2][SB][kBlk / 16];
   __shared__ StageBuf lds0, lds1;
+  __shared__ mf_u32x4 ldsq[kQLds ? NW * 32 * 16 : 1];   // [wave][row][chunk ^ row % 16]
 
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -209,51 +220,71 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
   const int row_last = min(row_w + 31, tl.len - 1);
   const int end = min(tl.row + kRows, tl.len);     // keys: [0, end)
   const int win = kWindow ? p.window : 0;
-  const int st0 = kWindow ? max(0, tl.row - win + 1) / kPromptTok : 0;
-  const int st1 = (end + kPromptTok - 1) / kPromptTok;
+  const int st0 = kWindow ? max(0, tl.row - win + 1) / kTok : 0;
+  const int st1 = (end + kTok - 1) / kTok;
 
   const float scale2 = p.scale * kLog2E;
   const float inv_cap = kCap ? 1.f / p.softcap : 0.f, cap2 = p.softcap * kLog2E;
 
   const char* kb = p.k + tl.first * p.k_tok + hk * p.k_head;
   const char* vb = p.v + tl.first * p.v_tok + hk * p.v_head;
-  // this wave's block of a stage, K and V, straight into LDS; lane i of load u fetches
-  // the chunk that the swizzle (attn_chunk32.h) keeps in slot 64 u + i; tokens past
-  // the sequence's end come in as zeros
-  const int own = NW == SB ? wave : wave % SB;
+  // this wave's loads of a stage straight into LDS: load i of the stage's is part u of
+  // i / kBlkLoads, a block's K, then its V, then the next block's; lane l of it fetches the chunk that the
+  // swizzle (attn_chunk32.h) keeps in slot 64 u + l; tokens past the sequence's end come
+  // in as zeros
   auto dma_stage = [&](int st, StageBuf& dst) {
-    const int tok0 = st * kPromptTok + own * kBlockTok;
-    const int nt = min(max(tl.len - tok0, 0), kBlockTok);
-    const auto rk = make_rsrc(kb + tok0 * p.k_tok, nt ? (nt - 1) * (int)p.k_tok + kRow : 0);
-    const auto rv = make_rsrc(vb + tok0 * p.v_tok, nt ? (nt - 1) * (int)p.v_tok + kRow : 0);
 #pragma unroll
-    for (int u = 0; u < kBlkLoads; ++u) {
+    for (int k = 0; k < kLoads; ++k) {
+      const int i = wave * kLoads + k, kb_v = i / kBlkLoads, u = i % kBlkLoads;
+      const int blk = kb_v / 2, is_v = kb_v % 2;                       // (uniform)
+      const int tok0 = st * kTok + blk * kBlockTok;
+      const int nt = min(max(tl.len - tok0, 0), kBlockTok);
+      const int64_t stride = is_v ? p.v_tok : p.k_tok;
+      const auto rs = make_rsrc((is_v ? vb : kb) + tok0 * stride,
+                                nt ? (nt - 1) * (int)stride + kRow : 0);
       const int t = (64 / CPR) * u + lane / CPR;
-      const int c = 16 * ((lane % CPR) ^ swz<D>(t));
-      if (NW == SB || wave < SB) buf_load16_lds(rk, &dst[0][own][64 * u], t * (int)p.k_tok + c);
-      if (NW == SB || wave >= SB) buf_load16_lds(rv, &dst[1][own][64 * u], t * (int)p.v_tok + c);
+      buf_load16_lds(rs, &dst[is_v][blk][64 * u],
+                     t * (int)stride + 16 * ((lane % CPR) ^ swz<D>(t)));
     }
   };
 
   dma_stage(st0, lds0);                     // (on its way before the query rows)
-  mf_u32x4 qop[NK];
+  mf_u32x4 qop[NQ];
+  mf_u32x4* qs = &ldsq[kQLds ? (wave * 32 + jr) * 16 : 0];
   {
     const char* qp = p.q + (int64_t)(tl.first + (row_ok ? row : 0)) * p.q_tok + hq * p.q_head;
 #pragma unroll
     for (int i = 0; i < NK; ++i) {
       const mf_u32x4 w = *reinterpret_cast<const mf_u32x4*>(qp + 16 * (2 * i + hh));
-      qop[i] = row_ok ? w ^ p.q_sign : mf_u32x4{0u, 0u, 0u, 0u};
+      const mf_u32x4 x = row_ok ? w ^ p.q_sign : mf_u32x4{0u, 0u, 0u, 0u};
+      if (i < NQ) qop[i < NQ ? i : 0] = x;
+      else qs[(2 * (i - NQ) + hh) ^ (jr & 15)] = x;     // (read by this wave alone)
     }
   }
   const int g_a = jr >> 3, h_a = (jr >> 2) & 1, t_a = jr & 3;
   const int tau = 16 * (g_a >> 1) + 8 * h_a + 4 * (g_a & 1) + t_a;
   const int kblk = tau >> 4, ktok = tau & 15;
   const int nl = lane & 15;
-  auto vaddr = [&](const StageBuf& cur, int blk, int z, int e) -> const char* {
-    const int vtok = 8 * hh + 4 * z + (nl >> 2);
-    const int chunk = 4 * e + 2 * (jr >> 4) + ((nl & 3) >> 1);
-    return reinterpret_cast<const char*>(&cur[1][blk][vtok * CPR + (chunk ^ swz<D>(vtok))]) +
-           8 * (nl & 1);
+  // Byte offsets of a step's operands in its stage buffer: the swizzle is an XOR below the
+  // row's size, so every operand lies at one offset XOR a constant.  (D = 256 does that
+  // anew for each read: kept in registers, 24 offsets would push others to memory.)
+  const int k_off = kblk * kBlk + ktok * kRow + 16 * (hh ^ swz<D>(ktok));
+  const int v_tok0 = 8 * hh + (nl >> 2);
+  const int v_off = v_tok0 * kRow + 16 * ((2 * (jr >> 4) + ((nl & 3) >> 1)) ^ swz<D>(v_tok0)) +
+                    8 * (nl & 1);
+  const int q_off = 16 * (hh ^ (jr & 15));
+  auto anew = [](int off) {
+    if constexpr (kQLds) asm volatile("" : "+v"(off));
+    return off;
+  };
+  auto k_operand = [&](const StageBuf& cur, int bp, int i, int off) {
+    return *reinterpret_cast<const mf_u32x4*>(reinterpret_cast<const char*>(&cur[0][bp][0]) +
+                                              (off ^ (32 * i)));
+  };
+  auto v_operand = [&](const StageBuf& cur, int blk, int z, int e, int off) {
+    // token v_tok0 + 4 z: the row four further, whose swizzle differs by z's bit
+    return ld_tr16(reinterpret_cast<const char*>(&cur[1][blk][0]) + (off ^ (64 * e) ^ (16 * z)) +
+                   4 * kRow * z);
   };
 
   float m, lsum;
@@ -263,9 +294,15 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
     mf_f32x16 sc;
 #pragma unroll
     for (int r = 0; r < 16; ++r) sc[r] = 0.f;
+    const int ko = anew(k_off), qo = anew(q_off);
 #pragma unroll
-    for (int i = 0; i < NK; ++i)
-      sc = M32::mma(cur[0][bp + kblk][ktok * CPR + ((2 * i + hh) ^ swz<D>(ktok))], qop[i], sc);
+    for (int i = 0; i < NK; ++i) {
+      const mf_u32x4 q = i < NQ ? qop[i < NQ ? i : 0]
+                                : *reinterpret_cast<const mf_u32x4*>(
+                                      reinterpret_cast<const char*>(qs) + (qo ^ (32 * (i - NQ))));
+      sc = M32::mma(k_operand(cur, bp, i, ko), q, sc);
+      if (kQLds && i % 4 == 3) __builtin_amdgcn_sched_barrier(0);   // (few operands ahead)
+    }
     float x[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) x[r] = sc[r];
@@ -306,13 +343,14 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
         some[i] = (w0 != 0.f ? one & 0xffffu : 0u) | (w1 != 0.f ? one & 0xffff0000u : 0u);
       }
     }
+    const int vo = anew(v_off);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const mf_u32x4 pop{w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]};
 #pragma unroll
       for (int e = 0; e < NE; ++e) {
-        const uint2 a0 = ld_tr16(vaddr(cur, bp + u, 0, e));
-        const uint2 a1 = ld_tr16(vaddr(cur, bp + u, 1, e));
+        const uint2 a0 = v_operand(cur, bp + u, 0, e, vo);
+        const uint2 a1 = v_operand(cur, bp + u, 1, e, vo);
         mf_u32x4 vop{a0.x, a0.y, a1.x, a1.y};
         if constexpr (careful.value) {
           mf_u32x4 bad;
@@ -349,6 +387,7 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
           }
         }
         o[e] = M32::mma(vop, pop, o[e]);
+        if (kQLds && e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
       }
     }
   };
@@ -361,7 +400,7 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
       for (int r = 0; r < 16; ++r) o[e][r] = 0.f;
     // a step none of whose tokens any row of the wave sees is left out (uniform)
     auto part = [&](int st, int bp, const StageBuf& cur) {
-      const int tok0 = st * kPromptTok + bp * kBlockTok;
+      const int tok0 = st * kTok + bp * kBlockTok;
       if (wave_rows && tok0 <= row_last && !(kWindow && tok0 + 31 <= row_w - win))
         step(careful, tok0, bp, cur);
     };
@@ -382,7 +421,7 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
         __syncthreads();
         if (st + 1 < st1) dma_stage(st + 1, nxt);
         part(st, 0, cur);
-        part(st, 2, cur);
+        if constexpr (SB > 2) part(st, 2, cur);
       };
       for (int st = st0; st < st1; st += 2) {
         stage(st, lds0, lds1);
@@ -408,44 +447,49 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
   // bound short prompts: EPILOGUE.)
   const float l = lsum + __shfl_xor(lsum, 32, 64);
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  char* rows = reinterpret_cast<char*>(&lds0[0][0][0]) + wave * (32 * kRow);
+  // (D = 256: half a row at a time, where the query's half was)
+  constexpr int kHalves = kQLds ? 2 : 1, EH = NE / kHalves, CH = CPR / kHalves;
+  char* rows = kQLds ? reinterpret_cast<char*>(&ldsq[wave * 32 * 16])
+                     : reinterpret_cast<char*>(&lds0[0][0][0]) + wave * (32 * kRow);
+  char* op = p.out + (int64_t)(tl.first + row_w) * p.o_tok + hq * p.o_head + 16 * (lane % CH);
 #pragma unroll
-  for (int e = 0; e < NE; ++e)
+  for (int half = 0; half < kHalves; ++half) {
 #pragma unroll
-    for (int g = 0; g < 4; ++g)
-      *reinterpret_cast<uint2*>(rows + jr * kRow + 16 * ((4 * e + g) ^ (jr % CPR)) + 8 * hh) =
-          make_uint2(Ops::pk(o[e][4 * g] * inv, o[e][4 * g + 1] * inv),
-                     Ops::pk(o[e][4 * g + 2] * inv, o[e][4 * g + 3] * inv));
-  char* op = p.out + (int64_t)(tl.first + row_w) * p.o_tok + hq * p.o_head + 16 * (lane % CPR);
+    for (int e = 0; e < EH; ++e)
 #pragma unroll
-  for (int i = 0; i < 32 * CPR / 64; ++i) {
-    const int r = (64 / CPR) * i + lane / CPR;
-    const mf_u32x4 w =
-        *reinterpret_cast<const mf_u32x4*>(rows + r * kRow + 16 * ((lane % CPR) ^ (r % CPR)));
-    if (row_w + r < tl.len) *reinterpret_cast<mf_u32x4*>(op + r * p.o_tok) = w;
+      for (int g = 0; g < 4; ++g) {
+        const mf_f32x16& oe = o[half * EH + e];
+        *reinterpret_cast<uint2*>(rows + jr * (16 * CH) + 16 * ((4 * e + g) ^ (jr % CH)) + 8 * hh) =
+            make_uint2(Ops::pk(oe[4 * g] * inv, oe[4 * g + 1] * inv),
+                       Ops::pk(oe[4 * g + 2] * inv, oe[4 * g + 3] * inv));
+      }
+#pragma unroll
+    for (int i = 0; i < 32 * CH / 64; ++i) {
+      const int r = (64 / CH) * i + lane / CH;
+      const mf_u32x4 w =
+          *reinterpret_cast<const mf_u32x4*>(rows + r * (16 * CH) + 16 * ((lane % CH) ^ (r % CH)));
+      if (row_w + r < tl.len)
+        *reinterpret_cast<mf_u32x4*>(op + r * p.o_tok + 16 * CH * half) = w;
+    }
   }
 }
 
-template <typename T, int D, int NW, bool kCap, bool kWindow>
-__global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void prompt_attn_kernel(PromptParams p) {
-  prompt_body<T, D, NW, kCap, kWindow>(p);
+template <typename T, int D, bool kCap, bool kWindow>
+__global__ __launch_bounds__(64 * PromptShape<D>::kWaves, 2) void prompt_attn_kernel(PromptParams p) {
+  prompt_body<T, D, kCap, kWindow>(p);
 }
 
-template <typename T, int D, int NW>
-hipError_t launch_prompt_waves(PromptParams p, hipStream_t st) {
+template <typename T, int D>
+hipError_t launch_prompt_dim(PromptParams p, hipStream_t st) {
+  constexpr int NW = PromptShape<D>::kWaves;
   p.tiles = (p.N + 32 * NW - 1) / (32 * NW) + p.B;
   const dim3 grid((uint32_t)p.tiles * p.Hq), block(64 * NW);
   const bool cap = p.softcap > 0.f, win = p.window > 0;
-  if (cap && win) hipLaunchKernelGGL((prompt_attn_kernel<T, D, NW, true, true>), grid, block, 0, st, p);
-  else if (cap) hipLaunchKernelGGL((prompt_attn_kernel<T, D, NW, true, false>), grid, block, 0, st, p);
-  else if (win) hipLaunchKernelGGL((prompt_attn_kernel<T, D, NW, false, true>), grid, block, 0, st, p);
-  else hipLaunchKernelGGL((prompt_attn_kernel<T, D, NW, false, false>), grid, block, 0, st, p);
+  if (cap && win) hipLaunchKernelGGL((prompt_attn_kernel<T, D, true, true>), grid, block, 0, st, p);
+  else if (cap) hipLaunchKernelGGL((prompt_attn_kernel<T, D, true, false>), grid, block, 0, st, p);
+  else if (win) hipLaunchKernelGGL((prompt_attn_kernel<T, D, false, true>), grid, block, 0, st, p);
+  else hipLaunchKernelGGL((prompt_attn_kernel<T, D, false, false>), grid, block, 0, st, p);
   return hipGetLastError();
-}
-template <typename T, int D>
-hipError_t launch_prompt_dim(const PromptParams& p, hipStream_t st) {
-  if (D == 128 && getenv("PNW8")) return launch_prompt_waves<T, D, D == 256 ? 4 : 8>(p, st);
-  return launch_prompt_waves<T, D, 4>(p, st);
 }
 
 // One per element type, each in a source of its own (prompt_bf16.hip, prompt_f16.hip).
