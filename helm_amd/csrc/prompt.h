@@ -4,7 +4,7 @@
 //
 // Bound by the matrix cores: 4 D operations a visible (row, head) pair against
 // 8 bytes a row and head dim.  A workgroup owns 128 rows of one query head, a wave
-// 32 of them; it walks the keys in stages of 64 tokens, whose K and V go straight
+// 32 of them (D = 256: 256 rows); it walks the keys in stages, whose K and V go straight
 // from memory into LDS (two stage buffers, one barrier a stage), and computes 32
 // tokens a step.  Lane l = 32 hh + jr owns query row jr:
 //   S^T = K Q^T  (v_mfma_f32_32x32x16): A is K of token tau(jr), B query row jr; with
@@ -15,7 +15,7 @@
 //         32 e + 8 g + 4 hh + t of row jr.
 // So a row's scores, maximum, sum and output sit in the two lanes (*, jr).  The
 // running maximum is refreshed only when a score passes it by 2^8 (base-2 units).
-// Weights are rounded once to the 16-bit type (half a step, 2^-9 or 2^-12 of the
+// Weights are rounded once to the 16-bit type (by half a step, 2^-8 or 2^-11 at most, of the
 // weight, at random: below the output's own rounding) and the row's sum adds the
 // rounded ones; f16 weights are taken times 2^9 (weight_shift: nothing above 2^-34
 // of the largest is lost).
@@ -32,12 +32,19 @@
 
 namespace helm {
 
-// Tokens of a stage, waves of a workgroup: D = 256 would need 64 + 128 registers for a
-// wave's query operand and output alone, which left one wave a SIMD and its products
-// waiting for its softmax.  There half of the query operand stays in LDS (8 of the 40
-// KiB a step reads), eight waves share stages of 32 tokens, and each SIMD has two.
+// Tokens of a stage, waves of a workgroup, waves a SIMD holds, whether the upper half of
+// the query operand stays in LDS, and whether a step works its LDS offsets out anew.
+// The query operand and the output of 32 rows take 48, 96 or 192 registers: with the
+// query's half in LDS and stages of 32 tokens three waves fit a SIMD at D = 128 and two at
+// 256, where one wave's products wait for its own softmax.  bf16, 32 / 8 heads,
+// us: D = 128, 16,384 tokens 2,012 -> 1,954, ragged to 2,033 130 -> 120, 14 of 512
+// (40 heads) 77 -> 67; D = 256, 10,180 tokens of four prompts, 16 / 8 heads, soft-capped,
+// 1,024 window 322 -> 223.  D = 64 is no faster for it (8,192 tokens 315; stages of 32 326,
+// four waves a SIMD by force 309 to 502).
 template <int D> struct PromptShape {
-  static constexpr int kTok = D == 256 ? 32 : 64, kWaves = D == 256 ? 8 : 4;
+  static constexpr int kTok = D == 64 ? 64 : 32, kWaves = D == 256 ? 8 : 4;
+  static constexpr int kPerSimd = D == 128 ? 3 : 2;
+  static constexpr bool kQLds = D != 64, kAnew = D == 256;
 };
 
 struct PromptParams {
@@ -184,13 +191,14 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
   constexpr int kBlkLoads = kBlk / 1024;
   // 16-byte-a-lane loads of a wave and stage: neighbours of one block of K or V, or two
   constexpr int kLoads = 2 * SB * kBlkLoads / NW;
-  constexpr bool kQLds = D == 256;           // query dims 128 .. 255 in LDS
+  constexpr bool kQLds = PromptShape<D>::kQLds;
+  constexpr int QC = CPR / 2;                // 16-byte chunks of half a query row
   constexpr int NQ = kQLds ? NK / 2 : NK;
   using Ops = MfmaOps<T>;
   using M32 = Mfma32<T>;
   typedef mf_u32x4 StageBuf[2][SB][kBlk / 16];
   __shared__ StageBuf lds0, lds1;
-  __shared__ mf_u32x4 ldsq[kQLds ? NW * 32 * 16 : 1];   // [wave][row][chunk ^ row % 16]
+  __shared__ mf_u32x4 ldsq[kQLds ? NW * 32 * QC : 1];   // [wave][row][chunk ^ row % QC]
 
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -250,7 +258,7 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
 
   dma_stage(st0, lds0);                     // (on its way before the query rows)
   mf_u32x4 qop[NQ];
-  mf_u32x4* qs = &ldsq[kQLds ? (wave * 32 + jr) * 16 : 0];
+  mf_u32x4* qs = &ldsq[kQLds ? (wave * 32 + jr) * QC : 0];
   {
     const char* qp = p.q + (int64_t)(tl.first + (row_ok ? row : 0)) * p.q_tok + hq * p.q_head;
 #pragma unroll
@@ -258,7 +266,7 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
       const mf_u32x4 w = *reinterpret_cast<const mf_u32x4*>(qp + 16 * (2 * i + hh));
       const mf_u32x4 x = row_ok ? w ^ p.q_sign : mf_u32x4{0u, 0u, 0u, 0u};
       if (i < NQ) qop[i < NQ ? i : 0] = x;
-      else qs[(2 * (i - NQ) + hh) ^ (jr & 15)] = x;     // (read by this wave alone)
+      else qs[(2 * (i - NQ) + hh) ^ (jr % QC)] = x;     // (read by this wave alone)
     }
   }
   const int g_a = jr >> 3, h_a = (jr >> 2) & 1, t_a = jr & 3;
@@ -267,14 +275,14 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
   const int nl = lane & 15;
   // Byte offsets of a step's operands in its stage buffer: the swizzle is an XOR below the
   // row's size, so every operand lies at one offset XOR a constant.  (D = 256 does that
-  // anew for each read: kept in registers, 24 offsets would push others to memory.)
+  // anew for each read: kept in registers, 24 offsets pushed others to memory.)
   const int k_off = kblk * kBlk + ktok * kRow + 16 * (hh ^ swz<D>(ktok));
   const int v_tok0 = 8 * hh + (nl >> 2);
   const int v_off = v_tok0 * kRow + 16 * ((2 * (jr >> 4) + ((nl & 3) >> 1)) ^ swz<D>(v_tok0)) +
                     8 * (nl & 1);
-  const int q_off = 16 * (hh ^ (jr & 15));
+  const int q_off = 16 * (hh ^ (jr % QC));
   auto anew = [](int off) {
-    if constexpr (kQLds) asm volatile("" : "+v"(off));
+    if constexpr (PromptShape<D>::kAnew) asm volatile("" : "+v"(off));
     return off;
   };
   auto k_operand = [&](const StageBuf& cur, int bp, int i, int off) {
@@ -301,7 +309,7 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
                                 : *reinterpret_cast<const mf_u32x4*>(
                                       reinterpret_cast<const char*>(qs) + (qo ^ (32 * (i - NQ))));
       sc = M32::mma(k_operand(cur, bp, i, ko), q, sc);
-      if (kQLds && i % 4 == 3) __builtin_amdgcn_sched_barrier(0);   // (few operands ahead)
+      if (PromptShape<D>::kAnew && i % 4 == 3) __builtin_amdgcn_sched_barrier(0);   // (few operands ahead)
     }
     float x[16];
 #pragma unroll
@@ -387,7 +395,7 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
           }
         }
         o[e] = M32::mma(vop, pop, o[e]);
-        if (kQLds && e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+        if (PromptShape<D>::kAnew && e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
       }
     }
   };
@@ -444,12 +452,12 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
   // The rows leave through LDS, each wave's in a part of its own (chunk c of row r at
   // slot c ^ r, so that neither side meets bank conflicts): 16 bytes a lane, whole rows
   // a store.  (Straight from the registers a row's lines went out in 16-byte pieces, which
-  // bound short prompts: EPILOGUE.)
+  // bound short prompts: 14 of 512 tokens, 40 heads of 128, 89 -> 72 us.)
   const float l = lsum + __shfl_xor(lsum, 32, 64);
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  // (D = 256: half a row at a time, where the query's half was)
+  // (with the query's half in LDS: half a row at a time, where that was)
   constexpr int kHalves = kQLds ? 2 : 1, EH = NE / kHalves, CH = CPR / kHalves;
-  char* rows = kQLds ? reinterpret_cast<char*>(&ldsq[wave * 32 * 16])
+  char* rows = kQLds ? reinterpret_cast<char*>(&ldsq[wave * 32 * QC])
                      : reinterpret_cast<char*>(&lds0[0][0][0]) + wave * (32 * kRow);
   char* op = p.out + (int64_t)(tl.first + row_w) * p.o_tok + hq * p.o_head + 16 * (lane % CH);
 #pragma unroll
@@ -475,7 +483,7 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
 }
 
 template <typename T, int D, bool kCap, bool kWindow>
-__global__ __launch_bounds__(64 * PromptShape<D>::kWaves, 2) void prompt_attn_kernel(PromptParams p) {
+__global__ __launch_bounds__(64 * PromptShape<D>::kWaves, PromptShape<D>::kPerSimd) void prompt_attn_kernel(PromptParams p) {
   prompt_body<T, D, kCap, kWindow>(p);
 }
 
