@@ -27,6 +27,7 @@ int report_error(int code, const std::string& msg);
 namespace {
 
 constexpr int kThreads4 = 256;
+constexpr int kRowsLaunch = 1 << 24;   // rows of a launch (its threads stay below 2^32)
 
 constexpr int kRowsPer = 2;         // consecutive rows of a thread
 
@@ -280,12 +281,20 @@ int rows_call(bool write, const char* name, void* pool, int64_t n_slots, int pag
   a.v_tok = v_tok;
   a.v_head = v_head;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  if (dtype == HELM_F16) launch_rows_d<f16_t>(write, D, a, st);
-  else if (dtype == HELM_BF16) launch_rows_d<bf16_t>(write, D, a, st);
-  else launch_rows_d<float>(write, D, a, st);
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess)
-    return report_error((int)e, std::string(name) + " launch: " + hipGetErrorString(e));
+  for (int n0 = 0; n0 < n_tok; n0 += kRowsLaunch) {
+    P4Rows part = a;
+    part.n_tok = std::min(kRowsLaunch, n_tok - n0);
+    part.slots += n0;
+    part.k += n0 * k_tok * eb;
+    part.v += n0 * v_tok * eb;
+    if (dtype == HELM_F16) launch_rows_d<f16_t>(write, D, part, st);
+    else if (dtype == HELM_BF16) launch_rows_d<bf16_t>(write, D, part, st);
+    else launch_rows_d<float>(write, D, part, st);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess)
+      return report_error((int)e, std::string(name) + " launch: " + hipGetErrorString(e));
+    if (n_tok - n0 <= kRowsLaunch) break;
+  }
   return HELM_OK;
 }
 

@@ -587,16 +587,19 @@ struct P4Plan {
   int splits, row_tiles;
   size_t parts, bytes;
 };
-// Splits (grid.x) from the widest table: two workgroups a CU over the whole launch
-// (64 k x 4: 53.2 us, one a CU 55.8; 32 k: 14.6, 14.1), at least one per 128 blocks, so
-// that a long sequence of a ragged batch does not trail behind, and no more workgroups
-// than that gains from (their partials are 16 rows each).  A split has a block a wave.
+// Splits (grid.x) from the widest table: a workgroup a CU over the whole launch, two
+// where a wave would still have eight blocks or more (64 k x 4 sequences: 53.2 us against
+// 55.8 with one; 32 k, one sequence, 14.6 against 14.1, whose joining kernel has half the
+// partials); at least one per 128 blocks, so that a long sequence of a ragged batch does
+// not trail behind, and no more workgroups than that gains from (their partials are 16
+// rows each).  A split has a block a wave.
 P4Plan p4_plan(int B, int Hq, int Hkv, int S, int D, int max_pages, int page_size) {
   P4Plan p{};
   const int64_t blocks = ((int64_t)max_pages * (page_size / kP4Tok) + 1) / 2;
   p.row_tiles = ((int64_t)(Hq / Hkv) * S + kP4Rows - 1) / kP4Rows;
   const int64_t wgs = (int64_t)B * Hkv * p.row_tiles;
-  int64_t n = std::max<int64_t>(512 / wgs, (blocks + 127) / 128);
+  const int64_t target = wgs * blocks >= 512 * kP4Waves * 8 ? 512 : 256;
+  int64_t n = std::max<int64_t>(target / wgs, (blocks + 127) / 128);
   n = std::min<int64_t>(n, 16384 / wgs);
   n = std::min<int64_t>(n, (blocks + kP4Waves - 1) / kP4Waves);
   p.splits = (int)std::max<int64_t>(1, n);
@@ -636,7 +639,7 @@ extern "C" int helm_pool4_decode_attn(const void* q, void* out, const void* pool
   if (D != 64 && D != 128 && D != 256)
     return report_error(HELM_E_UNSUPPORTED, "a 4-bit pool has head_dim 64, 128 or 256");
   if (!p4_shape_ok(B, Hq, Hkv, q_len, max_pages, page_size) || n_slots < 0 ||
-      n_slots > 0x7fffffff || table_stride < max_pages)
+      n_slots > 0x7fffffff || table_stride < 0)
     return report_error(HELM_E_INVALID, "bad 4-bit decode shape");
   if (mask && mask_dtype != HELM_F32 && mask_dtype != HELM_BF16 && mask_dtype != HELM_F16)
     return report_error(HELM_E_INVALID, "unknown mask dtype");

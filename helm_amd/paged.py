@@ -203,11 +203,12 @@ def batch_tables(new_lens: torch.Tensor, cached_lens: torch.Tensor, page_table: 
     if not (new_lens.is_contiguous() and cached_lens.is_contiguous()
             and free_slots.is_contiguous()):
         raise ValueError("new_lens, cached_lens and free_slots must be contiguous")
-    if B < 1 or B > 4096 or page_size < 1 or max_tokens < 0:
+    if not (1 <= B <= 4096 and 1 <= page_size < 2 ** 31 and 0 <= max_tokens < 2 ** 31
+            and free_slots.numel() < 2 ** 31):
         raise ValueError("batch_tables takes 1 to 4096 sequences, page_size >= 1, max_tokens >= 0")
     if out is None:
         idx = _engine.common_device("batch_tables", new_lens, cached_lens, page_table, free_slots)
-        cu, seq, taken = new_lens.new_empty(2 * B + 2).split((B + 1, B, 1))
+        cu, seq, taken = new_lens.new_empty(2 * B + 2).split_with_sizes((B + 1, B, 1))
         pos, slot = new_lens.new_empty((2, max_tokens), dtype=torch.int64).unbind(0)
         out = BatchTables(cu, pos, slot, seq, taken)
     else:

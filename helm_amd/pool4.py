@@ -30,7 +30,7 @@ class Pool4:
     """`n_slots` pages of `page_size` tokens (a multiple of 16) of `num_kv_heads` heads
     of `head_dim` 64, 128 or 256, in 4 bits.  ``data`` is the storage, uint8
     ``[n_slots, Hkv, page_size / 16, 17 * head_dim]``; what its bytes mean is the
-    library's affair."""
+    library's affair (copying whole slots of it moves pages)."""
 
     def __init__(self, n_slots: int, num_kv_heads: int, head_dim: int, page_size: int = 16,
                  device="cuda"):
@@ -42,12 +42,16 @@ class Pool4:
             raise ValueError("page_size must be a multiple of 16")
         self.n_slots, self.num_kv_heads = n_slots, num_kv_heads
         self.head_dim, self.page_size = head_dim, page_size
-        self.data = torch.zeros((n_slots, num_kv_heads, page_size // 16, 17 * head_dim),
+        self._data = torch.zeros((n_slots, num_kv_heads, page_size // 16, 17 * head_dim),
                                 dtype=torch.uint8, device=device)
 
-        self._idx = self.data.get_device()
         # the C-ABI's leading arguments of a write or read
-        self._shape = (self.data.data_ptr(), n_slots, page_size, num_kv_heads, head_dim)
+        self._shape = (self._data.data_ptr(), n_slots, page_size, num_kv_heads, head_dim)
+
+    @property
+    def data(self) -> torch.Tensor:
+        """The storage (one tensor for the pool's life)."""
+        return self._data
 
     def _slots(self, slot_map: torch.Tensor) -> int:
         if slot_map.dtype != torch.int64:
@@ -69,7 +73,7 @@ class Pool4:
         if code is None or v.dtype != k.dtype:
             raise TypeError("k and v must share float16, bfloat16 or float32")
         _engine.refuse_grad("Pool4.write", k, v)
-        idx = _engine.common_device("Pool4.write", self.data, k, v, slot_map)
+        idx = _engine.common_device("Pool4.write", self._data, k, v, slot_map)
         k, v = _aligned_rows(k), _aligned_rows(v)
         ks, vs = k.stride(), v.stride()
         _engine.launch_on(idx, "helm_pool4_write", *self._shape, slot_map.data_ptr(), n,
@@ -83,7 +87,7 @@ class Pool4:
         code = _CODES.get(dtype)
         if code is None:
             raise TypeError("values are read as float16, bfloat16 or float32")
-        idx = _engine.common_device("Pool4.read", self.data, slot_map)
+        idx = _engine.common_device("Pool4.read", self._data, slot_map)
         H, D = self.num_kv_heads, self.head_dim
         k, v = slot_map.new_empty((2, n, H, D), dtype=dtype).unbind(0)
         _engine.launch_on(idx, "helm_pool4_read", *self._shape, slot_map.data_ptr(), n,
@@ -215,7 +219,7 @@ def _decode_args(q, pool, page_table, seq_lens, max_pages, scale, softcap, mask,
     # (a call of its own takes a workspace of its own: calls on other streams, captured ones)
     ws = torch.empty(need, dtype=torch.uint8, device=q.device)
     args = (q.data_ptr(), out.data_ptr(), pool.data.data_ptr(), pool.n_slots, pool.page_size,
-            page_table.data_ptr(), max(page_table.stride(0), max_pages), max_pages,
+            page_table.data_ptr(), page_table.stride(0), max_pages,
             seq_lens.data_ptr(), B, Hq, pool.num_kv_heads, S, D, scale, cap,
             m.data_ptr() if m is not None else None, *ms, width,
             _CODES[m.dtype] if m is not None else _native.HELM_F32, int(bool(causal)),

@@ -199,6 +199,22 @@ def test_long_context_and_splits():
     _assert_close(c, out, heads=[0, 3, 7])
 
 
+@pytest.mark.parametrize("B,D,t,S", [(16384, 64, 4400, 1), (16384, 256, 4400, 1), (8192, 128, 12350, 1)])
+def test_many_sequences_of_long_contexts(B, D, t, S):
+    """So many sequences that a split holds more blocks than a wave looks up at once; they
+    share one context's pages (a table row expanded) and end at different tokens."""
+    c = _case(D, [t], 1, 1, D, S, 16, torch.bfloat16)
+    q = (1.5 * _randn(77, B, 1, S, D)).to(torch.bfloat16)
+    table = c["table"].expand(B, -1)
+    assert table.stride(0) == 0
+    lens = (t - torch.arange(B, device=DEV) % 97).to(torch.int32)
+    out = pool4.pool4_decode_attention(q, c["pool"], table, lens)
+    for b in (0, 1, 50, B // 2, B - 1):
+        n = int(lens[b])
+        d = dict(q=q[b:b + 1], ks=[c["ks"][0][:n]], vs=[c["vs"][0][:n]])
+        _assert_close(d, out[b:b + 1])
+
+
 @pytest.mark.parametrize("mdt", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("D,S,cap", [(64, 1, 0.0), (128, 1, 30.0), (256, 4, 50.0), (128, 3, 0.0)])
 def test_masks_and_softcap(mdt, D, S, cap):

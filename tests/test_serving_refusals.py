@@ -32,6 +32,7 @@ def _tables(B=2, width=4, **kw):
     (dict(max_tokens=-1), ValueError),
     (dict(new_lens=torch.ones(4097, dtype=I32), cached_lens=torch.zeros(4097, dtype=I32),
           page_table=torch.zeros((4097, 1), dtype=I32)), ValueError),
+    (dict(max_tokens=2 ** 31), ValueError), (dict(page_size=2 ** 31), ValueError),
     ({}, RuntimeError),            # CPU tensors
 ])
 def test_batch_tables_refusals(bad, err):
@@ -177,7 +178,7 @@ def test_c_entries_refuse_before_device_work():
         return lib.helm_pool4_decode_attn(q, p, p, 1, page, p, ts, mp, p, B, Hq, Hkv, S, D, 1.0, 0.0,
                                           mask, 0, 0, 0, ml, mdt, 0, dt, ws, wb, None)
     assert attn(D=80) == U and attn(dt=F32) == U and attn(page=20) == E and attn(Hq=3, Hkv=2) == E
-    assert attn(S=0) == E and attn(mp=2) == E and attn(p=None) == E and attn(q=8) == E
+    assert attn(S=0) == E and attn(ts=-1) == E and attn(p=None) == E and attn(q=8) == E
     assert attn(mask=16, ml=0) == E and attn(mask=16, ml=4, mdt=7) == E
     assert attn(mp=4096, ts=4096) == W and attn(B=0) == 0
     assert lib.helm_pool4_workspace_bytes(1, 2, 1, 1, 64, 4096, 16) > 0
