@@ -171,6 +171,13 @@ __device__ __forceinline__ PromptTile prompt_tile_in_order(const PromptParams& p
   return {-1, 0, 0, j - base};
 }
 
+// Rows of CH 16-byte chunks in LDS (half a query row, an output row on its way out): chunk
+// c of row r sits at slot c ^ out_swz(r), so that 16 lanes that read one chunk of 16 rows,
+// or write one, meet every bank group once (rows of 128 bytes: two share 256).
+template <int CH> __device__ __forceinline__ int out_swz(int r) {
+  return CH == 8 ? (r >> 1) & 7 : r & (CH - 1);
+}
+
 template <typename T> __device__ __forceinline__ uint32_t nonfinite_halves(uint32_t w) {
   constexpr uint32_t kExp = std::is_same<T, bf16_t>::value ? 0x7f80u : 0x7c00u;
   uint32_t r = 0;
@@ -198,7 +205,7 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
   using M32 = Mfma32<T>;
   typedef mf_u32x4 StageBuf[2][SB][kBlk / 16];
   __shared__ StageBuf lds0, lds1;
-  __shared__ mf_u32x4 ldsq[kQLds ? NW * 32 * QC : 1];   // [wave][row][chunk ^ row % QC]
+  __shared__ mf_u32x4 ldsq[kQLds ? NW * 32 * QC : 1];   // [wave][row][slot]
 
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -266,7 +273,7 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
       const mf_u32x4 w = *reinterpret_cast<const mf_u32x4*>(qp + 16 * (2 * i + hh));
       const mf_u32x4 x = row_ok ? w ^ p.q_sign : mf_u32x4{0u, 0u, 0u, 0u};
       if (i < NQ) qop[i < NQ ? i : 0] = x;
-      else qs[(2 * (i - NQ) + hh) ^ (jr % QC)] = x;     // (read by this wave alone)
+      else qs[(2 * (i - NQ) + hh) ^ out_swz<QC>(jr)] = x;     // (read by this wave alone)
     }
   }
   const int g_a = jr >> 3, h_a = (jr >> 2) & 1, t_a = jr & 3;
@@ -280,7 +287,7 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
   const int v_tok0 = 8 * hh + (nl >> 2);
   const int v_off = v_tok0 * kRow + 16 * ((2 * (jr >> 4) + ((nl & 3) >> 1)) ^ swz<D>(v_tok0)) +
                     8 * (nl & 1);
-  const int q_off = 16 * (hh ^ (jr % QC));
+  const int q_off = 16 * (hh ^ out_swz<QC>(jr));
   auto anew = [](int off) {
     if constexpr (PromptShape<D>::kAnew) asm volatile("" : "+v"(off));
     return off;
@@ -449,9 +456,8 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
     __syncthreads();
   }
 
-  // The rows leave through LDS, each wave's in a part of its own (chunk c of row r at
-  // slot c ^ r, so that neither side meets bank conflicts): 16 bytes a lane, whole rows
-  // a store.  (Straight from the registers a row's lines went out in 16-byte pieces, which
+  // The rows leave through LDS, each wave's in a part of its own: 16 bytes a lane, whole
+  // rows a store.  (Straight from the registers a row's lines went out in 16-byte pieces, which
   // bound short prompts: 14 of 512 tokens, 40 heads of 128, 89 -> 72 us.)
   const float l = lsum + __shfl_xor(lsum, 32, 64);
   const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -467,7 +473,7 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const mf_f32x16& oe = o[half * EH + e];
-        *reinterpret_cast<uint2*>(rows + jr * (16 * CH) + 16 * ((4 * e + g) ^ (jr % CH)) + 8 * hh) =
+        *reinterpret_cast<uint2*>(rows + jr * (16 * CH) + 16 * ((4 * e + g) ^ out_swz<CH>(jr)) + 8 * hh) =
             make_uint2(Ops::pk(oe[4 * g] * inv, oe[4 * g + 1] * inv),
                        Ops::pk(oe[4 * g + 2] * inv, oe[4 * g + 3] * inv));
       }
@@ -475,7 +481,7 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
     for (int i = 0; i < 32 * CH / 64; ++i) {
       const int r = (64 / CH) * i + lane / CH;
       const mf_u32x4 w =
-          *reinterpret_cast<const mf_u32x4*>(rows + r * (16 * CH) + 16 * ((lane % CH) ^ (r % CH)));
+          *reinterpret_cast<const mf_u32x4*>(rows + r * (16 * CH) + 16 * ((lane % CH) ^ out_swz<CH>(r)));
       if (row_w + r < tl.len)
         *reinterpret_cast<mf_u32x4*>(op + r * p.o_tok + 16 * CH * half) = w;
     }
