@@ -94,7 +94,8 @@ template <typename T> __device__ __forceinline__ void load8(const char* p, int64
   }
 }
 
-template <typename T> __device__ __forceinline__ void store8(char* p, int64_t elem, const float* x) {
+template <typename T>
+__device__ __forceinline__ void store8(char* p, int64_t elem, const float* x) {
   if constexpr (std::is_same<T, float>::value) {
     reinterpret_cast<float4*>(p + 4 * elem)[0] = make_float4(x[0], x[1], x[2], x[3]);
     reinterpret_cast<float4*>(p + 4 * elem)[1] = make_float4(x[4], x[5], x[6], x[7]);
@@ -252,7 +253,8 @@ int rows_call(bool write, const char* name, void* pool, int64_t n_slots, int pag
     return report_error(HELM_E_INVALID, "unknown dtype");
   if (D != 64 && D != 128 && D != 256)
     return report_error(HELM_E_UNSUPPORTED, "a 4-bit pool has head_dim 64, 128 or 256");
-  if (n_slots < 0 || page_size < kP4Tok || page_size % kP4Tok || Hkv < 1 || Hkv > 65535 || n_tok < 0)
+  if (n_slots < 0 || page_size < kP4Tok || page_size % kP4Tok || Hkv < 1 || Hkv > 65535 ||
+      n_tok < 0)
     return report_error(HELM_E_INVALID,
                         "bad 4-bit pool shape (page_size a multiple of 16, 1 to 65535 heads)");
   if (n_tok == 0) return HELM_OK;

@@ -29,7 +29,7 @@
 // Hidden tokens (past the sequence's length, past the causal limit, or under a
 // mask of -inf) take no part whatever their K and V hold: their scores are
 // overwritten, and where V's group stands for NaN the products take zeros there
-// and the NaN is put into the rows that weigh such a token (block_nan).
+// and the NaN is put into the rows that weigh such a token.
 // A row with nothing visible is zeros.
 #include <algorithm>
 #include <string>
@@ -124,12 +124,13 @@ __device__ __forceinline__ P4Raw<D> p4_load(const char* tile, bool there, int n,
   return r;
 }
 
+// The two codes of byte B of w, or all eight, times s, as bf16 (exact).
+template <int B> __device__ __forceinline__ uint32_t p4_decode2(uint32_t w, float s) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, B));
+}
 __device__ __forceinline__ mf_u32x4 p4_decode8(uint32_t w, float s) {
-  return mf_u32x4{
-      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0)),
-      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1)),
-      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 2)),
-      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3))};
+  return mf_u32x4{p4_decode2<0>(w, s), p4_decode2<1>(w, s), p4_decode2<2>(w, s),
+                  p4_decode2<3>(w, s)};
 }
 // Pair c (dims 2c, 2c + 1 of the lane's chunk) of token j of a tile's four.
 template <int D>
@@ -138,10 +139,10 @@ __device__ __forceinline__ uint32_t p4_v_pair(const P4Raw<D>& r, int j, int c, f
   const int byte = j * PB + c;
   const uint32_t w = r.v[byte >> 2];
   switch (byte & 3) {
-    case 0: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0));
-    case 1: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1));
-    case 2: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 2));
-    default: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3));
+    case 0: return p4_decode2<0>(w, s);
+    case 1: return p4_decode2<1>(w, s);
+    case 2: return p4_decode2<2>(w, s);
+    default: return p4_decode2<3>(w, s);
   }
 }
 
@@ -649,7 +650,8 @@ extern "C" int helm_pool4_decode_attn(const void* q, void* out, const void* pool
     return report_error(HELM_E_INVALID, "null pointer argument");
   if ((reinterpret_cast<uint64_t>(q) | reinterpret_cast<uint64_t>(pool) |
        reinterpret_cast<uint64_t>(out) | reinterpret_cast<uint64_t>(workspace)) & 15)
-    return report_error(HELM_E_INVALID, "q, out, the pool and the workspace must be 16-byte aligned");
+    return report_error(HELM_E_INVALID,
+                        "q, out, the pool and the workspace must be 16-byte aligned");
   const P4Plan pl = p4_plan(B, Hq, Hkv, q_len, D, max_pages, page_size);
   if (pl.bytes && (!workspace || ws_bytes < pl.bytes))
     return report_error(HELM_E_WORKSPACE, "workspace too small: need " + std::to_string(pl.bytes));

@@ -244,9 +244,9 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
   const char* kb = p.k + tl.first * p.k_tok + hk * p.k_head;
   const char* vb = p.v + tl.first * p.v_tok + hk * p.v_head;
   // this wave's loads of a stage straight into LDS: load i of the stage's is part u of
-  // i / kBlkLoads, a block's K, then its V, then the next block's; lane l of it fetches the chunk that the
-  // swizzle (attn_chunk32.h) keeps in slot 64 u + l; tokens past the sequence's end come
-  // in as zeros
+  // i / kBlkLoads, a block's K, then its V, then the next block's; lane l of it fetches the
+  // chunk that the swizzle (attn_chunk32.h) keeps in slot 64 u + l; tokens past the
+  // sequence's end come in as zeros
   auto dma_stage = [&](int st, StageBuf& dst) {
 #pragma unroll
     for (int k = 0; k < kLoads; ++k) {
@@ -316,7 +316,8 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
                                 : *reinterpret_cast<const mf_u32x4*>(
                                       reinterpret_cast<const char*>(qs) + (qo ^ (32 * (i - NQ))));
       sc = M32::mma(k_operand(cur, bp, i, ko), q, sc);
-      if (PromptShape<D>::kAnew && i % 4 == 3) __builtin_amdgcn_sched_barrier(0);   // (few operands ahead)
+      // (few operands ahead)
+      if (PromptShape<D>::kAnew && i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
     }
     float x[16];
 #pragma unroll
@@ -473,15 +474,16 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const mf_f32x16& oe = o[half * EH + e];
-        *reinterpret_cast<uint2*>(rows + jr * (16 * CH) + 16 * ((4 * e + g) ^ out_swz<CH>(jr)) + 8 * hh) =
+        const int slot = (4 * e + g) ^ out_swz<CH>(jr);
+        *reinterpret_cast<uint2*>(rows + jr * (16 * CH) + 16 * slot + 8 * hh) =
             make_uint2(Ops::pk(oe[4 * g] * inv, oe[4 * g + 1] * inv),
                        Ops::pk(oe[4 * g + 2] * inv, oe[4 * g + 3] * inv));
       }
 #pragma unroll
     for (int i = 0; i < 32 * CH / 64; ++i) {
       const int r = (64 / CH) * i + lane / CH;
-      const mf_u32x4 w =
-          *reinterpret_cast<const mf_u32x4*>(rows + r * (16 * CH) + 16 * ((lane % CH) ^ out_swz<CH>(r)));
+      const int slot = (lane % CH) ^ out_swz<CH>(r);
+      const mf_u32x4 w = *reinterpret_cast<const mf_u32x4*>(rows + r * (16 * CH) + 16 * slot);
       if (row_w + r < tl.len)
         *reinterpret_cast<mf_u32x4*>(op + r * p.o_tok + 16 * CH * half) = w;
     }
@@ -489,7 +491,8 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
 }
 
 template <typename T, int D, bool kCap, bool kWindow>
-__global__ __launch_bounds__(64 * PromptShape<D>::kWaves, PromptShape<D>::kPerSimd) void prompt_attn_kernel(PromptParams p) {
+__global__ __launch_bounds__(64 * PromptShape<D>::kWaves, PromptShape<D>::kPerSimd)
+void prompt_attn_kernel(PromptParams p) {
   prompt_body<T, D, kCap, kWindow>(p);
 }
 

@@ -67,7 +67,8 @@ extern "C" int helm_prompt_attn(const void* q, int64_t q_tok_stride, int64_t q_h
   p.window = window;
   p.zero_rest = zero_rest;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  const hipError_t e = dtype == HELM_BF16 ? launch_prompt_bf16(p, D, st) : launch_prompt_f16(p, D, st);
+  const hipError_t e =
+      dtype == HELM_BF16 ? launch_prompt_bf16(p, D, st) : launch_prompt_f16(p, D, st);
   if (e != hipSuccess)
     return report_error((int)e, std::string("prompt attention launch: ") + hipGetErrorString(e));
   return HELM_OK;

@@ -96,9 +96,10 @@ class Pool4:
 
 
 def _aligned_rows(x: torch.Tensor) -> torch.Tensor:
-    """x [n, H, D] itself where its rows are dense and 16-byte aligned, else a copy."""
+    """x [n, H, D] itself where its rows are dense, 16-byte aligned and less than 2^25 elements
+    apart (the kernels' addressing), else a copy."""
     s, unit = x.stride(), 16 // x.element_size()
-    if s[2] != 1 or s[0] % unit or s[1] % unit or x.data_ptr() % 16:
+    if s[2] != 1 or s[0] % unit or s[1] % unit or s[0] > 1 << 25 or x.data_ptr() % 16:
         x = torch.empty(x.shape, dtype=x.dtype, device=x.device).copy_(x)
     return x
 
@@ -132,8 +133,8 @@ def prepare_pool4_decode(q: torch.Tensor, pool: Pool4, page_table: torch.Tensor,
     if m is not None and (m.dtype not in _CODES or m.stride(-1) != 1):
         raise ValueError("a prepared call reads the mask in place: float32, bfloat16 or "
                          "float16 with dense rows")
-    return PreparedPool4Decode(*_decode_args(q, pool, page_table, seq_lens, max_pages, scale, softcap,
-                                             attention_mask, causal, out, in_place=True))
+    return PreparedPool4Decode(*_decode_args(q, pool, page_table, seq_lens, max_pages, scale,
+                                             softcap, attention_mask, causal, out, in_place=True))
 
 
 def pool4_decode_attention(q: torch.Tensor, pool: Pool4, page_table: torch.Tensor,
@@ -142,7 +143,8 @@ def pool4_decode_attention(q: torch.Tensor, pool: Pool4, page_table: torch.Tenso
                            attention_mask: Optional[torch.Tensor] = None, causal: bool = False,
                            out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of q [B, Hq, q_len, D] (float16 or bfloat16) over 4-bit pages, the
-    arguments of ``paged.paged_decode_attention``.
+    arguments of ``paged.paged_decode_attention``; made for single tokens and a few drafts
+    (every 16 query rows of a KV head read its pages again).
 
     page_table: int32 [B, >= max_pages] slots of the pool (others count as hidden
     pages); seq_lens: int32 [B] tokens, on the device; attention_mask: additive

@@ -50,8 +50,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     idx = _engine.common_device("prompt_attention", q, k, v, cu_seqlens, out)
     q, k, v = _aligned_rows(q), _aligned_rows(k), _aligned_rows(v)
     sq, sk, sv = q.stride(), k.stride(), v.stride()
-    _engine.launch_on(idx, "helm_prompt_attn", q.data_ptr(), sq[0], sq[1], k.data_ptr(), sk[0], sk[1],
-                      v.data_ptr(), sv[0], sv[1], out.data_ptr(), Hq * D, D,
+    _engine.launch_on(idx, "helm_prompt_attn", q.data_ptr(), sq[0], sq[1], k.data_ptr(), sk[0],
+                      sk[1], v.data_ptr(), sv[0], sv[1], out.data_ptr(), Hq * D, D,
                       cu_seqlens.data_ptr(), B, N, Hq, Hkv, D, scale, cap,
                       min(window or 0, 0x7fffffff), rest, _CODES[dt])
     return out

@@ -77,3 +77,61 @@ def test_prompts_then_decode_steps(dtype, D, page):
         rk, rv = pool.read(slots, dtype=torch.float32)
         assert torch.equal(rk.double(), ks[b]) and torch.equal(rv.double(), vs[b])
     assert math.isfinite(out.float().abs().max().item())
+
+
+def test_a_captured_step():
+    """A decode step of every operator in one graph, replayed with other lengths, tables, free
+    slots and tokens: each replay equals the calls made one by one."""
+    B, Hq, Hkv, D, page, width, n_slots = 4, 8, 2, 128, 16, 12, 64
+    r = random.Random(5)
+    g = torch.Generator(device=DEV).manual_seed(5)
+    i32 = dict(dtype=torch.int32, device=DEV)
+    one, cached = torch.ones(B, **i32), torch.zeros(B, **i32)
+    table, free = torch.zeros((B, width), **i32), torch.zeros(n_slots, **i32)
+    q = torch.zeros(B, Hq, 1, D, dtype=torch.bfloat16, device=DEV)
+    kv = torch.zeros(2, B, Hkv, D, dtype=torch.bfloat16, device=DEV)
+    pool = pool4.Pool4(n_slots, Hkv, D, page_size=page, device=DEV)
+    t = paged.batch_tables(one, cached, table, free, page, B)
+    res = {}
+
+    def step(tables=None):
+        tb = paged.batch_tables(one, cached, table, free, page, B, out=tables)
+        pool.write(kv[0], kv[1], tb.slot_map)
+        k, v = pool.read(tb.slot_map)
+        own = prompt.prompt_attention(q[:, :, 0], k, v, tb.cu_seqlens)
+        return tb, k, v, own, pool4.pool4_decode_attention(q, pool, table, tb.seq_lens)
+
+    step(t)                                            # (libraries loaded before capture)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        res["out"] = step(t)
+    for i in range(4):
+        slots = list(range(n_slots))
+        r.shuffle(slots)
+        lens = [r.randint(0, width * page - 1) for _ in range(B)]
+        rows, at = [], 0
+        for n in lens:
+            have = -(-n // page)
+            rows.append(slots[at:at + have] + [-1] * (width - have))
+            at += have
+        pool.data.copy_(torch.randint(0, 100, pool.data.shape, generator=g, device=DEV))
+        q.copy_(torch.randn(q.shape, generator=g, device=DEV))
+        kv.copy_(torch.randn(kv.shape, generator=g, device=DEV))
+        rest = slots[at:] + [0] * at
+
+        def inputs():
+            cached.copy_(torch.tensor(lens, **i32))
+            table.copy_(torch.tensor(rows, **i32))
+            free.copy_(torch.tensor(rest, **i32))
+        inputs()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [x.clone() for x in (*res["out"][0], *res["out"][1:], table, pool.data)]
+        inputs()
+        eager = step()
+        torch.cuda.synchronize()
+        for a, b in zip(got, (*eager[0], *eager[1:], table, pool.data)):
+            assert torch.equal(a, b)
+        assert torch.equal(got[7], got[6].repeat_interleave(Hq // Hkv, 1))   # a row alone: its V
+        assert torch.isfinite(got[8].float()).all()
