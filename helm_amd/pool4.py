@@ -74,10 +74,11 @@ class Pool4:
             raise TypeError("k and v must share float16, bfloat16 or float32")
         _engine.refuse_grad("Pool4.write", k, v)
         idx = _engine.common_device("Pool4.write", self._data, k, v, slot_map)
-        k, v = _aligned_rows(k), _aligned_rows(v)
-        ks, vs = k.stride(), v.stride()
-        _engine.launch_on(idx, "helm_pool4_write", *self._shape, slot_map.data_ptr(), n,
-                          k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], code)
+        unit = 4 if code == _native.HELM_F32 else 8
+        k, *k_at = _rows16(k, unit)
+        v, *v_at = _rows16(v, unit)
+        _engine.launch_on(idx, "helm_pool4_write", *self._shape, slot_map.data_ptr(), n, *k_at,
+                          *v_at, code)
 
     def read(self, slot_map: torch.Tensor, dtype: torch.dtype = torch.bfloat16
              ) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -95,13 +96,16 @@ class Pool4:
         return k, v
 
 
-def _aligned_rows(x: torch.Tensor) -> torch.Tensor:
-    """x [n, H, D] itself where its rows are dense, 16-byte aligned and less than 2^25 elements
-    apart (the kernels' addressing), else a copy."""
-    s, unit = x.stride(), 16 // x.element_size()
-    if s[2] != 1 or s[0] % unit or s[1] % unit or s[0] > 1 << 25 or x.data_ptr() % 16:
+def _rows16(x: torch.Tensor, unit: int) -> tuple:
+    """(x, its address, token and head stride): x [n, H, D] itself where its rows are dense,
+    16-byte aligned (multiples of `unit` elements) and less than 2^25 elements apart (the
+    kernels' addressing), else a copy."""
+    s0, s1, s2 = x.stride()
+    at = x.data_ptr()
+    if s2 != 1 or s0 % unit or s1 % unit or s0 > 1 << 25 or at & 15:
         x = torch.empty(x.shape, dtype=x.dtype, device=x.device).copy_(x)
-    return x
+        (s0, s1, _), at = x.stride(), x.data_ptr()
+    return x, at, s0, s1
 
 
 class PreparedPool4Decode:

@@ -7,7 +7,7 @@ from typing import Optional
 
 import torch
 
-from helm_amd.pool4 import _CODES, _aligned_rows, check_scores
+from helm_amd.pool4 import _CODES, _rows16, check_scores
 from helm_amd.runtime import engine as _engine
 
 
@@ -48,10 +48,10 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         raise ValueError("out must be contiguous, of q's shape and dtype")
     _engine.refuse_grad("prompt_attention", q, k, v)
     idx = _engine.common_device("prompt_attention", q, k, v, cu_seqlens, out)
-    q, k, v = _aligned_rows(q), _aligned_rows(k), _aligned_rows(v)
-    sq, sk, sv = q.stride(), k.stride(), v.stride()
-    _engine.launch_on(idx, "helm_prompt_attn", q.data_ptr(), sq[0], sq[1], k.data_ptr(), sk[0],
-                      sk[1], v.data_ptr(), sv[0], sv[1], out.data_ptr(), Hq * D, D,
+    q, *q_at = _rows16(q, 8)
+    k, *k_at = _rows16(k, 8)
+    v, *v_at = _rows16(v, 8)
+    _engine.launch_on(idx, "helm_prompt_attn", *q_at, *k_at, *v_at, out.data_ptr(), Hq * D, D,
                       cu_seqlens.data_ptr(), B, N, Hq, Hkv, D, scale, cap,
                       min(window or 0, 0x7fffffff), rest, _CODES[dt])
     return out
