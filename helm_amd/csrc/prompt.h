@@ -4,9 +4,9 @@
 //
 // Bound by the matrix cores: 4 D operations a visible (row, head) pair against
 // 8 bytes a row and head dim.  A workgroup owns 128 rows of one query head, a wave
-// 32 of them (D = 256: 256 rows); it walks the keys in stages, whose K and V go straight
-// from memory into LDS (two stage buffers, one barrier a stage), and computes 32
-// tokens a step.  Lane l = 32 hh + jr owns query row jr:
+// 32 of them (D = 256: 256 rows; few tiles: 32 rows in all, PromptSplit); it walks the
+// keys in stages, whose K and V go straight from memory into LDS (two stage buffers,
+// one barrier a stage), and computes 32 tokens a step.  Lane l = 32 hh + jr owns query row jr:
 //   S^T = K Q^T  (v_mfma_f32_32x32x16): A is K of token tau(jr), B query row jr; with
 //         tau(8g + 4h + t) = 16 (g >> 1) + 8h + 4 (g & 1) + t the lane gets row jr's
 //         scores of tokens 8 hh .. 8 hh + 7 of both 16-token blocks of the step,
@@ -26,6 +26,7 @@
 // and NaN taken out of the products and added where a row weighs them (careful).
 #pragma once
 
+#include <cfloat>
 #include <type_traits>
 
 #include "attn_chunk32.h"
@@ -60,6 +61,26 @@ struct PromptParams {
   int window;          // <= 0: off
   int zero_rest;
 };
+
+// Few row tiles: the longest walk of one wave would be the launch's time.  There a workgroup
+// owns 32 rows: its waves deal the steps of their walk out among them, each through K and V
+// buffers of its own (no barrier in the walk), and join their sums at the end.  Every
+// workgroup then loads K and V for 32 rows, not 128 or 256, so this is for launches that
+// leave CUs idle: up to 512 such tiles (times heads), which are resident together (one a
+// CU, two rounds, at D = 256; up to 640 at D = 64, three a CU), or 1,280 where the sequences
+// are 2,048 tokens on average and an extra round's start and join are small beside the walks.  bf16, 8 / 2 heads, us without
+// and with: 1,200 tokens D = 64 20.8 -> 11.7, 128 29.7 -> 16.7, 256 67 -> 28; 4,800 tokens
+// (1,208 tiles) 69 -> 46, 103 -> 80, 241 -> 185.  Beyond, it loses: 4 of 1,200 (1,232 tiles)
+// 22.0 -> 21.4, 32.9 -> 37.0, 72 -> 86; 32 / 8 heads, 4 of 150 (736) 6.7 -> 7.6, 9.3 -> 14.1,
+// 18 -> 30; 600 tokens (640) 13.3 -> 10.0, 19.3 -> 18.2, 37 -> 39.  Eight waves: 8 / 2 heads, 2,400 tokens D = 64 19.8 -> 24.8, D = 128 28 -> 39.
+template <int D> struct PromptSplit {
+  static constexpr int kWaves = 4, kPerSimd = D == 256 ? 1 : 2;
+  static constexpr int kTiles = D == 64 ? 640 : 512, kTilesLong = 1280;
+};
+template <int D> bool prompt_splits(const PromptParams& p) {
+  const int64_t wgs = ((int64_t)(p.N + 31) / 32 + p.B) * p.Hq;
+  return wgs <= (p.N / 2048 >= p.B ? PromptSplit<D>::kTilesLong : PromptSplit<D>::kTiles);
+}
 
 // Sequence b's rows, clamped to the tensors.
 struct PromptSeq {
@@ -186,11 +207,64 @@ template <typename T> __device__ __forceinline__ uint32_t nonfinite_halves(uint3
   return r;
 }
 
-template <typename T, int D, bool kCap, bool kWindow>
+// Joins the waves' sums over 32 rows: a wave's part counts exp2(m - M) of itself, M the
+// largest of the row's maxima (at least the smallest normal number, so that an infinity or NaN
+// in the sums stays one).  Wave w's sums go where
+// its K (the row's first half) and its V were, 64 D bytes each: dims 32 e + 8 g + 4 hh .. + 3 of row r (chunk c = 4 e + g)
+// at 16-byte slot 64 c + 32 hh + (r ^ c % 16), so that writes (a chunk's rows) and reads
+// (a row's chunks) both meet every bank group.
+template <typename T, int D, int NW>
+__device__ __forceinline__ void prompt_join(const PromptParams& p, float m, float lsum,
+                                            mf_f32x16 (&o)[D / 32], mf_u32x4* kbuf, mf_u32x4* vbuf,
+                                            const PromptTile& tl, int hq) {
+  constexpr int CPR = D / 8;
+  __shared__ float tops[NW][32], sums[NW][32];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, jr = lane & 31, hh = lane >> 5;
+  lsum += __shfl_xor(lsum, 32, 64);
+  if (hh == 0) tops[wave][jr] = m;
+  __syncthreads();
+  float top = tops[0][jr];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) top = fmaxf(top, tops[w][jr]);
+  const float f = m == top ? 1.f : fmaxf(__builtin_amdgcn_exp2f(m - top), FLT_MIN);
+  if (hh == 0) sums[wave][jr] = lsum * f;
+  auto at = [&](int w, int c, int h, int r) {
+    return reinterpret_cast<mf_f32x4*>(c < CPR / 2 ? kbuf : vbuf) + 4 * D * w +
+           64 * (c % (CPR / 2)) + 32 * h + (r ^ c % 16);
+  };
+#pragma unroll
+  for (int c = 0; c < CPR; ++c) {
+    mf_f32x4 x;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) x[t] = o[c / 4][4 * (c % 4) + t] * f;
+    *at(wave, c, hh, jr) = x;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 32 * CPR; i += 64 * NW) {
+    const int r = i / CPR, c = i % CPR;
+    if (tl.row + r >= tl.len) break;
+    float l = 0.f;
+    mf_f32x4 a{0.f, 0.f, 0.f, 0.f}, b{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      l += sums[w][r];
+      a += *at(w, c, 0, r);
+      b += *at(w, c, 1, r);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    using Ops = MfmaOps<T>;
+    *reinterpret_cast<mf_u32x4*>(p.out + (int64_t)(tl.first + tl.row + r) * p.o_tok +
+                                 hq * p.o_head + 16 * c) =
+        mf_u32x4{Ops::pk(a[0] * inv, a[1] * inv), Ops::pk(a[2] * inv, a[3] * inv),
+                 Ops::pk(b[0] * inv, b[1] * inv), Ops::pk(b[2] * inv, b[3] * inv)};
+  }
+}
+
+template <typename T, int D, bool kCap, bool kWindow, bool kSplit>
 __device__ __forceinline__ void prompt_body(const PromptParams& p) {
-  constexpr int NW = PromptShape<D>::kWaves;
-  constexpr int kRows = 32 * NW;             // query rows of the workgroup
-  constexpr int kTok = PromptShape<D>::kTok, SB = kTok / kBlockTok;
+  constexpr int NW = kSplit ? PromptSplit<D>::kWaves : PromptShape<D>::kWaves;
+  constexpr int kRows = kSplit ? 32 : 32 * NW;       // query rows of the workgroup
+  constexpr int kTok = kSplit ? 32 : PromptShape<D>::kTok, SB = kTok / kBlockTok;
   constexpr int NK = D / 16, NE = D / 32, CPR = D / 8;
   constexpr int kRow = 2 * D, kBlk = kBlockTok * kRow;
   constexpr int kShift = std::is_same<T, f16_t>::value ? 9 : 0;
@@ -198,13 +272,15 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
   constexpr int kBlkLoads = kBlk / 1024;
   // 16-byte-a-lane loads of a wave and stage: neighbours of one block of K or V, or two
   constexpr int kLoads = 2 * SB * kBlkLoads / NW;
-  constexpr bool kQLds = PromptShape<D>::kQLds;
+  constexpr bool kQLds = PromptShape<D>::kQLds && !kSplit;
+  constexpr bool kAnew = PromptShape<D>::kAnew && !kSplit;
   constexpr int QC = CPR / 2;                // 16-byte chunks of half a query row
   constexpr int NQ = kQLds ? NK / 2 : NK;
   using Ops = MfmaOps<T>;
   using M32 = Mfma32<T>;
   typedef mf_u32x4 StageBuf[2][SB][kBlk / 16];
   __shared__ StageBuf lds0, lds1;
+  __shared__ mf_u32x4 ldsk[kSplit ? NW : 1][SB][kBlk / 16], ldsv[kSplit ? NW : 1][SB][kBlk / 16];
   __shared__ mf_u32x4 ldsq[kQLds ? NW * 32 * QC : 1];   // [wave][row][slot]
 
   const int tid = threadIdx.x;
@@ -228,7 +304,7 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
     }
     return;
   }
-  const int row_w = tl.row + 32 * wave;                  // the wave's first row
+  const int row_w = kSplit ? tl.row : tl.row + 32 * wave;    // the wave's first row
   const int row = row_w + jr;
   const bool row_ok = row < tl.len;
   const bool wave_rows = row_w < tl.len;
@@ -263,7 +339,36 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
     }
   };
 
-  dma_stage(st0, lds0);                     // (on its way before the query rows)
+  // split: the wave's own loads of stage st's K (0) or V (1) alone
+  constexpr int kOwnLoads = SB * kBlkLoads;
+  auto dma_own = [&](int st, int is_v) {
+#pragma unroll
+    for (int blk = 0; blk < SB; ++blk) {
+      const int tok0 = st * kTok + blk * kBlockTok;
+      const int nt = min(max(tl.len - tok0, 0), kBlockTok);
+      const int64_t stride = is_v ? p.v_tok : p.k_tok;
+      const auto rs = make_rsrc((is_v ? vb : kb) + tok0 * stride,
+                                nt ? (nt - 1) * (int)stride + kRow : 0);
+#pragma unroll
+      for (int u = 0; u < kBlkLoads; ++u) {
+        const int t = (64 / CPR) * u + lane / CPR;
+        buf_load16_lds(rs, &(is_v ? ldsv : ldsk)[wave][blk][64 * u],
+                       t * (int)stride + 16 * ((lane % CPR) ^ swz<D>(t)));
+      }
+    }
+  };
+  // (wave barrier of memory: every LDS read so far has returned)
+  auto reads_done = [] {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // all loads into LDS but the youngest kOwnLoads have landed
+  auto older_landed = [&] {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kOwnLoads) : "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+
+  if constexpr (!kSplit) dma_stage(st0, lds0);      // (on its way before the query rows)
   mf_u32x4 qop[NQ];
   mf_u32x4* qs = &ldsq[kQLds ? (wave * 32 + jr) * QC : 0];
   {
@@ -289,23 +394,24 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
                     8 * (nl & 1);
   const int q_off = 16 * (hh ^ out_swz<QC>(jr));
   auto anew = [](int off) {
-    if constexpr (PromptShape<D>::kAnew) asm volatile("" : "+v"(off));
+    if constexpr (kAnew) asm volatile("" : "+v"(off));
     return off;
   };
-  auto k_operand = [&](const StageBuf& cur, int bp, int i, int off) {
-    return *reinterpret_cast<const mf_u32x4*>(reinterpret_cast<const char*>(&cur[0][bp][0]) +
-                                              (off ^ (32 * i)));
+  // (from the first of the step's two blocks of K or V)
+  auto k_operand = [&](const mf_u32x4* kk, int i, int off) {
+    return *reinterpret_cast<const mf_u32x4*>(reinterpret_cast<const char*>(kk) + (off ^ (32 * i)));
   };
-  auto v_operand = [&](const StageBuf& cur, int blk, int z, int e, int off) {
+  auto v_operand = [&](const mf_u32x4* vv, int u, int z, int e, int off) {
     // token v_tok0 + 4 z: the row four further, whose swizzle differs by z's bit
-    return ld_tr16(reinterpret_cast<const char*>(&cur[1][blk][0]) + (off ^ (64 * e) ^ (16 * z)) +
+    return ld_tr16(reinterpret_cast<const char*>(vv) + (off ^ (64 * e) ^ (16 * z)) + u * kBlk +
                    4 * kRow * z);
   };
 
   float m, lsum;
   mf_f32x16 o[NE];
 
-  auto step = [&](auto careful, int tok0, int bp, const StageBuf& cur) {
+  auto step = [&](auto careful, int tok0, const mf_u32x4* kk, const mf_u32x4* vv) {
+    if constexpr (kSplit) older_landed();      // K
     mf_f32x16 sc;
 #pragma unroll
     for (int r = 0; r < 16; ++r) sc[r] = 0.f;
@@ -315,9 +421,13 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
       const mf_u32x4 q = i < NQ ? qop[i < NQ ? i : 0]
                                 : *reinterpret_cast<const mf_u32x4*>(
                                       reinterpret_cast<const char*>(qs) + (qo ^ (32 * (i - NQ))));
-      sc = M32::mma(k_operand(cur, bp, i, ko), q, sc);
+      sc = M32::mma(k_operand(kk, i, ko), q, sc);
       // (few operands ahead)
-      if (PromptShape<D>::kAnew && i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+      if (kAnew && i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (kSplit) {
+      reads_done();
+      dma_own(tok0 / kTok + NW, 0);            // (past the sequence: zeros, never used)
     }
     float x[16];
 #pragma unroll
@@ -339,7 +449,8 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
     if (__builtin_expect(__builtin_amdgcn_ballot_w64(top > m + kSlack) != 0, 0)) {
       float mn = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)));
       if constexpr (kShift) mn = ceilf(mn);    // (so that m - kShift is exact)
-      const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      if constexpr (careful.value) f = fmaxf(f, FLT_MIN);     // (an infinity in o stays one)
       m = mn;
       lsum *= f;
 #pragma unroll
@@ -347,7 +458,7 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
     }
     const float base = m == -INFINITY ? 0.f : m - kShift;
     uint32_t w[8];
-    uint32_t some[8];                          // careful: 1 where a weight is not zero
+    uint32_t some[8];                          // careful: 1 where the formula weighs the token
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float w0 = __builtin_amdgcn_exp2f(fmaf(x[2 * i], mul, -base));
@@ -356,17 +467,19 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
       lsum = dot2<T>(w[i], Ops::ones8()[0], lsum);
       if constexpr (careful.value) {
         const uint32_t one = Ops::ones8()[0];
-        some[i] = (w0 != 0.f ? one & 0xffffu : 0u) | (w1 != 0.f ? one & 0xffff0000u : 0u);
+        some[i] = (x[2 * i] != -INFINITY ? one & 0xffffu : 0u) |
+                  (x[2 * i + 1] != -INFINITY ? one & 0xffff0000u : 0u);
       }
     }
+    if constexpr (kSplit) older_landed();      // V
     const int vo = anew(v_off);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const mf_u32x4 pop{w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]};
 #pragma unroll
       for (int e = 0; e < NE; ++e) {
-        const uint2 a0 = v_operand(cur, bp + u, 0, e, vo);
-        const uint2 a1 = v_operand(cur, bp + u, 1, e, vo);
+        const uint2 a0 = v_operand(vv, u, 0, e, vo);
+        const uint2 a1 = v_operand(vv, u, 1, e, vo);
         mf_u32x4 vop{a0.x, a0.y, a1.x, a1.y};
         if constexpr (careful.value) {
           mf_u32x4 bad;
@@ -403,7 +516,7 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
           }
         }
         o[e] = M32::mma(vop, pop, o[e]);
-        if (PromptShape<D>::kAnew && e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+        if (kAnew && e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
       }
     }
   };
@@ -418,9 +531,21 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
     auto part = [&](int st, int bp, const StageBuf& cur) {
       const int tok0 = st * kTok + bp * kBlockTok;
       if (wave_rows && tok0 <= row_last && !(kWindow && tok0 + 31 <= row_w - win))
-        step(careful, tok0, bp, cur);
+        step(careful, tok0, &cur[0][bp][0], &cur[1][bp][0]);
     };
-    if constexpr (careful.value) {
+    if constexpr (kSplit) {
+      if (st0 + wave < st1) {
+        dma_own(st0 + wave, 0);
+        __builtin_amdgcn_sched_barrier(0);    // (K's loads are the older ones)
+        dma_own(st0 + wave, 1);
+      }
+      for (int st = st0 + wave; st < st1; st += NW) {
+        step(careful, st * kTok, &ldsk[wave][0][0], &ldsv[wave][0][0]);
+        reads_done();
+        dma_own(st + NW, 1);
+      }
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");    // (no load is on its way any more)
+    } else if constexpr (careful.value) {
       for (int st = st0; st < st1; ++st) {
         __syncthreads();                    // (every wave is done with the stage before)
         dma_stage(st, lds0);
@@ -451,6 +576,11 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
   for (int e = 0; e < NE; ++e)
 #pragma unroll
     for (int r = 0; r < 16; ++r) odd = odd || o[e][r] != o[e][r];
+  if constexpr (kSplit) {
+    if (__builtin_amdgcn_ballot_w64(odd && row_ok)) walk(std::true_type{});
+    prompt_join<T, D, NW>(p, m, lsum, o, &ldsk[0][0][0], &ldsv[0][0][0], tl, hq);
+    return;
+  }
   // (the barrier also ends every wave's reads of the buffers that a second walk fills)
   if (__syncthreads_or(odd && row_ok)) {
     walk(std::true_type{});
@@ -493,20 +623,35 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
 template <typename T, int D, bool kCap, bool kWindow>
 __global__ __launch_bounds__(64 * PromptShape<D>::kWaves, PromptShape<D>::kPerSimd)
 void prompt_attn_kernel(PromptParams p) {
-  prompt_body<T, D, kCap, kWindow>(p);
+  prompt_body<T, D, kCap, kWindow, false>(p);
+}
+template <typename T, int D, bool kCap, bool kWindow>
+__global__ __launch_bounds__(64 * PromptSplit<D>::kWaves, PromptSplit<D>::kPerSimd)
+void prompt_split_kernel(PromptParams p) {
+  prompt_body<T, D, kCap, kWindow, true>(p);
 }
 
-template <typename T, int D>
-hipError_t launch_prompt_dim(PromptParams p, hipStream_t st) {
-  constexpr int NW = PromptShape<D>::kWaves;
-  p.tiles = (p.N + 32 * NW - 1) / (32 * NW) + p.B;
-  const dim3 grid((uint32_t)p.tiles * p.Hq), block(64 * NW);
-  const bool cap = p.softcap > 0.f, win = p.window > 0;
-  if (cap && win) hipLaunchKernelGGL((prompt_attn_kernel<T, D, true, true>), grid, block, 0, st, p);
-  else if (cap) hipLaunchKernelGGL((prompt_attn_kernel<T, D, true, false>), grid, block, 0, st, p);
-  else if (win) hipLaunchKernelGGL((prompt_attn_kernel<T, D, false, true>), grid, block, 0, st, p);
-  else hipLaunchKernelGGL((prompt_attn_kernel<T, D, false, false>), grid, block, 0, st, p);
+template <typename T, int D, bool kCap, bool kWindow>
+hipError_t launch_prompt_form(PromptParams p, hipStream_t st) {
+  const bool split = prompt_splits<D>(p);
+  const int rows = split ? 32 : 32 * PromptShape<D>::kWaves;
+  p.tiles = (p.N + rows - 1) / rows + p.B;
+  const dim3 grid((uint32_t)p.tiles * p.Hq);
+  if (split)
+    hipLaunchKernelGGL((prompt_split_kernel<T, D, kCap, kWindow>), grid,
+                       dim3(64 * PromptSplit<D>::kWaves), 0, st, p);
+  else
+    hipLaunchKernelGGL((prompt_attn_kernel<T, D, kCap, kWindow>), grid,
+                       dim3(64 * PromptShape<D>::kWaves), 0, st, p);
   return hipGetLastError();
+}
+template <typename T, int D>
+hipError_t launch_prompt_dim(const PromptParams& p, hipStream_t st) {
+  const bool cap = p.softcap > 0.f, win = p.window > 0;
+  if (cap && win) return launch_prompt_form<T, D, true, true>(p, st);
+  if (cap) return launch_prompt_form<T, D, true, false>(p, st);
+  if (win) return launch_prompt_form<T, D, false, true>(p, st);
+  return launch_prompt_form<T, D, false, false>(p, st);
 }
 
 // One per element type, each in a source of its own (prompt_bf16.hip, prompt_f16.hip).

@@ -161,6 +161,55 @@ def test_infinities_and_nan_where_they_are_hidden(dtype, D, window):
     assert torch.isfinite(out[30:49, 0, 7]).all() and (out[31, :, 3] == math.inf).all()
 
 
+# Up to 512 or 640 tiles of 32 rows (times heads; 1,280 for long prompts) a workgroup's waves share a
+# tile's keys, beyond each has rows of its own: the same edges on either side.
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lens,Hq,Hkv,D,window,cap", [
+    ([127, 128, 129, 0, 1, 33], 36, 4, 64, 0, 0.0), ([127, 128, 129, 0, 1, 33], 36, 4, 128, 0, 0.0),
+    ([255, 256, 257, 1], 40, 8, 256, 0, 0.0), ([400, 31], 72, 8, 64, 129, 30.0),
+    ([400, 31], 72, 8, 128, 33, 30.0), ([400, 31], 72, 8, 256, 97, 30.0),
+    ([2500], 2, 1, 64, 0, 0.0), ([2049], 3, 1, 128, 1000, 0.0), ([1, 700, 64], 3, 1, 256, 0, 20.0),
+    ([4100], 1, 1, 256, 4000, 0.0), ([97], 8, 2, 128, 96, 0.0)])
+def test_either_form(dtype, lens, Hq, Hkv, D, window, cap):
+    q, k, v = _case(len(lens) + D, sum(lens), Hq, Hkv, D, dtype)
+    out = prompt.prompt_attention(q, k, v, _cu(lens), window=window or None, softcap=cap or None)
+    _assert_close(out, q, k, v, lens, cap=cap, window=window, heads=[0, Hq // 2, Hq - 1])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("window", [0, 40])
+def test_infinities_and_nan_with_many_heads(dtype, D, window):
+    lens, H = [100, 70], 66
+    q, k, v = (x.contiguous() for x in _case(D + 1, 170, H, H // 2, D, dtype))
+    v[30, :, 3], v[50, :, 4], v[60, :, 5] = math.inf, -math.inf, math.nan
+    v[70, :, 3], v[100, :, 6] = -math.inf, math.nan
+    k[80, :, 1], q[20, 1, 0] = math.nan, math.inf
+    out = prompt.prompt_attention(q, k, v, _cu(lens), window=window or None)
+    _assert_close(out, q, k, v, lens, window=window, heads=[0, 1, H - 1])
+    assert torch.isfinite(out[:20, 0]).all() and torch.isnan(out[20, 1]).all()
+    assert (out[31, :, 3] == math.inf).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("H", [2, 66])
+def test_a_visible_infinity_counts_however_small_its_weight(dtype, D, H):
+    """One key 150 nats above the others (e^-150 is no fp32 number), an infinity before it
+    and one behind it: the formula weighs both."""
+    n = 200
+    q, k, v = _case(5, n, H, 1, D, dtype)
+    q, k, v = torch.zeros_like(q), torch.zeros_like(k), v.contiguous()
+    q[:, :, 0], k[40, :, 0] = 8.0, 150.0
+    v[5, :, 3], v[70, :, 4] = math.inf, -math.inf
+    out = prompt.prompt_attention(q, k, v, _cu([n]), scale=0.125)
+    _assert_close(out, q, k, v, [n], scale=0.125, heads=[0, H - 1])
+    assert torch.isfinite(out[:5]).all() and (out[5:, :, 3] == math.inf).all()
+    assert torch.isfinite(out[:70, :, 4]).all() and (out[70:, :, 4] == -math.inf).all()
+    rest = [d for d in range(D) if d not in (3, 4)]
+    assert torch.equal(out[40:, 0, rest], v[40, 0, rest].expand(n - 40, D - 2))
+
+
 def test_captured_call_follows_its_operands():
     n = 160
     q, k, v = (x.contiguous() for x in _case(12, n, 4, 2, 128, torch.bfloat16))
