@@ -14,7 +14,9 @@
 // the pages: B is small against the tokens, and a sum in one workgroup that the
 // others wait for would cost a second launch.  Entries of the table that this
 // call writes are never read by it: a token on a new page takes its slot from
-// the free list.
+// the free list.  The lengths are read until the last workgroup ends, so no
+// output may lie over an input; seq_lens alone may be cached_lens itself (a loop's
+// lengths, kept in place), and is then written by a second launch.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -120,7 +122,7 @@ __global__ __launch_bounds__(kThreads) void batch_tables_kernel(TablesArgs a) {
     const Seq s = load_seq(a, b);
     cu[b] = clamp_i32(t0);
     pg[b] = clamp_i32(p0);
-    if (blockIdx.x == 0) a.seq_lens[b] = s.total;
+    if (blockIdx.x == 0 && a.seq_lens) a.seq_lens[b] = s.total;
     t0 += s.total - s.cached;
     p0 += s.need;
   }
@@ -170,6 +172,32 @@ __global__ __launch_bounds__(kThreads) void batch_tables_kernel(TablesArgs a) {
   }
 }
 
+// lens[b] += new_lens[b], as load_seq adds them, once the tables are done.
+__global__ __launch_bounds__(kThreads) void add_lens_kernel(TablesArgs a, int32_t* lens) {
+  const int b = blockIdx.x * kThreads + threadIdx.x;
+  if (b < a.B) lens[b] = load_seq(a, b).total;
+}
+
+// `rows` rows of `bytes` bytes, `step` (>= bytes) apart.
+struct Range {
+  uintptr_t at;
+  int64_t rows, bytes, step;
+};
+template <typename T>
+Range range(const T* p, int64_t n, int64_t rows = 1, int64_t stride = 0) {
+  const int64_t e = sizeof(T);
+  return {reinterpret_cast<uintptr_t>(p), rows, n * e, (rows > 1 ? stride : n) * e};
+}
+// Whether a byte of x (one row) is one of y's.
+bool overlap(const Range& x, const Range& y) {
+  if (!x.bytes || !y.bytes || !y.rows || x.at + x.bytes <= y.at) return false;
+  if (x.at < y.at + y.bytes) return true;
+  const int64_t row = (int64_t)(x.at - y.at) / y.step;      // the last that starts at or before x
+  if (row >= y.rows) return false;
+  const int64_t in = (int64_t)(x.at - y.at) - row * y.step;
+  return in < y.bytes || (row + 1 < y.rows && in + x.bytes > y.step);
+}
+
 }  // namespace
 
 extern "C" int helm_batch_tables(const int32_t* new_lens, const int32_t* cached_lens, int B,
@@ -188,9 +216,26 @@ extern "C" int helm_batch_tables(const int32_t* new_lens, const int32_t* cached_
     return helm::report_error(HELM_E_INVALID, "null pointer argument");
   TablesArgs a{new_lens, cached_lens, page_table, table_stride, table_width, free_slots, n_free,
                page_size, B, max_tokens, cu_seqlens, positions, slot_map, seq_lens, pages_taken};
+  // the table (read and written), what is only read, what is only written
+  const bool in_place = seq_lens == cached_lens;
+  const Range r[] = {range(page_table, table_width, B, table_stride),
+                     range(new_lens, B), range(cached_lens, B), range(free_slots, n_free),
+                     range(cu_seqlens, B + 1), range(positions, max_tokens),
+                     range(slot_map, max_tokens), range(seq_lens, B), range(pages_taken, 1)};
+  constexpr int kIn = 1, kCached = 2, kOut = 4, kLens = 7, kRanges = 9;
+  for (int i = kIn; i < kRanges; ++i)
+    for (int j = 0; j < std::min(i, i < kOut ? kIn : kRanges); ++j)
+      if (overlap(r[i], r[j]) && !(in_place && i == kLens && j == kCached))
+        return helm::report_error(HELM_E_INVALID,
+                                  "an output lies over another operand (seq_lens may be "
+                                  "cached_lens itself, nothing else)");
+  if (in_place) a.seq_lens = nullptr;
   const int grid = std::max(1, std::min(256, (max_tokens + 2 * kThreads - 1) / (2 * kThreads)));
   hipLaunchKernelGGL(batch_tables_kernel, dim3(grid), dim3(kThreads), 2 * (B + 1) * sizeof(int),
                      reinterpret_cast<hipStream_t>(stream), a);
+  if (in_place)
+    hipLaunchKernelGGL(add_lens_kernel, dim3((B + kThreads - 1) / kThreads), dim3(kThreads), 0,
+                       reinterpret_cast<hipStream_t>(stream), a, seq_lens);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess)
     return helm::report_error((int)e, std::string("batch tables launch: ") + hipGetErrorString(e));

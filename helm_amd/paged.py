@@ -179,7 +179,9 @@ def batch_tables(new_lens: torch.Tensor, cached_lens: torch.Tensor, page_table: 
     need come from free_slots (int32, in order) and are written behind the pages
     the sequence has, ceil(cached / page_size).  max_tokens: rows of the packed
     step, at least the sum of new_lens (a captured step keeps it fixed).  out: a
-    former result of the same sizes, written instead of new tensors.
+    former result of the same sizes, written instead of new tensors; its seq_lens may
+    be cached_lens itself, which then holds the next step's.  No other output may share
+    memory with an operand (ValueError).
 
     Token i of the step, of sequence b, has position cached + i - cu_seqlens[b]
     and row page_table[b, position // page_size] * page_size + position %

@@ -379,6 +379,8 @@ int helm_prefetch_pages(helm_engine* eng, int n, const uint64_t* src_host,
  * needs more than table_width pages, the missing pages' tokens get slot -1 and
  * their entries inside the table -1.  Entries that the call does not take are
  * not written; tokens past max_tokens are left out.  Sums stop at 2^31 - 1.
+ * seq_lens may be cached_lens itself (a second launch then writes it); any other
+ * output over an operand, or page_table over one, is HELM_E_INVALID.
  * B <= HELM_TABLES_MAX_SEQS. */
 #define HELM_TABLES_MAX_SEQS 4096
 int helm_batch_tables(const int32_t* new_lens, const int32_t* cached_lens, int B,

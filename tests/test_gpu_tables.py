@@ -107,3 +107,64 @@ def test_results_written_again_and_replayed():
         want = R.tables(nl, cl, tb, fl, page, N)
         assert [out[i].tolist() for i in range(4)] == [list(w) for w in want[:4]]
         assert out.pages_taken.item() == want[4] and table.tolist() == want[5]
+
+
+def _loop(r, B, N, top, captured):
+    """Steps whose cached lengths are the outputs' seq_lens, kept in place: each step's tables
+    are the oracle's, and the lengths after it the next step's."""
+    page, width = 16, 60
+    used = 0
+    new, free = _i32([0] * B), _i32([0] * 400)
+    table = torch.full((B, width), -3, dtype=torch.int32, device=DEV)
+    out = paged.batch_tables(new, _i32([0] * B), table, free, page, N)
+    cached, lens = out.seq_lens, [0] * B
+    rows = table.tolist()
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            paged.batch_tables(new, cached, table, free, page, N, out=out)
+        cached.zero_()
+    for _ in range(5):
+        nl = [r.randint(0, top) for _ in range(B)]
+        fl = list(range(used, used + 400))
+        new.copy_(_i32(nl))
+        free.copy_(_i32(fl))
+        if captured:
+            graph.replay()
+        else:
+            assert paged.batch_tables(new, cached, table, free, page, N, out=out) is out
+        torch.cuda.synchronize()
+        want = R.tables(nl, lens, rows, fl, page, N)
+        assert [out[i].tolist() for i in range(4)] == [list(w) for w in want[:4]]
+        assert out.pages_taken.item() == want[4] and table.tolist() == want[5]
+        lens, rows, used = want[3], want[5], used + want[4]
+
+
+@pytest.mark.parametrize("B,N,top", [(1, 3, 1), (3, 16, 4), (70, 500, 6), (300, 12000, 30)])
+@pytest.mark.parametrize("captured", [False, True])
+def test_lengths_kept_in_place(B, N, top, captured):
+    """One workgroup's steps and many workgroups'."""
+    _loop(random.Random(B), B, N, top, captured)
+
+
+def test_outputs_over_operands_are_refused():
+    B, page, N = 4, 16, 20
+    new, cached = _i32([3] * B), _i32([5] * B)
+    back = torch.zeros((B, 40), dtype=torch.int32, device=DEV)
+    table, free = back[:, :8], _i32(list(range(10, 40)))
+    out = paged.batch_tables(new, cached, table, free, page, N)
+    shifted = _i32([5] * (B + 1))
+    wide = torch.zeros(40, dtype=torch.int64, device=DEV)
+    for lens, o in ((cached, out._replace(seq_lens=new)), (shifted[:B], out._replace(seq_lens=shifted[1:])),
+                    (cached, out._replace(positions=wide[:N], slot_map=wide[N - 1:2 * N - 1])),
+                    (cached, out._replace(pages_taken=free[7:8])), (cached, out._replace(seq_lens=back[2, 6:10])),
+                    (out.cu_seqlens[1:], out), (out.pages_taken.expand(B).contiguous()[:B], out._replace(
+                        seq_lens=out.cu_seqlens[:B]))):
+        with pytest.raises(ValueError, match="over another operand"):
+            paged.batch_tables(new, lens, table, free, page, N, out=o)
+    with pytest.raises(ValueError, match="over another operand"):
+        paged.batch_tables(new, back[1, 4:8], table, free, page, N)
+    # columns of the table's buffer that are not the table's are nobody else's either
+    got = paged.batch_tables(new, back[1, 8:8 + B], table, free, page, N,
+                             out=out._replace(seq_lens=back[2, 12:12 + B]))
+    assert got.seq_lens.tolist() == [3] * B

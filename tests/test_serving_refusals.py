@@ -193,6 +193,28 @@ def test_c_entries_refuse_before_device_work():
     assert prom(N=0x7fffffff, Hq=64) == E
 
 
+def test_batch_tables_c_entry_refuses_outputs_over_operands():
+    lib, E = _native.load(), _native.HELM_E_INVALID
+    # (addresses of nothing: the call ends at its checks)
+    at = dict(new=0x1000, cached=0x2000, table=0x3000, free=0x4000, cu=0x5000, pos=0x6000,
+              slot=0x7000, lens=0x8000, taken=0x9000)
+    B, width, stride, n_free, N = 4, 8, 40, 30, 20
+
+    def refused(**kw):
+        a = dict(at, **kw)
+        rc = lib.helm_batch_tables(a["new"], a["cached"], B, a["table"], stride, width, a["free"], n_free,
+                                   16, N, a["cu"], a["pos"], a["slot"], a["lens"], a["taken"], None)
+        return rc == E and b"over another operand" in lib.helm_last_error_string()
+
+    t, row, used = at["table"], 4 * stride, 4 * width
+    for lens in (at["new"], at["cached"] + 4, at["cached"] - 12, t, t + used - 4, t + row, t + row - 4,
+                 t + 3 * row + used - 4, t - 12, t + 2 * row - 16 + 4, at["free"] + 4 * n_free - 4):
+        assert refused(lens=lens)
+    assert refused(pos=at["slot"] - 8 * N + 8) and refused(slot=at["pos"] + 8 * N - 8)
+    assert refused(cu=at["taken"] - 4 * B) and refused(taken=at["pos"]) and refused(cu=at["cached"])
+    assert refused(new=t + used - 4) and refused(cached=t + 3 * row) and refused(free=t - 4)
+
+
 # ---- the oracle ------------------------------------------------------------------------
 def test_stored_values_are_nearest_within_half_a_step():
     g = torch.Generator().manual_seed(0)
