@@ -44,9 +44,9 @@ class Pool4:
         self.head_dim, self.page_size = head_dim, page_size
         self._data = torch.zeros((n_slots, num_kv_heads, page_size // 16, 17 * head_dim),
                                 dtype=torch.uint8, device=device)
-
-        # the C-ABI's leading arguments of a write or read
-        self._shape = (self._data.data_ptr(), n_slots, page_size, num_kv_heads, head_dim)
+        # the C-ABI's arguments of a write or read behind the storage's address, which is
+        # taken at each call: a copied or unpickled pool has its own
+        self._shape = (n_slots, page_size, num_kv_heads, head_dim)
 
     @property
     def data(self) -> torch.Tensor:
@@ -77,8 +77,8 @@ class Pool4:
         unit = 4 if code == _native.HELM_F32 else 8
         k, *k_at = _rows16(k, unit)
         v, *v_at = _rows16(v, unit)
-        _engine.launch_on(idx, "helm_pool4_write", *self._shape, slot_map.data_ptr(), n, *k_at,
-                          *v_at, code)
+        _engine.launch_on(idx, "helm_pool4_write", self._data.data_ptr(), *self._shape,
+                          slot_map.data_ptr(), n, *k_at, *v_at, code)
 
     def read(self, slot_map: torch.Tensor, dtype: torch.dtype = torch.bfloat16
              ) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -91,8 +91,9 @@ class Pool4:
         idx = _engine.common_device("Pool4.read", self._data, slot_map)
         H, D = self.num_kv_heads, self.head_dim
         k, v = slot_map.new_empty((2, n, H, D), dtype=dtype).unbind(0)
-        _engine.launch_on(idx, "helm_pool4_read", *self._shape, slot_map.data_ptr(), n,
-                          k.data_ptr(), H * D, D, v.data_ptr(), H * D, D, code)
+        _engine.launch_on(idx, "helm_pool4_read", self._data.data_ptr(), *self._shape,
+                          slot_map.data_ptr(), n, k.data_ptr(), H * D, D, v.data_ptr(), H * D, D,
+                          code)
         return k, v
 
 

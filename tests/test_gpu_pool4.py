@@ -7,6 +7,7 @@ off by at most (D + 4) 2^-24 L, L the largest sum of its terms' magnitudes (the 
 are exact: bf16 codes and queries in parts), plus 2^-22 of the logit's size for its
 scaling and exponent; a weight's relative error e moves the mean by at most 2 e max|v|;
 sums of T terms in fp32 add T 2^-24 max|v| (far more than their trees do)."""
+import copy
 import math
 
 import pytest
@@ -332,3 +333,15 @@ def test_calls_on_two_streams():
     torch.cuda.synchronize()
     for i, o in enumerate(outs):
         assert torch.equal(o, want[i % 2])
+
+
+def test_a_copied_pool_has_its_own_pages():
+    pool = pool4.Pool4(3, 2, 64, device=DEV)
+    slots = torch.arange(48, device=DEV)
+    k, v = _randn(1, 48, 2, 64), _randn(2, 48, 2, 64)
+    pool.write(k, v, slots)
+    twin = copy.deepcopy(pool)
+    twin.write(v, k, slots)
+    for p, a, b in ((pool, k, v), (twin, v, k)):
+        rk, rv = p.read(slots, dtype=torch.float32)
+        assert torch.equal(rk.double(), R.stored4(a)) and torch.equal(rv.double(), R.stored4(b))

@@ -1,7 +1,10 @@
 """What the serving operators refuse, and what they do not need a GPU for: argument
 checks of the Python entry points and of the C-ABI (which return before any device
 work), the oracle's own properties."""
+import copy
+import io
 import math
+import pickle
 
 import pytest
 import torch
@@ -79,6 +82,31 @@ def test_pool4_write_refusals(k, v, slots, err):
     if err is RuntimeError:
         with pytest.raises(err):
             pool.read(slots)
+
+
+def _saved(pool):
+    f = io.BytesIO()
+    torch.save(pool, f)
+    f.seek(0)
+    return torch.load(f, weights_only=False)
+
+
+@pytest.mark.parametrize("twin", [copy.deepcopy, lambda p: pickle.loads(pickle.dumps(p)), _saved])
+def test_a_copied_pool_is_written_and_read_in_its_own_storage(twin, monkeypatch):
+    pool = pool4.Pool4(3, 2, 64, device="cpu")
+    pool.data.random_(0, 256)
+    other, calls = twin(pool), []
+    assert torch.equal(other.data, pool.data) and other.data.data_ptr() != pool.data.data_ptr()
+    monkeypatch.setattr(pool4._engine, "common_device", lambda what, *t: 0)
+    monkeypatch.setattr(pool4._engine, "launch_on", lambda idx, fn, *args: calls.append((fn, args)))
+    rows, slots = torch.zeros(3, 2, 64), torch.zeros(3, dtype=I64)
+    for p in (pool, other):
+        p.write(rows, rows, slots)
+        p.read(slots)
+        for fn, args in calls:
+            assert args[:5] == (p.data.data_ptr(), 3, 16, 2, 64), fn
+        assert [fn for fn, _ in calls] == ["helm_pool4_write", "helm_pool4_read"]
+        calls.clear()
 
 
 def _decode(**kw):
