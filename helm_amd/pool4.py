@@ -114,10 +114,16 @@ class PreparedPool4Decode:
     once, for loops that issue the same shape every step.  ``run`` reads q, page table,
     lengths, mask and pool as they are then, on torch's current stream; runs of one
     object (its replays in graphs among them) share its workspace and `out` and must
-    not overlap."""
+    not overlap.  It holds addresses: a deep copy or pickle of it is refused."""
 
     def __init__(self, idx, args, out, keep):
         self._idx, self._args, self.out, self._keep = idx, args, out, keep
+
+    def __copy__(self) -> "PreparedPool4Decode":
+        return PreparedPool4Decode(self._idx, self._args, self.out, self._keep)
+
+    def __reduce_ex__(self, protocol):
+        raise TypeError("a prepared call holds its operands' addresses: prepare the copies' own")
 
     def run(self) -> torch.Tensor:
         _engine.launch_on(self._idx, "helm_pool4_decode_attn", *self._args)

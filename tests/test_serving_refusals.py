@@ -150,6 +150,15 @@ def test_prepared_pool4_decode_reads_in_place():
         pool4.prepare_pool4_decode(**_decode(attention_mask=torch.zeros(2, 1, 1, 32).double()))
 
 
+def test_a_prepared_call_is_not_copied_with_its_addresses():
+    step = pool4.PreparedPool4Decode(0, (1, 2), torch.zeros(2), (torch.zeros(3),))
+    for twin in (copy.deepcopy, pickle.dumps, lambda s: copy.deepcopy({"layer": [s]})):
+        with pytest.raises(TypeError, match="prepare"):
+            twin(step)
+    same = copy.copy(step)                      # of the same operands
+    assert same.out is step.out and same._args is step._args and same._keep is step._keep
+
+
 def _prompt(**kw):
     a = dict(q=torch.zeros(5, 4, 64).half(), k=torch.zeros(5, 2, 64).half(),
              v=torch.zeros(5, 2, 64).half(), cu_seqlens=torch.tensor([0, 5], dtype=I32))
