@@ -114,10 +114,13 @@ class PreparedPool4Decode:
     once, for loops that issue the same shape every step.  ``run`` reads q, page table,
     lengths, mask and pool as they are then, on torch's current stream; runs of one
     object (its replays in graphs among them) share its workspace and `out` and must
-    not overlap.  It holds addresses: a deep copy or pickle of it is refused."""
+    not overlap.  It may be dropped while runs are on their way, on any stream, but not
+    before the last replay of a graph that holds one.  It holds addresses: a deep copy or
+    pickle of it is refused."""
 
     def __init__(self, idx, args, out, keep):
         self._idx, self._args, self.out, self._keep = idx, args, out, keep
+        self._streams = set()              # those that the workspace and out are recorded on
 
     def __copy__(self) -> "PreparedPool4Decode":
         return PreparedPool4Decode(self._idx, self._args, self.out, self._keep)
@@ -126,7 +129,11 @@ class PreparedPool4Decode:
         raise TypeError("a prepared call holds its operands' addresses: prepare the copies' own")
 
     def run(self) -> torch.Tensor:
-        _engine.launch_on(self._idx, "helm_pool4_decode_attn", *self._args)
+        stream = _engine.launch_on(self._idx, "helm_pool4_decode_attn", *self._args)
+        if stream not in self._streams:
+            for t in (self.out, self._keep[-1]):
+                t.record_stream(torch.cuda.current_stream(self._idx))
+            self._streams.add(stream)
         return self.out
 
 

@@ -65,10 +65,10 @@ def stream_ptr(device: torch.device) -> int:
 _get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
-def launch_on(idx: int, fn: str, *args) -> None:
+def launch_on(idx: int, fn: str, *args) -> int:
     """One native call that launches on HIP device `idx`, on torch's current stream
-    there (its last argument): the device is current for it (and the one before is
-    again afterwards); raises as ``_native.call`` does."""
+    there (its last argument, returned): the device is current for it (and the one before
+    is again afterwards); raises as ``_native.call`` does."""
     f = _native.entry(fn)
     stream = _raw_stream(idx) if _raw_stream is not None else \
         torch.cuda.current_stream(idx).cuda_stream
@@ -79,6 +79,7 @@ def launch_on(idx: int, fn: str, *args) -> None:
             rc = f(*args, stream)
     if rc:
         _native.check(fn, rc)
+    return stream
 
 
 def common_device(what: str, *tensors: torch.Tensor) -> int:

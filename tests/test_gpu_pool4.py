@@ -345,3 +345,23 @@ def test_a_copied_pool_has_its_own_pages():
     for p, a, b in ((pool, k, v), (twin, v, k)):
         rk, rv = p.read(slots, dtype=torch.float32)
         assert torch.equal(rk.double(), R.stored4(a)) and torch.equal(rv.double(), R.stored4(b))
+
+
+def test_a_prepared_step_dropped_while_it_runs_on_another_stream():
+    """Its workspace and output are not handed out again before that stream is done."""
+    c = _case(73, [5000], 8, 2, 128, 1, 16, torch.bfloat16)
+    want = pool4.pool4_decode_attention(c["q"], c["pool"], c["table"], c["lens"])
+    step = pool4.prepare_pool4_decode(c["q"], c["pool"], c["table"], c["lens"])
+    ws, at = step._keep[-1].numel(), (step._keep[-1].data_ptr(), step.out.data_ptr())
+    assert ws > 0
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)
+        kept = step.run().clone()
+    del step
+    fresh = [torch.zeros(ws, dtype=torch.uint8, device=DEV), torch.zeros_like(c["q"])]
+    running = not side.query()
+    assert not running or not set(at) & {t.data_ptr() for t in fresh}
+    torch.cuda.synchronize()
+    assert torch.equal(kept, want)
