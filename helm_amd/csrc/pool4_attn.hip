@@ -29,7 +29,7 @@
 // Hidden tokens (past the sequence's length, past the causal limit, or under a
 // mask of -inf) take no part whatever their K and V hold: their scores are
 // overwritten, and where V's group stands for NaN the products take zeros there
-// and the NaN is put into the rows that weigh such a token.
+// and the NaN is put into the rows that see such a token, however small its weight.
 // A row with nothing visible is zeros.
 #include <algorithm>
 #include <string>
@@ -422,14 +422,18 @@ __global__ __launch_bounds__(64 * kP4Waves) void pool4_attn_kernel(P4Attn a) {
       o[2 * c + 1] = Ops::mma(odd, lo, o[2 * c + 1]);
     }
     if (__builtin_expect(nan, 0)) {
-      // ones at the NaN tokens (a whole chunk lies in one group): a row that
-      // weighs any gets NaN in every dim of the chunk
-      mf_u32x4 one;
+      // ones at the NaN tokens (a whole chunk lies in one group) times ones at those that
+      // the row sees (not its weights, which may be zero by rounding): a row that sees any
+      // gets NaN in every dim of the chunk, and no later factor takes that away
+      mf_u32x4 one, sees;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+      for (int j = 0; j < 4; ++j) {
         one[j] = (((ff >> (2 * j)) & 1u) ? 0x3F80u : 0u) |
                  (((ff >> (2 * j + 1)) & 1u) ? 0x3F800000u : 0u);
-      const mf_f32x4 hit = Ops::mma(one, hi, mf_f32x4{0.f, 0.f, 0.f, 0.f});
+        sees[j] = (x[2 * j] != -INFINITY ? 0x3F80u : 0u) |
+                  (x[2 * j + 1] != -INFINITY ? 0x3F800000u : 0u);
+      }
+      const mf_f32x4 hit = Ops::mma(one, sees, mf_f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
       for (int r4 = 0; r4 < 4; ++r4)
         if (!(hit[r4] == 0.f))

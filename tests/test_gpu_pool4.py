@@ -365,3 +365,39 @@ def test_a_prepared_step_dropped_while_it_runs_on_another_stream():
     assert not running or not set(at) & {t.data_ptr() for t in fresh}
     torch.cuda.synchronize()
     assert torch.equal(kept, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("T", [60, 500, 1500])
+@pytest.mark.parametrize("mdt", [None, torch.float32, torch.bfloat16])
+def test_a_visible_nan_group_counts_however_small_its_weight(dtype, D, T, mdt):
+    """One key 153.6 nats above the others (e^-153.6 is no fp32 number), a NaN group of V
+    before it and one behind: the formula weighs both, in one split and in several.  A mask's
+    lowest finite value hides nothing, -inf does."""
+    c = _case(D + T, [T], 2, 1, D, 2, 16, dtype)
+    q, k, v = c["q"].zero_(), torch.zeros(T, 1, D, device=DEV), _randn(9, T, 1, D)
+    q[..., 0], k[40, 0, 0] = 8.0, 128.0                      # 8 * 128 * 0.15
+    v[5, 0, 3], v[T - 8, 0, 40] = math.inf, math.nan         # groups 0 and 1
+    v[T - 1, 0, D - 1] = math.nan                            # the last row's alone
+    pos = torch.arange(T)
+    slots = (c["table"].cpu()[0][pos // 16].long() * 16 + pos % 16).to(DEV)
+    c["pool"].write(k, v, slots)
+    c["ks"], c["vs"] = [R.stored4(k)], [R.stored4(v)]
+    m = None
+    if mdt is not None:
+        m = torch.zeros(1, 1, 1, T, dtype=mdt, device=DEV)
+        m[..., 5] = torch.finfo(mdt).min
+    def attend():
+        return pool4.pool4_decode_attention(c["q"], c["pool"], c["table"], c["lens"], scale=0.15,
+                                            attention_mask=m, causal=True)
+    out = attend()
+    _assert_close(c, out, True, scale=0.15, mask=m)
+    assert torch.isnan(out[..., :64]).all() and torch.isnan(out[0, :, 1, D - 32:]).all()
+    if D > 64:
+        assert torch.isfinite(out[0, :, 0, 64:]).all() and torch.isfinite(out[0, :, 1, 64:D - 32]).all()
+    if m is not None:
+        m[..., 5] = m[..., T - 8] = -math.inf
+        out = attend()
+        _assert_close(c, out, True, scale=0.15, mask=m)
+        assert torch.isfinite(out[0, :, 0]).all()
