@@ -26,7 +26,6 @@
 // and NaN taken out of the products and added where a row weighs them (careful).
 #pragma once
 
-#include <cfloat>
 #include <type_traits>
 
 #include "attn_chunk32.h"
@@ -207,10 +206,15 @@ template <typename T> __device__ __forceinline__ uint32_t nonfinite_halves(uint3
   return r;
 }
 
+// x f, but an infinity or NaN (a visible one, which counts at any weight) stays what it is where
+// f is zero.
+__device__ __forceinline__ float scale_finite(float x, float f) {
+  return fabsf(x) < INFINITY ? x * f : x;
+}
+
 // Joins the waves' sums over 32 rows: a wave's part counts exp2(m - M) of itself, M the
-// largest of the row's maxima (at least the smallest normal number, so that an infinity or NaN
-// in the sums stays one).  Wave w's sums go where
-// its K (the row's first half) and its V were, 64 D bytes each: dims 32 e + 8 g + 4 hh .. + 3 of row r (chunk c = 4 e + g)
+// largest of the row's maxima.  Wave w's sums go where its K (the row's first half) and
+// its V were, 64 D bytes each: dims 32 e + 8 g + 4 hh .. + 3 of row r (chunk c = 4 e + g)
 // at 16-byte slot 64 c + 32 hh + (r ^ c % 16), so that writes (a chunk's rows) and reads
 // (a row's chunks) both meet every bank group.
 template <typename T, int D, int NW>
@@ -226,7 +230,7 @@ __device__ __forceinline__ void prompt_join(const PromptParams& p, float m, floa
   float top = tops[0][jr];
 #pragma unroll
   for (int w = 1; w < NW; ++w) top = fmaxf(top, tops[w][jr]);
-  const float f = m == top ? 1.f : fmaxf(__builtin_amdgcn_exp2f(m - top), FLT_MIN);
+  const float f = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top);
   if (hh == 0) sums[wave][jr] = lsum * f;
   auto at = [&](int w, int c, int h, int r) {
     return reinterpret_cast<mf_f32x4*>(c < CPR / 2 ? kbuf : vbuf) + 4 * D * w +
@@ -236,7 +240,7 @@ __device__ __forceinline__ void prompt_join(const PromptParams& p, float m, floa
   for (int c = 0; c < CPR; ++c) {
     mf_f32x4 x;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) x[t] = o[c / 4][4 * (c % 4) + t] * f;
+    for (int t = 0; t < 4; ++t) x[t] = scale_finite(o[c / 4][4 * (c % 4) + t], f);
     *at(wave, c, hh, jr) = x;
   }
   __syncthreads();
@@ -449,12 +453,18 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
     if (__builtin_expect(__builtin_amdgcn_ballot_w64(top > m + kSlack) != 0, 0)) {
       float mn = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)));
       if constexpr (kShift) mn = ceilf(mn);    // (so that m - kShift is exact)
-      float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-      if constexpr (careful.value) f = fmaxf(f, FLT_MIN);     // (an infinity in o stays one)
+      const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
       m = mn;
       lsum *= f;
 #pragma unroll
-      for (int e = 0; e < NE; ++e) o[e] *= f;
+      for (int e = 0; e < NE; ++e) {
+        if constexpr (careful.value) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[e][r] = scale_finite(o[e][r], f);
+        } else {
+          o[e] *= f;
+        }
+      }
     }
     const float base = m == -INFINITY ? 0.f : m - kShift;
     uint32_t w[8];

@@ -228,3 +228,24 @@ def test_captured_call_follows_its_operands():
         assert torch.equal(out[:sum(lens)], prompt.prompt_attention(q, k, v, cu)[:sum(lens)])
         assert (out[sum(lens):] == 7).all()
         _assert_close(out, q, k, v, lens)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("H", [2, 82])
+@pytest.mark.parametrize("window", [0, 120])
+def test_large_values_without_weight_add_nothing(D, H, window):
+    """One key 150 nats above the others and finite values of 1e38 before it and behind: e^-150 of
+    them is below half a step of any output.  A NaN that some rows of a tile do not see
+    (which makes a workgroup walk twice) changes nothing for those."""
+    n = 200
+    q, k, v = (x.contiguous() for x in _case(6, n, H, 1, D, torch.bfloat16))
+    q.zero_(), k.zero_()
+    q[:, :, 0], k[40, :, 0] = 8.0, 150.0
+    v[5, :, 3], v[20, :, 7], v[70, :, 4] = 1e38, -1e38, 1e38
+    v[110, :, 9] = math.nan
+    out = prompt.prompt_attention(q, k, v, _cu([n]), scale=0.125, window=window or None)
+    seen = min(n, 40 + window) if window else n              # rows that see token 40
+    assert torch.equal(out[40:110], v[40].expand(70, H, D))
+    rest = [d for d in range(D) if d != 9]
+    assert torch.equal(out[110:seen, :, rest], v[40, :, rest].expand(seen - 110, H, D - 1))
+    assert torch.isnan(out[110:, :, 9]).all()
