@@ -401,3 +401,22 @@ def test_a_visible_nan_group_counts_however_small_its_weight(dtype, D, T, mdt):
         out = attend()
         _assert_close(c, out, True, scale=0.15, mask=m)
         assert torch.isfinite(out[0, :, 0]).all()
+
+
+@pytest.mark.parametrize("D,Hkv,page", [(64, 3, 16), (128, 2, 48), (256, 1, 32)])
+def test_rows_that_no_slot_names_keep_k_and_v(D, Hkv, page):
+    pool = pool4.Pool4(7, Hkv, D, page_size=page, device=DEV)
+    rows = 7 * page
+    every = torch.arange(rows, device=DEV)
+    pool.write(_randn(1, rows, Hkv, D), _randn(2, rows, Hkv, D), every)
+    k0, v0 = pool.read(every, dtype=torch.float32)
+    before = pool.data.clone()
+    slots = _slots(3, 33, 7, page)
+    k, v = _randn(4, 33, Hkv, D), _randn(5, 33, Hkv, D)
+    pool.write(k[:0], v[:0], slots[:0])
+    pool.write(k, v, torch.full_like(slots, -1))
+    assert torch.equal(pool.data, before)
+    pool.write(k, v, slots)
+    k1, v1 = pool.read(every, dtype=torch.float32)
+    k0[slots], v0[slots] = R.stored4(k).float(), R.stored4(v).float()
+    assert torch.equal(k1, k0) and torch.equal(v1, v0)

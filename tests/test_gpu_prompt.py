@@ -249,3 +249,31 @@ def test_large_values_without_weight_add_nothing(D, H, window):
     rest = [d for d in range(D) if d != 9]
     assert torch.equal(out[110:seen, :, rest], v[40, :, rest].expand(seen - 110, H, D - 1))
     assert torch.isnan(out[110:, :, 9]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("B", [255, 256, 257, 700])
+@pytest.mark.parametrize("Hq,Hkv,D", [(1, 1, 128), (40, 4, 64), (6, 2, 256)])
+def test_many_sequences_of_any_number(dtype, B, Hq, Hkv, D):
+    """Up to 256 sequences the longest walks come first over the batch, beyond each sequence's
+    in turn: empty sequences, one of several tiles in each window of 64, rows outside."""
+    lens = [(i * 37) % 5 for i in range(B)]
+    lens[3], lens[70], lens[140], lens[B - 1] = 300, 0, 129, 257
+    n, first = sum(lens), 9
+    q, k, v = _case(B + D, first + n + 70, Hq, Hkv, D, dtype)
+    cu = _cu(lens) + first
+    out = prompt.prompt_attention(q, k, v, cu)
+    _assert_close(out, q, k, v, lens, first=first, heads=[0, Hq - 1])
+    assert (out[:first] == 0).all() and (out[first + n:] == 0).all()
+    kept = torch.full_like(out, 3.0)
+    prompt.prompt_attention(q, k, v, cu, out=kept)
+    assert torch.equal(kept[first:first + n], out[first:first + n])
+    assert (kept[:first] == 3).all() and (kept[first + n:] == 3).all()
+
+
+@pytest.mark.parametrize("heads", [2, 40])
+def test_more_sequences_than_rows(heads):
+    """300 empty sequences: every row is outside."""
+    q, k, v = _case(1, 150, heads, 1, 64, torch.bfloat16)
+    cu = torch.full((301,), 60, dtype=torch.int32, device=DEV)
+    assert (prompt.prompt_attention(q, k, v, cu) == 0).all()
