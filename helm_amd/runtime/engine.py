@@ -12,6 +12,7 @@ import os
 from typing import Dict
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from helm_amd import _native
 
@@ -94,11 +95,16 @@ def common_device(what: str, *tensors: torch.Tensor) -> int:
 
 
 def refuse_grad(what: str, *tensors: torch.Tensor) -> None:
-    """The package serves models: its attention records nothing for a backward pass."""
+    """The package serves models: its attention records nothing for a backward pass, and
+    has no tangent to give (which no_grad does not drop)."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t.requires_grad:
                 raise RuntimeError(f"{what} records no gradient: call it under torch.no_grad()")
+    if _forward_ad._current_level >= 0:
+        for t in tensors:
+            if _forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{what} gives no forward-mode tangent: unpack its operands")
 
 
 @atexit.register

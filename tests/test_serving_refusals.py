@@ -194,6 +194,31 @@ def test_operands_that_ask_for_a_gradient_are_refused():
         prompt.prompt_attention(**a)
 
 
+@pytest.mark.parametrize("quiet", [False, True])
+def test_operands_with_a_tangent_are_refused(quiet):
+    from torch.autograd import forward_ad
+    with forward_ad.dual_level(), torch.set_grad_enabled(not quiet):
+        for name in "qkv":
+            a = _prompt()
+            a[name] = forward_ad.make_dual(a[name], torch.ones_like(a[name]))
+            with pytest.raises(RuntimeError, match="tangent"):
+                prompt.prompt_attention(**a)
+            a = dict(q=torch.zeros(3, 2, 64), k=torch.zeros(3, 2, 64))
+            a["k" if name == "k" else "q"] = forward_ad.make_dual(torch.zeros(3, 2, 64),
+                                                                  torch.ones(3, 2, 64))
+            with pytest.raises(RuntimeError, match="tangent"):
+                pool4.Pool4(2, 2, 64, device="cpu").write(a["q"], a["k"], torch.zeros(3, dtype=I64))
+        m = forward_ad.make_dual(torch.zeros(1, 1, 1, 9), torch.ones(1, 1, 1, 9))
+        for call in (pool4.pool4_decode_attention, pool4.prepare_pool4_decode):
+            with pytest.raises(RuntimeError, match="tangent"):
+                call(**_decode(attention_mask=m))
+        with pytest.raises(RuntimeError, match="HIP tensors"):
+            prompt.prompt_attention(**_prompt())       # operands without one
+    with pytest.raises(RuntimeError, match="tangent|functorch|storage"):
+        torch.func.jvp(lambda q: prompt.prompt_attention(**_prompt(q=q)), (_prompt()["q"],),
+                       (torch.ones(5, 4, 64).half(),))
+
+
 def test_c_entries_refuse_before_device_work():
     lib = _native.load()
     E, U, W = _native.HELM_E_INVALID, _native.HELM_E_UNSUPPORTED, _native.HELM_E_WORKSPACE
