@@ -254,6 +254,13 @@ __device__ __forceinline__ void softcap_scores(float (&x)[N], float k, float cap
     for (int r = 0; r < N; ++r) x[r] = tanhf(x[r] * k) * cap;
   }
 }
+// Whether a call's scale and soft-cap (<= 0: off), their quotient and products with
+// log2 e are finite in fp32: a zero score times an infinity would be NaN.
+inline bool scores_ok(float scale, float softcap) {
+  constexpr float kMax = 0x1p126f;
+  if (!(fabsf(scale) <= kMax) || !(softcap <= kMax)) return false;
+  return !(softcap > 0.f) || (softcap >= 1.f / kMax && fabsf(scale) / softcap <= kMax);
+}
 
 // LDS transpose read of 16-bit elements (ds_read_b64_tr_b16): within each
 // 16-lane group, lane c = 4a + b receives element b of the 8 bytes that

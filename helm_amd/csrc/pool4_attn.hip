@@ -651,6 +651,8 @@ extern "C" int helm_pool4_decode_attn(const void* q, void* out, const void* pool
   if (mask && mask_dtype != HELM_F32 && mask_dtype != HELM_BF16 && mask_dtype != HELM_F16)
     return report_error(HELM_E_INVALID, "unknown mask dtype");
   if (mask && mask_len < 1) return report_error(HELM_E_INVALID, "mask without a column");
+  if (!scores_ok(scale, softcap))
+    return report_error(HELM_E_INVALID, "scale, softcap or their quotient out of fp32's range");
   if (B == 0) return HELM_OK;
   if (!q || !out || (!pool && n_slots) || (!page_table && max_pages) || !seq_lens)
     return report_error(HELM_E_INVALID, "null pointer argument");

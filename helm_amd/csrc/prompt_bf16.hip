@@ -24,8 +24,10 @@ extern "C" int helm_prompt_attn(const void* q, int64_t q_tok_stride, int64_t q_h
     return report_error(HELM_E_UNSUPPORTED, "prompt attention takes float16 or bfloat16");
   if (D != 64 && D != 128 && D != 256)
     return report_error(HELM_E_UNSUPPORTED, "prompt attention takes head_dim 64, 128 or 256");
-  if (B < 0 || N < 0 || Hq < 1 || Hkv < 1 || Hq % Hkv || !(scale == scale))
-    return report_error(HELM_E_INVALID, "bad prompt attention shape or scale");
+  if (B < 0 || N < 0 || Hq < 1 || Hkv < 1 || Hq % Hkv)
+    return report_error(HELM_E_INVALID, "bad prompt attention shape");
+  if (!scores_ok(scale, softcap))
+    return report_error(HELM_E_INVALID, "scale, softcap or their quotient out of fp32's range");
   if (N == 0) return HELM_OK;
   if (!q || !k || !v || !out || !cu_seqlens)
     return report_error(HELM_E_INVALID, "null pointer argument");

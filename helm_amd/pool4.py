@@ -24,6 +24,7 @@ from helm_amd.runtime import engine as _engine
 _DIMS = (64, 128, 256)
 _CODES = {torch.float16: _native.HELM_F16, torch.bfloat16: _native.HELM_BF16,
           torch.float32: _native.HELM_F32}
+_SCORE_MAX = 2.0 ** 126
 
 
 class Pool4:
@@ -177,13 +178,16 @@ def pool4_decode_attention(q: torch.Tensor, pool: Pool4, page_table: torch.Tenso
 
 
 def check_scores(scale: Optional[float], softcap: Optional[float], D: int) -> Tuple[float, float]:
-    """(scale, softcap or 0) of an attention call."""
+    """(scale, softcap or 0) of an attention call: numbers whose products in the kernels'
+    fp32 (by log2 e, by one another's inverse) stay finite."""
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     cap = 0.0 if softcap is None else float(softcap)
-    if not math.isfinite(scale):
-        raise ValueError("scale must be finite")
-    if not (0.0 <= cap < math.inf):
-        raise ValueError("softcap must be a positive number (None or 0: off)")
+    if not abs(scale) <= _SCORE_MAX:
+        raise ValueError("scale must be finite, 2^126 at most in magnitude")
+    if cap and not 1.0 / _SCORE_MAX <= cap <= _SCORE_MAX:
+        raise ValueError("softcap must be a positive number, 2^-126 to 2^126 (None or 0: off)")
+    if cap and abs(scale) / cap > _SCORE_MAX:
+        raise ValueError("scale / softcap must be 2^126 at most")
     return scale, cap
 
 

@@ -185,6 +185,29 @@ def test_prompt_refusals(bad, err):
         prompt.prompt_attention(**_prompt(**bad))
 
 
+@pytest.mark.parametrize("bad", [
+    dict(scale=1e300), dict(scale=-1e39), dict(softcap=1e39), dict(softcap=1e-60), dict(softcap=1e-39),
+    dict(softcap=math.nan), dict(scale=1e20, softcap=1e-20), dict(scale=-3e38)])
+def test_scores_out_of_fp32s_range_are_refused(bad):
+    """1e-60 is 0 in fp32, which would turn the cap off; a factor of infinity makes NaN of
+    zero scores."""
+    with pytest.raises(ValueError, match="scale|softcap"):
+        pool4.pool4_decode_attention(**_decode(**bad))
+    with pytest.raises(ValueError, match="scale|softcap"):
+        prompt.prompt_attention(**_prompt(**bad))
+    lib, E, BF = _native.load(), _native.HELM_E_INVALID, _native.HELM_BF16
+    scale, cap = bad.get("scale", 0.125), bad.get("softcap", 0.0)
+    if cap != 1e-60:                           # (0 as the C entries get it: off)
+        assert lib.helm_pool4_decode_attn(16, 16, 16, 1, 16, 16, 1, 1, 16, 1, 2, 1, 1, 64, scale, cap, None,
+                                          0, 0, 0, 0, BF, 0, BF, None, 0, None) == E
+        assert lib.helm_prompt_attn(16, 128, 64, 16, 64, 64, 16, 64, 64, 16, 128, 64, 16, 1, 1, 2, 1, 64,
+                                    scale, cap, 0, 0, BF, None) == E
+    for good in (dict(scale=0.0), dict(scale=2.0 ** 126), dict(softcap=2.0 ** -126),
+                 dict(softcap=2.0 ** 126), dict(softcap=0.0)):
+        with pytest.raises(RuntimeError, match="HIP tensors"):
+            prompt.prompt_attention(**_prompt(**good))
+
+
 def test_operands_that_ask_for_a_gradient_are_refused():
     a = _prompt()
     a["q"].requires_grad_()
