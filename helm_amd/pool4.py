@@ -170,7 +170,8 @@ def pool4_decode_attention(q: torch.Tensor, pool: Pool4, page_table: torch.Tenso
     [B|1, Hq|1, q_len|1, T], tokens from T on are hidden; causal: the q_len rows are
     the sequence's last tokens, each sees those up to its own.  Hidden tokens (-inf in
     the mask among them) take no part whatever they hold, and a row that sees nothing
-    is zeros.  Returns out [B, Hq, q_len, D] in q's dtype."""
+    is zeros.  out: contiguous; it may be q itself, but share memory with no other
+    operand.  Returns out [B, Hq, q_len, D] in q's dtype."""
     idx, args, out, _ = _decode_args(q, pool, page_table, seq_lens, max_pages, scale, softcap,
                                      attention_mask, causal, out)
     _engine.launch_on(idx, "helm_pool4_decode_attn", *args)
@@ -224,7 +225,8 @@ def _decode_args(q, pool, page_table, seq_lens, max_pages, scale, softcap, mask,
             m = m.contiguous()
         ms = tuple(m.stride(i) if m.size(i) > 1 else 0 for i in range(3))
         width = m.size(3)
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty((B, Hq, S, D), dtype=q.dtype, device=q.device)
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
         raise ValueError("out must be contiguous, of q's shape and dtype")
@@ -237,6 +239,9 @@ def _decode_args(q, pool, page_table, seq_lens, max_pages, scale, softcap, mask,
         if in_place:
             raise ValueError("a prepared call reads q in place: it must be 16-byte aligned")
         q = q.clone()
+    if given:
+        _engine.refuse_overlap("pool4_decode_attention", out, q, pool.data, page_table, seq_lens,
+                               *masks)
     lib = _native.load()
     need = lib.helm_pool4_workspace_bytes(B, Hq, pool.num_kv_heads, S, D, max_pages,
                                           pool.page_size)

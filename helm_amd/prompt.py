@@ -22,7 +22,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     b is rows cu_seqlens[b] .. cu_seqlens[b + 1] (int32 [B + 1] on the device, ascending
     within 0 .. N, as ``paged.batch_tables`` gives it).  window: a row sees its last
     `window` rows only, itself included.  Rows outside every sequence are left as they
-    are in `out`, and zeros where `out` is not given.  Returns [N, Hq, D] in q's dtype."""
+    are in `out`, and zeros where `out` is not given.  out: contiguous; it may be q itself,
+    but share memory with no other operand.  Returns [N, Hq, D] in q's dtype."""
     qs, kv = q.shape, k.shape
     if len(qs) != 3 or len(kv) != 3 or v.shape != kv or kv[0] != qs[0] or kv[2] != qs[2]:
         raise ValueError("q must be [N, Hq, D], k and v [N, Hkv, D]")
@@ -51,6 +52,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     q, *q_at = _rows16(q, 8)
     k, *k_at = _rows16(k, 8)
     v, *v_at = _rows16(v, 8)
+    if not rest:
+        _engine.refuse_overlap("prompt_attention", out, q, k, v, cu_seqlens)
     _engine.launch_on(idx, "helm_prompt_attn", *q_at, *k_at, *v_at, out.data_ptr(), Hq * D, D,
                       cu_seqlens.data_ptr(), B, N, Hq, Hkv, D, scale, cap,
                       min(window or 0, 0x7fffffff), rest, _CODES[dt])

@@ -94,6 +94,21 @@ def common_device(what: str, *tensors: torch.Tensor) -> int:
     return idx
 
 
+def refuse_overlap(what: str, out: torch.Tensor, *inputs: torch.Tensor) -> None:
+    """Refuses a contiguous `out` that shares memory with an operand (other workgroups
+    may still be reading it).  The first of them may be `out` itself: a workgroup
+    reads its own rows of it and then writes them."""
+    lo = out.data_ptr()
+    hi = lo + out.numel() * out.element_size()
+    for i, t in enumerate(inputs):
+        at = t.data_ptr()
+        if at >= hi or lo == hi or not t.numel() or (i == 0 and at == lo and t.is_contiguous()):
+            continue
+        span = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1
+        if at + span * t.element_size() > lo:
+            raise ValueError(f"{what}: out lies over another operand (only q itself may be out)")
+
+
 def refuse_grad(what: str, *tensors: torch.Tensor) -> None:
     """The package serves models: its attention records nothing for a backward pass, and
     has no tangent to give (which no_grad does not drop)."""

@@ -424,7 +424,8 @@ int helm_pool4_read(const void* pool, int64_t n_slots, int page_size, int Hkv, i
  * hidden.  Hidden tokens (those, past the limit, or under -inf) take no part
  * whatever they hold; a row that sees nothing is zeros.  Pages whose slot is
  * outside [0, n_slots), and tokens past max_pages, count as hidden.  q, out,
- * the pool and the workspace are 16-byte aligned.  The workspace
+ * the pool and the workspace are 16-byte aligned; out may be q, but lie over
+ * nothing else.  The workspace
  * (helm_pool4_workspace_bytes; 0: none needed) needs no contents before or
  * after a call; calls that may overlap need one each. */
 size_t helm_pool4_workspace_bytes(int B, int Hq, int Hkv, int q_len, int D, int max_pages,
@@ -447,7 +448,8 @@ int helm_pool4_decode_attn(const void* q, void* out, const void* pool, int64_t n
  * rows cu_seqlens[b] .. cu_seqlens[b + 1] (device int32, ascending; clamped to
  * [0, N]); row i of it sees rows j <= i, with window > 0 only j > i - window.
  * softcap <= 0: off.  Rows before cu_seqlens[0] and from cu_seqlens[B] on: left
- * as they are, or zeros with zero_rest != 0.  head_dim 64, 128 or 256. */
+ * as they are, or zeros with zero_rest != 0.  out may be q (at q's strides), but
+ * lie over nothing else.  head_dim 64, 128 or 256. */
 int helm_prompt_attn(const void* q, int64_t q_tok_stride, int64_t q_head_stride, const void* k,
                      int64_t k_tok_stride, int64_t k_head_stride, const void* v,
                      int64_t v_tok_stride, int64_t v_head_stride, void* out,

@@ -420,3 +420,12 @@ def test_rows_that_no_slot_names_keep_k_and_v(D, Hkv, page):
     k1, v1 = pool.read(every, dtype=torch.float32)
     k0[slots], v0[slots] = R.stored4(k).float(), R.stored4(v).float()
     assert torch.equal(k1, k0) and torch.equal(v1, v0)
+
+
+@pytest.mark.parametrize("lens,S", [([200, 31], 1), ([5000, 100], 4)])
+def test_out_may_be_q(lens, S):
+    c = _case(81, lens, 10, 2, 128, S, 16, torch.float16)
+    want = pool4.pool4_decode_attention(c["q"], c["pool"], c["table"], c["lens"], causal=True)
+    q = c["q"].clone()
+    assert pool4.pool4_decode_attention(q, c["pool"], c["table"], c["lens"], causal=True, out=q) is q
+    assert torch.equal(q, want)

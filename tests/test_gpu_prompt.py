@@ -277,3 +277,15 @@ def test_more_sequences_than_rows(heads):
     q, k, v = _case(1, 150, heads, 1, 64, torch.bfloat16)
     cu = torch.full((301,), 60, dtype=torch.int32, device=DEV)
     assert (prompt.prompt_attention(q, k, v, cu) == 0).all()
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("lens,Hq,Hkv", [([333, 1, 150], 4, 2), ([700, 400], 40, 8)])
+def test_out_may_be_q(D, lens, Hq, Hkv):
+    n = sum(lens) + 5
+    q, k, v = (x.contiguous() for x in _case(D, n, Hq, Hkv, D, torch.bfloat16))
+    v[100, :, 3] = math.nan                     # (some workgroups walk twice)
+    want, rest = prompt.prompt_attention(q, k, v, _cu(lens)), q[sum(lens):].clone()
+    assert prompt.prompt_attention(q, k, v, _cu(lens), out=q) is q
+    same = (q == want) | (torch.isnan(q) & torch.isnan(want))
+    assert same[:sum(lens)].all() and torch.equal(q[sum(lens):], rest)

@@ -185,6 +185,40 @@ def test_prompt_refusals(bad, err):
         prompt.prompt_attention(**_prompt(**bad))
 
 
+def test_out_over_another_operand_is_refused(monkeypatch):
+    monkeypatch.setattr(prompt._engine, "common_device", lambda what, *t: 0)
+    monkeypatch.setattr(prompt._engine, "launch_on", lambda idx, fn, *args: 0)
+    back = torch.zeros(16 * 4 * 64).half()
+    qkv = torch.zeros(3, 5, 4, 64).half()
+
+    def prom(out, **kw):
+        a = dict(q=qkv[0], k=qkv[1, :, :2], v=qkv[2, :, :2], cu_seqlens=torch.tensor([0, 5], dtype=I32))
+        return prompt.prompt_attention(**dict(a, **kw), out=out)
+    for out in (qkv[1], qkv[2], qkv.view(-1)[256:256 + 1280].view(5, 4, 64),
+                qkv.view(-1)[1280 - 8:2560 - 8].view(5, 4, 64)):
+        with pytest.raises(ValueError, match="out lies over"):
+            prom(out)
+    with pytest.raises(ValueError, match="out lies over"):
+        prom(back[:1280].view(5, 4, 64), cu_seqlens=back[1270:1274].view(I32))
+    fused = torch.zeros(5, 8, 64).half()
+    with pytest.raises(ValueError, match="out lies over"):           # q's rows, but not at q's strides
+        prom(fused.view(-1)[:1280].view(5, 4, 64), q=fused[:, :4])
+    for out in (qkv[0], torch.zeros(5, 4, 64).half(), back[:1280].view(5, 4, 64)):
+        assert prom(out, cu_seqlens=back[1280:1284].view(I32)) is out
+    turned = torch.zeros(4, 5, 64).half().transpose(0, 1)
+    assert prom(torch.zeros(5, 4, 64).half(), q=turned).shape == (5, 4, 64)
+    assert prom(torch.zeros(0, 4, 64).half(), q=qkv[0, :0], k=qkv[1, :0, :2], v=qkv[2, :0, :2]).numel() == 0
+
+    d = _decode()
+    mask = torch.zeros(2, 4, 1, 64).bfloat16()
+    for out, kw in ((mask, dict(attention_mask=mask)),
+                    (d["pool"].data.view(-1)[4096:4096 + 1024].view(torch.bfloat16).view(2, 4, 1, 64), {})):
+        for call in (pool4.pool4_decode_attention, pool4.prepare_pool4_decode):
+            with pytest.raises(ValueError, match="out lies over"):
+                call(**dict(d, **kw), out=out)
+    assert pool4.pool4_decode_attention(**d, out=d["q"]) is d["q"]
+
+
 @pytest.mark.parametrize("bad", [
     dict(scale=1e300), dict(scale=-1e39), dict(softcap=1e39), dict(softcap=1e-60), dict(softcap=1e-39),
     dict(softcap=math.nan), dict(scale=1e20, softcap=1e-20), dict(scale=-3e38)])
