@@ -62,7 +62,7 @@ __device__ __forceinline__ P4Place p4_place(const P4Rows& a, int64_t slot) {
     s = slot / a.page;
     r = (int)(slot - s * a.page);
   }
-  return {a.pool + s * a.slot_bytes + (r / kP4Tok) * P4<D>::kBytes, r % kP4Tok};
+  return {a.pool + s * a.slot_bytes + (int64_t)(r / kP4Tok) * P4<D>::kBytes, r % kP4Tok};
 }
 
 // Byte of the codes of dims 8c .. 8c + 7 of token t (V at D = 64: the first of its two

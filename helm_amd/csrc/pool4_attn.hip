@@ -305,7 +305,9 @@ __global__ __launch_bounds__(64 * kP4Waves) void pool4_attn_kernel(P4Attn a) {
       // (a slot that the pool does not have hides its tile)
       const bool there = (j < mine) & (2 * (blk0 + hop * j) + s < sq.tiles) &
                          ((uint32_t)slot < (uint32_t)a.n_slots);
-      const char* tile = head_base + (there ? slot : 0) * a.slot_bytes + in[s] * P4<D>::kBytes;
+      // (64 bits: a page of eight million tokens of 256 dims passes 2^31 bytes)
+      const char* tile = head_base + (there ? slot : 0) * a.slot_bytes +
+                         (int64_t)in[s] * P4<D>::kBytes;
       k.r[s] = p4_load<D>(tile, there, n, h);
       if (!there) k.gone |= 1 << s;
     }

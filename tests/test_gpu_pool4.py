@@ -429,3 +429,27 @@ def test_out_may_be_q(lens, S):
     q = c["q"].clone()
     assert pool4.pool4_decode_attention(q, c["pool"], c["table"], c["lens"], causal=True, out=q) is q
     assert torch.equal(q, want)
+
+
+@pytest.mark.parametrize("D,page", [(64, 2 ** 25), (128, 2 ** 24 + 48), (256, 2 ** 23 + 32)])
+def test_one_page_past_32_bits(D, page):
+    """A page of more than 2^31 bytes a head: rows before, at and behind that byte, and the last."""
+    pool = pool4.Pool4(1, 1, D, page_size=page, device=DEV)
+    assert pool.data.numel() > 2 ** 31
+    edge = 2 ** 31 // (17 * D) * 16
+    slots = torch.tensor([edge - 3, edge + 5, edge + 21, page - 1, 7], device=DEV)
+    k, v = torch.zeros(5, 1, D, device=DEV), _randn(2, 5, 1, D)
+    k[:, 0, 0] = 128.0
+    pool.write(k, v, slots)
+    rk, rv = pool.read(slots, dtype=torch.float32)
+    assert torch.equal(rk, k) and torch.equal(rv.double(), R.stored4(v))
+    # 102 nats above everything else, which holds zeros: its V
+    q = torch.zeros(1, 2, 1, D, dtype=torch.bfloat16, device=DEV)
+    q[..., 0] = 8.0
+    table = torch.zeros(1, 1, dtype=torch.int32, device=DEV)
+    for i in range(4):
+        pool.data.zero_()
+        pool.write(k[i:i + 1], v[i:i + 1], slots[i:i + 1])
+        n = torch.tensor([int(slots[i]) + 1], dtype=torch.int32, device=DEV)
+        out = pool4.pool4_decode_attention(q, pool, table, n, scale=0.1)
+        assert torch.equal(out[0, :, 0].double(), R.stored4(v[i]).expand(2, D).bfloat16().double())
