@@ -9,7 +9,8 @@
 // On N(0, 1) rows that keeps an rms error of 0.1119 of the values' rms, against
 // 0.1149 where the group's exponent is the largest value's (which cuts 6 to 8
 // down to 6) and 0.1155 where no value is cut.  A group that holds an infinity
-// or NaN has the exponent byte 255 and stands for NaN.
+// or NaN has the exponent byte 255 and stands for NaN; bytes that no write leaves
+// (below 2, 253, 254) are hidden tokens' only, and attention takes 253 and 254 for 255.
 //
 // The limits of e keep every code times 2^e a normal bf16 and fp32 number, so
 // that the matrix cores' bf16 operands hold K and V exactly (f16 would not: its

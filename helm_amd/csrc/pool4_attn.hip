@@ -151,9 +151,10 @@ __device__ __forceinline__ mf_u32x2 load8_any(const char* p) {
   return reinterpret_cast<const Any*>(p)->v;
 }
 
-// Any byte of x equal to 255.
-__device__ __forceinline__ bool any_ff(uint32_t x) {
-  return ((~x - 0x01010101u) & x & 0x80808080u) != 0u;
+// Any byte of x or y from 192 on: a group past 2^65, a NaN (255), or a byte that no write leaves
+// (253 and 254, whose codes pass bf16's range).
+__device__ __forceinline__ bool any_high(uint32_t x, uint32_t y) {
+  return (((x & (x << 1)) | (y & (y << 1))) & 0x80808080u) != 0u;
 }
 
 __device__ __forceinline__ void add_scaled(float4& acc, float f, const float4 v) {
@@ -394,13 +395,13 @@ __global__ __launch_bounds__(64 * kP4Waves) void pool4_attn_kernel(P4Attn a) {
       hi[j] = a0;
       lo[j] = b0;
     }
-    const bool nan = __builtin_amdgcn_ballot_w64(any_ff(r[0].ve) || any_ff(r[1].ve)) != 0;
+    const bool high = __builtin_amdgcn_ballot_w64(any_high(r[0].ve, r[1].ve)) != 0;
     uint32_t ff = 0;                         // bit j: token j's group stands for NaN
-    if (__builtin_expect(nan, 0)) {
+    if (__builtin_expect(high, 0)) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         uint32_t& ve = r[j >> 2].ve;
-        if (((ve >> (8 * (j & 3))) & 255u) == 255u) {
+        if (((ve >> (8 * (j & 3))) & 255u) > 252u) {
           ff |= 1u << j;
           ve &= ~(255u << (8 * (j & 3)));
         }
@@ -423,7 +424,7 @@ __global__ __launch_bounds__(64 * kP4Waves) void pool4_attn_kernel(P4Attn a) {
       o[2 * c] = Ops::mma(even, lo, o[2 * c]);
       o[2 * c + 1] = Ops::mma(odd, lo, o[2 * c + 1]);
     }
-    if (__builtin_expect(nan, 0)) {
+    if (__builtin_expect(high, 0)) {
       // ones at the NaN tokens (a whole chunk lies in one group) times ones at those that
       // the row sees (not its weights, which may be zero by rounding): a row that sees any
       // gets NaN in every dim of the chunk, and no later factor takes that away

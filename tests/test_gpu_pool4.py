@@ -453,3 +453,43 @@ def test_one_page_past_32_bits(D, page):
         n = torch.tensor([int(slots[i]) + 1], dtype=torch.int32, device=DEV)
         out = pool4.pool4_decode_attention(q, pool, table, n, scale=0.1)
         assert torch.equal(out[0, :, 0].double(), R.stored4(v[i]).expand(2, D).bfloat16().double())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("T", [70, 1400])
+def test_hidden_tokens_may_hold_any_bytes(dtype, D, T):
+    """Tokens inside the sequence that were never written, under -inf or past a row's
+    causal limit: any exponent byte, 253 and 254 among them."""
+    c = _case(D + T, [T], 2, 1, D, 2, 16, dtype)
+    g = torch.Generator(device=DEV).manual_seed(T)
+    c["pool"].data.copy_(torch.randint(244, 256, c["pool"].data.shape, generator=g, device=DEV))
+    live = torch.arange(3, T - 1, 2)                     # (the second row sees T - 1 under -inf)
+    k, v = _randn(1, T, 1, D), _randn(2, T, 1, D)
+    slots = (c["table"].cpu()[0][live // 16].long() * 16 + live % 16).to(DEV)
+    live = live.to(DEV)
+    c["pool"].write(k[live], v[live], slots)
+    m = torch.full((1, 1, 2, T), -math.inf, device=DEV)
+    m[..., live] = 0.0
+    m[:, :, 0, T - 1] = 0.0                              # (hidden by the causal limit)
+    c["ks"], c["vs"] = [R.stored4(k)], [R.stored4(v)]
+    out = pool4.pool4_decode_attention(c["q"], c["pool"], c["table"], c["lens"], attention_mask=m,
+                                       causal=True)
+    _assert_close(c, out, True, mask=m)
+    assert torch.isfinite(out).all()
+
+
+def test_the_largest_groups_are_attended():
+    """Exponents of 252, the largest that a write leaves, are values and no NaN."""
+    c = _case(7, [40], 2, 1, 64, 1, 16, torch.bfloat16)
+    k, v = 0 * _randn(1, 40, 1, 64), _randn(2, 40, 1, 64)
+    v[17] *= 2.0 ** 126
+    v[17, 0, 5], v[17, 0, 40] = 6 * 2.0 ** 125, -6 * 2.0 ** 125
+    pos = torch.arange(40)
+    slots = (c["table"].cpu()[0][pos // 16].long() * 16 + pos % 16).to(DEV)
+    c["pool"].write(k, v, slots)
+    out = pool4.pool4_decode_attention(c["q"], c["pool"], c["table"], c["lens"])
+    want = R.stored4(v)[:, 0].mean(0)
+    # (equal weights: the sum of 40 exact values in fp32, 1 / 40, the output's rounding)
+    assert ((out[0, :, 0].double() - want).abs()
+            <= 2.0 ** -8 * want.abs() + 45 * 2.0 ** -24 * R.stored4(v).abs().max() / 40).all()
