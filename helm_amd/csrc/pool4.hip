@@ -9,7 +9,7 @@
 // rows of a tile, which share cache lines, meet in one L2 instead of leaving it in
 // parts.  16,384 rows of 8 heads of 128, bf16, write / read: a thread a row and place
 // 31 / 28.5 us (half of it divisions), four rows 26 / 22, on one XCD 18.8 / 18.9, two
-// rows 18.1 / 17.5 (8: 21 / 24); 85 MB each, 16.7 us at a large copy's rate.
+// rows 18.1 / 17.5 (8: 21 / 24); 85 MB each, 14.7 us at 5.78 TB/s.
 // The conversions of gfx950 encode and decode two values an instruction, exactly and
 // with ties to the even code (checked over every code and exponent).
 #include "pool4.h"

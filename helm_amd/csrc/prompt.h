@@ -14,16 +14,19 @@
 //         transpose reads.  O register 4g + t of dim group e is dim
 //         32 e + 8 g + 4 hh + t of row jr.
 // So a row's scores, maximum, sum and output sit in the two lanes (*, jr).  The
-// running maximum is refreshed only when a score passes it by 2^8 (base-2 units).
-// Weights are rounded once to the 16-bit type (by half a step, 2^-8 or 2^-11 at most, of the
-// weight, at random: below the output's own rounding) and the row's sum adds the
-// rounded ones; f16 weights are taken times 2^9 (weight_shift: nothing above 2^-34
-// of the largest is lost).
+// running maximum is refreshed only when a score passes it by 2^8 (f16: 2^6) in weight.
+// Weights are rounded once to the 16-bit type, by half a step: 2^-8 (bf16) or 2^-11 (f16) of
+// the weight at most, at random, and the row's sum adds the rounded ones.  f16 weights are
+// taken times 2^9; those below 2^-23 of the running maximum's fall under the type's normal
+// range and are off by 2^-34 of that at most.  An output's relative rms error is 2.0e-3 to
+// 2.1e-3 in bf16 and 2.2e-4 to 2.6e-4 in f16, against 1.6e-3 and 1.9e-4 to 2.0e-4 where weights
+// stay in fp32 (its own rounding); the low parts of the weights would be a second product of P . V, half
+// as much matrix work again.
 //
 // Hidden tokens take no part whatever they hold: their scores are overwritten,
 // and an infinity or NaN in V (which would turn a weight of zero into NaN) shows
 // as NaN in an output, upon which the workgroup walks again with V's infinities
-// and NaN taken out of the products and added where a row weighs them (careful).
+// and NaN taken out of the products and added where a row sees them (careful).
 #pragma once
 
 #include <type_traits>
@@ -67,11 +70,17 @@ struct PromptParams {
 // workgroup then loads K and V for 32 rows, not 128 or 256, so this is for launches that
 // leave CUs idle: up to 512 such tiles (times heads), which are resident together (one a
 // CU, two rounds, at D = 256; up to 640 at D = 64, three a CU), or 1,280 where the sequences
-// are 2,048 tokens on average and an extra round's start and join are small beside the walks.  bf16, 8 / 2 heads, us without
-// and with: 1,200 tokens D = 64 20.8 -> 11.7, 128 29.7 -> 16.7, 256 67 -> 28; 4,800 tokens
-// (1,208 tiles) 69 -> 46, 103 -> 80, 241 -> 185.  Beyond, it loses: 4 of 1,200 (1,232 tiles)
-// 22.0 -> 21.4, 32.9 -> 37.0, 72 -> 86; 32 / 8 heads, 4 of 150 (736) 6.7 -> 7.6, 9.3 -> 14.1,
-// 18 -> 30; 600 tokens (640) 13.3 -> 10.0, 19.3 -> 18.2, 37 -> 39.  Eight waves: 8 / 2 heads, 2,400 tokens D = 64 19.8 -> 24.8, D = 128 28 -> 39.
+// are 2,048 tokens on average and an extra round's start and join are small beside the
+// walks.  The host knows N and B alone: a padded N counts as rows, and one long prompt
+// among short ones as their average.
+// bf16, us without and with, D = 64 / 128 / 256:
+//   8 / 2 heads, 1,200 tokens            20.8 -> 11.7, 29.7 -> 16.7, 67 -> 28
+//   8 / 2 heads, 4,800 (1,208 tiles)     69 -> 46,     103 -> 80,    241 -> 185
+//   32 / 8 heads, 600 (640)              13.3 -> 10.0, 19.3 -> 18.2, 37 -> 39
+// and beyond, where it loses:
+//   8 / 2 heads, 4 of 1,200 (1,232)      22.0 -> 21.4, 32.9 -> 37.0, 72 -> 86
+//   32 / 8 heads, 4 of 150 (736)         6.7 -> 7.6,   9.3 -> 14.1,  18 -> 30
+// Eight waves for four, 8 / 2 heads, 2,400 tokens: D = 64 19.8 -> 24.8, 128 28 -> 39.
 template <int D> struct PromptSplit {
   static constexpr int kWaves = 4, kPerSimd = D == 256 ? 1 : 2;
   static constexpr int kTiles = D == 64 ? 640 : 512, kTilesLong = 1280;
@@ -468,7 +477,7 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
     }
     const float base = m == -INFINITY ? 0.f : m - kShift;
     uint32_t w[8];
-    uint32_t some[8];                          // careful: 1 where the formula weighs the token
+    uint32_t some[8];                          // careful: 1 where the row sees the token
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float w0 = __builtin_amdgcn_exp2f(fmaf(x[2 * i], mul, -base));

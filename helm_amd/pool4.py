@@ -64,8 +64,9 @@ class Pool4:
     def write(self, k: torch.Tensor, v: torch.Tensor, slot_map: torch.Tensor) -> None:
         """Rows n of k and v ([n, Hkv, D] float16, bfloat16 or float32, any strides) into
         row slot_map[n] (int64, slot * page_size + token; outside the pool, -1 for
-        instance: skipped).  Rows of one call that share a slot leave either's values,
-        group by group: give each its own."""
+        instance: skipped).  Each row needs a slot of its own: what two rows of one call
+        leave in one they share is undefined (codes of one under the other's exponents;
+        other rows are as they should be)."""
         n = self._slots(slot_map)
         want = (n, self.num_kv_heads, self.head_dim)
         if k.shape != want or v.shape != want:

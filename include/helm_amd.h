@@ -404,8 +404,8 @@ int helm_batch_tables(const int32_t* new_lens, const int32_t* cached_lens, int B
  * helm_pool4_write: row n of k and v ([n_tok, Hkv, D], strides in elements, D
  * contiguous, rows 16-byte aligned, HELM_F16 / BF16 / F32) into row
  * slot_map[n] = slot * page_size + token of the pool; rows outside
- * [0, n_slots * page_size) are skipped.  Two rows of one call with the same
- * slot leave either's values, group by group.
+ * [0, n_slots * page_size) are skipped.  What two rows of one call leave in a
+ * slot that they share is undefined; no other row is affected.
  * helm_pool4_read: the values of those rows, exact but for the rounding to
  * the output type; zeros for rows outside the pool. */
 int helm_pool4_write(void* pool, int64_t n_slots, int page_size, int Hkv, int D,
