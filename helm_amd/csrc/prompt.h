@@ -20,8 +20,8 @@
 // taken times 2^9; those below 2^-23 of the running maximum's fall under the type's normal
 // range and are off by 2^-34 of that at most.  An output's relative rms error is 2.0e-3 to
 // 2.1e-3 in bf16 and 2.2e-4 to 2.6e-4 in f16, against 1.6e-3 and 1.9e-4 to 2.0e-4 where weights
-// stay in fp32 (its own rounding); the low parts of the weights would be a second product of P . V, half
-// as much matrix work again.
+// stay in fp32 (its own rounding); the low parts of the weights would be a second product
+// of P . V, half as much matrix work again.
 //
 // Hidden tokens take no part whatever they hold: their scores are overwritten,
 // and an infinity or NaN in V (which would turn a weight of zero into NaN) shows
