@@ -1,0 +1,798 @@
+// Beam search over a paged cache: the choice of a step's continuations (helm_beam_select)
+// and the block tables that follow from it (helm_beam_tables).
+//
+// Selection.  Beam k of a request with running score s_k offers token t at
+//   s_k + x_kt - lse_k,   lse_k = log(sum over t of e^{x_kt}),
+// and the n best of the request's K V candidates are wanted, ties to the lowest k V + t.
+// Within a row the order is the logits' own, so one pass over them gives a chunk's
+// largest value, its sum and its n best, and the rows meet in a second, small kernel.
+// Bound by memory: the logits are read once.  The order between rows is of sums, which are
+// formed in 64 bits: exponentials in 32 (off by 2^-23 each, their argument exact to that),
+// their sums, logarithms and the scores in 64, so that lse is off by about 1e-8 and two
+// candidates change places only where their scores are as near as that.
+//
+// A chunk's n best: the n-th largest of a wave's 64 lane maxima (a search over the bits of
+// the value with ballots) is at most the n-th largest of its values; the largest such bound
+// of the four waves leaves few values, which are put in a list and ranked by counting.  Where
+// ties or a sorted row leave more than the list holds, the workgroup searches value and
+// index bit by bit instead.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <cfloat>
+#include <string>
+
+#include "attn_kernel.h"
+#include "helm_amd.h"
+#include "ranges.h"
+
+namespace helm {
+int report_error(int code, const std::string& msg);
+}
+
+namespace {
+
+using helm::bf16_t;
+using helm::f16_t;
+
+constexpr int kBeamThreads = 256;
+constexpr int kBeamWaves = kBeamThreads / 64;
+constexpr int kList = 512;                   // values that a chunk's bound may leave
+constexpr int kJoinList = 2048;              // and a request's
+
+struct SelectArgs {
+  const void* logits;
+  int64_t b_stride, k_stride;                // elements
+  const float* scores;
+  int B, K, V, n, chunks;
+  double* part_sum;                          // [B K][chunks]
+  float* part_max;                           // [B K][chunks]
+  float* cand_x;                             // [B][n][K chunks], -inf: none; a chunk's n best are
+  int* cand_t;                               // a column, best first
+  float* out_scores;
+  int64_t* out_tokens;
+  int32_t* out_parents;
+};
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+struct __attribute__((packed)) Any16 { u32x4 v; };
+
+// e^d for d <= 0 (NaN: NaN), its argument in base 2 as a whole number and an exact rest.
+__device__ __forceinline__ float exp_low(float d) {
+  d = d < -150.f ? -150.f : d;                // (zero from there on)
+  const float n = rintf(d * 1.44269504f);
+  const float f = fmaf(d, 1.44269504f, -n) + d * 1.92596299e-8f;   // log2 e = hi + lo
+  return ldexpf(__builtin_amdgcn_exp2f(f), (int)n);
+}
+
+// Whole numbers in the order of the floats (no NaN).
+__device__ __forceinline__ uint32_t ordered(float x) {
+  const uint32_t u = __float_as_uint(x + 0.f);          // (-0 is +0)
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float unordered(uint32_t u) {
+  return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
+}
+__device__ __forceinline__ uint64_t ordered(double x) {
+  const uint64_t u = (uint64_t)__double_as_longlong(x + 0.0);
+  return u >> 63 ? ~u : u | 0x8000000000000000ull;
+}
+__device__ __forceinline__ double unordered(uint64_t u) {
+  return __longlong_as_double((long long)(u >> 63 ? u & 0x7fffffffffffffffull : ~u));
+}
+// The n-th largest of the wave's 64 keys (1 <= n <= 64).
+template <typename U> __device__ __forceinline__ U wave_nth(U key, int n) {
+  U t = 0;
+#pragma unroll
+  for (int b = 8 * (int)sizeof(U) - 1; b >= 0; --b) {
+    const U c = t | (U)1 << b;
+    if (__builtin_popcountll(__builtin_amdgcn_ballot_w64(key >= c)) >= n) t = c;
+  }
+  return t;
+}
+
+__device__ __forceinline__ int block_sum(int x, int* sh) {
+#pragma unroll
+  for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d, 64);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = x;
+  __syncthreads();
+  int s = 0;
+#pragma unroll
+  for (int w = 0; w < kBeamWaves; ++w) s += sh[w];
+  return s;
+}
+
+template <typename T> struct Elem;           // the values of 16 bytes
+template <> struct Elem<float> {
+  static constexpr int kPer = 4;
+  __device__ static float get(const u32x4& w, int j) { return __uint_as_float(w[j]); }
+};
+template <> struct Elem<bf16_t> {
+  static constexpr int kPer = 8;
+  __device__ static float get(const u32x4& w, int j) {
+    return __uint_as_float(j & 1 ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16);
+  }
+};
+template <> struct Elem<f16_t> {
+  static constexpr int kPer = 8;
+  __device__ static float get(const u32x4& w, int j) {
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)(w[j >> 1] >> (16 * (j & 1))));
+  }
+};
+
+// Chunk blockIdx.x of row blockIdx.y: its maximum, sum and n best.  A thread holds NV runs
+// of 16 bytes in registers, a chunk is 256 times that.
+template <typename T, int NV>
+__global__ __launch_bounds__(kBeamThreads) void beam_scan_kernel(SelectArgs a) {
+  constexpr int E = Elem<T>::kPer;
+  constexpr int kSize = kBeamThreads * NV * E;
+  __shared__ float sh_max[kBeamWaves];
+  __shared__ uint32_t sh_bound[kBeamWaves];
+  __shared__ double sh_sum[kBeamWaves];
+  __shared__ int sh_n[kBeamWaves], sh_count;
+  __shared__ float list_x[kList];
+  __shared__ int list_t[kList];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int row = blockIdx.y, n = a.n;
+  const int first = blockIdx.x * kSize;
+  const T* x = reinterpret_cast<const T*>(a.logits) + row / a.K * a.b_stride +
+               row % a.K * a.k_stride + first;
+  const int left = a.V - first;               // values of this chunk and those behind it
+  u32x4 raw[NV];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int at = (v * kBeamThreads + tid) * E;
+    if (at + E <= left) {
+      raw[v] = reinterpret_cast<const Any16*>(x + at)->v;   // (rows at any alignment)
+    } else {
+      // the row's last values and -inf behind them
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (sizeof(T) == 4) {
+          w[j] = at + j < left ? reinterpret_cast<const uint32_t*>(x)[at + j] : 0xff800000u;
+        } else {
+          const uint32_t none = sizeof(T) == 2 && __is_same(T, bf16_t) ? 0xff80u : 0xfc00u;
+          const uint16_t* h = reinterpret_cast<const uint16_t*>(x);
+          const uint32_t lo = at + 2 * j < left ? h[at + 2 * j] : none;
+          const uint32_t hi = at + 2 * j + 1 < left ? h[at + 2 * j + 1] : none;
+          w[j] = lo | hi << 16;
+        }
+      }
+      raw[v] = u32x4{w[0], w[1], w[2], w[3]};
+    }
+  }
+  if (tid == 0) sh_count = 0;
+  float top = -INFINITY;
+#pragma unroll
+  for (int v = 0; v < NV; ++v)
+#pragma unroll
+    for (int j = 0; j < E; ++j) top = fmaxf(top, Elem<T>::get(raw[v], j));
+  float m = top;
+#pragma unroll
+  for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+  const uint32_t bound = wave_nth(ordered(top), n);
+  if (lane == 0) {
+    sh_max[wave] = m;
+    sh_bound[wave] = bound;
+  }
+  __syncthreads();
+  uint32_t b0 = 0;
+#pragma unroll
+  for (int w = 0; w < kBeamWaves; ++w) {
+    m = fmaxf(m, sh_max[w]);
+    b0 = max(b0, sh_bound[w]);
+  }
+  const float least = unordered(b0);
+
+  // the sum (NaN where the row has one or an infinity), and the list
+  const float base = m == -INFINITY ? 0.f : m;
+  float part = 0.f;
+#pragma unroll
+  for (int v = 0; v < NV; ++v)
+#pragma unroll
+    for (int j = 0; j < E; ++j) part += exp_low(Elem<T>::get(raw[v], j) - base);
+  double sum = part;
+#pragma unroll
+  for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
+  if (lane == 0) sh_sum[wave] = sum;
+  // (of a thread's values, those that may be among the n best: none of most threads')
+  if (top >= least && top > -INFINITY) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const float y = Elem<T>::get(raw[v], j);
+        if (y >= least && y > -INFINITY) {
+          const int i = atomicAdd(&sh_count, 1);
+          if (i < kList) {
+            list_x[i] = y;
+            list_t[i] = (v * kBeamThreads + tid) * E + j;
+          }
+        }
+      }
+  }
+  __syncthreads();
+  const int64_t p = (int64_t)row * a.chunks + blockIdx.x;
+  if (tid == 0) {
+    a.part_max[p] = m;
+    a.part_sum[p] = (sh_sum[0] + sh_sum[1]) + (sh_sum[2] + sh_sum[3]);
+  }
+  int count = sh_count;
+  if (count > kList) {
+    // exactly n: the n-th largest value, and how far among its equals
+    auto at_least = [&](uint32_t key) {
+      int c = 0;
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int j = 0; j < E; ++j) c += ordered(Elem<T>::get(raw[v], j)) >= key;
+      return block_sum(c, sh_n);
+    };
+    uint32_t key = 0;
+    for (int b = 31; b >= 0; --b) {
+      const uint32_t c = key | 1u << b;
+      if (at_least(c) >= n) key = c;
+    }
+    const float edge = unordered(key);
+    const int need = n - at_least(key + 1);
+    int last = 0;                             // of the equals, those before it are less than need
+    for (int b = 30; b >= 0; --b) {
+      const int c = last | 1 << b;
+      if (c >= kSize) continue;
+      int k = 0;
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+          k += Elem<T>::get(raw[v], j) == edge && (v * kBeamThreads + tid) * E + j < c;
+      if (block_sum(k, sh_n) < need) last = c;
+    }
+    __syncthreads();
+    if (tid == 0) sh_count = 0;
+    __syncthreads();
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const float y = Elem<T>::get(raw[v], j);
+        const int t = (v * kBeamThreads + tid) * E + j;
+        if (y > edge || (y == edge && t <= last)) {
+          const int i = atomicAdd(&sh_count, 1);
+          if (i < kList) {
+            list_x[i] = y;
+            list_t[i] = t;
+          }
+        }
+      }
+    __syncthreads();
+    count = min(sh_count, kList);
+  }
+  const int lists = a.K * a.chunks;
+  const int64_t col = (int64_t)(row / a.K) * n * lists + row % a.K * a.chunks + blockIdx.x;
+  float* cx = a.cand_x + col;
+  int* ct = a.cand_t + col;
+  for (int i = tid; i < count; i += kBeamThreads) {
+    const float y = list_x[i];
+    const int t = list_t[i];
+    int rank = 0;
+    for (int k = 0; k < count; ++k) {
+      const float z = list_x[k];
+      rank += z > y || (z == y && list_t[k] < t);
+    }
+    if (rank < n) {
+      cx[rank * lists] = y;
+      ct[rank * lists] = first + t;
+    }
+  }
+  for (int i = count + tid; i < n; i += kBeamThreads) {
+    cx[i * lists] = -INFINITY;
+    ct[i * lists] = 0;
+  }
+}
+
+// The n best of request blockIdx.x from its rows' chunks.
+__global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(SelectArgs a) {
+  __shared__ double base[64];                // s_k - lse_k; -inf: the row offers nothing
+  __shared__ uint64_t sh_bound[kBeamWaves];
+  __shared__ int sh_n[kBeamWaves], sh_count;
+  __shared__ double list_x[kJoinList];
+  __shared__ int64_t list_i[kJoinList];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int b = blockIdx.x, n = a.n, C = a.chunks;
+  if (tid == 0) sh_count = 0;
+  for (int k = wave; k < a.K; k += kBeamWaves) {
+    const int64_t p = ((int64_t)b * a.K + k) * C;
+    float m = -INFINITY;
+    for (int c = lane; c < C; c += 64) m = fmaxf(m, a.part_max[p + c]);
+#pragma unroll
+    for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+    double s = 0.0;
+    for (int c = lane; c < C; c += 64) {
+      // (a chunk's own -inf maximum has a sum of zero, or of NaN)
+      const float mc = a.part_max[p + c];
+      s += mc == -INFINITY ? a.part_sum[p + c]
+                           : a.part_sum[p + c] * exp((double)mc - (double)m);
+    }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d, 64);
+    if (lane == 0) {
+      const float score = a.scores[b * a.K + k];
+      const double x = (double)score - ((double)m + log(s));
+      base[k] = fabsf(score) < INFINITY && fabs(x) < INFINITY ? x : -INFINITY;
+    }
+  }
+  __syncthreads();
+  // candidate i of the request: of list i % (K C), that is of a row's chunk, the (i / (K C))th
+  const int lists = a.K * C, all = lists * n;
+  const float* cx = a.cand_x + (int64_t)b * all;
+  const int* ct = a.cand_t + (int64_t)b * all;
+  auto value = [&](int i) {
+    const double s = base[i % lists / C];
+    return s == -INFINITY ? s : s + (double)cx[i];
+  };
+  auto index = [&](int i) { return (int64_t)(i % lists / C) * a.V + ct[i]; };
+  double top = -INFINITY;
+  for (int i = tid; i < min(all, max(lists, kBeamThreads)); i += kBeamThreads)
+    top = fmax(top, value(i));
+  const uint64_t bound = wave_nth(ordered(top), n);
+  if (lane == 0) sh_bound[wave] = bound;
+  __syncthreads();
+  uint64_t b0 = 0;
+#pragma unroll
+  for (int w = 0; w < kBeamWaves; ++w) b0 = max(b0, sh_bound[w]);
+  const double least = unordered(b0);
+  auto keep = [&](double y, int i) {
+    const int at = atomicAdd(&sh_count, 1);
+    if (at < kJoinList) {
+      list_x[at] = y;
+      list_i[at] = index(i);
+    }
+  };
+  // the lists side by side from their best on, until none of them has one left
+  const int sweep = (lists + kBeamThreads - 1) / kBeamThreads * kBeamThreads;
+  for (int i0 = 0; i0 < all; i0 += sweep) {
+    bool any = false;
+    for (int i = i0 + tid; i < min(all, i0 + sweep); i += kBeamThreads) {
+      const double y = value(i);
+      if (y >= least && y > -INFINITY) {
+        any = true;
+        keep(y, i);
+      }
+    }
+    if (!__syncthreads_or(any)) break;
+  }
+  int count = sh_count;
+  if (count > kJoinList) {
+    auto counted = [&](auto wanted) {
+      int c = 0;
+      for (int i = tid; i < all; i += kBeamThreads) c += wanted(value(i), i);
+      return block_sum(c, sh_n);
+    };
+    uint64_t key = 0;
+    for (int bit = 63; bit >= 0; --bit) {
+      const uint64_t c = key | 1ull << bit;
+      if (counted([&](double y, int) { return ordered(y) >= c; }) >= n) key = c;
+    }
+    const double edge = unordered(key);
+    const int need = n - counted([&](double y, int) { return ordered(y) > key; });
+    int64_t last = 0;
+    for (int bit = 40; bit >= 0; --bit) {
+      const int64_t c = last | 1ll << bit;
+      if (c >= (int64_t)a.K * a.V) continue;
+      if (counted([&](double y, int i) { return y == edge && index(i) < c; }) < need) last = c;
+    }
+    __syncthreads();
+    if (tid == 0) sh_count = 0;
+    __syncthreads();
+    for (int i = tid; i < all; i += kBeamThreads) {
+      const double y = value(i);
+      if (y > edge || (y == edge && index(i) <= last)) keep(y, i);
+    }
+    __syncthreads();
+    count = min(sh_count, kJoinList);
+  }
+  const int64_t o = (int64_t)b * n;
+  for (int i = tid; i < count; i += kBeamThreads) {
+    const double y = list_x[i];
+    const int64_t t = list_i[i];
+    int rank = 0;
+    for (int k = 0; k < count; ++k) {
+      const double z = list_x[k];
+      rank += z > y || (z == y && list_i[k] < t);
+    }
+    if (rank < n) {
+      // (never -inf, which stands for no candidate)
+      a.out_scores[o + rank] = (float)fmin(fmax(y, -(double)FLT_MAX), (double)FLT_MAX);
+      a.out_tokens[o + rank] = t % a.V;
+      a.out_parents[o + rank] = (int32_t)(t / a.V);
+    }
+  }
+  for (int i = count + tid; i < n; i += kBeamThreads) {
+    a.out_scores[o + i] = -INFINITY;
+    a.out_tokens[o + i] = -1;
+    a.out_parents[o + i] = -1;
+  }
+}
+
+// Chunks of a row: 16 bytes a thread where that many workgroups do not fill the device.
+struct SelectPlan {
+  int nv, chunks;
+  int64_t rows, bytes;
+};
+SelectPlan select_plan(int B, int K, int V, int n, int es) {
+  SelectPlan p{};
+  p.rows = (int64_t)B * K;
+  const int per = kBeamThreads * 16 / es;
+  p.nv = p.rows * ((V + 4 * per - 1) / (4 * per)) >= 512 ? 4 : 1;
+  p.chunks = (V + p.nv * per - 1) / (p.nv * per);
+  p.bytes = p.rows * p.chunks * (12 + 8 * (int64_t)n);
+  return p;
+}
+bool select_ok(int B, int K, int V, int n) {
+  return B >= 0 && K >= 1 && K <= HELM_BEAMS_MAX && V >= 1 && n >= 1 && n <= HELM_BEAMS_MAX &&
+         (int64_t)B * K <= 65535 &&
+         (int64_t)K * ((V + 1023) / 1024) * n <= 0x7fffffff;
+}
+
+template <typename T> void launch_scan(const SelectArgs& a, const SelectPlan& p, hipStream_t st) {
+  const dim3 grid(p.chunks, (uint32_t)p.rows);
+  if (p.nv == 4) hipLaunchKernelGGL((beam_scan_kernel<T, 4>), grid, dim3(kBeamThreads), 0, st, a);
+  else hipLaunchKernelGGL((beam_scan_kernel<T, 1>), grid, dim3(kBeamThreads), 0, st, a);
+}
+
+// ---- tables ----------------------------------------------------------------------------
+//
+// Row j of a request goes on from p_j = parents[j] (j itself where that is no row).  Full
+// pages are shared by name: new[j][c] = old[p_j][c].  A part-filled page is a row's own, since
+// its next token goes there: the keeper of parent p (p itself if it is its own child, else its
+// lowest child) keeps the page, and p's other children take, in ascending order, the
+// part-filled pages of the rows that no row goes on from.  There are as many of those as of
+// other children, no page is both read and written, and nothing is taken from a free list.
+//
+// The first launch, a workgroup per request and 128 columns, a column a thread, writes the
+// tables (in place too: a column's old entries are in LDS before its new ones are stored),
+// which page is copied where, and its columns' pages that no row names any more; the second
+// copies the pages' tokens in all layers' pools and joins the lists of released pages, in the
+// order of requests, columns and rows.
+constexpr int kCols = 128;
+constexpr int kPools = 128;                  // a launch's
+
+struct BeamTableArgs {
+  const int32_t* parents;
+  int B, K;
+  const int32_t* table;
+  int64_t stride;
+  int width, chunks;
+  const int32_t* lens;
+  int page;
+  const int32_t* shared;                     // may be null: none
+  int32_t* out;
+  int64_t out_stride;
+  int32_t* copies;                           // [B K][2]
+  int32_t* lists;                            // [B][chunks][K kCols]
+  int32_t* counts;                           // [B][chunks]
+  int32_t* released;
+  int32_t* n_released;
+};
+
+// The i-th set bit of x (there are more than i).
+__device__ __forceinline__ int nth_bit(uint64_t x, int i) {
+  for (; i > 0; --i) x &= x - 1;
+  return __builtin_ctzll(x);
+}
+
+__global__ __launch_bounds__(kCols) void beam_tables_kernel(BeamTableArgs a) {
+  extern __shared__ int32_t old[];           // [K][kCols]
+  __shared__ int par[64], tail[64], sh_first[2];
+  __shared__ uint64_t sh_dead;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int b = blockIdx.y, K = a.K, chunk = blockIdx.x;
+  const int col = chunk * kCols + tid;
+  const int32_t* rows = a.table + (int64_t)b * K * a.stride;
+  int32_t* outs = a.out + (int64_t)b * K * a.out_stride;
+  const bool in = col < a.width;
+  for (int k = 0; k < K; ++k) old[k * kCols + tid] = in ? rows[k * a.stride + col] : -1;
+  const int len = max(0, a.lens[(int64_t)b * K]);
+  const int full = len / a.page;             // columns of full pages
+  const bool part = len % a.page != 0;
+  const int shared = a.shared ? max(0, a.shared[b]) : 0;
+  if (wave == 0) {
+    int p = lane < K ? a.parents[(int64_t)b * K + lane] : -1;
+    if (p < 0 || p >= K) p = lane;
+    uint64_t kids = 0;                       // of row `lane`
+    for (int k = 0; k < K; ++k) {
+      const uint64_t x = __builtin_amdgcn_ballot_w64(lane < K && p == k);
+      if (lane == k) kids = x;
+    }
+    const int keeper = kids >> lane & 1 ? lane : kids ? __builtin_ctzll(kids) : -1;
+    const bool extra = __shfl(keeper, p, 64) != lane;
+    const uint64_t dead = __builtin_amdgcn_ballot_w64(lane < K && !kids);
+    const uint64_t extras = __builtin_amdgcn_ballot_w64(lane < K && extra);
+    int t = p;
+    if (lane < K && extra)
+      t = nth_bit(dead, __builtin_popcountll(extras & ((1ull << lane) - 1)));
+    par[lane] = p;
+    tail[lane] = t;
+    if (lane == 0) sh_dead = dead;
+  }
+  __syncthreads();
+  // (in place, the shared columns, the same in every row, stay as they are)
+  if (in && !(a.out == a.table && col < shared))
+    for (int k = 0; k < K; ++k) {
+      const int from = col < full ? par[k] : col == full && part ? tail[k] : k;
+      outs[k * a.out_stride + col] = old[from * kCols + tid];
+    }
+  // which page is copied where, by the workgroup that holds the column
+  if (chunk == min(full / kCols, a.chunks - 1))
+    for (int k = tid; k < K; k += kCols) {
+      int src = -1, dst = -1;
+      if (part && full < a.width && tail[k] != par[k]) {
+        src = old[par[k] * kCols + full % kCols];
+        dst = old[tail[k] * kCols + full % kCols];
+      }
+      a.copies[2 * ((int64_t)b * K + k)] = src;
+      a.copies[2 * ((int64_t)b * K + k) + 1] = dst;
+    }
+
+  // pages of full columns that only rows without a child name, each once
+  const uint64_t dead = sh_dead;
+  uint64_t gone = 0;
+  if (in && col >= shared && col < full)
+    for (uint64_t d = dead; d; d &= d - 1) {
+      const int k = __builtin_ctzll(d);
+      const int slot = old[k * kCols + tid];
+      bool held = slot < 0;
+      for (int i = 0; i < K && !held; ++i)
+        held = (i < k || !(dead >> i & 1)) && old[i * kCols + tid] == slot;
+      if (!held) gone |= 1ull << k;
+    }
+  const int mine = __builtin_popcountll(gone);
+  int incl = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int x = __shfl_up(incl, d, 64);
+    if (lane >= d) incl += x;
+  }
+  if (lane == 63) sh_first[wave] = incl;
+  __syncthreads();
+  int at = incl - mine + (wave ? sh_first[0] : 0);
+  const int64_t l = (int64_t)b * a.chunks + chunk;
+  int32_t* list = a.lists + l * K * kCols;
+  for (; gone; gone &= gone - 1) list[at++] = old[__builtin_ctzll(gone) * kCols + tid];
+  if (tid == 0) a.counts[l] = sh_first[0] + sh_first[1];
+}
+
+struct BeamPools {
+  int n, segs, unit_tokens, parts;
+  int n_slots;
+  int64_t slot, seg;                         // bytes between slots, between a slot's segments
+  int64_t unit;                              // bytes of unit_tokens tokens of a segment
+  char* at[kPools];
+};
+
+// Workgroups x < joins: each its share of the lists of released pages, behind those before.
+// The rest: page blockIdx.x - joins of the copies, in pool blockIdx.y, part blockIdx.z.
+template <typename W>
+__global__ __launch_bounds__(kBeamThreads) void beam_copy_kernel(BeamTableArgs a, BeamPools p,
+                                                             int joins) {
+  const int tid = threadIdx.x;
+  if ((int)blockIdx.x < joins) {
+    if (blockIdx.y || blockIdx.z) return;
+    __shared__ int sh[kBeamWaves];
+    const int n = a.B * a.chunks, per = (n + joins - 1) / joins;
+    const int l0 = min(n, (int)blockIdx.x * per), l1 = min(n, l0 + per);
+    int before = 0;
+    for (int l = tid; l < l0; l += kBeamThreads) before += a.counts[l];
+    int at = block_sum(before, sh);
+    for (int l = l0; l < l1; ++l) {
+      const int c = a.counts[l];
+      for (int i = tid; i < c; i += kBeamThreads)
+        a.released[at + i] = a.lists[(int64_t)l * a.K * kCols + i];
+      at += c;
+    }
+    if ((int)blockIdx.x == joins - 1 && tid == 0) *a.n_released = at;
+    return;
+  }
+  const int row = blockIdx.x - joins;
+  const int src = a.copies[2 * row], dst = a.copies[2 * row + 1];
+  if (src == dst || (uint32_t)src >= (uint32_t)p.n_slots || (uint32_t)dst >= (uint32_t)p.n_slots)
+    return;
+  const int used = max(0, a.lens[row / a.K * a.K]) % a.page;
+  // (a page's tokens stay within 2^31 words: checked on the host)
+  const uint32_t words = (uint32_t)((used + p.unit_tokens - 1) / p.unit_tokens * p.unit /
+                                    (int64_t)sizeof(W));
+  const char* s = p.at[blockIdx.y] + src * p.slot;
+  char* d = p.at[blockIdx.y] + dst * p.slot;
+  const uint32_t all = words * p.segs;
+  constexpr int U = 8;
+  for (uint32_t i0 = blockIdx.z * kBeamThreads * U; i0 < all; i0 += p.parts * kBeamThreads * U) {
+    W x[U];
+    int64_t off[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t i = min(i0 + u * kBeamThreads + tid, all - 1);
+      off[u] = i / words * p.seg + (int64_t)(i % words) * sizeof(W);
+      x[u] = *reinterpret_cast<const W*>(s + off[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i0 + u * kBeamThreads + tid < all) *reinterpret_cast<W*>(d + off[u]) = x[u];
+  }
+}
+
+bool tables_ok(int B, int K, int width) {
+  return B >= 0 && K >= 1 && K <= HELM_BEAMS_MAX && (int64_t)B * K <= 65535 && width >= 0 &&
+         (int64_t)B * K * width <= 0x7fffffff;
+}
+int table_chunks(int width) { return std::max(1, (width + kCols - 1) / kCols); }
+
+}  // namespace
+
+extern "C" size_t helm_beam_select_workspace_bytes(int B, int K, int V, int n, int dtype) {
+  if (!select_ok(B, K, V, n)) return 0;
+  return (size_t)select_plan(B, K, V, n, dtype == HELM_F32 ? 4 : 2).bytes;
+}
+
+extern "C" int helm_beam_select(const void* logits, int64_t b_stride, int64_t k_stride, int dtype,
+                                const float* scores, int B, int K, int V, int n,
+                                float* out_scores, int64_t* out_tokens, int32_t* out_parents,
+                                void* workspace, size_t ws_bytes, void* stream) {
+  using namespace helm;
+  if (dtype != HELM_F16 && dtype != HELM_BF16 && dtype != HELM_F32)
+    return report_error(HELM_E_UNSUPPORTED, "logits are float16, bfloat16 or float32");
+  if (!select_ok(B, K, V, n) || b_stride < 0 || k_stride < 0)
+    return report_error(HELM_E_INVALID, "bad beam selection shape (1 to " +
+                                            std::to_string(HELM_BEAMS_MAX) +
+                                            " beams and candidates, at most 65535 rows)");
+  if (B == 0) return HELM_OK;
+  if (!logits || !scores || !out_scores || !out_tokens || !out_parents)
+    return report_error(HELM_E_INVALID, "null pointer argument");
+  const int es = dtype == HELM_F32 ? 4 : 2;
+  if (reinterpret_cast<uint64_t>(logits) % es)
+    return report_error(HELM_E_INVALID, "logits must be aligned to their elements");
+  const SelectPlan p = select_plan(B, K, V, n, es);
+  if (!workspace || ws_bytes < (size_t)p.bytes || (reinterpret_cast<uint64_t>(workspace) & 7))
+    return report_error(HELM_E_WORKSPACE,
+                        "workspace too small or unaligned: need " + std::to_string(p.bytes));
+  SelectArgs a{};
+  a.logits = logits;
+  a.b_stride = b_stride;
+  a.k_stride = k_stride;
+  a.scores = scores;
+  a.B = B;
+  a.K = K;
+  a.V = V;
+  a.n = n;
+  a.chunks = p.chunks;
+  const int64_t parts = p.rows * p.chunks;
+  a.part_sum = static_cast<double*>(workspace);
+  a.part_max = reinterpret_cast<float*>(a.part_sum + parts);
+  a.cand_x = a.part_max + parts;
+  a.cand_t = reinterpret_cast<int*>(a.cand_x + parts * n);
+  a.out_scores = out_scores;
+  a.out_tokens = out_tokens;
+  a.out_parents = out_parents;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (dtype == HELM_F32) launch_scan<float>(a, p, st);
+  else if (dtype == HELM_BF16) launch_scan<bf16_t>(a, p, st);
+  else launch_scan<f16_t>(a, p, st);
+  hipLaunchKernelGGL(beam_join_kernel, dim3(B), dim3(kBeamThreads), 0, st, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess)
+    return report_error((int)e, std::string("beam selection launch: ") + hipGetErrorString(e));
+  return HELM_OK;
+}
+
+extern "C" size_t helm_beam_tables_workspace_bytes(int B, int K, int table_width) {
+  if (!tables_ok(B, K, table_width)) return 0;
+  return (size_t)B * table_chunks(table_width) * ((size_t)K * kCols + 1) * sizeof(int32_t);
+}
+
+extern "C" int helm_beam_tables(const int32_t* parents, int B, int K, const int32_t* page_table,
+                                int64_t table_stride, int table_width, const int32_t* seq_lens,
+                                int page_size, const int32_t* shared_pages, int32_t* new_table,
+                                int64_t new_stride, int32_t* copies, int32_t* released,
+                                int32_t* n_released, const void* const* pools, int n_pools,
+                                int64_t n_slots, int64_t slot_bytes, int segments,
+                                int64_t segment_bytes, int unit_tokens, int64_t unit_bytes,
+                                void* workspace, size_t ws_bytes, void* stream) {
+  using namespace helm;
+  if (!tables_ok(B, K, table_width) || page_size < 1 || table_stride < table_width ||
+      new_stride < table_width)
+    return report_error(HELM_E_INVALID, "bad beam table shape (1 to " +
+                                            std::to_string(HELM_BEAMS_MAX) +
+                                            " beams, at most 65535 rows, page_size >= 1)");
+  if (n_pools < 0 || (n_pools && (!pools || n_slots < 0 || n_slots > 0x7fffffff || slot_bytes < 0 ||
+                                  segments < 1 || segment_bytes < 0 || unit_tokens < 1 ||
+                                  unit_bytes < 1)))
+    return report_error(HELM_E_INVALID, "bad pool shape");
+  const int64_t units = n_pools ? ((int64_t)page_size + unit_tokens - 1) / unit_tokens : 1;
+  if (n_pools && (segments > 0x7fffffff / unit_bytes / units || segment_bytes < units * unit_bytes))
+    return report_error(HELM_E_INVALID, "a page's segments overlap or pass 2^31 bytes");
+  if (B == 0 && !n_released) return report_error(HELM_E_INVALID, "null pointer argument");
+  if (B && (!parents || !seq_lens || !copies || !n_released ||
+            (table_width && (!page_table || !new_table || !released))))
+    return report_error(HELM_E_INVALID, "null pointer argument");
+  const size_t need = helm_beam_tables_workspace_bytes(B, K, table_width);
+  if (need && (!workspace || ws_bytes < need || (reinterpret_cast<uint64_t>(workspace) & 3)))
+    return report_error(HELM_E_WORKSPACE,
+                        "workspace too small or unaligned: need " + std::to_string(need));
+  const int64_t R = (int64_t)B * K;
+  const bool in_place = new_table == page_table && new_stride == table_stride;
+  // what is read; what is written
+  auto rows = [&](const int32_t* t, int64_t stride) {
+    return stride == table_width ? range(t, R * table_width) : range(t, table_width, R, stride);
+  };
+  const Range r[] = {rows(page_table, table_stride), range(parents, R),
+                     range(seq_lens, R), range(shared_pages, shared_pages ? B : 0),
+                     rows(new_table, new_stride), range(copies, 2 * R),
+                     range(released, R * table_width), range(n_released, 1)};
+  constexpr int kOut = 4, kRanges = 8;
+  // (overlap takes one row of its first operand: the table's rows one by one)
+  auto meet = [](const Range& x, const Range& y) {
+    for (int64_t i = 0; i < x.rows; ++i)
+      if (overlap({x.at + (uintptr_t)(i * x.step), 1, x.bytes, x.bytes}, y)) return true;
+    return false;
+  };
+  for (int i = kOut; i < kRanges; ++i)
+    for (int j = 0; j < i; ++j) {
+      if (in_place && i == kOut && j == 0) continue;
+      if (j == 0 || j == kOut ? meet(r[i], r[j]) : meet(r[j], r[i]))
+        return report_error(HELM_E_INVALID, "an output lies over another operand (new_table may "
+                                            "be page_table itself, nothing else)");
+    }
+  BeamTableArgs a{};
+  a.parents = parents;
+  a.B = B;
+  a.K = K;
+  a.table = page_table;
+  a.stride = table_stride;
+  a.width = table_width;
+  a.chunks = table_chunks(table_width);
+  a.lens = seq_lens;
+  a.page = page_size;
+  a.shared = shared_pages;
+  a.out = new_table;
+  a.out_stride = new_stride;
+  a.copies = copies;
+  a.lists = static_cast<int32_t*>(workspace);
+  a.counts = a.lists + (size_t)B * a.chunks * K * kCols;
+  a.released = released;
+  a.n_released = n_released;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (B)
+    hipLaunchKernelGGL(beam_tables_kernel, dim3(a.chunks, B), dim3(kCols),
+                       K * kCols * sizeof(int32_t), st, a);
+  // 16 bytes a lane where every page's segments allow it; workgroups of 32 KB or more
+  BeamPools p{};
+  p.n_slots = (int)n_slots;
+  p.segs = segments;
+  p.unit_tokens = unit_tokens;
+  p.slot = slot_bytes;
+  p.seg = segment_bytes;
+  p.unit = unit_bytes;
+  p.parts = (int)std::min<int64_t>(64, std::max<int64_t>(1, units * unit_bytes * segments >> 16));
+  int joins = (int)std::max<int64_t>(1, std::min<int64_t>(64, (int64_t)B * a.chunks));
+  for (int i0 = 0; i0 == 0 || i0 < n_pools; i0 += kPools) {
+    p.n = std::min(kPools, n_pools - i0);
+    uint64_t bits = (uint64_t)slot_bytes | (uint64_t)segment_bytes | (uint64_t)unit_bytes;
+    for (int i = 0; i < p.n; ++i) {
+      if (!pools[i0 + i]) return report_error(HELM_E_INVALID, "null pool");
+      p.at[i] = static_cast<char*>(const_cast<void*>(pools[i0 + i]));
+      bits |= reinterpret_cast<uint64_t>(pools[i0 + i]);
+    }
+    const dim3 grid((uint32_t)(joins + (p.n ? R : 0)), std::max(1, p.n), p.n ? p.parts : 1);
+    if (bits % 16 == 0)
+      hipLaunchKernelGGL((beam_copy_kernel<u32x4>), grid, dim3(kBeamThreads), 0, st, a, p, joins);
+    else
+      hipLaunchKernelGGL((beam_copy_kernel<uint8_t>), grid, dim3(kBeamThreads), 0, st, a, p, joins);
+    joins = 0;
+  }
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess)
+    return report_error((int)e, std::string("beam tables launch: ") + hipGetErrorString(e));
+  return HELM_OK;
+}

@@ -24,6 +24,7 @@
 #include <string>
 
 #include "helm_amd.h"
+#include "ranges.h"
 
 namespace helm {
 int report_error(int code, const std::string& msg);
@@ -178,26 +179,6 @@ __global__ __launch_bounds__(kThreads) void add_lens_kernel(TablesArgs a, int32_
   if (b < a.B) lens[b] = load_seq(a, b).total;
 }
 
-// `rows` rows of `bytes` bytes, `step` (>= bytes) apart.
-struct Range {
-  uintptr_t at;
-  int64_t rows, bytes, step;
-};
-template <typename T>
-Range range(const T* p, int64_t n, int64_t rows = 1, int64_t stride = 0) {
-  const int64_t e = sizeof(T);
-  return {reinterpret_cast<uintptr_t>(p), rows, n * e, (rows > 1 ? stride : n) * e};
-}
-// Whether a byte of x (one row) is one of y's.
-bool overlap(const Range& x, const Range& y) {
-  if (!x.bytes || !y.bytes || !y.rows || x.at + x.bytes <= y.at) return false;
-  if (x.at < y.at + y.bytes) return true;
-  const int64_t row = (int64_t)(x.at - y.at) / y.step;      // the last that starts at or before x
-  if (row >= y.rows) return false;
-  const int64_t in = (int64_t)(x.at - y.at) - row * y.step;
-  return in < y.bytes || (row + 1 < y.rows && in + x.bytes > y.step);
-}
-
 }  // namespace
 
 extern "C" int helm_batch_tables(const int32_t* new_lens, const int32_t* cached_lens, int B,
@@ -216,6 +197,9 @@ extern "C" int helm_batch_tables(const int32_t* new_lens, const int32_t* cached_
     return helm::report_error(HELM_E_INVALID, "null pointer argument");
   TablesArgs a{new_lens, cached_lens, page_table, table_stride, table_width, free_slots, n_free,
                page_size, B, max_tokens, cu_seqlens, positions, slot_map, seq_lens, pages_taken};
+  using helm::Range;
+  using helm::overlap;
+  using helm::range;
   // the table (read and written), what is only read, what is only written
   const bool in_place = seq_lens == cached_lens;
   const Range r[] = {range(page_table, table_width, B, table_stride),

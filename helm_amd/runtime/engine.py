@@ -109,6 +109,19 @@ def refuse_overlap(what: str, out: torch.Tensor, *inputs: torch.Tensor) -> None:
             raise ValueError(f"{what}: out lies over another operand (only q itself may be out)")
 
 
+def refuse_shared(what: str, out: torch.Tensor, *others: torch.Tensor) -> None:
+    """Refuses a contiguous `out` that shares memory with any of `others` (from their first
+    byte to their last)."""
+    lo = out.data_ptr()
+    hi = lo + out.numel() * out.element_size()
+    for t in others:
+        if lo == hi or not t.numel():
+            continue
+        span = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1
+        if t.data_ptr() < hi and t.data_ptr() + span * t.element_size() > lo:
+            raise ValueError(f"{what}: an output lies over another operand")
+
+
 def refuse_grad(what: str, *tensors: torch.Tensor) -> None:
     """The package serves models: its attention records nothing for a backward pass, and
     has no tangent to give (which no_grad does not drop)."""

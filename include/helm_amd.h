@@ -458,6 +458,54 @@ int helm_prompt_attn(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
                      float scale, float softcap, int window, int zero_rest, int dtype,
                      void* stream);
 
+/* ---- beam search over a paged cache ------------------------------------------------ */
+
+#define HELM_BEAMS_MAX 64     /* beams of a request, candidates of a selection */
+
+/* The n best continuations of each of B requests' K beams.  Row (b, k) of logits
+ * (element strides b_stride and k_stride, V contiguous, HELM_F16 / BF16 / F32, aligned to
+ * the element) and its running score scores[b * K + k] offer token t at
+ *   score + logit[t] - log(sum over the row of exp(logit)).
+ * Out, [B, n], best first, ties to the lowest k * V + t: the score (past fp32's range: its
+ * largest or lowest number), the token, the beam (0 .. K - 1).  A logit of -inf is no candidate, nor is anything of a row whose score is not
+ * finite or whose logits hold a NaN or +inf; where fewer than n are left, -inf, -1, -1.  The
+ * order is of 64-bit sums.  1 <= K, n <= HELM_BEAMS_MAX, B K <= 65535.  The workspace is
+ * 8-byte aligned and needs no contents before or after a call; calls that may overlap need
+ * one each. */
+size_t helm_beam_select_workspace_bytes(int B, int K, int V, int n, int dtype);
+int helm_beam_select(const void* logits, int64_t b_stride, int64_t k_stride, int dtype,
+                     const float* scores, int B, int K, int V, int n, float* out_scores,
+                     int64_t* out_tokens, int32_t* out_parents, void* workspace,
+                     size_t ws_bytes, void* stream);
+
+/* The block tables after a beam step.  Rows b * K .. of page_table are request b's beams,
+ * all with seq_lens[b * K] tokens (device) in pages of page_size; row j goes on from row
+ * p_j = parents[b * K + j] of its request (j itself where that is outside 0 .. K - 1).
+ *   columns of full pages: new[j] = old[p_j];
+ *   the part-filled page's column, whose page is each row's own: one child of a row, itself if
+ *     it goes on from itself, else the lowest, keeps its page; the others take, in ascending
+ *     order, those of the rows without a child, and the parent's tokens are copied into them
+ *     in every pool;
+ *   columns behind that: new[j] = old[j].
+ * shared_pages [B] (may be NULL: 0): leading columns in which the request's rows are the same.
+ * copies [B K, 2]: the pages copied from and to for each row, -1, -1 where none.
+ * released: full pages behind the shared ones that no row names any more, each once, by request,
+ * column, row (negative entries are no pages); n_released: how many; behind them released (room
+ * for B K table_width) is left as it is.  new_table may be page_table itself (at its stride); no
+ * other output may lie over an operand.
+ * pools: n_pools (0: none) addresses on the host, all of n_slots pages slot_bytes apart, a page
+ * being `segments` segments segment_bytes apart whose every unit_tokens tokens are unit_bytes
+ * bytes; pages outside [0, n_slots) are not copied.  K <= HELM_BEAMS_MAX, B K <= 65535. */
+size_t helm_beam_tables_workspace_bytes(int B, int K, int table_width);
+int helm_beam_tables(const int32_t* parents, int B, int K, const int32_t* page_table,
+                     int64_t table_stride, int table_width, const int32_t* seq_lens,
+                     int page_size, const int32_t* shared_pages, int32_t* new_table,
+                     int64_t new_stride, int32_t* copies, int32_t* released,
+                     int32_t* n_released, const void* const* pools, int n_pools,
+                     int64_t n_slots, int64_t slot_bytes, int segments, int64_t segment_bytes,
+                     int unit_tokens, int64_t unit_bytes, void* workspace, size_t ws_bytes,
+                     void* stream);
+
 /* ---- device profile ------------------------------------------------------- */
 
 /* Bandwidths of one device, as HELM's device profiler measures them for its

@@ -1,0 +1,189 @@
+"""What the beam operators refuse: argument checks of the Python entry points and of the C-ABI
+(which return before any device work), and the restatements' own properties."""
+import ctypes
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from helm_amd import _native, beams, pool4
+from helm_amd.runtime import engine
+from oracle import beams as R
+
+I32, I64, F32 = torch.int32, torch.int64, torch.float32
+
+
+def _select(B=2, K=3, V=8, **kw):
+    return dict(dict(logits=torch.zeros((B, K, V)), scores=torch.zeros((B, K))), **kw)
+
+
+@pytest.mark.parametrize("bad,err", [
+    (dict(logits=torch.zeros((6, 8))), ValueError),
+    (dict(scores=torch.zeros((2, 4))), ValueError),
+    (dict(logits=torch.zeros((2, 3, 8), dtype=torch.float64)), TypeError),
+    (dict(logits=torch.zeros((2, 3, 8), dtype=I32)), TypeError),
+    (dict(scores=torch.zeros((2, 3), dtype=torch.bfloat16)), TypeError),
+    (dict(scores=torch.zeros((3, 2)).t()), ValueError),
+    (dict(n=0), ValueError), (dict(n=65), ValueError),
+    (dict(logits=torch.zeros((2, 65, 8)), scores=torch.zeros((2, 65))), ValueError),
+    (dict(logits=torch.zeros((2, 3, 0))), ValueError),
+    (dict(logits=torch.zeros((1, 1)).expand(65536, 1, 1), scores=torch.zeros((65536, 1))), ValueError),
+    (dict(logits=torch.zeros((2, 3, 8), requires_grad=True)), RuntimeError),
+    ({}, RuntimeError),            # CPU tensors
+])
+def test_select_refusals(bad, err):
+    with pytest.raises(err):
+        beams.beam_select(**_select(**bad))
+
+
+def test_select_out_refusals(monkeypatch):
+    good = beams.BeamChoice(torch.zeros((2, 3)), torch.zeros((2, 3), dtype=I64),
+                            torch.zeros((2, 3), dtype=I32))
+    for bad in (good._replace(scores=torch.zeros((2, 4))),
+                good._replace(tokens=torch.zeros((2, 3), dtype=I32)),
+                good._replace(parents=torch.zeros((3, 2), dtype=I32).t())):
+        with pytest.raises(ValueError):
+            beams.beam_select(**_select(), out=bad)
+    monkeypatch.setattr(engine, "common_device", lambda *a: 0)
+    a = _select()
+    buf = torch.zeros(12)
+    for bad in (good._replace(scores=a["scores"]),                  # read until the last row is
+                good._replace(scores=a["logits"].view(-1)[40:46].view(2, 3)),
+                good._replace(scores=buf[:6].view(2, 3), parents=buf.view(I32)[5:11].view(2, 3))):
+        with pytest.raises(ValueError, match="lies over"):
+            beams.beam_select(**a, out=bad)
+
+
+def _tables(B=2, K=3, W=4, **kw):
+    return dict(dict(parents=torch.zeros((B, K), dtype=I32),
+                     page_table=torch.zeros((B * K, W), dtype=I32),
+                     seq_lens=torch.zeros(B * K, dtype=I32), page_size=16), **kw)
+
+
+@pytest.mark.parametrize("bad,err", [
+    (dict(parents=torch.zeros((2, 3), dtype=I64)), TypeError),
+    (dict(page_table=torch.zeros((6, 4), dtype=I64)), TypeError),
+    (dict(seq_lens=torch.zeros(6, dtype=I64)), TypeError),
+    (dict(parents=torch.zeros(6, dtype=I32)), ValueError),
+    (dict(parents=torch.zeros((3, 2), dtype=I32).t()), ValueError),
+    (dict(page_table=torch.zeros((5, 4), dtype=I32)), ValueError),
+    (dict(page_table=torch.zeros((4, 6), dtype=I32).t()), ValueError),
+    (dict(page_table=torch.zeros((1, 4), dtype=I32).expand(6, 4)), ValueError),
+    (dict(seq_lens=torch.zeros(2, dtype=I32)), ValueError),
+    (dict(seq_lens=torch.zeros(12, dtype=I32)[::2]), ValueError),
+    (dict(page_size=0), ValueError),
+    (dict(shared_pages=torch.zeros(2, dtype=I64)), TypeError),
+    (dict(shared_pages=torch.zeros(6, dtype=I32)), ValueError),
+    (dict(parents=torch.zeros((1, 65), dtype=I32), page_table=torch.zeros((65, 4), dtype=I32),
+          seq_lens=torch.zeros(65, dtype=I32)), ValueError),
+    (dict(pages=beams.PageStore([torch.zeros(4, 2, 32, 8)])), ValueError),     # 32, not 16
+    (dict(out=beams.BeamTables(torch.zeros((6, 4), dtype=I32), torch.zeros((6, 2), dtype=I32),
+                               torch.zeros(23, dtype=I32), torch.zeros(1, dtype=I32))), ValueError),
+    (dict(out=beams.BeamTables(torch.zeros((6, 4), dtype=I64), torch.zeros((6, 2), dtype=I32),
+                               torch.zeros(24, dtype=I32), torch.zeros(1, dtype=I32))), ValueError),
+    ({}, RuntimeError),            # CPU tensors
+])
+def test_tables_refusals(bad, err):
+    with pytest.raises(err):
+        beams.beam_tables(**_tables(**bad))
+
+
+@pytest.mark.parametrize("bad", [
+    [], [torch.zeros(4, 16)], [torch.zeros(4, 2, 16, 8), torch.zeros(4, 2, 16, 4)],
+    [torch.zeros(4, 2, 16, 8), torch.zeros(4, 2, 16, 8).half()],
+    [torch.zeros(4, 2, 16, 8), torch.zeros(8, 2, 16, 8)[::2]],
+    [torch.zeros(4, 2, 8, 16).transpose(2, 3)], [torch.zeros(4, 2, 16, 16)[..., :8]],
+    [torch.zeros(4, 3, 2, 16, 8)[:, :, :1].expand(4, 3, 2, 16, 8)],       # parts over each other
+    [torch.zeros(4, 3, 5, 16, 8)[:, :, ::2]],                             # no one stride
+    [torch.zeros(1, 2, 16, 8).expand(4, 2, 16, 8)],                       # pages over each other
+    [torch.zeros(4, 2, 16, 0)],
+    [pool4.Pool4(4, 2, 64, device="cpu"), pool4.Pool4(4, 2, 64, device="cpu").data],
+])
+def test_page_store_refusals(bad):
+    with pytest.raises(ValueError):
+        beams.PageStore(bad)
+
+
+def test_page_store_layouts():
+    """(slots, bytes between slots, segments, bytes between them, tokens and bytes of a unit)"""
+    assert beams.PageStore([torch.zeros(5, 2, 3, 16, 8)])._shape == (5, 3072 * 1, 6, 512, 1, 32)
+    a = torch.zeros(5, 2, 3, 16, 8).half()
+    assert beams.PageStore([a[:, 0], a[:, 1]])._shape == (5, 1536, 3, 256, 1, 16)
+    assert beams.PageStore([torch.zeros(5, 16, 8).half()])._shape == (5, 256, 1, 256, 1, 16)
+    p = pool4.Pool4(5, 2, 64, page_size=32, device="cpu")
+    s = beams.PageStore([p])
+    assert s._shape == (5, 2 * 2 * 17 * 64, 2, 2 * 17 * 64, 16, 17 * 64) and s.page_size == 32
+
+
+def _i32(n):
+    a = np.zeros(max(1, n), dtype=np.int32)
+    return a, a.ctypes.data
+
+
+def test_c_entries_refuse_before_device_work():
+    lib = _native.load()
+    f = np.zeros(4096, dtype=np.float32)
+    at, E = f.ctypes.data, (_native.HELM_E_INVALID, _native.HELM_E_UNSUPPORTED,
+                            _native.HELM_E_WORKSPACE)
+
+    def select(logits=at, bs=24, ks=8, dt=2, scores=at, B=2, K=3, V=8, n=3, o=at, ws=at, nb=4096):
+        return lib.helm_beam_select(logits, bs, ks, dt, scores, B, K, V, n, o, o, o, ws, nb, None)
+    assert select(dt=7) == E[1]
+    for kw in (dict(K=0), dict(K=65), dict(n=0), dict(n=65), dict(V=0), dict(B=-1), dict(B=30000),
+               dict(bs=-1), dict(logits=None), dict(scores=None), dict(o=None),
+               dict(logits=at + 2)):
+        assert select(**kw) == E[0], kw
+    for kw in (dict(ws=None), dict(nb=8), dict(ws=at + 4)):
+        assert select(**kw) == E[2], kw
+    assert select(B=0) == 0
+    assert lib.helm_beam_select_workspace_bytes(2, 3, 8, 3, 2) == 6 * (12 + 24)
+    assert lib.helm_beam_select_workspace_bytes(2, 0, 8, 3, 2) == 0
+
+    arr = {k: _i32(n) for k, n in dict(par=6, tab=24, lens=6, new=24, cop=12, rel=24, cnt=1).items()}
+    ptr = {k: v[1] for k, v in arr.items()}
+    need = lib.helm_beam_tables_workspace_bytes(2, 3, 4)
+    ws = np.zeros(need // 4, dtype=np.int32)
+    pool = (ctypes.c_void_p * 1)(at)
+
+    def tables(B=2, K=3, W=4, ts=4, ns=4, page=16, pools=None, n=0, geo=(4, 64, 2, 32, 1, 2),
+               wsp=ws.ctypes.data, nb=need, **kw):
+        p = dict(ptr, **kw)
+        return lib.helm_beam_tables(p["par"], B, K, p["tab"], ts, W, p["lens"], page, None,
+                                    p["new"], ns, p["cop"], p["rel"], p["cnt"], pools, n, *geo,
+                                    wsp, nb, None)
+    for kw in (dict(K=0), dict(K=65), dict(B=-1), dict(W=-1), dict(ts=3), dict(ns=3), dict(page=0),
+               dict(par=None), dict(tab=None), dict(lens=None), dict(new=None), dict(cop=None),
+               dict(rel=None), dict(cnt=None), dict(n=-1), dict(n=1),
+               dict(n=1, pools=pool, geo=(-1, 64, 2, 32, 1, 2)),
+               dict(n=1, pools=pool, geo=(4, 64, 0, 32, 1, 2)),
+               dict(n=1, pools=pool, geo=(4, 64, 2, 16, 1, 2)),        # segments over each other
+               dict(n=1, pools=pool, geo=(4, 64, 2, 2 ** 31, 1, 2 ** 30))):
+        assert tables(**kw) == E[0], kw
+    for kw in (dict(wsp=None), dict(nb=need - 4)):
+        assert tables(**kw) == E[2], kw
+    # an output over an operand, byte by byte; the table may be its own
+    tab = ptr["tab"]
+    for kw in (dict(cop=tab), dict(rel=ptr["par"]), dict(new=tab + 4), dict(cnt=tab + 92),
+               dict(cop=ptr["lens"]), dict(rel=ptr["cop"]), dict(cnt=ptr["new"] + 20),
+               dict(new=tab, ns=5)):
+        assert tables(**kw) == E[0], kw
+        assert b"lies over" in lib.helm_last_error_string()
+
+
+def test_the_restated_choice():
+    """By hand: two beams of two tokens, and ties."""
+    x = torch.tensor([[[0.0, 0.0], [0.0, 0.0]]])
+    y, tok, par = R.select(x, torch.tensor([[0.0, 0.0]]), 5)
+    assert tok.tolist() == [[0, 1, 0, 1, -1]] and par.tolist() == [[0, 0, 1, 1, -1]]
+    assert torch.allclose(y[0, :4], torch.full((4,), -math.log(2.0), dtype=torch.float64))
+    assert y[0, 4] == -math.inf
+
+
+def test_the_restated_tables():
+    """By hand: pages of 4, 6 tokens; beams 1 and 2 go on from 1, beam 0 from 2."""
+    table = [[10, 20, 0], [11, 21, 0], [11, 22, 0]]
+    new, copies, released = R.tables([[2, 1, 1]], table, [6] * 3, 4)
+    # beam 2's page goes on under row 0, beam 1's under row 1; row 2 takes the page of beam 0
+    assert new == [[11, 22, 0], [11, 21, 0], [11, 20, 0]]
+    assert copies == [(-1, -1), (-1, -1), (21, 20)] and released == [10]
