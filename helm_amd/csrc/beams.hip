@@ -7,21 +7,22 @@
 // Within a row the order is the logits' own, so one pass over them gives a chunk's
 // largest value, its sum and its n best, and the rows meet in a second, small kernel.
 // Bound by memory: the logits are read once.  The order between rows is of sums, which are
-// formed in 64 bits: exponentials in 32 (off by 2^-23 each, their argument exact to that),
-// their sums, logarithms and the scores in 64, so that lse is off by about 1e-8 and two
-// candidates change places only where their scores are as near as that.
+// formed in 64 bits: exponentials in 32 (each off at random by some 2^-21 at most, most of it
+// its argument's rounding), their sums, logarithms and the scores in 64, so that two
+// candidates of different rows change places only where their scores are within some 1e-7.
 //
-// A chunk's n best: the n-th largest of a wave's 64 lane maxima (a search over the bits of
-// the value with ballots) is at most the n-th largest of its values; the largest such bound
-// of the four waves leaves few values, which are put in a list and ranked by counting.  Where
-// ties or a sorted row leave more than the list holds, the workgroup searches value and
-// index bit by bit instead.
+// A chunk's n best: the n-th largest of the 256 threads' maxima, which every wave finds for
+// itself by a search over the value's leading bits with ballots, is at most the n-th largest of
+// the chunk and leaves little more than n values (34 of 32, 74 of 64 in a random row).  They
+// are put in a list and ranked by counting.  Where ties or a sorted row leave more than the
+// list holds, the workgroup searches value and index bit by bit instead.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
 #include <algorithm>
 #include <cfloat>
 #include <string>
+#include <type_traits>
 
 #include "attn_kernel.h"
 #include "helm_amd.h"
@@ -47,7 +48,7 @@ struct SelectArgs {
   const float* scores;
   int B, K, V, n, chunks;
   double* part_sum;                          // [B K][chunks]
-  float* part_max;                           // [B K][chunks]
+  float* part_max;                          // [B K][chunks]
   float* cand_x;                             // [B][n][K chunks], -inf: none; a chunk's n best are
   int* cand_t;                               // a column, best first
   float* out_scores;
@@ -57,14 +58,6 @@ struct SelectArgs {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 struct __attribute__((packed)) Any16 { u32x4 v; };
-
-// e^d for d <= 0 (NaN: NaN), its argument in base 2 as a whole number and an exact rest.
-__device__ __forceinline__ float exp_low(float d) {
-  d = d < -150.f ? -150.f : d;                // (zero from there on)
-  const float n = rintf(d * 1.44269504f);
-  const float f = fmaf(d, 1.44269504f, -n) + d * 1.92596299e-8f;   // log2 e = hi + lo
-  return ldexpf(__builtin_amdgcn_exp2f(f), (int)n);
-}
 
 // Whole numbers in the order of the floats (no NaN).
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -81,13 +74,49 @@ __device__ __forceinline__ uint64_t ordered(double x) {
 __device__ __forceinline__ double unordered(uint64_t u) {
   return __longlong_as_double((long long)(u >> 63 ? u & 0x7fffffffffffffffull : ~u));
 }
-// The n-th largest of the wave's 64 keys (1 <= n <= 64).
-template <typename U> __device__ __forceinline__ U wave_nth(U key, int n) {
-  U t = 0;
+// A reduction over the wave's 64 lanes, `none` its neutral value; the result is uniform.
+template <typename F> __device__ __forceinline__ float wave_reduce(float x, float none, F f) {
+  const int o = __builtin_bit_cast(int, none);
+  auto with = [&](auto ctrl, auto rows) {
+    const int y = __builtin_amdgcn_update_dpp(o, __builtin_bit_cast(int, x), decltype(ctrl)::value,
+                                              decltype(rows)::value, 0xf, false);
+    x = f(x, __builtin_bit_cast(float, y));
+  };
+  using std::integral_constant;
+  with(integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{});   // row_shr 1, 2, 4, 8
+  with(integral_constant<int, 0x112>{}, integral_constant<int, 0xf>{});
+  with(integral_constant<int, 0x114>{}, integral_constant<int, 0xf>{});
+  with(integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{});
+  with(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});   // row_bcast 15, 31
+  with(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
+}
+
+// The n-th largest (1 <= n <= 64) of the workgroup's keys in sh, one a thread, in its leading
+// kBits bits, the others zero: every wave finds it for itself.  Up to 40 of them, of the
+// largest of each four, of which there are 64: nearly as good a bound (44 values for the best 32
+// of a random row) for a quarter of the ballots.
+// (Rolled up: a kernel's first pass over its code waits for it, 64 bytes at a time.)
+template <int kBits> __device__ __forceinline__ uint32_t nth_key(const uint32_t* sh, int n) {
+  u32x4 k = reinterpret_cast<const u32x4*>(sh)[threadIdx.x & 63];
+  uint32_t t = 0;
+  if (n <= 40) {
+    const uint32_t top = max(max(k[0], k[1]), max(k[2], k[3]));
+#pragma unroll 2
+    for (int b = 31; b >= 32 - kBits; --b) {
+      const uint32_t c = t | 1u << b;
+      if (__builtin_popcountll(__builtin_amdgcn_ballot_w64(top >= c)) >= n) t = c;
+    }
+    return t;
+  }
+#pragma unroll 1
+  for (int b = 31; b >= 32 - kBits; --b) {
+    const uint32_t c = t | 1u << b;
+    int have = 0;
 #pragma unroll
-  for (int b = 8 * (int)sizeof(U) - 1; b >= 0; --b) {
-    const U c = t | (U)1 << b;
-    if (__builtin_popcountll(__builtin_amdgcn_ballot_w64(key >= c)) >= n) t = c;
+    for (int i = 0; i < 4; ++i)
+      have += __builtin_popcountll(__builtin_amdgcn_ballot_w64(k[i] >= c));
+    if (have >= n) t = c;
   }
   return t;
 }
@@ -108,18 +137,21 @@ template <typename T> struct Elem;           // the values of 16 bytes
 template <> struct Elem<float> {
   static constexpr int kPer = 4;
   __device__ static float get(const u32x4& w, int j) { return __uint_as_float(w[j]); }
+  __device__ static float read(const float* x) { return *x; }
 };
 template <> struct Elem<bf16_t> {
   static constexpr int kPer = 8;
   __device__ static float get(const u32x4& w, int j) {
     return __uint_as_float(j & 1 ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16);
   }
+  __device__ static float read(const bf16_t* x) { return __uint_as_float((uint32_t)x->x << 16); }
 };
 template <> struct Elem<f16_t> {
   static constexpr int kPer = 8;
   __device__ static float get(const u32x4& w, int j) {
     return (float)__builtin_bit_cast(_Float16, (uint16_t)(w[j >> 1] >> (16 * (j & 1))));
   }
+  __device__ static float read(const f16_t* x) { return (float)__builtin_bit_cast(_Float16, x->x); }
 };
 
 // Chunk blockIdx.x of row blockIdx.y: its maximum, sum and n best.  A thread holds NV runs
@@ -129,11 +161,11 @@ __global__ __launch_bounds__(kBeamThreads) void beam_scan_kernel(SelectArgs a) {
   constexpr int E = Elem<T>::kPer;
   constexpr int kSize = kBeamThreads * NV * E;
   __shared__ float sh_max[kBeamWaves];
-  __shared__ uint32_t sh_bound[kBeamWaves];
-  __shared__ double sh_sum[kBeamWaves];
+  __shared__ __attribute__((aligned(16))) uint32_t sh_key[kBeamThreads];
+  __shared__ float sh_sum[kBeamWaves];
   __shared__ int sh_n[kBeamWaves], sh_count;
-  __shared__ float list_x[kList];
   __shared__ int list_t[kList];
+  __shared__ uint64_t list[kList];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int row = blockIdx.y, n = a.n;
   const int first = blockIdx.x * kSize;
@@ -170,55 +202,50 @@ __global__ __launch_bounds__(kBeamThreads) void beam_scan_kernel(SelectArgs a) {
   for (int v = 0; v < NV; ++v)
 #pragma unroll
     for (int j = 0; j < E; ++j) top = fmaxf(top, Elem<T>::get(raw[v], j));
-  float m = top;
-#pragma unroll
-  for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
-  const uint32_t bound = wave_nth(ordered(top), n);
-  if (lane == 0) {
-    sh_max[wave] = m;
-    sh_bound[wave] = bound;
-  }
+  float m = wave_reduce(top, -INFINITY, [](float p, float q) { return fmaxf(p, q); });
+  if (lane == 0) sh_max[wave] = m;
+  sh_key[tid] = ordered(top);
   __syncthreads();
-  uint32_t b0 = 0;
 #pragma unroll
-  for (int w = 0; w < kBeamWaves; ++w) {
-    m = fmaxf(m, sh_max[w]);
-    b0 = max(b0, sh_bound[w]);
-  }
-  const float least = unordered(b0);
+  for (int w = 0; w < kBeamWaves; ++w) m = fmaxf(m, sh_max[w]);
+  // (16 bits of it: a bf16 value whole; 32 took half as long again as the sums)
+  const float least =
+      fmaxf(unordered(max(nth_key<16>(sh_key, n), ordered(-INFINITY))), -FLT_MAX);
 
-  // the sum (NaN where the row has one or an infinity), and the list
+  // the sum of e^(x - m) (NaN or an infinity where the row has one): 1 for the largest itself
   const float base = m == -INFINITY ? 0.f : m;
   float part = 0.f;
 #pragma unroll
   for (int v = 0; v < NV; ++v)
 #pragma unroll
-    for (int j = 0; j < E; ++j) part += exp_low(Elem<T>::get(raw[v], j) - base);
-  double sum = part;
+    for (int j = 0; j < E; ++j)
+      part += __builtin_amdgcn_exp2f((Elem<T>::get(raw[v], j) - base) * 1.44269504f);
+  part = wave_reduce(part, 0.f, [](float p, float q) { return p + q; });
+  if (lane == 0) sh_sum[wave] = part;
+  // of a thread's values, those that may be among the n best: none of most threads'
+  if (top >= least) {
+    uint64_t mine = 0;
 #pragma unroll
-  for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
-  if (lane == 0) sh_sum[wave] = sum;
-  // (of a thread's values, those that may be among the n best: none of most threads')
-  if (top >= least && top > -INFINITY) {
-#pragma unroll
-    for (int v = 0; v < NV; ++v)
+    for (int v = 0; v < NV; ++v) {
+      uint32_t some = 0;                      // the last value in the lowest bit
 #pragma unroll
       for (int j = 0; j < E; ++j) {
         const float y = Elem<T>::get(raw[v], j);
-        if (y >= least && y > -INFINITY) {
-          const int i = atomicAdd(&sh_count, 1);
-          if (i < kList) {
-            list_x[i] = y;
-            list_t[i] = (v * kBeamThreads + tid) * E + j;
-          }
-        }
+        some = 2 * some + (y >= least ? 1u : 0u);
       }
+      mine |= (uint64_t)some << (E * v);
+    }
+    for (; mine; mine &= mine - 1) {
+      const int e = __builtin_ctzll(mine), v = e / E, j = E - 1 - e % E;
+      const int i = atomicAdd(&sh_count, 1);
+      if (i < kList) list_t[i] = (v * kBeamThreads + tid) * E + j;
+    }
   }
   __syncthreads();
   const int64_t p = (int64_t)row * a.chunks + blockIdx.x;
   if (tid == 0) {
-    a.part_max[p] = m;
-    a.part_sum[p] = (sh_sum[0] + sh_sum[1]) + (sh_sum[2] + sh_sum[3]);
+    a.part_max[p] = base;
+    a.part_sum[p] = ((double)sh_sum[0] + sh_sum[1]) + ((double)sh_sum[2] + sh_sum[3]);
   }
   int count = sh_count;
   if (count > kList) {
@@ -259,32 +286,36 @@ __global__ __launch_bounds__(kBeamThreads) void beam_scan_kernel(SelectArgs a) {
       for (int j = 0; j < E; ++j) {
         const float y = Elem<T>::get(raw[v], j);
         const int t = (v * kBeamThreads + tid) * E + j;
-        if (y > edge || (y == edge && t <= last)) {
+        if (y > -INFINITY && (y > edge || (y == edge && t <= last))) {
           const int i = atomicAdd(&sh_count, 1);
-          if (i < kList) {
-            list_x[i] = y;
-            list_t[i] = t;
-          }
+          if (i < kList) list_t[i] = t;
         }
       }
     __syncthreads();
     count = min(sh_count, kList);
   }
+  // one number a value: better ones are larger, and of equals those before
+  for (int i = tid; i < count; i += kBeamThreads) {
+    const int t = list_t[i];
+    list[i] = (uint64_t)ordered(Elem<T>::read(x + t)) << 32 | (uint32_t)~t;
+  }
+  __syncthreads();
   const int lists = a.K * a.chunks;
   const int64_t col = (int64_t)(row / a.K) * n * lists + row % a.K * a.chunks + blockIdx.x;
   float* cx = a.cand_x + col;
   int* ct = a.cand_t + col;
-  for (int i = tid; i < count; i += kBeamThreads) {
-    const float y = list_x[i];
-    const int t = list_t[i];
+  // ranked by counting, four threads a value
+  for (int i0 = 0; i0 < count; i0 += kBeamThreads / 4) {
+    const int i = i0 + tid / 4;
+    const uint64_t mine = list[min(i, count - 1)];
     int rank = 0;
-    for (int k = 0; k < count; ++k) {
-      const float z = list_x[k];
-      rank += z > y || (z == y && list_t[k] < t);
-    }
-    if (rank < n) {
-      cx[rank * lists] = y;
-      ct[rank * lists] = first + t;
+#pragma unroll 4
+    for (int k = tid & 3; k < count; k += 4) rank += list[k] > mine;
+    rank += __shfl_xor(rank, 1, 64);
+    rank += __shfl_xor(rank, 2, 64);
+    if (i < count && rank < n && (tid & 3) == 0) {
+      cx[rank * lists] = unordered((uint32_t)(mine >> 32));
+      ct[rank * lists] = first + (int)~(uint32_t)mine;
     }
   }
   for (int i = count + tid; i < n; i += kBeamThreads) {
@@ -296,74 +327,140 @@ __global__ __launch_bounds__(kBeamThreads) void beam_scan_kernel(SelectArgs a) {
 // The n best of request blockIdx.x from its rows' chunks.
 __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(SelectArgs a) {
   __shared__ double base[64];                // s_k - lse_k; -inf: the row offers nothing
-  __shared__ uint64_t sh_bound[kBeamWaves];
+  __shared__ __attribute__((aligned(16))) uint32_t sh_key[kBeamThreads];
   __shared__ int sh_n[kBeamWaves], sh_count;
   __shared__ double list_x[kJoinList];
   __shared__ int64_t list_i[kJoinList];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int b = blockIdx.x, n = a.n, C = a.chunks;
   if (tid == 0) sh_count = 0;
-  for (int k = wave; k < a.K; k += kBeamWaves) {
+  // candidate i of the request: of list i % (K C), that is of a row's chunk, the (i / (K C))th.
+  // The lists lie side by side, from their best on; eight a thread are on their way at once,
+  // the first of them before the rows' sums.
+  constexpr int U = 8, kBatch = U * kBeamThreads;
+  const int lists = a.K * C, all = lists * n;
+  const float* cx = a.cand_x + (int64_t)b * all;
+  const int* ct = a.cand_t + (int64_t)b * all;
+  float x[U];
+  int t0[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int i = u * kBeamThreads + tid;
+    x[u] = i < all ? cx[i] : -INFINITY;
+    t0[u] = i < all ? ct[i] : 0;
+  }
+  // the rows' sums, a row to the first power of two of lanes that holds its chunks
+  const int wide = C > 32 ? 64 : C > 1 ? 2 << (31 - __builtin_clz(C - 1)) : 1;
+  const int per_wave = 64 / wide, c1 = lane & (wide - 1);
+  for (int k0 = wave * per_wave; k0 < a.K; k0 += kBeamWaves * per_wave) {
+    const int k = min(k0 + lane / wide, a.K - 1);
     const int64_t p = ((int64_t)b * a.K + k) * C;
-    float m = -INFINITY;
-    for (int c = lane; c < C; c += 64) m = fmaxf(m, a.part_max[p + c]);
-#pragma unroll
-    for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+    const float score = a.scores[b * a.K + k];
+    // against the row's largest (a chunk of -inf has 0 for it and for a sum)
+    float top = -INFINITY;
     double s = 0.0;
-    for (int c = lane; c < C; c += 64) {
-      // (a chunk's own -inf maximum has a sum of zero, or of NaN)
-      const float mc = a.part_max[p + c];
-      s += mc == -INFINITY ? a.part_sum[p + c]
-                           : a.part_sum[p + c] * exp((double)mc - (double)m);
+    for (int c = c1; c < C + c1; c += wide) {
+      const double part = c < C ? a.part_sum[p + c] : 0.0;
+      const float max_c = c < C ? a.part_max[p + c] : 0.f;
+      const float at = part != 0.0 ? max_c : -INFINITY;
+      float m = at;
+      for (int d = wide / 2; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+      if (m > top) {
+        s *= exp((double)top - (double)m);
+        top = m;
+      }
+      if (part != 0.0) s += part * exp((double)at - (double)top);
     }
-#pragma unroll
-    for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d, 64);
-    if (lane == 0) {
-      const float score = a.scores[b * a.K + k];
-      const double x = (double)score - ((double)m + log(s));
+    for (int d = wide / 2; d; d >>= 1) s += __shfl_xor(s, d, 64);
+    if (c1 == 0 && k0 + lane / wide < a.K) {
+      const double x = (double)score - ((double)top + log(s));
       base[k] = fabsf(score) < INFINITY && fabs(x) < INFINITY ? x : -INFINITY;
     }
   }
   __syncthreads();
-  // candidate i of the request: of list i % (K C), that is of a row's chunk, the (i / (K C))th
-  const int lists = a.K * C, all = lists * n;
-  const float* cx = a.cand_x + (int64_t)b * all;
-  const int* ct = a.cand_t + (int64_t)b * all;
-  auto value = [&](int i) {
-    const double s = base[i % lists / C];
-    return s == -INFINITY ? s : s + (double)cx[i];
+  auto sum = [&](int list, float v) {
+    const double s = base[list / C];
+    return v == -INFINITY || s == -INFINITY ? -INFINITY : s + (double)v;
   };
-  auto index = [&](int i) { return (int64_t)(i % lists / C) * a.V + ct[i]; };
-  double top = -INFINITY;
-  for (int i = tid; i < min(all, max(lists, kBeamThreads)); i += kBeamThreads)
-    top = fmax(top, value(i));
-  const uint64_t bound = wave_nth(ordered(top), n);
-  if (lane == 0) sh_bound[wave] = bound;
-  __syncthreads();
-  uint64_t b0 = 0;
+  const int hop = kBeamThreads % lists;
+  auto next = [&](int l) { return l + hop < lists ? l + hop : l + hop - lists; };
+  int at[U];                                 // the eight's lists
 #pragma unroll
-  for (int w = 0; w < kBeamWaves; ++w) b0 = max(b0, sh_bound[w]);
-  const double least = unordered(b0);
-  auto keep = [&](double y, int i) {
-    const int at = atomicAdd(&sh_count, 1);
-    if (at < kJoinList) {
-      list_x[at] = y;
-      list_i[at] = index(i);
+  for (int u = 0; u < U; ++u) at[u] = u ? next(at[u - 1]) : tid % lists;
+  // a bound: up to 16, the n-th largest of the threads' maxima; beyond (where one row may hold
+  // most of the best, several a thread: 4 x 16 rows, n = 32: 21 -> 16 us) of each wave's 512
+  // values the n-th largest, to eight bits of its mantissa
+  double y0[U], top = -INFINITY;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    y0[u] = sum(at[u], x[u]);
+    top = fmax(top, y0[u]);
+  }
+  uint32_t bound = 0;
+  if (n <= 16) {
+    sh_key[tid] = (uint32_t)(ordered(top) >> 32);
+    __syncthreads();
+    bound = nth_key<24>(sh_key, n);
+  } else {
+    uint32_t key[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) key[u] = (uint32_t)(ordered(y0[u]) >> 32);
+#pragma unroll 1
+    for (int bit = 31; bit >= 12; --bit) {
+      const uint32_t c = bound | 1u << bit;
+      int have = 0;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        have += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key[u] >= c));
+      if (have >= n) bound = c;
+    }
+    if (lane == 0) sh_key[wave] = bound;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kBeamWaves; ++w) bound = max(bound, sh_key[w]);
+  }
+  const double least = unordered(max((uint64_t)bound << 32, ordered(-(double)INFINITY)));
+  auto keep = [&](double y, int64_t t) {
+    const int i = atomicAdd(&sh_count, 1);
+    if (i < kJoinList) {
+      list_x[i] = y;
+      list_i[i] = t;
     }
   };
-  // the lists side by side from their best on, until none of them has one left
-  const int sweep = (lists + kBeamThreads - 1) / kBeamThreads * kBeamThreads;
-  for (int i0 = 0; i0 < all; i0 += sweep) {
-    bool any = false;
-    for (int i = i0 + tid; i < min(all, i0 + sweep); i += kBeamThreads) {
-      const double y = value(i);
+  bool any = false;
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (y0[u] >= least && y0[u] > -INFINITY) {
+      any = true;
+      keep(y0[u], (int64_t)(at[u] / C) << 32 | t0[u]);
+    }
+  // on until none of the lists has one left (a sweep holds one of each)
+  const int sweep = (lists + kBatch - 1) / kBatch * kBatch;
+  auto value = [&](int i) { return sum(i % lists, cx[i]); };
+  auto index = [&](int i) { return (int64_t)(i % lists / C) << 32 | ct[i]; };   // (row, token)
+  for (int i0 = kBatch; i0 < all; i0 += kBatch) {
+    if (i0 % sweep == 0) {
+      if (!__syncthreads_or(any)) break;
+      any = false;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * kBeamThreads + tid;
+      x[u] = i < all ? cx[i] : -INFINITY;
+    }
+    int l = next(at[U - 1]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      at[u] = l;
+      l = next(l);
+      const double y = sum(at[u], x[u]);
       if (y >= least && y > -INFINITY) {
         any = true;
-        keep(y, i);
+        keep(y, index(i0 + u * kBeamThreads + tid));
       }
     }
-    if (!__syncthreads_or(any)) break;
   }
+  __syncthreads();
   int count = sh_count;
   if (count > kJoinList) {
     auto counted = [&](auto wanted) {
@@ -379,9 +476,8 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(SelectArgs a) {
     const double edge = unordered(key);
     const int need = n - counted([&](double y, int) { return ordered(y) > key; });
     int64_t last = 0;
-    for (int bit = 40; bit >= 0; --bit) {
+    for (int bit = 37; bit >= 0; --bit) {
       const int64_t c = last | 1ll << bit;
-      if (c >= (int64_t)a.K * a.V) continue;
       if (counted([&](double y, int i) { return y == edge && index(i) < c; }) < need) last = c;
     }
     __syncthreads();
@@ -389,25 +485,29 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(SelectArgs a) {
     __syncthreads();
     for (int i = tid; i < all; i += kBeamThreads) {
       const double y = value(i);
-      if (y > edge || (y == edge && index(i) <= last)) keep(y, i);
+      if (y > edge || (y == edge && index(i) <= last)) keep(y, index(i));
     }
     __syncthreads();
     count = min(sh_count, kJoinList);
   }
   const int64_t o = (int64_t)b * n;
-  for (int i = tid; i < count; i += kBeamThreads) {
-    const double y = list_x[i];
-    const int64_t t = list_i[i];
+  for (int i0 = 0; i0 < count; i0 += kBeamThreads / 4) {
+    const int i = i0 + tid / 4;
+    const double y = list_x[min(i, count - 1)];
+    const int64_t t = list_i[min(i, count - 1)];
     int rank = 0;
-    for (int k = 0; k < count; ++k) {
+#pragma unroll 4
+    for (int k = tid & 3; k < count; k += 4) {
       const double z = list_x[k];
       rank += z > y || (z == y && list_i[k] < t);
     }
-    if (rank < n) {
+    rank += __shfl_xor(rank, 1, 64);
+    rank += __shfl_xor(rank, 2, 64);
+    if (i < count && rank < n && (tid & 3) == 0) {
       // (never -inf, which stands for no candidate)
       a.out_scores[o + rank] = (float)fmin(fmax(y, -(double)FLT_MAX), (double)FLT_MAX);
-      a.out_tokens[o + rank] = t % a.V;
-      a.out_parents[o + rank] = (int32_t)(t / a.V);
+      a.out_tokens[o + rank] = t & 0xffffffff;
+      a.out_parents[o + rank] = (int32_t)(t >> 32);
     }
   }
   for (int i = count + tid; i < n; i += kBeamThreads) {
@@ -426,7 +526,7 @@ SelectPlan select_plan(int B, int K, int V, int n, int es) {
   SelectPlan p{};
   p.rows = (int64_t)B * K;
   const int per = kBeamThreads * 16 / es;
-  p.nv = p.rows * ((V + 4 * per - 1) / (4 * per)) >= 512 ? 4 : 1;
+  p.nv = es / 2 * (p.rows * ((V + 8191) / 8192) >= 512 ? 4 : 1);
   p.chunks = (V + p.nv * per - 1) / (p.nv * per);
   p.bytes = p.rows * p.chunks * (12 + 8 * (int64_t)n);
   return p;
@@ -439,8 +539,9 @@ bool select_ok(int B, int K, int V, int n) {
 
 template <typename T> void launch_scan(const SelectArgs& a, const SelectPlan& p, hipStream_t st) {
   const dim3 grid(p.chunks, (uint32_t)p.rows);
-  if (p.nv == 4) hipLaunchKernelGGL((beam_scan_kernel<T, 4>), grid, dim3(kBeamThreads), 0, st, a);
-  else hipLaunchKernelGGL((beam_scan_kernel<T, 1>), grid, dim3(kBeamThreads), 0, st, a);
+  constexpr int S = sizeof(T) / 2;
+  if (p.nv == S) hipLaunchKernelGGL((beam_scan_kernel<T, S>), grid, dim3(kBeamThreads), 0, st, a);
+  else hipLaunchKernelGGL((beam_scan_kernel<T, 4 * S>), grid, dim3(kBeamThreads), 0, st, a);
 }
 
 // ---- tables ----------------------------------------------------------------------------
@@ -485,68 +586,72 @@ __device__ __forceinline__ int nth_bit(uint64_t x, int i) {
 }
 
 __global__ __launch_bounds__(kCols) void beam_tables_kernel(BeamTableArgs a) {
-  extern __shared__ int32_t old[];           // [K][kCols]
-  __shared__ int par[64], tail[64], sh_first[2];
-  __shared__ uint64_t sh_dead;
+  extern __shared__ int32_t old[];           // [K][kCols], a column its thread's own
+  __shared__ int sh_first[2];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int b = blockIdx.y, K = a.K, chunk = blockIdx.x;
   const int col = chunk * kCols + tid;
   const int32_t* rows = a.table + (int64_t)b * K * a.stride;
   int32_t* outs = a.out + (int64_t)b * K * a.out_stride;
   const bool in = col < a.width;
-  for (int k = 0; k < K; ++k) old[k * kCols + tid] = in ? rows[k * a.stride + col] : -1;
+  int p = lane < K ? a.parents[(int64_t)b * K + lane] : -1;   // row `lane` goes on from it
   const int len = max(0, a.lens[(int64_t)b * K]);
+  const int shared = a.shared ? max(0, a.shared[b]) : 0;
+  for (int k0 = 0; k0 < K; k0 += 8) {        // (eight loads on their way at once)
+    int32_t x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = in && k0 + i < K ? rows[(k0 + i) * a.stride + col] : -1;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (k0 + i < K) old[(k0 + i) * kCols + tid] = x[i];
+  }
   const int full = len / a.page;             // columns of full pages
   const bool part = len % a.page != 0;
-  const int shared = a.shared ? max(0, a.shared[b]) : 0;
-  if (wave == 0) {
-    int p = lane < K ? a.parents[(int64_t)b * K + lane] : -1;
-    if (p < 0 || p >= K) p = lane;
-    uint64_t kids = 0;                       // of row `lane`
-    for (int k = 0; k < K; ++k) {
-      const uint64_t x = __builtin_amdgcn_ballot_w64(lane < K && p == k);
-      if (lane == k) kids = x;
-    }
-    const int keeper = kids >> lane & 1 ? lane : kids ? __builtin_ctzll(kids) : -1;
-    const bool extra = __shfl(keeper, p, 64) != lane;
-    const uint64_t dead = __builtin_amdgcn_ballot_w64(lane < K && !kids);
-    const uint64_t extras = __builtin_amdgcn_ballot_w64(lane < K && extra);
-    int t = p;
-    if (lane < K && extra)
-      t = nth_bit(dead, __builtin_popcountll(extras & ((1ull << lane) - 1)));
-    par[lane] = p;
-    tail[lane] = t;
-    if (lane == 0) sh_dead = dead;
+  // which row's page row `lane` has in the part-filled page's column (each wave for itself)
+  if (p < 0 || p >= K) p = lane;
+  uint64_t kids = 0;                         // of row `lane`
+  for (int k = 0; k < K; ++k) {
+    const uint64_t x = __builtin_amdgcn_ballot_w64(lane < K && p == k);
+    if (lane == k) kids = x;
   }
-  __syncthreads();
+  const int keeper = kids >> lane & 1 ? lane : kids ? __builtin_ctzll(kids) : -1;
+  const bool extra = lane < K && __shfl(keeper, p, 64) != lane;
+  const uint64_t dead = __builtin_amdgcn_ballot_w64(lane < K && !kids);
+  const uint64_t extras = __builtin_amdgcn_ballot_w64(extra);
+  int tail = p;
+  if (extra) tail = nth_bit(dead, __builtin_popcountll(extras & ((1ull << lane) - 1)));
   // (in place, the shared columns, the same in every row, stay as they are)
-  if (in && !(a.out == a.table && col < shared))
+  if (in && !(a.out == a.table && col < shared)) {
+#pragma unroll 4
     for (int k = 0; k < K; ++k) {
-      const int from = col < full ? par[k] : col == full && part ? tail[k] : k;
+      const int par_k = __builtin_amdgcn_readlane(p, k);
+      const int tail_k = __builtin_amdgcn_readlane(tail, k);
+      const int from = col < full ? par_k : col == full && part ? tail_k : k;
       outs[k * a.out_stride + col] = old[from * kCols + tid];
     }
-  // which page is copied where, by the workgroup that holds the column
-  if (chunk == min(full / kCols, a.chunks - 1))
-    for (int k = tid; k < K; k += kCols) {
-      int src = -1, dst = -1;
-      if (part && full < a.width && tail[k] != par[k]) {
-        src = old[par[k] * kCols + full % kCols];
-        dst = old[tail[k] * kCols + full % kCols];
-      }
-      a.copies[2 * ((int64_t)b * K + k)] = src;
-      a.copies[2 * ((int64_t)b * K + k) + 1] = dst;
+  }
+  // which page is copied where, by the thread that holds the column (or the last there is)
+  if (col == min(full, max(1, a.width) - 1))
+    for (int k = 0; k < K; ++k) {
+      const int par_k = __builtin_amdgcn_readlane(p, k);
+      const int tail_k = __builtin_amdgcn_readlane(tail, k);
+      const bool moved = part && full < a.width && tail_k != par_k;
+      a.copies[2 * ((int64_t)b * K + k)] = moved ? old[par_k * kCols + tid] : -1;
+      a.copies[2 * ((int64_t)b * K + k) + 1] = moved ? old[tail_k * kCols + tid] : -1;
     }
 
   // pages of full columns that only rows without a child name, each once
-  const uint64_t dead = sh_dead;
   uint64_t gone = 0;
   if (in && col >= shared && col < full)
     for (uint64_t d = dead; d; d &= d - 1) {
       const int k = __builtin_ctzll(d);
       const int slot = old[k * kCols + tid];
       bool held = slot < 0;
-      for (int i = 0; i < K && !held; ++i)
-        held = (i < k || !(dead >> i & 1)) && old[i * kCols + tid] == slot;
+      for (int i0 = 0; i0 < K; i0 += 8) {
+#pragma unroll
+        for (int i = i0; i < i0 + 8; ++i)
+          held |= i < K && (i < k || !(dead >> i & 1)) && old[min(i, K - 1) * kCols + tid] == slot;
+      }
       if (!held) gone |= 1ull << k;
     }
   const int mine = __builtin_popcountll(gone);
