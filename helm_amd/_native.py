@@ -120,6 +120,12 @@ SIGNATURES = {
         _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p, _i64,
         _i64, _c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
         _f32, _f32, ctypes.c_int, ctypes.c_int, ctypes.c_int, _c_void_p]),
+    "helm_prefix_workspace_bytes": (_sz, [ctypes.c_int] * 6),
+    "helm_prefix_decode_attn": (ctypes.c_int, [
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i64, ctypes.c_int, _c_void_p,
+        _i64, ctypes.c_int, _c_void_p, _c_void_p, _c_void_p, ctypes.c_int, ctypes.c_int,
+        ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, _f32, _f32, ctypes.c_int,
+        ctypes.c_int, _c_void_p, _sz, _c_void_p]),
     "helm_beam_select_workspace_bytes": (_sz, [ctypes.c_int] * 5),
     "helm_beam_select": (ctypes.c_int, [
         _c_void_p, _i64, _i64, ctypes.c_int, _c_void_p, ctypes.c_int, ctypes.c_int,

@@ -120,18 +120,20 @@ class PreparedPool4Decode:
     before the last replay of a graph that holds one.  It holds addresses: a deep copy or
     pickle of it is refused."""
 
+    _entry = "helm_pool4_decode_attn"
+
     def __init__(self, idx, args, out, keep):
         self._idx, self._args, self.out, self._keep = idx, args, out, keep
         self._streams = set()              # those that the workspace and out are recorded on
 
     def __copy__(self) -> "PreparedPool4Decode":
-        return PreparedPool4Decode(self._idx, self._args, self.out, self._keep)
+        return type(self)(self._idx, self._args, self.out, self._keep)
 
     def __reduce_ex__(self, protocol):
         raise TypeError("a prepared call holds its operands' addresses: prepare the copies' own")
 
     def run(self) -> torch.Tensor:
-        stream = _engine.launch_on(self._idx, "helm_pool4_decode_attn", *self._args)
+        stream = _engine.launch_on(self._idx, self._entry, *self._args)
         if stream not in self._streams:
             for t in (self.out, self._keep[-1]):
                 t.record_stream(torch.cuda.current_stream(self._idx))

@@ -458,6 +458,35 @@ int helm_prompt_attn(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
                      float scale, float softcap, int window, int zero_rest, int dtype,
                      void* stream);
 
+/* ---- sequences that share their first pages ----------------------------------------- */
+
+/* helm_paged_decode_attn of R sequences in groups whose first pages are the same ones (beams
+ * of a prompt, requests under one system prompt): those are read once for a group, and
+ * the answer is the one that each sequence's whole table gives.  Slot s of the pools starts at
+ * s * slot_stride elements, its KV head h head_stride elements further on, a page being dense
+ * [page_size, D] rows, 16-byte aligned; page_size a multiple of 16.  Group g is sequences
+ * group_starts[g] .. group_starts[g + 1] (device int32 [n_groups + 1], ascending within 0 .. R);
+ * the first shared_pages[g] columns of their table rows hold the same slots, and it is the
+ * first row's that are read.  Sequences outside every group share nothing.
+ * q and out [R, Hq, q_len, D] dense, of the pools' type (HELM_F16, HELM_BF16): the q_len rows
+ * are the sequence's last tokens, row s sees tokens j <= p = seq_lens[r] - q_len + s, with
+ * window > 0 only j > p - window.  Hidden tokens, those past max_pages and those of pages whose
+ * slot is outside [0, n_slots) among them, take no part whatever they hold; a row that sees
+ * nothing is zeros.  softcap <= 0: off.  out may be q, but lie over nothing else.  The workspace
+ * (16-byte aligned) needs no contents before or after a call; calls that may overlap need one
+ * each.  head_dim 64, 128 or 256. */
+#define HELM_PREFIX_MAX_SEQS 4096
+#define HELM_PREFIX_MAX_GROUPS 1024
+size_t helm_prefix_workspace_bytes(int R, int Hq, int Hkv, int q_len, int D, int n_groups);
+int helm_prefix_decode_attn(const void* q, void* out, const void* k_pool, const void* v_pool,
+                            int64_t n_slots, int64_t slot_stride, int64_t head_stride,
+                            int page_size, const int32_t* page_table, int64_t table_stride,
+                            int max_pages, const int32_t* seq_lens,
+                            const int32_t* group_starts, const int32_t* shared_pages,
+                            int n_groups, int R, int Hq, int Hkv, int q_len, int D, float scale,
+                            float softcap, int window, int dtype, void* workspace,
+                            size_t ws_bytes, void* stream);
+
 /* ---- beam search over a paged cache ------------------------------------------------ */
 
 #define HELM_BEAMS_MAX 64     /* beams of a request, candidates of a selection */
