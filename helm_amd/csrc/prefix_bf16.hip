@@ -17,15 +17,16 @@ struct PfPlan {
   int wgs, own_tiles, own_rows;
   int64_t group_slots, own_slots, bytes;
 };
-// Workgroups of a KV head: as many as the device holds at once.
+// Workgroups of a KV head: a workgroup a CU in all.
 PfPlan pf_plan(int R, int Hq, int Hkv, int S, int D, int n_groups) {
   PfPlan p{};
   const int64_t rows = (int64_t)S * (Hq / Hkv);
-  p.wgs = std::max(1, (D == 256 ? 256 : 512) / Hkv);
+  const int waves = pf_waves(D);
+  p.wgs = std::max(1, 256 / Hkv);
   p.own_tiles = (int)((rows + kPfRows - 1) / kPfRows);
   p.own_rows = (int)std::min<int64_t>(rows, kPfRows);
-  p.group_slots = n_groups ? n_groups + R * rows / kPfRows + p.wgs : 0;
-  p.own_slots = (int64_t)R * p.own_tiles + p.wgs;
+  p.group_slots = n_groups ? n_groups + R * rows / kPfRows + waves * p.wgs : 0;
+  p.own_slots = (int64_t)R * p.own_tiles + waves * p.wgs;
   auto room = [](int64_t n) { return (n + 15) / 16 * 16; };
   p.bytes = room(R * (int64_t)sizeof(PfSeq)) +
             room(Hkv * p.group_slots * kPfRows * 2 * 4) + room(Hkv * p.own_slots * p.own_rows * 2 * 4) +
@@ -37,13 +38,13 @@ bool pf_shape_ok(int R, int Hq, int Hkv, int S, int max_pages, int page, int n_g
   if (R < 0 || R > HELM_PREFIX_MAX_SEQS || n_groups < 0 || n_groups > HELM_PREFIX_MAX_GROUPS ||
       Hkv < 1 || Hq < 1 || Hq % Hkv || S < 1 || max_pages < 0 || page < kBlockTok ||
       page % kBlockTok || (int64_t)max_pages * page > 0x7fffff00 ||
-      (int64_t)R * Hq * S > 0x7fffffff / kPfThreads || Hkv > 65536)
+      (int64_t)R * Hq * S > 0x7fffffff / kPfJoinThreads || Hkv > 65536)
     return false;
-  // the line of a KV head's walks stays within 2^31 steps, its slots within 2^31 rows
+  // the line of a KV head's walks stays within 2^30 steps
   const int64_t rows = (int64_t)S * (Hq / Hkv);
   const int64_t walks = (int64_t)R * ((rows + kPfRows - 1) / kPfRows) + n_groups + R * rows / kPfRows;
   const int64_t steps = ((int64_t)max_pages * page + kPfStep - 1) / kPfStep + 1;
-  return walks * steps <= 0x7fffffff - 512;
+  return walks * steps <= 0x3fffffff;
 }
 
 }  // namespace
@@ -75,7 +76,7 @@ extern "C" int helm_prefix_decode_attn(const void* q, void* out, const void* k_p
                         "bad shared-prefix decode shape (at most " +
                             std::to_string(HELM_PREFIX_MAX_SEQS) + " sequences, " +
                             std::to_string(HELM_PREFIX_MAX_GROUPS) +
-                            " groups, 2^31 steps of 32 tokens a KV head)");
+                            " groups, 2^30 steps of 32 tokens a KV head)");
   if (!scores_ok(scale, softcap))
     return report_error(HELM_E_INVALID, "scale, softcap or their quotient out of fp32's range");
   if (R == 0) return HELM_OK;

@@ -12,7 +12,7 @@ from helm_amd import _native
 from helm_amd.pool4 import _CODES, PreparedPool4Decode, check_scores
 from helm_amd.runtime import engine as _engine
 
-_MAX_SEQS, _MAX_GROUPS = 4096, 1024      # HELM_PREFIX_MAX_SEQS, _GROUPS
+_MAX_SEQS, _MAX_GROUPS = 4096, 512      # HELM_PREFIX_MAX_SEQS, _GROUPS
 
 
 class PreparedPrefixDecode(PreparedPool4Decode):
@@ -62,7 +62,7 @@ def prefix_decode_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
     The q_len rows are the sequence's last tokens: row s stands at p = len - q_len + s and
     sees tokens up to p, with `window` only the last `window` of those.  Hidden tokens take
     no part whatever they hold, and a row that sees nothing is zeros.  At most 4,096
-    sequences and 1,024 groups.  out: contiguous; it may be q itself, but share memory with
+    sequences and 512 groups.  out: contiguous; it may be q itself, but share memory with
     no other operand.  Returns out [R, Hq, q_len, D] in q's dtype."""
     idx, args, out, _ = _decode_args(q, k_pool, v_pool, page_table, seq_lens, group_starts,
                                      shared_pages, max_pages, scale, softcap, window, out)

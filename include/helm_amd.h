@@ -476,7 +476,7 @@ int helm_prompt_attn(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
  * (16-byte aligned) needs no contents before or after a call; calls that may overlap need one
  * each.  head_dim 64, 128 or 256. */
 #define HELM_PREFIX_MAX_SEQS 4096
-#define HELM_PREFIX_MAX_GROUPS 1024
+#define HELM_PREFIX_MAX_GROUPS 512
 size_t helm_prefix_workspace_bytes(int R, int Hq, int Hkv, int q_len, int D, int n_groups);
 int helm_prefix_decode_attn(const void* q, void* out, const void* k_pool, const void* v_pool,
                             int64_t n_slots, int64_t slot_stride, int64_t head_stride,

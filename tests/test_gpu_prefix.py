@@ -162,7 +162,7 @@ def test_long_shared_document():
     check(c, call(c, window=5000), window=5000, rows=[0, 7, 19])
 
 
-@pytest.mark.parametrize("R,n_groups", [(300, 100), (4096, 1024), (1000, 3), (65, 1)])
+@pytest.mark.parametrize("R,n_groups", [(300, 100), (4096, 512), (1000, 3), (65, 1)])
 def test_many_sequences(R, n_groups):
     r = random.Random(R)
     groups = []
