@@ -17,21 +17,26 @@ struct PfPlan {
   int wgs, own_tiles, own_rows;
   int64_t group_slots, own_slots, bytes;
 };
-// Workgroups of a KV head: a workgroup a CU in all.
-PfPlan pf_plan(int R, int Hq, int Hkv, int S, int D, int n_groups) {
+// Workgroups of a KV head: as many as the device holds at once.
+template <int D> PfPlan pf_plan_dim(int R, int Hq, int Hkv, int S, int n_groups) {
   PfPlan p{};
   const int64_t rows = (int64_t)S * (Hq / Hkv);
-  const int waves = pf_waves(D);
-  p.wgs = std::max(1, 256 / Hkv);
-  p.own_tiles = (int)((rows + kPfRows - 1) / kPfRows);
-  p.own_rows = (int)std::min<int64_t>(rows, kPfRows);
+  constexpr int waves = PfShape<D>::kWaves, tile = PfShape<D>::kTile;
+  p.wgs = std::max(1, 256 * PfShape<D>::kPerCu / Hkv);
+  p.own_tiles = (int)((rows + tile - 1) / tile);
+  p.own_rows = (int)std::min<int64_t>(rows, tile);
   p.group_slots = n_groups ? n_groups + R * rows / kPfRows + waves * p.wgs : 0;
-  p.own_slots = (int64_t)R * p.own_tiles + waves * p.wgs;
+  p.own_slots = (int64_t)R * p.own_tiles + p.wgs;
   auto room = [](int64_t n) { return (n + 15) / 16 * 16; };
-  p.bytes = room(R * (int64_t)sizeof(PfSeq)) +
-            room(Hkv * p.group_slots * kPfRows * 2 * 4) + room(Hkv * p.own_slots * p.own_rows * 2 * 4) +
+  p.bytes = room(R * (int64_t)sizeof(PfSeq)) + room(Hkv * p.group_slots * kPfRows * 2 * 4) +
+            room(Hkv * p.own_slots * p.own_rows * 2 * 4) +
             4 * Hkv * (p.group_slots * kPfRows + p.own_slots * p.own_rows) * D;
   return p;
+}
+PfPlan pf_plan(int R, int Hq, int Hkv, int S, int D, int n_groups) {
+  return D == 64 ? pf_plan_dim<64>(R, Hq, Hkv, S, n_groups)
+                 : D == 128 ? pf_plan_dim<128>(R, Hq, Hkv, S, n_groups)
+                            : pf_plan_dim<256>(R, Hq, Hkv, S, n_groups);
 }
 
 bool pf_shape_ok(int R, int Hq, int Hkv, int S, int max_pages, int page, int n_groups) {
@@ -42,8 +47,8 @@ bool pf_shape_ok(int R, int Hq, int Hkv, int S, int max_pages, int page, int n_g
     return false;
   // the line of a KV head's walks stays within 2^30 steps
   const int64_t rows = (int64_t)S * (Hq / Hkv);
-  const int64_t walks = (int64_t)R * ((rows + kPfRows - 1) / kPfRows) + n_groups + R * rows / kPfRows;
-  const int64_t steps = ((int64_t)max_pages * page + kPfStep - 1) / kPfStep + 1;
+  const int64_t walks = (int64_t)R * ((rows + 127) / 128) + n_groups + R * rows / 128;
+  const int64_t steps = ((int64_t)max_pages * page + kPfStep - 1) / kPfStep + 1 + kPfFixed;
   return walks * steps <= 0x3fffffff;
 }
 
