@@ -14,6 +14,9 @@
 // equal stretch of it.  So any lengths are spread evenly, and the launch depends on none:
 // every workgroup sums them up for itself.  A piece of a walk leaves its partials at slot
 // (walk + workgroup), of which no two pieces are alike, as both only grow along the line.
+// Walks of a group that has several come first on the line, each from a stretch's start on:
+// so the workgroups that read the same tokens for different rows do so side by side, through
+// one XCD's L2 (a KV head's workgroups are on one where 8, 16, ... heads lie round the XCDs).
 //
 // A walk is that of prompt.h: 32 x 32 matrix tiles, 32 rows a wave, K and V straight from memory
 // into LDS (two stage buffers, one barrier a stage), half of the query operand in LDS at
@@ -39,7 +42,7 @@ namespace helm {
 constexpr int kPfRows = 32;          // of a wave, and of a slot of the groups' partials
 constexpr int kPfStep = 32;          // tokens of a step
 // What a walk costs before its first step and behind its last, in steps.
-constexpr int kPfFixed = 2;
+constexpr int kPfFixed = 8;
 // A workgroup's least stretch.
 constexpr int kPfLeast = 4;
 constexpr int kPfJoinThreads = 256;
@@ -73,14 +76,13 @@ struct PfParams {
   float *group_ml, *group_o, *own_ml, *own_o;
 };
 
-// Where the partials of sequence r's rows are: walk t is [at + t each, at + (t + 1) each) of the
-// line (each: 0, there is none), its first kPfFixed before its steps.
+// Where the partials of sequence r's rows are: walk t is from at + t each on of the line, its
+// steps (0: there is none) from kPfFixed behind that on.
 struct PfSeq {
   int row0;                          // its first row among its group's
-  int group_at, group_each, group_slot;
-  int own_at, own_each;
+  int group_at, group_each, group_steps, group_slot;
+  int own_at, own_steps;
   int stretch;                       // of a workgroup
-  int pad;
 };
 
 // What a sequence of len tokens sees: [first, end) of its table, first a block's.
@@ -441,6 +443,36 @@ __device__ __forceinline__ void pf_store(const PfRowsOf<D>& s, float* ml, float*
           make_float4(s.o[e][4 * g], s.o[e][4 * g + 1], s.o[e][4 * g + 2], s.o[e][4 * g + 3]);
 }
 
+// Running sums of N numbers over the workgroup's threads before this one, and in all.
+template <int NW, int N>
+__device__ __forceinline__ void pf_scan(const int (&x)[N], int (&before)[N], int (&all)[N],
+                                        int (*sh)[NW]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int i = 0; i < N; ++i) before[i] = x[i];
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int t = __shfl_up(before[i], d, 64);
+      if (lane >= d) before[i] += t;
+    }
+  if (lane == 63)
+#pragma unroll
+    for (int i = 0; i < N; ++i) sh[i][wave] = before[i];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    before[i] -= x[i];
+    all[i] = 0;
+#pragma unroll
+    for (int v = 0; v < NW; ++v) {
+      if (v < wave) before[i] += sh[i][v];
+      all[i] += sh[i][v];
+    }
+  }
+}
+
 template <typename T, int D, bool kCap>
 __global__ __launch_bounds__(64 * PfShape<D>::kWaves, D == 256 ? 2 : 3)
 void prefix_attn_kernel(PfParams p) {
@@ -456,7 +488,7 @@ void prefix_attn_kernel(PfParams p) {
   __shared__ mf_u32x4 ldsq[PfShape<D>::kQLds ? NW * kPfRows * QC : 1];   // [wave][row][slot]
   extern __shared__ PfGroup groups[];                  // [n_groups + 1], then int [R]:
   int* ends = reinterpret_cast<int*>(groups + p.n_groups + 1);   // the sequences' tokens
-  __shared__ int sh_sum[2][NW], sh_found[4];
+  __shared__ int sh_sum[5][NW], sh_found[4];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hk = blockIdx.x % p.Hkv, wg = blockIdx.x / p.Hkv;
@@ -500,51 +532,59 @@ void prefix_attn_kernel(PfParams p) {
     const int r = e - n_groups, g = group_of(r);
     return {r, sg, max(g < 0 ? 0 : groups[g].shared, pf_view(p, ends[r]).first), ends[r]};
   };
-  auto tiles_of = [&](const Entity& e) { return (e.rows + kTile - 1) / kTile; };
-  auto each_of = [&](const Entity& e) {
-    const int n = pf_steps(e.first, e.end);
-    return n ? n + kPfFixed : 0;
-  };
-  // each thread sums a run of entities, of lengths and of the groups' slots
+  auto tiles_of = [&](int rows) { return (rows + kTile - 1) / kTile; };
+  auto slots_of = [&](int e, int rows) { return e < n_groups ? (rows + kPfRows - 1) / kPfRows : 0; };
+  auto several = [&](int e, int rows) { return e < n_groups && rows > kTile; };
+  // each thread sums a run of entities: lengths, walks and slots of the groups of several
+  // walks, lengths and slots of the others
   const int per = (E + kThreads - 1) / kThreads;
   const int e0 = min(E, tid * per), e1 = min(E, e0 + per);
-  int sum = 0, slots = 0;
+  constexpr int N = 5;
+  int sum[N] = {}, at[N], total[N];
   for (int e = e0; e < e1; ++e) {
     const Entity n = entity(e);
-    sum += tiles_of(n) * each_of(n);
-    if (e < n_groups) slots += (n.rows + kPfRows - 1) / kPfRows;
-  }
-  int at = sum, slot = slots, total = 0;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int x = __shfl_up(at, d, 64), y = __shfl_up(slot, d, 64);
-    if (lane >= d) {
-      at += x;
-      slot += y;
+    const int steps = pf_steps(n.first, n.end), tiles = tiles_of(n.rows);
+    const int len = steps ? tiles * (steps + kPfFixed) : 0;
+    if (several(e, n.rows)) {
+      sum[0] += len;
+      sum[1] += tiles;
+      sum[2] += slots_of(e, n.rows);
+    } else {
+      sum[3] += len;
+      sum[4] += slots_of(e, n.rows);
     }
   }
-  if (lane == 63) {
-    sh_sum[0][wave] = at;
-    sh_sum[1][wave] = slot;
-  }
-  __syncthreads();
-  at -= sum;
-  slot -= slots;
-#pragma unroll
-  for (int v = 0; v < NW; ++v) {
-    if (v < wave) {
-      at += sh_sum[0][v];
-      slot += sh_sum[1][v];
+  pf_scan<NW, N>(sum, at, total, sh_sum);
+  // whether a stretch's start is worth it: half a stretch a walk is left unused
+  const bool align = total[1] > 0 && 2 * total[1] <= p.wgs;
+  const int room = p.wgs - (align ? total[1] : 0);
+  const int stretch = max(kPfLeast, (total[0] + total[3] + room - 1) / room);
+  auto each_of = [&](bool multi, int steps) {
+    const int n = steps ? steps + kPfFixed : 0;
+    return multi && align ? (n + stretch - 1) / stretch * stretch : n;
+  };
+  if (align) {
+    int len[1] = {0}, to[1], all[1];
+    for (int e = e0; e < e1; ++e) {
+      const Entity n = entity(e);
+      if (several(e, n.rows)) len[0] += tiles_of(n.rows) * each_of(true, pf_steps(n.first, n.end));
     }
-    total += sh_sum[0][v];
+    __syncthreads();                                   // (sh_sum has been read)
+    pf_scan<NW, 1>(len, to, all, sh_sum);
+    at[0] = to[0];
+    total[0] = all[0];
   }
-  total = __builtin_amdgcn_readfirstlane(total);
-  const int stretch = max(kPfLeast, (total + p.wgs - 1) / p.wgs);
-  const int a = wg * stretch, b = min(a + stretch, total);
-  for (int e = e0, x = at, y = slot; e < e1; ++e) {
+  const int end_all = __builtin_amdgcn_readfirstlane(total[0] + total[3]);
+  const int a = wg * stretch, b = min(a + stretch, end_all);
+  at[3] += total[0];
+  at[4] += total[2];
+  for (int e = e0; e < e1; ++e) {
     const Entity n = entity(e);
-    const int each = each_of(n), len = tiles_of(n) * each;
-    if (a >= x && a < x + len) {
+    const bool multi = several(e, n.rows);
+    const int steps = pf_steps(n.first, n.end), tiles = tiles_of(n.rows);
+    const int each = each_of(multi, steps);
+    int &x = at[multi ? 0 : 3], &y = at[multi ? 2 : 4];
+    if (a >= x && a < x + tiles * each) {
       sh_found[0] = e;
       sh_found[1] = x;
       sh_found[2] = y;
@@ -556,22 +596,25 @@ void prefix_attn_kernel(PfParams p) {
       } else {
         PfSeq& q = p.seqs[e - n_groups];
         q.own_at = x;
-        q.own_each = each;
+        q.own_steps = steps;
         q.stretch = stretch;
       }
     }
-    x += len;
-    if (e < n_groups) y += (n.rows + kPfRows - 1) / kPfRows;
+    x += tiles * each;
+    y += slots_of(e, n.rows);
   }
   __syncthreads();
   if (blockIdx.x == 0) {
     for (int r = tid; r < p.R; r += kThreads) {
       const int g = group_of(r);
+      const Entity n = g < 0 ? Entity{0, 0, 0, 0} : entity(g);
+      const int steps = pf_steps(n.first, n.end);
       PfSeq& q = p.seqs[r];
-      q.row0 = g < 0 ? 0 : (r - groups[g].start) * sg;
+      q.row0 = g < 0 ? 0 : (r - n.seq0) * sg;
       q.group_at = g < 0 ? 0 : lds0.at.at[g];
       q.group_slot = g < 0 ? 0 : lds0.at.slot[g];
-      q.group_each = g < 0 ? 0 : each_of(entity(g));
+      q.group_each = each_of(several(g < 0 ? E : g, n.rows), steps);
+      q.group_steps = steps;
     }
     __syncthreads();                                   // (the walks' buffers may be written)
   }
@@ -580,6 +623,10 @@ void prefix_attn_kernel(PfParams p) {
   int e = __builtin_amdgcn_readfirstlane(sh_found[0]);
   int x = __builtin_amdgcn_readfirstlane(sh_found[1]);
   int y = __builtin_amdgcn_readfirstlane(sh_found[2]);
+  auto rows_at = [&](int i) {
+    return i < n_groups ? max(0, groups[i + 1].start - groups[i].start) * sg : sg;
+  };
+  bool multi = e < E && several(e, rows_at(e));
   PfRowsOf<D> s;
   s.qs = &ldsq[PfShape<D>::kQLds ? (wave * kPfRows + (lane & 31)) * QC : 0];
   for (int t = -1; e < E && x < b;) {
@@ -589,13 +636,17 @@ void prefix_attn_kernel(PfParams p) {
     w.first = __builtin_amdgcn_readfirstlane(n.first);
     w.end = __builtin_amdgcn_readfirstlane(n.end);
     const int rows = __builtin_amdgcn_readfirstlane(n.rows);
-    const int tiles = (rows + kTile - 1) / kTile, steps = pf_steps(w.first, w.end);
-    const int each = steps ? steps + kPfFixed : 0;
+    const int tiles = tiles_of(rows), steps = pf_steps(w.first, w.end);
+    const int each = each_of(multi, steps);
     t = t < 0 ? (each ? max(0, (a - x) / each) : tiles) : t + 1;
-    if (t >= tiles || x + t * each >= b) {             // the next group, sequence
+    if (t >= tiles || x + t * each >= b) {             // the next group of its kind, sequence
       x += tiles * each;
-      if (e < n_groups) y += (rows + kPfRows - 1) / kPfRows;
-      ++e;
+      y += slots_of(e, rows);
+      for (++e; e < n_groups && several(e, rows_at(e)) != multi;) ++e;
+      if (multi && e >= n_groups) {                    // (no more of several walks)
+        multi = false;
+        for (e = 0; e < n_groups && several(e, rows_at(e));) ++e;
+      }
       t = -1;
       continue;
     }
@@ -639,15 +690,16 @@ __global__ __launch_bounds__(kPfJoinThreads) void prefix_join_kernel(PfParams p)
   const int s = blockIdx.x % p.S, hq = blockIdx.x / p.S % p.Hq, r = blockIdx.x / p.S / p.Hq;
   const int hk = hq / p.G, row = s * p.G + hq % p.G;
   const PfSeq q = p.seqs[r];
-  // the pieces of a walk at [at, at + each) of the line: on the stretches of its steps
-  auto pieces = [&](int at, int each, int& first) {
-    first = each > 0 ? (at + kPfFixed) / q.stretch : 0;
-    return each > 0 ? (at + each - 1) / q.stretch - first + 1 : 0;
+  // the pieces of a walk whose steps start kPfFixed behind `at` on the line
+  auto pieces = [&](int at, int steps, int& first) {
+    first = (at + kPfFixed) / q.stretch;
+    return steps > 0 ? (at + kPfFixed + steps - 1) / q.stretch - first + 1 : 0;
   };
   const int grow = q.row0 + row, gt = grow / kTile, ot = row / kTile;
   int w0, v0;
-  int n_group = pieces(q.group_at + gt * q.group_each, q.group_each, w0);
-  const int n_own = pieces(q.own_at + ot * q.own_each, q.own_each, v0);
+  int n_group = pieces(q.group_at + gt * q.group_each, q.group_steps, w0);
+  const int own_each = q.own_steps > 0 ? q.own_steps + kPfFixed : 0;
+  const int n_own = pieces(q.own_at + ot * own_each, q.own_steps, v0);
   const int g0 = q.group_slot + grow / kPfRows + NW * w0, o0 = r * p.own_tiles + ot + v0;
   n_group = min(n_group, max(0, (p.group_slots - g0 + NW - 1) / NW));
   const int n = n_group + n_own;
