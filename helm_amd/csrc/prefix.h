@@ -19,9 +19,10 @@
 // one XCD's L2 (a KV head's workgroups are on one where 8, 16, ... heads lie round the XCDs).
 //
 // A walk is that of prompt.h: 32 x 32 matrix tiles, 32 rows a wave, K and V straight from memory
-// into LDS (two stage buffers, one barrier a stage), half of the query operand in LDS at
-// D = 128 and 256.  Few rows keep few of the waves busy, which is enough: a step of one wave
-// takes 0.6 us at most, its 64 D bytes of K and V 2 us of a third of a CU's share of the memory.
+// into LDS, one barrier a stage.  Few rows keep few of the waves busy, which is enough: a step of
+// one wave takes 0.6 us, its 128 D bytes of K and V 1.6 us of half a CU's share of the memory.
+// Here K and V come from HBM, not from L2: three stages are on their way (one at D = 256, whose
+// buffers are twice as large and share LDS with half of the query operand).
 // Weights are rounded once to the 16-bit type (2^-8 of the weight in bf16, 2^-11 in f16, and the
 // row's sum adds the rounded ones); f16 weights are taken times 2^9.
 //
@@ -46,11 +47,12 @@ constexpr int kPfFixed = 8;
 // A workgroup's least stretch.
 constexpr int kPfLeast = 4;
 constexpr int kPfJoinThreads = 256;
-// Waves of a workgroup, tokens of a stage, workgroups of a CU.
+// Waves of a workgroup, tokens of a stage, stage buffers, workgroups of a CU, whether the upper
+// half of the query operand stays in LDS.
 template <int D> struct PfShape {
-  static constexpr int kWaves = PromptShape<D>::kWaves, kTok = PromptShape<D>::kTok;
-  static constexpr int kPerCu = D == 256 ? 1 : 3;
-  static constexpr bool kQLds = PromptShape<D>::kQLds;
+  static constexpr int kWaves = D == 256 ? 8 : 4, kTok = D == 64 ? 64 : 32;
+  static constexpr int kBufs = D == 256 ? 2 : 4, kPerCu = D == 256 ? 1 : 2;
+  static constexpr bool kQLds = D == 256;
   static constexpr int kTile = kPfRows * kWaves;       // rows of a walk
 };
 
@@ -112,11 +114,15 @@ struct PfAt {
   int at[HELM_PREFIX_MAX_GROUPS], slot[HELM_PREFIX_MAX_GROUPS];
 };
 
-// A stage of K and V in LDS, blocks of 16 tokens.
+// A stage of K and V in LDS, blocks of 16 tokens.  The stage buffers are objects of their own, so
+// that the compiler sees that loads into one do not touch the reads of another.
 template <int D> struct PfBuf {
   static constexpr int kBlocks = PfShape<D>::kTok / kBlockTok, kChunks = 2 * D;
   typedef mf_u32x4 type[2][kBlocks][kChunks];
 };
+template <int D> using PfLds = typename PfBuf<D>::type;
+template <int D>
+using PfMore = std::conditional_t<(PfShape<D>::kBufs > 2), PfLds<D>, mf_u32x4>;
 
 // A walk's piece: rows [row0, row0 + rows) of sequences seq0 .. (S G rows each), steps [i0, i1)
 // of tokens [first, end).
@@ -326,14 +332,14 @@ __device__ __forceinline__ void pf_add_special(const PfParams& p, const PfPiece&
 // done again, with V's infinities and NaN taken for zeros.
 template <typename T, int D, bool kCap>
 __device__ __forceinline__ bool pf_walk(const PfParams& p, const PfPiece& w, int hk, const int* ends,
-                                        PfRowsOf<D>& s, typename PfBuf<D>::type& lds0,
-                                        typename PfBuf<D>::type& lds1) {
-  using Buf = typename PfBuf<D>::type;
-  constexpr int NW = PfShape<D>::kWaves, SB = PfBuf<D>::kBlocks, kSteps = SB / 2;
+                                        PfRowsOf<D>& s, PfLds<D>& lds0, PfLds<D>& lds1,
+                                        PfMore<D>& lds2, PfMore<D>& lds3) {
+  using Buf = PfLds<D>;
+  constexpr int NW = PfShape<D>::kWaves, NB = PfShape<D>::kBufs;
+  constexpr int SB = PfBuf<D>::kBlocks, kSteps = SB / 2;
   constexpr int CPR = D / 8, kRow = 2 * D, kBlk = kBlockTok * kRow, kBlkLoads = kBlk / 1024;
   constexpr int kLoads = 2 * SB * kBlkLoads / NW;      // a wave's, of one block
   constexpr int NK = D / 16, NQ = PfRowsOf<D>::NQ, QC = PfRowsOf<D>::QC;
-  __shared__ int sh_gone[2][SB];
   const int lane = threadIdx.x & 63, jr = lane & 31, hh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const bool wave_rows = kPfRows * wave < w.rows;
@@ -342,25 +348,36 @@ __device__ __forceinline__ bool pf_walk(const PfParams& p, const PfPiece& w, int
   const int32_t* trow = p.table + (int64_t)w.seq0 * p.table_stride;
   // load i of the stage's is part i % kBlkLoads of a block's K, its V, the next block's, ...
   const int my_blk = wave * kLoads / kBlkLoads / 2;
-  // lane i holds the slot of this wave's block of stage win0 + i (-1: none), its place there
+  // lane SB k + u holds the slot of block u of stage win0 + k (-1: none), its place there
+  constexpr int kWin = 64 / SB;
   struct Window {
     int slot, in;
   };
   auto window = [&](int s0) -> Window {
-    const int block = (tok0 >> 4) + SB * (s0 + lane) + my_blk;
+    const int st = s0 + lane / SB;
+    const int block = (tok0 >> 4) + SB * st + lane % SB;
     const int page = (unsigned)block / (unsigned)p.bpp;
-    return {s0 + lane < stages && page < p.max_pages ? trow[page] : -1, block - page * p.bpp};
+    return {st < stages && page < p.max_pages ? trow[page] : -1, block - page * p.bpp};
   };
   Window win = window(0), next{-1, 0};
   int win0 = 0;
+  uint32_t gone = 0;                                   // a byte a stage on its way: blocks not there
+  // (past the last stage: nothing, zeros, so that every stage waits for the same)
   auto dma = [&](int st, Buf& dst) {
-    if (st == win0 + 64) {
+    if (st == win0 + kWin) {
       win = next;
-      win0 += 64;
-      next = window(win0 + 64);
+      win0 += kWin;
+      next = window(win0 + kWin);
     }
-    const int slot = __builtin_amdgcn_readlane(win.slot, (st - win0) & 63);
-    const int in = __builtin_amdgcn_readlane(win.in, (st - win0) & 63);
+    uint32_t g = 0;
+#pragma unroll
+    for (int u = 0; u < SB; ++u)
+      if ((uint32_t)__builtin_amdgcn_readlane(win.slot, SB * (st - win0) + u) >=
+          (uint32_t)p.n_slots)
+        g |= 1u << u;
+    gone = gone >> 8 | g << 24;
+    const int slot = __builtin_amdgcn_readlane(win.slot, SB * (st - win0) + my_blk);
+    const int in = __builtin_amdgcn_readlane(win.in, SB * (st - win0) + my_blk);
     const PfBlock b = pf_block(p, w, hk, slot, in, tok0 + 16 * (SB * st + my_blk), kBlk);
 #pragma unroll
     for (int k = 0; k < kLoads; ++k) {
@@ -370,7 +387,6 @@ __device__ __forceinline__ bool pf_walk(const PfParams& p, const PfPiece& w, int
       buf_load16_lds(make_rsrc((is_v ? p.v : p.k) + b.at, b.nt * kRow), &dst[is_v][my_blk][64 * u],
                      t * kRow + 16 * ((lane % CPR) ^ swz<D>(t)));
     }
-    if (lane == 0) sh_gone[st & 1][my_blk] = (uint32_t)slot >= (uint32_t)p.n_slots;
   };
   // careful: infinities and NaN in what this wave has loaded of V, taken for zeros
   auto clean = [&](Buf& buf) {
@@ -389,8 +405,17 @@ __device__ __forceinline__ bool pf_walk(const PfParams& p, const PfPiece& w, int
   mf_u32x4 q[NK];
 #pragma unroll
   for (int i = 0; i < NK; ++i) q[i] = *reinterpret_cast<const mf_u32x4*>(qp + 16 * (2 * i + hh));
-  dma(0, lds0);
-  if (stages > 64) next = window(64);
+  auto start = [&] {
+    dma(0, lds0);
+    if constexpr (NB > 2) {
+      __builtin_amdgcn_sched_barrier(0);               // (in this order)
+      dma(1, lds1);
+      __builtin_amdgcn_sched_barrier(0);
+      dma(2, lds2);
+    }
+    if (stages > kWin) next = window(kWin);
+  };
+  start();
 #pragma unroll
   for (int i = 0; i < NK; ++i) {
     const mf_u32x4 x = s.ok ? q[i] ^ p.q_sign : mf_u32x4{0u, 0u, 0u, 0u};
@@ -400,31 +425,49 @@ __device__ __forceinline__ bool pf_walk(const PfParams& p, const PfPiece& w, int
   for (bool careful = false;; careful = true) {
     pf_zero(s);
     auto stage = [&](int st, Buf& cur, Buf& nxt) {
-      // the stage is in LDS (this wave's loads done, then everyone's), and every wave is
-      // done with the other buffer, which the next stage's loads fill
-      __builtin_amdgcn_s_waitcnt(0x0F70);              // vmcnt(0)
-      if (careful) clean(cur);
-      __syncthreads();
-      const int gone = (int)__builtin_amdgcn_ballot_w64(lane < SB && sh_gone[st & 1][lane % SB]);
-      if (st + 1 < stages) dma(st + 1, nxt);
+      // the stage is in LDS (this wave's loads done, all but those of the NB - 2 stages behind
+      // it, then everyone's), and every wave is done with the buffer of the stage before,
+      // which loads of a later one fill (a plain barrier would wait for all loads)
+      if (careful) {
+        __builtin_amdgcn_s_waitcnt(0x0F70 | (NB - 2) * kLoads);    // vmcnt
+        clean(cur);
+      }
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NB - 2) * kLoads)
+                   : "memory");
+      __builtin_amdgcn_sched_barrier(0);
+      const uint32_t there = gone >> (32 - 8 * (NB - 1));          // this stage's
+      dma(st + NB - 1, nxt);
       if (!wave_rows) return;
 #pragma unroll
       for (int j = 0; j < kSteps; ++j)
         if (j == 0 || w.i0 + kSteps * st + j < w.i1)
-          pf_step<T, D, kCap>(p, s, tok0 + kPfStep * (kSteps * st + j), gone >> (2 * j) & 3,
+          pf_step<T, D, kCap>(p, s, tok0 + kPfStep * (kSteps * st + j), there >> (2 * j) & 3,
                               reinterpret_cast<const char*>(&cur[0][2 * j][0]),
                               reinterpret_cast<const char*>(&cur[1][2 * j][0]));
     };
-    for (int st = 0; st < stages; st += 2) {
-      stage(st, lds0, lds1);
-      if (st + 1 < stages) stage(st + 1, lds1, lds0);
+    // (left from within: a round's end always has the same loads on their way)
+    for (int st = 0;; st += NB) {
+      if constexpr (NB > 2) {
+        stage(st, lds0, lds3);
+        if (st + 1 >= stages) break;
+        stage(st + 1, lds1, lds0);
+        if (st + 2 >= stages) break;
+        stage(st + 2, lds2, lds1);
+        if (st + 3 >= stages) break;
+        stage(st + 3, lds3, lds2);
+      } else {
+        stage(st, lds0, lds1);
+        if (st + 1 >= stages) break;
+        stage(st + 1, lds1, lds0);
+      }
+      if (st + NB >= stages) break;
     }
-    // (the barrier also ends every wave's reads of the buffers)
+    // (no load is on its way any more, and the barrier ends every wave's reads of the buffers)
+    __builtin_amdgcn_s_waitcnt(0x0F70);
     if (!__syncthreads_or(wave_rows && pf_odd(s)) || careful) return careful;
     win = window(0);
     win0 = 0;
-    if (stages > 64) next = window(64);
-    dma(0, lds0);
+    start();
   }
 }
 
@@ -474,17 +517,17 @@ __device__ __forceinline__ void pf_scan(const int (&x)[N], int (&before)[N], int
 }
 
 template <typename T, int D, bool kCap>
-__global__ __launch_bounds__(64 * PfShape<D>::kWaves, D == 256 ? 2 : 3)
+__global__ __launch_bounds__(64 * PfShape<D>::kWaves, 2)
 void prefix_attn_kernel(PfParams p) {
   constexpr int NW = PfShape<D>::kWaves, kThreads = 64 * NW, kTile = PfShape<D>::kTile;
   constexpr int QC = PfRowsOf<D>::QC;
-  typedef typename PfBuf<D>::type Buf;
   __shared__ union Lds {
     __device__ Lds() {}
-    Buf buf;
+    PfLds<D> buf;
     PfAt at;
   } lds0;
-  __shared__ Buf lds1;
+  __shared__ PfLds<D> lds1;
+  __shared__ PfMore<D> lds2, lds3;
   __shared__ mf_u32x4 ldsq[PfShape<D>::kQLds ? NW * kPfRows * QC : 1];   // [wave][row][slot]
   extern __shared__ PfGroup groups[];                  // [n_groups + 1], then int [R]:
   int* ends = reinterpret_cast<int*>(groups + p.n_groups + 1);   // the sequences' tokens
@@ -669,7 +712,7 @@ void prefix_attn_kernel(PfParams p) {
       ml = p.own_ml + 2 * at;
       part = p.own_o + at * D;
     }
-    const bool careful = pf_walk<T, D, kCap>(p, w, hk, ends, s, lds0.buf, lds1);
+    const bool careful = pf_walk<T, D, kCap>(p, w, hk, ends, s, lds0.buf, lds1, lds2, lds3);
     if (kPfRows * wave < w.rows)
       pf_store(s, ml + 2 * kPfRows * wave, part + (int64_t)kPfRows * wave * D);
     if (careful) {
