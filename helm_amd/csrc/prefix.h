@@ -9,7 +9,7 @@
 // Bound by memory up to some 400 rows a KV head (4 D operations a row and token against
 // 4 D bytes a token), by the matrix cores beyond.
 //
-// Work: a KV head's walks, the groups' (128 rows each, 256 at D = 256) and then the sequences',
+// Work: a KV head's walks, the groups' (128 rows each) and then the sequences',
 // lie end to end on one line of steps of 32 tokens, and each of the head's workgroups takes an
 // equal stretch of it.  So any lengths are spread evenly, and the launch depends on none:
 // every workgroup sums them up for itself.  A piece of a walk leaves its partials at slot
@@ -21,10 +21,12 @@
 // A walk is that of prompt.h: 32 x 32 matrix tiles, 32 rows a wave, K and V straight from memory
 // into LDS, one barrier a stage.  Few rows keep few of the waves busy, which is enough: a step of
 // one wave takes 0.6 us, its 128 D bytes of K and V 1.6 us of half a CU's share of the memory.
-// Here K and V come from HBM, not from L2: three stages are on their way (one at D = 256, whose
-// buffers are twice as large and share LDS with half of the query operand).
+// Here K and V come from HBM, not from L2: three stages are on their way.
 // Weights are rounded once to the 16-bit type (2^-8 of the weight in bf16, 2^-11 in f16, and the
-// row's sum adds the rounded ones); f16 weights are taken times 2^9.
+// row's sum adds the rounded ones); f16 weights are taken times 2^9, those under 2^-34 of the
+// largest are lost.  An output's relative rms error is 2.3e-3 in bf16 and 2.7e-4 in f16, against
+// 1.7e-3 and 2.1e-4 where weights stay in fp32.  (A second product for what the rounding leaves,
+// in walks of up to 64 rows: 4 to 13% of the call, 32k tokens under 64 sequences 81 -> 92 us.)
 //
 // Hidden tokens (past a row's position or out of its window, past a sequence's end, in pages
 // that the pool does not have) take no part whatever they hold: their scores are overwritten,
@@ -43,17 +45,17 @@ namespace helm {
 constexpr int kPfRows = 32;          // of a wave, and of a slot of the groups' partials
 constexpr int kPfStep = 32;          // tokens of a step
 // What a walk costs before its first step and behind its last, in steps.
-constexpr int kPfFixed = 8;
+constexpr int kPfFixed = 5;
 // A workgroup's least stretch.
 constexpr int kPfLeast = 4;
 constexpr int kPfJoinThreads = 256;
-// Waves of a workgroup, tokens of a stage, stage buffers, workgroups of a CU, whether the upper
-// half of the query operand stays in LDS.
+constexpr int kPfWaves = 4;          // of a workgroup
+constexpr int kPfThreads = 64 * kPfWaves;
+constexpr int kPfTile = kPfRows * kPfWaves;            // rows of a walk
+constexpr int kPfBufs = 4;           // stage buffers
+// Tokens of a stage; workgroups of a CU, which the buffers (16 KB, 32 at D = 256) leave room for.
 template <int D> struct PfShape {
-  static constexpr int kWaves = D == 256 ? 8 : 4, kTok = D == 64 ? 64 : 32;
-  static constexpr int kBufs = D == 256 ? 2 : 4, kPerCu = D == 256 ? 1 : 2;
-  static constexpr bool kQLds = D == 256;
-  static constexpr int kTile = kPfRows * kWaves;       // rows of a walk
+  static constexpr int kTok = D == 64 ? 64 : 32, kPerCu = D == 256 ? 1 : 2;
 };
 
 struct PfParams {
@@ -94,8 +96,9 @@ struct PfView {
 __device__ __forceinline__ int pf_room(const PfParams& p) { return p.max_pages * p.page; }
 __device__ __forceinline__ PfView pf_view(const PfParams& p, int len) {
   const int end = min(max(len, 0), pf_room(p));
-  const int first = p.window > 0 ? max(0, end - p.S + 1 - p.window) : 0;
-  return {min(first, end) & ~15, end};
+  // (row 0's first: end - S + 1 - window, or 0)
+  const int first = p.window > 0 && end - p.window >= p.S ? end - p.window - p.S + 1 : 0;
+  return {first & ~15, end};
 }
 // Tokens in the shared pages of a group.
 __device__ __forceinline__ int pf_shared(const PfParams& p, int pages) {
@@ -121,8 +124,6 @@ template <int D> struct PfBuf {
   typedef mf_u32x4 type[2][kBlocks][kChunks];
 };
 template <int D> using PfLds = typename PfBuf<D>::type;
-template <int D>
-using PfMore = std::conditional_t<(PfShape<D>::kBufs > 2), PfLds<D>, mf_u32x4>;
 
 // A walk's piece: rows [row0, row0 + rows) of sequences seq0 .. (S G rows each), steps [i0, i1)
 // of tokens [first, end).
@@ -130,13 +131,10 @@ struct PfPiece {
   int seq0, row0, rows, first, end, i0, i1;
 };
 
-// What a wave holds: 32 query rows (their operand's upper half in LDS at qs, kQLds), what they
-// see, their sums.
+// What a wave holds: 32 query rows, what they see, their sums.
 template <int D> struct PfRowsOf {
   static constexpr int NK = D / 16, NE = D / 32;
-  static constexpr int NQ = PfShape<D>::kQLds ? NK / 2 : NK, QC = D / 16;
-  mf_u32x4 q[NQ];
-  mf_u32x4* qs;                      // row jr's chunks
+  mf_u32x4 q[NK];
   int last, from;                    // row jr's last and first visible token
   int all_to, all_from;              // every row sees the tokens between
   bool ok;
@@ -157,7 +155,7 @@ __device__ __forceinline__ PfRow pf_row(const PfParams& p, const PfPiece& w, int
   r.g = row % (unsigned)p.G;
   const int at = ends[r.seq] - p.S + r.s;
   r.last = min(at, w.end - 1);
-  r.from = p.window > 0 ? max(0, at - p.window + 1) : 0;
+  r.from = p.window > 0 && at >= p.window ? at - p.window + 1 : 0;
   return r;
 }
 // The wave's rows first ..: what they see, and the address of row jr's query.
@@ -203,10 +201,8 @@ template <typename T, int D, bool kCap>
 __device__ __forceinline__ void pf_step(const PfParams& p, PfRowsOf<D>& s, int tok0, int gone,
                                         const char* kk, const char* vv) {
   constexpr int NK = D / 16, NE = D / 32, kRow = 2 * D, kBlk = kBlockTok * kRow;
-  constexpr int NQ = PfRowsOf<D>::NQ, QC = PfRowsOf<D>::QC;
   constexpr int kShift = std::is_same<T, f16_t>::value ? 9 : 0;
   constexpr float kSlack = chunk_slack(kShift);
-  constexpr bool kAnew = PromptShape<D>::kAnew;        // (offsets in few registers)
   using Ops = MfmaOps<T>;
   using M32 = Mfma32<T>;
   const int lane = threadIdx.x & 63, jr = lane & 31, hh = lane >> 5;
@@ -214,23 +210,16 @@ __device__ __forceinline__ void pf_step(const PfParams& p, PfRowsOf<D>& s, int t
   const int g_a = jr >> 3, h_a = (jr >> 2) & 1, t_a = jr & 3;
   const int tau = 16 * (g_a >> 1) + 8 * h_a + 4 * (g_a & 1) + t_a;
   const int ktok = tau & 15, nl = lane & 15;
-  int k_off = (tau >> 4) * kBlk + ktok * kRow + 16 * (hh ^ swz<D>(ktok));
+  const int k_off = (tau >> 4) * kBlk + ktok * kRow + 16 * (hh ^ swz<D>(ktok));
   const int v_tok0 = 8 * hh + (nl >> 2);
-  int v_off = v_tok0 * kRow + 16 * ((2 * (jr >> 4) + ((nl & 3) >> 1)) ^ swz<D>(v_tok0)) +
-              8 * (nl & 1);
-  int q_off = 16 * (hh ^ out_swz<QC>(jr));
-  if constexpr (kAnew) asm volatile("" : "+v"(k_off), "+v"(v_off), "+v"(q_off));
+  const int v_off = v_tok0 * kRow + 16 * ((2 * (jr >> 4) + ((nl & 3) >> 1)) ^ swz<D>(v_tok0)) +
+                    8 * (nl & 1);
   mf_f32x16 sc;
 #pragma unroll
   for (int r = 0; r < 16; ++r) sc[r] = 0.f;
 #pragma unroll
-  for (int i = 0; i < NK; ++i) {
-    const mf_u32x4 q = i < NQ ? s.q[i < NQ ? i : 0]
-                              : *reinterpret_cast<const mf_u32x4*>(
-                                    reinterpret_cast<const char*>(s.qs) + (q_off ^ (32 * (i - NQ))));
-    sc = M32::mma(*reinterpret_cast<const mf_u32x4*>(kk + (k_off ^ (32 * i))), q, sc);
-    if (kAnew && i % 4 == 3) __builtin_amdgcn_sched_barrier(0);      // (few operands ahead)
-  }
+  for (int i = 0; i < NK; ++i)
+    sc = M32::mma(*reinterpret_cast<const mf_u32x4*>(kk + (k_off ^ (32 * i))), s.q[i], sc);
   const float scale2 = p.scale * kLog2E;
   const float mul = kCap ? 1.f : scale2;                     // logits in base-2 units
   float x[16];
@@ -275,7 +264,6 @@ __device__ __forceinline__ void pf_step(const PfParams& p, PfRowsOf<D>& s, int t
       const uint2 a0 = ld_tr16(at + (v_off ^ (64 * e)));
       const uint2 a1 = ld_tr16(at + (v_off ^ (64 * e) ^ 16) + 4 * kRow);
       s.o[e] = M32::mma(mf_u32x4{a0.x, a0.y, a1.x, a1.y}, pop, s.o[e]);
-      if (kAnew && e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
     }
   }
 }
@@ -331,16 +319,16 @@ __device__ __forceinline__ void pf_add_special(const PfParams& p, const PfPiece&
 // The workgroup's walk through the stages of a piece, 32 rows a wave.  Returns whether it was
 // done again, with V's infinities and NaN taken for zeros.
 template <typename T, int D, bool kCap>
-__device__ __forceinline__ bool pf_walk(const PfParams& p, const PfPiece& w, int hk, const int* ends,
-                                        PfRowsOf<D>& s, PfLds<D>& lds0, PfLds<D>& lds1,
-                                        PfMore<D>& lds2, PfMore<D>& lds3) {
+__device__ __forceinline__ bool pf_walk(const PfParams& p, const PfPiece& w, int hk,
+                                        const int* ends, PfRowsOf<D>& s, PfLds<D>& lds0,
+                                        PfLds<D>& lds1, PfLds<D>& lds2, PfLds<D>& lds3) {
   using Buf = PfLds<D>;
-  constexpr int NW = PfShape<D>::kWaves, NB = PfShape<D>::kBufs;
+  constexpr int NW = kPfWaves, NB = kPfBufs;
   constexpr int SB = PfBuf<D>::kBlocks, kSteps = SB / 2;
   constexpr int CPR = D / 8, kRow = 2 * D, kBlk = kBlockTok * kRow, kBlkLoads = kBlk / 1024;
   constexpr int kLoads = 2 * SB * kBlkLoads / NW;      // a wave's, of one block
-  constexpr int NK = D / 16, NQ = PfRowsOf<D>::NQ, QC = PfRowsOf<D>::QC;
-  const int lane = threadIdx.x & 63, jr = lane & 31, hh = lane >> 5;
+  constexpr int NK = D / 16;
+  const int lane = threadIdx.x & 63, hh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const bool wave_rows = kPfRows * wave < w.rows;
   const int stages = (w.i1 - w.i0 + kSteps - 1) / kSteps;
@@ -361,7 +349,7 @@ __device__ __forceinline__ bool pf_walk(const PfParams& p, const PfPiece& w, int
   };
   Window win = window(0), next{-1, 0};
   int win0 = 0;
-  uint32_t gone = 0;                                   // a byte a stage on its way: blocks not there
+  uint32_t gone = 0;                                   // a byte a stage: its blocks not there
   // (past the last stage: nothing, zeros, so that every stage waits for the same)
   auto dma = [&](int st, Buf& dst) {
     if (st == win0 + kWin) {
@@ -402,26 +390,19 @@ __device__ __forceinline__ bool pf_walk(const PfParams& p, const PfPiece& w, int
     }
   };
   const char* qp = pf_rows<D>(p, w, wave_rows ? kPfRows * wave : 0, hk, ends, s);
-  mf_u32x4 q[NK];
 #pragma unroll
-  for (int i = 0; i < NK; ++i) q[i] = *reinterpret_cast<const mf_u32x4*>(qp + 16 * (2 * i + hh));
+  for (int i = 0; i < NK; ++i) s.q[i] = *reinterpret_cast<const mf_u32x4*>(qp + 16 * (2 * i + hh));
   auto start = [&] {
     dma(0, lds0);
-    if constexpr (NB > 2) {
-      __builtin_amdgcn_sched_barrier(0);               // (in this order)
-      dma(1, lds1);
-      __builtin_amdgcn_sched_barrier(0);
-      dma(2, lds2);
-    }
+    __builtin_amdgcn_sched_barrier(0);                 // (in this order)
+    dma(1, lds1);
+    __builtin_amdgcn_sched_barrier(0);
+    dma(2, lds2);
     if (stages > kWin) next = window(kWin);
   };
   start();
 #pragma unroll
-  for (int i = 0; i < NK; ++i) {
-    const mf_u32x4 x = s.ok ? q[i] ^ p.q_sign : mf_u32x4{0u, 0u, 0u, 0u};
-    if (i < NQ) s.q[i < NQ ? i : 0] = x;
-    else s.qs[(2 * (i - NQ) + hh) ^ out_swz<QC>(jr)] = x;             // (read by this wave alone)
-  }
+  for (int i = 0; i < NK; ++i) s.q[i] = s.ok ? s.q[i] ^ p.q_sign : mf_u32x4{0u, 0u, 0u, 0u};
   for (bool careful = false;; careful = true) {
     pf_zero(s);
     auto stage = [&](int st, Buf& cur, Buf& nxt) {
@@ -447,19 +428,13 @@ __device__ __forceinline__ bool pf_walk(const PfParams& p, const PfPiece& w, int
     };
     // (left from within: a round's end always has the same loads on their way)
     for (int st = 0;; st += NB) {
-      if constexpr (NB > 2) {
-        stage(st, lds0, lds3);
-        if (st + 1 >= stages) break;
-        stage(st + 1, lds1, lds0);
-        if (st + 2 >= stages) break;
-        stage(st + 2, lds2, lds1);
-        if (st + 3 >= stages) break;
-        stage(st + 3, lds3, lds2);
-      } else {
-        stage(st, lds0, lds1);
-        if (st + 1 >= stages) break;
-        stage(st + 1, lds1, lds0);
-      }
+      stage(st, lds0, lds3);
+      if (st + 1 >= stages) break;
+      stage(st + 1, lds1, lds0);
+      if (st + 2 >= stages) break;
+      stage(st + 2, lds2, lds1);
+      if (st + 3 >= stages) break;
+      stage(st + 3, lds3, lds2);
       if (st + NB >= stages) break;
     }
     // (no load is on its way any more, and the barrier ends every wave's reads of the buffers)
@@ -517,22 +492,19 @@ __device__ __forceinline__ void pf_scan(const int (&x)[N], int (&before)[N], int
 }
 
 template <typename T, int D, bool kCap>
-__global__ __launch_bounds__(64 * PfShape<D>::kWaves, 2)
+__global__ __launch_bounds__(kPfThreads, PfShape<D>::kPerCu)
 void prefix_attn_kernel(PfParams p) {
-  constexpr int NW = PfShape<D>::kWaves, kThreads = 64 * NW, kTile = PfShape<D>::kTile;
-  constexpr int QC = PfRowsOf<D>::QC;
+  constexpr int NW = kPfWaves, kThreads = kPfThreads, kTile = kPfTile;
   __shared__ union Lds {
     __device__ Lds() {}
     PfLds<D> buf;
     PfAt at;
   } lds0;
-  __shared__ PfLds<D> lds1;
-  __shared__ PfMore<D> lds2, lds3;
-  __shared__ mf_u32x4 ldsq[PfShape<D>::kQLds ? NW * kPfRows * QC : 1];   // [wave][row][slot]
+  __shared__ PfLds<D> lds1, lds2, lds3;
   extern __shared__ PfGroup groups[];                  // [n_groups + 1], then int [R]:
   int* ends = reinterpret_cast<int*>(groups + p.n_groups + 1);   // the sequences' tokens
   __shared__ int sh_sum[5][NW], sh_found[4];
-  const int tid = threadIdx.x, lane = tid & 63;
+  const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hk = blockIdx.x % p.Hkv, wg = blockIdx.x / p.Hkv;
   const int n_groups = p.n_groups, sg = p.S * p.G, E = n_groups + p.R;
@@ -576,7 +548,9 @@ void prefix_attn_kernel(PfParams p) {
     return {r, sg, max(g < 0 ? 0 : groups[g].shared, pf_view(p, ends[r]).first), ends[r]};
   };
   auto tiles_of = [&](int rows) { return (rows + kTile - 1) / kTile; };
-  auto slots_of = [&](int e, int rows) { return e < n_groups ? (rows + kPfRows - 1) / kPfRows : 0; };
+  auto slots_of = [&](int e, int rows) {
+    return e < n_groups ? (rows + kPfRows - 1) / kPfRows : 0;
+  };
   auto several = [&](int e, int rows) { return e < n_groups && rows > kTile; };
   // each thread sums a run of entities: lengths, walks and slots of the groups of several
   // walks, lengths and slots of the others
@@ -584,8 +558,10 @@ void prefix_attn_kernel(PfParams p) {
   const int e0 = min(E, tid * per), e1 = min(E, e0 + per);
   constexpr int N = 5;
   int sum[N] = {}, at[N], total[N];
+  const Entity mine = e0 < e1 ? entity(e0) : Entity{0, 0, 0, 0};       // (mostly its only one)
+  auto entity_of_run = [&](int e) { return e == e0 ? mine : entity(e); };
   for (int e = e0; e < e1; ++e) {
-    const Entity n = entity(e);
+    const Entity n = entity_of_run(e);
     const int steps = pf_steps(n.first, n.end), tiles = tiles_of(n.rows);
     const int len = steps ? tiles * (steps + kPfFixed) : 0;
     if (several(e, n.rows)) {
@@ -609,7 +585,7 @@ void prefix_attn_kernel(PfParams p) {
   if (align) {
     int len[1] = {0}, to[1], all[1];
     for (int e = e0; e < e1; ++e) {
-      const Entity n = entity(e);
+      const Entity n = entity_of_run(e);
       if (several(e, n.rows)) len[0] += tiles_of(n.rows) * each_of(true, pf_steps(n.first, n.end));
     }
     __syncthreads();                                   // (sh_sum has been read)
@@ -622,7 +598,7 @@ void prefix_attn_kernel(PfParams p) {
   at[3] += total[0];
   at[4] += total[2];
   for (int e = e0; e < e1; ++e) {
-    const Entity n = entity(e);
+    const Entity n = entity_of_run(e);
     const bool multi = several(e, n.rows);
     const int steps = pf_steps(n.first, n.end), tiles = tiles_of(n.rows);
     const int each = each_of(multi, steps);
@@ -671,7 +647,6 @@ void prefix_attn_kernel(PfParams p) {
   };
   bool multi = e < E && several(e, rows_at(e));
   PfRowsOf<D> s;
-  s.qs = &ldsq[PfShape<D>::kQLds ? (wave * kPfRows + (lane & 31)) * QC : 0];
   for (int t = -1; e < E && x < b;) {
     const Entity n = entity(e);
     PfPiece w;
@@ -725,7 +700,7 @@ void prefix_attn_kernel(PfParams p) {
 // Row blockIdx.x of the output, (r, hq, s), from its walks' partials.
 template <typename T, int D>
 __global__ __launch_bounds__(kPfJoinThreads) void prefix_join_kernel(PfParams p) {
-  constexpr int NW = PfShape<D>::kWaves, kTile = PfShape<D>::kTile;
+  constexpr int NW = kPfWaves, kTile = kPfTile;
   constexpr int C = D / 4, N = kPfJoinThreads / C, U = 4;
   __shared__ float4 sh_o[N][C];
   __shared__ float2 sh_ml[N];
@@ -760,7 +735,8 @@ __global__ __launch_bounds__(kPfJoinThreads) void prefix_join_kernel(PfParams p)
         ml[u] = reinterpret_cast<const float2*>(p.group_ml)[at];
         v[u] = reinterpret_cast<const float4*>(p.group_o)[at * C + c];
       } else {
-        const int64_t at = ((int64_t)hk * p.own_slots + o0 + i - n_group) * p.own_rows + row % kTile;
+        const int64_t at =
+            ((int64_t)hk * p.own_slots + o0 + i - n_group) * p.own_rows + row % kTile;
         ml[u] = reinterpret_cast<const float2*>(p.own_ml)[at];
         v[u] = reinterpret_cast<const float4*>(p.own_o)[at * C + c];
       }
@@ -816,9 +792,9 @@ hipError_t launch_prefix_dim(const PfParams& p, hipStream_t st) {
   const dim3 grid((uint32_t)(p.Hkv * p.wgs));
   const size_t dyn = sizeof(PfGroup) * (p.n_groups + 1) + sizeof(int) * (size_t)p.R;
   if (p.softcap > 0.f)
-    hipLaunchKernelGGL((prefix_attn_kernel<T, D, true>), grid, dim3(64 * PfShape<D>::kWaves), dyn, st, p);
+    hipLaunchKernelGGL((prefix_attn_kernel<T, D, true>), grid, dim3(kPfThreads), dyn, st, p);
   else
-    hipLaunchKernelGGL((prefix_attn_kernel<T, D, false>), grid, dim3(64 * PfShape<D>::kWaves), dyn, st, p);
+    hipLaunchKernelGGL((prefix_attn_kernel<T, D, false>), grid, dim3(kPfThreads), dyn, st, p);
   hipLaunchKernelGGL((prefix_join_kernel<T, D>), dim3((uint32_t)(p.R * p.Hq * p.S)),
                      dim3(kPfJoinThreads), 0, st, p);
   return hipGetLastError();

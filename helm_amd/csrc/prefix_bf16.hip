@@ -18,14 +18,13 @@ struct PfPlan {
   int64_t group_slots, own_slots, bytes;
 };
 // Workgroups of a KV head: as many as the device holds at once.
-template <int D> PfPlan pf_plan_dim(int R, int Hq, int Hkv, int S, int n_groups) {
+PfPlan pf_plan(int R, int Hq, int Hkv, int S, int D, int n_groups) {
   PfPlan p{};
   const int64_t rows = (int64_t)S * (Hq / Hkv);
-  constexpr int waves = PfShape<D>::kWaves, tile = PfShape<D>::kTile;
-  p.wgs = std::max(1, 256 * PfShape<D>::kPerCu / Hkv);
-  p.own_tiles = (int)((rows + tile - 1) / tile);
-  p.own_rows = (int)std::min<int64_t>(rows, tile);
-  p.group_slots = n_groups ? n_groups + R * rows / kPfRows + waves * p.wgs : 0;
+  p.wgs = std::max(1, 256 * (D == 256 ? PfShape<256>::kPerCu : PfShape<128>::kPerCu) / Hkv);
+  p.own_tiles = (int)((rows + kPfTile - 1) / kPfTile);
+  p.own_rows = (int)std::min<int64_t>(rows, kPfTile);
+  p.group_slots = n_groups ? n_groups + R * rows / kPfRows + kPfWaves * p.wgs : 0;
   p.own_slots = (int64_t)R * p.own_tiles + p.wgs;
   auto room = [](int64_t n) { return (n + 15) / 16 * 16; };
   p.bytes = room(R * (int64_t)sizeof(PfSeq)) + room(Hkv * p.group_slots * kPfRows * 2 * 4) +
@@ -33,21 +32,16 @@ template <int D> PfPlan pf_plan_dim(int R, int Hq, int Hkv, int S, int n_groups)
             4 * Hkv * (p.group_slots * kPfRows + p.own_slots * p.own_rows) * D;
   return p;
 }
-PfPlan pf_plan(int R, int Hq, int Hkv, int S, int D, int n_groups) {
-  return D == 64 ? pf_plan_dim<64>(R, Hq, Hkv, S, n_groups)
-                 : D == 128 ? pf_plan_dim<128>(R, Hq, Hkv, S, n_groups)
-                            : pf_plan_dim<256>(R, Hq, Hkv, S, n_groups);
-}
 
 bool pf_shape_ok(int R, int Hq, int Hkv, int S, int max_pages, int page, int n_groups) {
   if (R < 0 || R > HELM_PREFIX_MAX_SEQS || n_groups < 0 || n_groups > HELM_PREFIX_MAX_GROUPS ||
       Hkv < 1 || Hq < 1 || Hq % Hkv || S < 1 || max_pages < 0 || page < kBlockTok ||
-      page % kBlockTok || (int64_t)max_pages * page > 0x7fffff00 ||
+      page % kBlockTok || (int64_t)max_pages * page > 0x7ffff000 ||
       (int64_t)R * Hq * S > 0x7fffffff / kPfJoinThreads || Hkv > 65536)
     return false;
   // the line of a KV head's walks stays within 2^30 steps
   const int64_t rows = (int64_t)S * (Hq / Hkv);
-  const int64_t walks = (int64_t)R * ((rows + 127) / 128) + n_groups + R * rows / 128;
+  const int64_t walks = R * ((rows + kPfTile - 1) / kPfTile) + n_groups + R * rows / kPfTile;
   const int64_t steps = ((int64_t)max_pages * page + kPfStep - 1) / kPfStep + 1 + kPfFixed;
   return walks * steps <= 0x3fffffff;
 }
@@ -128,7 +122,8 @@ extern "C" int helm_prefix_decode_attn(const void* q, void* out, const void* k_p
   p.q_sign = scale < 0.f ? 0x80008000u : 0u;
   p.scale = std::max(scale < 0.f ? -scale : scale, FLT_MIN);
   p.softcap = softcap;
-  p.window = window;
+  // (one of the whole table's length hides nothing)
+  p.window = window < (int64_t)max_pages * page_size ? window : 0;
   char* ws = static_cast<char*>(workspace);
   auto take = [&](int64_t n) {
     char* at = ws;
@@ -144,6 +139,7 @@ extern "C" int helm_prefix_decode_attn(const void* q, void* out, const void* k_p
   const hipError_t e =
       dtype == HELM_BF16 ? launch_prefix_bf16(p, D, st) : launch_prefix_f16(p, D, st);
   if (e != hipSuccess)
-    return report_error((int)e, std::string("shared-prefix decode launch: ") + hipGetErrorString(e));
+    return report_error((int)e,
+                        std::string("shared-prefix decode launch: ") + hipGetErrorString(e));
   return HELM_OK;
 }

@@ -28,7 +28,8 @@ def _select(B=2, K=3, V=8, **kw):
     (dict(n=0), ValueError), (dict(n=65), ValueError),
     (dict(logits=torch.zeros((2, 65, 8)), scores=torch.zeros((2, 65))), ValueError),
     (dict(logits=torch.zeros((2, 3, 0))), ValueError),
-    (dict(logits=torch.zeros((1, 1)).expand(65536, 1, 1), scores=torch.zeros((65536, 1))), ValueError),
+    (dict(logits=torch.zeros((1, 1)).expand(65536, 1, 1), scores=torch.zeros((65536, 1))),
+     ValueError),
     (dict(logits=torch.zeros((2, 3, 8), requires_grad=True)), RuntimeError),
     ({}, RuntimeError),            # CPU tensors
 ])
@@ -140,7 +141,8 @@ def test_c_entries_refuse_before_device_work():
     assert lib.helm_beam_select_workspace_bytes(2, 3, 8, 3, 2) == 6 * (12 + 24)
     assert lib.helm_beam_select_workspace_bytes(2, 0, 8, 3, 2) == 0
 
-    arr = {k: _i32(n) for k, n in dict(par=6, tab=24, lens=6, new=24, cop=12, rel=24, cnt=1).items()}
+    sizes = dict(par=6, tab=24, lens=6, new=24, cop=12, rel=24, cnt=1)
+    arr = {k: _i32(n) for k, n in sizes.items()}
     ptr = {k: v[1] for k, v in arr.items()}
     need = lib.helm_beam_tables_workspace_bytes(2, 3, 4)
     ws = np.zeros(need // 4, dtype=np.int32)

@@ -62,8 +62,10 @@ def test_select_ties_and_orders(make, n):
         x = torch.zeros((B, K, V), device=DEV)
         x[:, 1, 4096:4196] = 5.0
     else:
-        x = torch.where(torch.arange(V, device=DEV) % 2 == 0, 0.0, -0.0).expand(B, K, V).contiguous()
-    for scores in (torch.zeros((B, K), device=DEV), torch.tensor([[0.0, -1.0, 0.5]] * B, device=DEV)):
+        x = torch.where(torch.arange(V, device=DEV) % 2 == 0, 0.0, -0.0)
+        x = x.expand(B, K, V).contiguous()
+    for scores in (torch.zeros((B, K), device=DEV),
+                   torch.tensor([[0.0, -1.0, 0.5]] * B, device=DEV)):
         check_select(x, scores, n)
         check_select(x.bfloat16(), scores, n)
 
@@ -180,14 +182,15 @@ def test_tables(B, K, page, width, seed):
     lens, shared = [], []
     for b in range(B):
         full = r.choice([0, r.randrange(width + 1), width])
-        lens.append(min(full, width) * page + (r.choice([0, r.randrange(page)]) if full < width else 0))
+        lens.append(full * page + (r.choice([0, r.randrange(page)]) if full < width else 0))
         shared.append(r.randint(0, lens[-1] // page))
     table, n = make_tables(r, B, K, page, width, lens, shared)
     slots = list(range(n + 3))
     r.shuffle(slots)
     table = [[slots[s] for s in row] for row in table]
     kinds = ["same", "one", "reverse", "any", "none", "outside"]
-    parents = [parents_of(r, kinds[(b + seed) % 6] if B > 1 else kinds[seed % 4], K) for b in range(B)]
+    parents = [parents_of(r, kinds[(b + seed) % 6] if B > 1 else kinds[seed % 4], K)
+               for b in range(B)]
     rows = [t for t in lens for _ in range(K)]
     want, copies, released = R.tables(parents, table, rows, page, shared)
     args = (torch.tensor(parents, **I32), torch.tensor(table, **I32), torch.tensor(rows, **I32))

@@ -53,7 +53,8 @@ def make(groups, Hq, Hkv, D, page, dtype, S=1, seed=0, alone=(), extra=3):
         starts.append(starts[-1] + len(n))
     return {"q": _randn(seed, (len(lens), Hq, S, D), dtype, 1.5),
             "arena": _randn(seed + 1, (n_slots, 2, Hkv, page, D), dtype), "table": table,
-            "lens": lens, "len_t": torch.tensor(lens, **I32), "start_t": torch.tensor(starts, **I32),
+            "lens": lens, "len_t": torch.tensor(lens, **I32),
+            "start_t": torch.tensor(starts, **I32),
             "shared_t": torch.tensor([s for s, _ in groups], **I32), "page": page}
 
 
@@ -91,7 +92,8 @@ def check(c, out, scale=None, cap=0.0, window=0, rows=None, heads=None):
             tol = u * want.abs() + 1.01 * u * (mag + want.abs()) \
                 + vmax * (2 * e + t * (2.0 ** -24 + 2.0 ** -34)) + 1e-30
             got = out[r, h].double()
-            ok = ((got - want).abs() <= tol) | (torch.isnan(got) & torch.isnan(want)) | (got == want)
+            ok = ((got - want).abs() <= tol) | (got == want) | \
+                (torch.isnan(got) & torch.isnan(want))
             assert ok.all(), (r, h, (got - want).abs().max().item(), tol.min().item())
 
 
@@ -128,8 +130,8 @@ def test_lengths(lens):
 @pytest.mark.parametrize("window", [0, 1, 40, 300])
 def test_drafts_and_windows(S, G, window):
     """The last S tokens, each up to its own; rows before a sequence's first token see nothing."""
-    c = make([(8, [8 * 16 + n for n in (0, 1, 3, 150)]), (3, [48, 20, 2, 400])], 2 * G, 2, 64, 16, HF,
-             S=S, seed=10 * S + G, alone=[1, 0, 9, 333])
+    c = make([(8, [8 * 16 + n for n in (0, 1, 3, 150)]), (3, [48, 20, 2, 400])], 2 * G, 2, 64, 16,
+             HF, S=S, seed=10 * S + G, alone=[1, 0, 9, 333])
     out = call(c, window=window)
     check(c, out, window=window)
     for r, t in enumerate(c["lens"]):
@@ -139,7 +141,8 @@ def test_drafts_and_windows(S, G, window):
 
 
 @pytest.mark.parametrize("dtype,D", [(BF, 64), (HF, 128), (BF, 256)])
-@pytest.mark.parametrize("cap,scale", [(50.0, None), (5.0, 0.3), (0.0, -0.2), (0.0, 0.0), (30.0, -1.0)])
+@pytest.mark.parametrize("cap,scale", [(50.0, None), (5.0, 0.3), (0.0, -0.2), (0.0, 0.0),
+                                       (30.0, -1.0)])
 def test_softcap_and_scale(dtype, D, cap, scale):
     c = make([(6, [120, 130, 99])], 4, 2, D, 16, dtype, seed=D, alone=[50])
     check(c, call(c, softcap=cap or None, scale=scale), scale=scale, cap=cap)
@@ -150,8 +153,8 @@ def test_softcap_and_scale(dtype, D, cap, scale):
 def test_many_rows_of_a_group(dtype, D, Hkv, n):
     """More rows than a walk has, split over many workgroups."""
     r = random.Random(n)
-    c = make([(70, [70 * 16 + r.randint(0, 90) for _ in range(n)]), (3, [60] * 3)], 4 * Hkv, Hkv, D, 16,
-             dtype, seed=n)
+    c = make([(70, [70 * 16 + r.randint(0, 90) for _ in range(n)]), (3, [60] * 3)], 4 * Hkv, Hkv,
+             D, 16, dtype, seed=n)
     check(c, call(c), rows=[0, 1, n // 2, n - 1, n], heads=[0, 4 * Hkv - 1])
 
 
@@ -181,12 +184,12 @@ def test_many_sequences(R, n_groups):
 
 
 def test_hidden_rows_hold_anything():
-    """NaN and infinities in pages' unused rows, in pages of no sequence, past a causal limit and out
-    of the window; slots that the pool does not have."""
+    """NaN and infinities in pages' unused rows, in pages of no sequence, past a causal limit and
+    out of the window; slots that the pool does not have."""
     for window in (0, 30):
         for S in (1, 3):
-            c = make([(4, [64 + 5, 64 + 20, 64, 40, 3]), (2, [32, 33])], 4, 2, 128, 16, BF, S=S, seed=6,
-                     alone=[18])
+            c = make([(4, [64 + 5, 64 + 20, 64, 40, 3]), (2, [32, 33])], 4, 2, 128, 16, BF, S=S,
+                     seed=6, alone=[18])
             clean = call(c, window=window)
             used = torch.zeros(c["arena"].size(0) * 16, dtype=torch.bool, device=DEV)
             for r, t in enumerate(c["lens"]):
@@ -309,7 +312,8 @@ def test_the_same_as_paged_decode():
     got = call(c)
     tab = torch.where((c["table"] < 0) | (c["table"] >= c["arena"].size(0)), 0, c["table"])
     want = paged.paged_decode_attention(c["q"], c["arena"][:, 0], c["arena"][:, 1], tab, c["len_t"])
-    assert ((got.float() - want.float()).abs() <= 2 * 2.0 ** -8 * want.float().abs() + 2.0 ** -10).all()
+    assert ((got.float() - want.float()).abs()
+            <= 2 * 2.0 ** -8 * want.float().abs() + 2.0 ** -10).all()
 
 
 def test_prepared_runs_streams_and_graphs():
@@ -360,7 +364,7 @@ def test_no_sequence():
     c = make([], 2, 2, 64, 16, BF, seed=18)
     assert call(c).shape == (0, 2, 1, 64)
     e = torch.zeros((0, 2, 16, 64), dtype=BF, device=DEV)              # a pool without a slot
-    out = prefix.prefix_decode_attention(_randn(0, (2, 2, 1, 64), BF), e, e, torch.zeros((2, 0), **I32),
-                                         torch.tensor([5, 0], **I32), torch.tensor([0, 2], **I32),
-                                         torch.zeros(1, **I32))
+    out = prefix.prefix_decode_attention(_randn(0, (2, 2, 1, 64), BF), e, e,
+                                         torch.zeros((2, 0), **I32), torch.tensor([5, 0], **I32),
+                                         torch.tensor([0, 2], **I32), torch.zeros(1, **I32))
     assert (out == 0).all()
