@@ -16,12 +16,18 @@
 // (walk + workgroup), of which no two pieces are alike, as both only grow along the line.
 // Walks of a group that has several come first on the line, each from a stretch's start on:
 // so the workgroups that read the same tokens for different rows do so side by side, through
-// one XCD's L2 (a KV head's workgroups are on one where 8, 16, ... heads lie round the XCDs).
+// one XCD's L2 (a KV head's workgroups are on one where 8, 16, ... heads lie round the XCDs):
+// 32k tokens under 64 sequences 93 -> 88 us.
 //
 // A walk is that of prompt.h: 32 x 32 matrix tiles, 32 rows a wave, K and V straight from memory
-// into LDS, one barrier a stage.  Few rows keep few of the waves busy, which is enough: a step of
-// one wave takes 0.6 us, its 128 D bytes of K and V 1.6 us of half a CU's share of the memory.
-// Here K and V come from HBM, not from L2: three stages are on their way.
+// into LDS, one barrier a stage.  Few rows keep few of the waves busy; such a walk is bound by
+// memory.  K and V come from HBM here, not from L2: three stages are on their way.
+//
+// Bound, measured at D = 128, bf16 (walks and their joining, us a call): 4 beams of 16 prompts of
+// 4k tokens 48, 2.8 TB/s of K and V; 16 chats behind 8k shared tokens 33, of which the joining
+// takes 5 and the line 3.5; 32k tokens under 64 sequences 81, where the walks' arithmetic alone
+// takes 66 and their loads alone 57: two waves a SIMD hide part of the one behind the other.
+//
 // Weights are rounded once to the 16-bit type (2^-8 of the weight in bf16, 2^-11 in f16, and the
 // row's sum adds the rounded ones); f16 weights are taken times 2^9, those under 2^-34 of the
 // largest are lost.  An output's relative rms error is 2.3e-3 in bf16 and 2.7e-4 in f16, against
@@ -44,15 +50,19 @@ namespace helm {
 
 constexpr int kPfRows = 32;          // of a wave, and of a slot of the groups' partials
 constexpr int kPfStep = 32;          // tokens of a step
-// What a walk costs before its first step and behind its last, in steps.
+// What a walk costs before its first step and behind its last, in steps.  (32k tokens under 64
+// sequences 81.5 us, with 8 84.8, with 12 88; with 2, workgroups of several short walks end late:
+// 4 beams of 16 prompts 63 us against 58 with 4 and 55 with 6.)
 constexpr int kPfFixed = 5;
-// A workgroup's least stretch.
+// A workgroup's least stretch (a prompt of 2k tokens, 4 beams: 17.1 us, with 2 18.4, with 8 21.9).
 constexpr int kPfLeast = 4;
 constexpr int kPfJoinThreads = 256;
 constexpr int kPfWaves = 4;          // of a workgroup
 constexpr int kPfThreads = 64 * kPfWaves;
 constexpr int kPfTile = kPfRows * kPfWaves;            // rows of a walk
-constexpr int kPfBufs = 4;           // stage buffers
+// Stage buffers.  (Two, and three workgroups a CU: 16 chats 39.6 us, 4 beams of 16 prompts 55, 32k
+// tokens 88; three buffers, three workgroups 39.7, 58, 88; four and two 33.9, 48, 84.)
+constexpr int kPfBufs = 4;
 // Tokens of a stage; workgroups of a CU, which the buffers (16 KB, 32 at D = 256) leave room for.
 template <int D> struct PfShape {
   static constexpr int kTok = D == 64 ? 64 : 32, kPerCu = D == 256 ? 1 : 2;
@@ -503,19 +513,22 @@ void prefix_attn_kernel(PfParams p) {
   __shared__ PfLds<D> lds1, lds2, lds3;
   extern __shared__ PfGroup groups[];                  // [n_groups + 1], then int [R]:
   int* ends = reinterpret_cast<int*>(groups + p.n_groups + 1);   // the sequences' tokens
-  __shared__ int sh_sum[5][NW], sh_found[4];
+  __shared__ int sh_sum[5][NW], sh_found[4], sh_down;
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hk = blockIdx.x % p.Hkv, wg = blockIdx.x / p.Hkv;
-  const int n_groups = p.n_groups, sg = p.S * p.G, E = n_groups + p.R;
+  const int sg = p.S * p.G;
+  int n_groups = p.n_groups;
 
   // ---- the line: the walks' lengths, and where this workgroup's stretch starts
   const int len0 = tid < p.R ? p.lens[tid] : 0;
   for (int g = tid; g <= n_groups; g += kThreads)
     groups[g] = {n_groups ? min(max(p.starts[g], 0), p.R) : 0,
                  g < n_groups ? pf_shared(p, p.shared[g]) : 0, 0x7fffffff, 0};
-  if (tid == 0) sh_found[0] = E;
+  if (tid == 0) sh_down = 0;
   __syncthreads();
+  for (int g = tid; g < n_groups; g += kThreads)
+    if (groups[g].start > groups[g + 1].start) sh_down = 1;
   auto group_of = [&](int r) {                         // -1: none
     int lo = 0, hi = n_groups;
     while (hi - lo > 1) {
@@ -535,6 +548,10 @@ void prefix_attn_kernel(PfParams p) {
     }
   }
   __syncthreads();
+  // (starts that do not ascend: no groups, as the line's length would have no bound)
+  if (sh_down) n_groups = 0;
+  const int E = n_groups + p.R;
+  if (tid == 0) sh_found[0] = E;
   // entity e, a group or a sequence: its rows and tokens
   struct Entity {
     int seq0, rows, first, end;
@@ -677,8 +694,6 @@ void prefix_attn_kernel(PfParams p) {
     float *ml, *part;
     if (e < n_groups) {
       const int to = y + t * NW + NW * wg;
-      // (starts that do not ascend may have more rows than there are)
-      if (to + (w.rows + kPfRows - 1) / kPfRows > p.group_slots) continue;
       const int64_t at = ((int64_t)hk * p.group_slots + to) * kPfRows;
       ml = p.group_ml + 2 * at;
       part = p.group_o + at * D;
@@ -715,11 +730,10 @@ __global__ __launch_bounds__(kPfJoinThreads) void prefix_join_kernel(PfParams p)
   };
   const int grow = q.row0 + row, gt = grow / kTile, ot = row / kTile;
   int w0, v0;
-  int n_group = pieces(q.group_at + gt * q.group_each, q.group_steps, w0);
+  const int n_group = pieces(q.group_at + gt * q.group_each, q.group_steps, w0);
   const int own_each = q.own_steps > 0 ? q.own_steps + kPfFixed : 0;
   const int n_own = pieces(q.own_at + ot * own_each, q.own_steps, v0);
   const int g0 = q.group_slot + grow / kPfRows + NW * w0, o0 = r * p.own_tiles + ot + v0;
-  n_group = min(n_group, max(0, (p.group_slots - g0 + NW - 1) / NW));
   const int n = n_group + n_own;
   const int c = threadIdx.x % C, g = threadIdx.x / C;
   float m = -INFINITY, l = 0.f;

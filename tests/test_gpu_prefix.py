@@ -306,6 +306,23 @@ def test_groups_past_the_batch_and_counts_past_the_table():
     check(c, none)
 
 
+@pytest.mark.parametrize("starts", [[0, 5, 2, 7], [7, 0], [3, 2 ** 31 - 1, -2 ** 31, 1]])
+def test_starts_that_do_not_ascend_share_nothing(starts):
+    c = make([(6, [6 * 16 + 20 * i for i in range(7)])], 4, 2, 64, 16, BF, seed=21)
+    n = len(starts) - 1
+    got = call(dict(c, start_t=torch.tensor(starts, **I32), shared_t=torch.full((n,), 6, **I32)))
+    check(c, got)
+    none = dict(c, start_t=torch.zeros(1, **I32), shared_t=torch.zeros(0, **I32))
+    check(c, call(none))
+
+
+def test_the_most_sequences_of_the_widest_heads():
+    r = random.Random(5)
+    c = make([(1, [r.randint(16, 40) for _ in range(8)]) for _ in range(512)], 1, 1, 256, 16, BF,
+             seed=22)
+    check(c, call(c), rows=r.sample(range(4096), 40) + [0, 4095])
+
+
 def test_the_same_as_paged_decode():
     """Whole tables: the answer of the operator that reads every sequence's pages by itself."""
     c = make([(30, [30 * 16 + n for n in (5, 60, 130, 700)])], 16, 4, 128, 16, BF, seed=14)
