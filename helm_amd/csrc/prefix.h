@@ -24,7 +24,7 @@
 // memory.  K and V come from HBM here, not from L2: three stages are on their way.
 //
 // Bound, measured at D = 128, bf16 (walks and their joining, us a call): 4 beams of 16 prompts of
-// 4k tokens 48, 2.8 TB/s of K and V; 16 chats behind 8k shared tokens 33, of which the joining
+// up to 4k tokens 48, 2.8 TB/s of K and V; 24 chats behind 8k shared tokens 33, of which the joining
 // takes 5 and the line 3.5; 32k tokens under 64 sequences 81, where the walks' arithmetic alone
 // takes 66 and their loads alone 57: two waves a SIMD hide part of the one behind the other.
 //
@@ -60,7 +60,7 @@ constexpr int kPfJoinThreads = 256;
 constexpr int kPfWaves = 4;          // of a workgroup
 constexpr int kPfThreads = 64 * kPfWaves;
 constexpr int kPfTile = kPfRows * kPfWaves;            // rows of a walk
-// Stage buffers.  (Two, and three workgroups a CU: 16 chats 39.6 us, 4 beams of 16 prompts 55, 32k
+// Stage buffers.  (Two, and three workgroups a CU: 24 chats 39.6 us, 4 beams of 16 prompts 55, 32k
 // tokens 88; three buffers, three workgroups 39.7, 58, 88; four and two 33.9, 48, 84.)
 constexpr int kPfBufs = 4;
 // Tokens of a stage; workgroups of a CU, which the buffers (16 KB, 32 at D = 256) leave room for.
