@@ -24,9 +24,9 @@
 // memory.  K and V come from HBM here, not from L2: three stages are on their way.
 //
 // Bound, measured at D = 128, bf16 (walks and their joining, us a call): 4 beams of 16 prompts of
-// up to 4k tokens 48, 2.8 TB/s of K and V; 24 chats behind 8k shared tokens 33, of which the joining
-// takes 5 and the line 3.5; 32k tokens under 64 sequences 81, where the walks' arithmetic alone
-// takes 66 and their loads alone 57: two waves a SIMD hide part of the one behind the other.
+// up to 4k tokens 48, 2.8 TB/s of K and V; 24 chats behind 8k shared tokens 33, of which the
+// joining takes 5 and the line 3.5; 32k tokens under 64 sequences 81, where the walks' arithmetic
+// alone takes 66 and their loads alone 57: two waves a SIMD hide part of the one behind the other.
 //
 // Weights are rounded once to the 16-bit type (2^-8 of the weight in bf16, 2^-11 in f16, and the
 // row's sum adds the rounded ones); f16 weights are taken times 2^9, those under 2^-34 of the

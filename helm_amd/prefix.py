@@ -56,8 +56,9 @@ def prefix_decode_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
     table, slots outside the pool count as hidden pages; seq_lens: int32 [R] tokens.
     group_starts: int32 [n + 1], ascending: group g is sequences group_starts[g] ..
     group_starts[g + 1], whose first shared_pages[g] (int32 [n]) table columns hold the same
-    slots, full pages or not; sequences outside every group share nothing.  All on the
-    device and read there: one launch shape serves any lengths and groups.
+    slots, full pages or not; sequences outside every group share nothing, nor does any where
+    the starts do not ascend.  All on the device and read there: one launch shape serves any
+    lengths and groups.
 
     The q_len rows are the sequence's last tokens: row s stands at p = len - q_len + s and
     sees tokens up to p, with `window` only the last `window` of those.  Hidden tokens take

@@ -465,7 +465,8 @@ int helm_prompt_attn(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
  * the answer is the one that each sequence's whole table gives.  Slot s of the pools starts at
  * s * slot_stride elements, its KV head h head_stride elements further on, a page being dense
  * [page_size, D] rows, 16-byte aligned; page_size a multiple of 16.  Group g is sequences
- * group_starts[g] .. group_starts[g + 1] (device int32 [n_groups + 1], ascending within 0 .. R);
+ * group_starts[g] .. group_starts[g + 1] (device int32 [n_groups + 1], ascending within 0 .. R;
+ * any that do not ascend: no groups);
  * the first shared_pages[g] columns of their table rows hold the same slots, and it is the
  * first row's that are read.  Sequences outside every group share nothing.
  * q and out [R, Hq, q_len, D] dense, of the pools' type (HELM_F16, HELM_BF16): the q_len rows
@@ -496,11 +497,12 @@ int helm_prefix_decode_attn(const void* q, void* out, const void* k_pool, const 
  * the element) and its running score scores[b * K + k] offer token t at
  *   score + logit[t] - log(sum over the row of exp(logit)).
  * Out, [B, n], best first, ties to the lowest k * V + t: the score (past fp32's range: its
- * largest or lowest number), the token, the beam (0 .. K - 1).  A logit of -inf is no candidate, nor is anything of a row whose score is not
- * finite or whose logits hold a NaN or +inf; where fewer than n are left, -inf, -1, -1.  The
- * order is of 64-bit sums.  1 <= K, n <= HELM_BEAMS_MAX, B K <= 65535.  The workspace is
- * 8-byte aligned and needs no contents before or after a call; calls that may overlap need
- * one each. */
+ * largest or lowest number), the token, the beam (0 .. K - 1).  A logit of -inf is no
+ * candidate, nor is anything of a row whose score is not finite or whose logits hold a NaN or
+ * +inf; where fewer than n are left, -inf, -1, -1.  The order is of 64-bit sums.
+ * 1 <= K, n <= HELM_BEAMS_MAX, B K <= 65535.  The workspace is 8-byte aligned and needs no
+ * contents before or after a call; calls that may overlap need one each.  No output may
+ * lie over the logits or scores. */
 size_t helm_beam_select_workspace_bytes(int B, int K, int V, int n, int dtype);
 int helm_beam_select(const void* logits, int64_t b_stride, int64_t k_stride, int dtype,
                      const float* scores, int B, int K, int V, int n, float* out_scores,
