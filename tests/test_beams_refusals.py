@@ -108,7 +108,7 @@ def test_page_store_refusals(bad):
 
 def test_page_store_layouts():
     """(slots, bytes between slots, segments, bytes between them, tokens and bytes of a unit)"""
-    assert beams.PageStore([torch.zeros(5, 2, 3, 16, 8)])._shape == (5, 3072 * 1, 6, 512, 1, 32)
+    assert beams.PageStore([torch.zeros(5, 2, 3, 16, 8)])._shape == (5, 768 * 4, 6, 512, 1, 32)
     a = torch.zeros(5, 2, 3, 16, 8).half()
     assert beams.PageStore([a[:, 0], a[:, 1]])._shape == (5, 1536, 3, 256, 1, 16)
     assert beams.PageStore([torch.zeros(5, 16, 8).half()])._shape == (5, 256, 1, 256, 1, 16)
