@@ -30,11 +30,11 @@
 // (From 32k to 64k tokens 64 sequences take 37 us more, 32 sequences 24, which is 5.7 TB/s; some
 // 30 us of a call do not grow with the tokens, the partials' 33 MB out and back half of them.)
 //
-// Weights are rounded once to the 16-bit type (2^-8 of the weight in bf16, 2^-11 in f16, and the
-// row's sum adds the rounded ones); f16 weights are taken times 2^9, those under 2^-34 of the
-// largest are lost.  An output's relative rms error is 2.3e-3 in bf16 and 2.7e-4 in f16, against
-// 1.7e-3 and 2.1e-4 where weights stay in fp32.  (A second product for what the rounding leaves,
-// in walks of up to 64 rows: 4 to 13% of the call, 32k tokens under 64 sequences 81 -> 92 us.)
+// Weights enter P . V in two 16-bit parts (2^-16 of the weight in bf16, 2^-22 in f16) and the row's
+// sum in fp32, as in the decode kernels; f16 weights are taken times 2^9, what is under 2^-34 of
+// the largest is lost.  An output is then off by its own rounding and hardly more: relative rms
+// error 1.7e-3 in bf16, 2.1e-4 in f16.  (In one part: 2.3e-3 and up to 3.0e-4, for 24 chats 34 us
+// against 36, 4 beams of 16 prompts 48.7 against 49.4, 32k tokens under 64 sequences 82 against 91.)
 //
 // Hidden tokens (past a row's position or out of its window, past a sequence's end, in pages
 // that the pool does not have) take no part whatever they hold: their scores are overwritten,
@@ -259,24 +259,32 @@ __device__ __forceinline__ void pf_step(const PfParams& p, PfRowsOf<D>& s, int t
     for (int e = 0; e < NE; ++e) s.o[e] *= f;
   }
   const float base = s.m == -INFINITY ? 0.f : s.m - kShift;
-  uint32_t w[8];
+  uint32_t hi[8], lo[8];
+  float ws[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float w0 = __builtin_amdgcn_exp2f(fmaf(x[2 * i], mul, -base));
     const float w1 = __builtin_amdgcn_exp2f(fmaf(x[2 * i + 1], mul, -base));
-    w[i] = Ops::pk(w0, w1);
-    s.lsum = dot2<T>(w[i], Ops::ones8()[0], s.lsum);
+    ws[i] = w0 + w1;
+    if constexpr (std::is_same<T, f16_t>::value) Ops::split2_mix(w0, w1, hi[i], lo[i]);
+    else Ops::split2(w0, w1, hi[i], lo[i]);
   }
+  s.lsum += ((ws[0] + ws[1]) + (ws[2] + ws[3])) + ((ws[4] + ws[5]) + (ws[6] + ws[7]));
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
-    const mf_u32x4 pop{w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]};
+    const mf_u32x4 pop{hi[4 * u], hi[4 * u + 1], hi[4 * u + 2], hi[4 * u + 3]};
+    const mf_u32x4 rest{lo[4 * u], lo[4 * u + 1], lo[4 * u + 2], lo[4 * u + 3]};
+    mf_u32x4 vop[NE];
 #pragma unroll
     for (int e = 0; e < NE; ++e) {
       const char* at = vv + u * kBlk;
       const uint2 a0 = ld_tr16(at + (v_off ^ (64 * e)));
       const uint2 a1 = ld_tr16(at + (v_off ^ (64 * e) ^ 16) + 4 * kRow);
-      s.o[e] = M32::mma(mf_u32x4{a0.x, a0.y, a1.x, a1.y}, pop, s.o[e]);
+      vop[e] = mf_u32x4{a0.x, a0.y, a1.x, a1.y};
+      s.o[e] = M32::mma(vop[e], pop, s.o[e]);
     }
+#pragma unroll
+    for (int e = 0; e < NE; ++e) s.o[e] = M32::mma(vop[e], rest, s.o[e]);
   }
 }
 

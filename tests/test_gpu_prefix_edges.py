@@ -1,0 +1,47 @@
+"""prefix_decode_attention at its edges, against 64 bits: what its roundings are."""
+import math
+
+import pytest
+import torch
+
+from oracle import serving as R
+from test_gpu_prefix import BF, DEV, HALF, HF, call, make
+
+pytestmark = pytest.mark.gpu
+
+
+def _attend(c, r, h):
+    """Sequence r's row h in 64 bits, and the mean of |v| under its weights."""
+    Hq, D = c["q"].size(1), c["q"].size(3)
+    t, page = c["lens"][r], c["page"]
+    kv = c["arena"][c["table"][r, :-(-t // page)].long(), :, h // (Hq // c["arena"].size(2))]
+    k, v = (kv[:, i].reshape(-1, D)[:t] for i in (0, 1))
+    want, mag = R.attend(c["q"][r, h][None], k, v, c["scale"])
+    return want[0, 0], mag[0, 0]
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_weights_are_held_in_two_parts(dtype, D):
+    """An output is off by its own rounding and hardly more.  q and k of -1, 0, 1 and a scale that
+    is a power of two: logits are exact.  Weights are off by at most w of themselves: u^2, their
+    second part's rounding; 2^-24 3 L, L the largest logit, for log2(e) in fp32 and the exponent's
+    rounding; 2^-24 16 for exponentials, the joining's among them.  The mean is then off by
+    d <= 2 w (mean |v| + |o|); where that changes its rounding, the value was within d of the
+    middle, so each error is at most its rounding's + 2 d, and so are their norms."""
+    c = make([(1, [16 + n for n in range(1, 25)]), (2, [32 + n for n in range(8)])], 8, 2, D, 16,
+             dtype, seed=D)
+    g = torch.Generator(device=DEV).manual_seed(D + 1)
+    for x in (c["q"], c["arena"][:, 0]):
+        x.copy_(torch.randint(-1, 2, x.shape, generator=g, device=DEV).float())
+    c["scale"] = 2.0 ** -round(math.log2(D) / 2 + 2)
+    out = call(c, scale=c["scale"])
+    rows = [(r, h) for r in range(out.size(0)) for h in range(8)]
+    want, mag = (torch.stack(x) for x in zip(*(_attend(c, r, h) for r, h in rows)))
+    got = torch.stack([out[r, h, 0] for r, h in rows]).double()
+    largest = max(R.logit_size(c["q"][r], c["arena"][:, 0].reshape(-1, D), c["scale"])
+                  for r in range(out.size(0)))
+    u = HALF[dtype]
+    d = 2 * (u * u + 2.0 ** -24 * (3 * largest + 16)) * (mag + want.abs())
+    rounding = (want.to(dtype).double() - want).norm()
+    assert (got - want).norm() <= rounding + 2 * d.norm()
