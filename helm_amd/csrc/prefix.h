@@ -101,16 +101,15 @@ struct PfSeq {
   int stretch;                       // of a workgroup
 };
 
-// What a sequence of len tokens sees: [first, end) of its table, first a block's.
+// What a sequence of len >= 0 tokens sees: [first, end) of its table, first a block's.
 struct PfView {
   int first, end;
 };
 __device__ __forceinline__ int pf_room(const PfParams& p) { return p.max_pages * p.page; }
 __device__ __forceinline__ PfView pf_view(const PfParams& p, int len) {
-  const int end = min(max(len, 0), pf_room(p));
-  // (row 0's first: end - S + 1 - window, or 0)
-  const int first = p.window > 0 && end - p.window >= p.S ? end - p.window - p.S + 1 : 0;
-  return {first & ~15, end};
+  // (row 0's first: len - S + 1 - window, or 0)
+  const int first = p.window > 0 && len - p.window >= p.S ? len - p.window - p.S + 1 : 0;
+  return {first & ~15, min(len, pf_room(p))};
 }
 // Tokens in the shared pages of a group.
 __device__ __forceinline__ int pf_shared(const PfParams& p, int pages) {
@@ -159,13 +158,13 @@ struct PfRow {
   int seq, s, g, last, from;
 };
 __device__ __forceinline__ PfRow pf_row(const PfParams& p, const PfPiece& w, int i,
-                                        const int* ends) {
+                                        const int* lens) {
   const unsigned row = w.row0 + i, sg = p.S * p.G;
   PfRow r;
   r.seq = w.seq0 + row / sg;
   r.s = row % sg / (unsigned)p.G;
   r.g = row % (unsigned)p.G;
-  const int at = ends[r.seq] - p.S + r.s;
+  const int at = lens[r.seq] - p.S + r.s;
   r.last = min(at, w.end - 1);
   r.from = p.window > 0 && at >= p.window ? at - p.window + 1 : 0;
   return r;
@@ -173,10 +172,10 @@ __device__ __forceinline__ PfRow pf_row(const PfParams& p, const PfPiece& w, int
 // The wave's rows first ..: what they see, and the address of row jr's query.
 template <int D>
 __device__ __forceinline__ const char* pf_rows(const PfParams& p, const PfPiece& w, int first,
-                                               int hk, const int* ends, PfRowsOf<D>& s) {
+                                               int hk, const int* lens, PfRowsOf<D>& s) {
   const int jr = threadIdx.x & 31;
   s.ok = first + jr < w.rows;
-  const PfRow r = pf_row(p, w, s.ok ? first + jr : 0, ends);
+  const PfRow r = pf_row(p, w, s.ok ? first + jr : 0, lens);
   s.last = s.ok ? r.last : -1;
   s.from = r.from;
   int to = s.ok ? s.last : 0x7fffffff, from = s.ok ? s.from : 0;
@@ -304,7 +303,7 @@ __device__ __forceinline__ PfBlock pf_block(const PfParams& p, const PfPiece& w,
 // has two dims of every (n / (D / 2))th row.
 template <typename T, int D>
 __device__ __forceinline__ void pf_add_special(const PfParams& p, const PfPiece& w, int hk,
-                                            const int* ends, float* part, int id, int n) {
+                                            const int* lens, float* part, int id, int n) {
   constexpr int kRow = 2 * D, kBlk = kBlockTok * kRow, kPairs = D / 2;
   const int every = max(1, n / kPairs);
   for (int item = id; item < kPairs * every; item += n) {
@@ -320,7 +319,7 @@ __device__ __forceinline__ void pf_add_special(const PfParams& p, const PfPiece&
         const uint32_t bad = nonfinite_halves<T>(v);
         if (!bad) continue;
         for (int r = r0; r < w.rows; r += every) {
-          const PfRow row = pf_row(p, w, r, ends);
+          const PfRow row = pf_row(p, w, r, lens);
           if (16 * block + t > row.last || 16 * block + t < row.from) continue;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -340,7 +339,7 @@ __device__ __forceinline__ void pf_add_special(const PfParams& p, const PfPiece&
 // done again, with V's infinities and NaN taken for zeros.
 template <typename T, int D, bool kCap>
 __device__ __forceinline__ bool pf_walk(const PfParams& p, const PfPiece& w, int hk,
-                                        const int* ends, PfRowsOf<D>& s, PfLds<D>& lds0,
+                                        const int* lens, PfRowsOf<D>& s, PfLds<D>& lds0,
                                         PfLds<D>& lds1, PfLds<D>& lds2, PfLds<D>& lds3) {
   using Buf = PfLds<D>;
   constexpr int NW = kPfWaves, NB = kPfBufs;
@@ -409,7 +408,7 @@ __device__ __forceinline__ bool pf_walk(const PfParams& p, const PfPiece& w, int
       v = x;
     }
   };
-  const char* qp = pf_rows<D>(p, w, wave_rows ? kPfRows * wave : 0, hk, ends, s);
+  const char* qp = pf_rows<D>(p, w, wave_rows ? kPfRows * wave : 0, hk, lens, s);
 #pragma unroll
   for (int i = 0; i < NK; ++i) s.q[i] = *reinterpret_cast<const mf_u32x4*>(qp + 16 * (2 * i + hh));
   auto start = [&] {
@@ -524,7 +523,7 @@ void prefix_attn_kernel(PfParams p) {
   } lds0;
   __shared__ PfLds<D> lds1, lds2, lds3;
   extern __shared__ PfGroup groups[];                  // [n_groups + 1], then int [R]:
-  int* ends = reinterpret_cast<int*>(groups + p.n_groups + 1);   // the sequences' tokens
+  int* lens = reinterpret_cast<int*>(groups + p.n_groups + 1);   // the sequences' tokens
   __shared__ int sh_sum[5][NW], sh_found[4], sh_down;
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -551,8 +550,9 @@ void prefix_attn_kernel(PfParams p) {
     return n_groups && groups[lo].start <= r && r < groups[lo + 1].start ? lo : -1;
   };
   for (int r = tid; r < p.R; r += kThreads) {
-    const PfView v = pf_view(p, r == tid ? len0 : p.lens[r]);
-    ends[r] = v.end;
+    const int len = max(r == tid ? len0 : p.lens[r], 0);
+    const PfView v = pf_view(p, len);
+    lens[r] = len;
     const int g = group_of(r);
     if (g >= 0) {
       atomicMin(&groups[g].lo, v.first);
@@ -574,7 +574,8 @@ void prefix_attn_kernel(PfParams p) {
       return {g.start, max(0, groups[e + 1].start - g.start) * sg, g.lo, g.hi};
     }
     const int r = e - n_groups, g = group_of(r);
-    return {r, sg, max(g < 0 ? 0 : groups[g].shared, pf_view(p, ends[r]).first), ends[r]};
+    const PfView v = pf_view(p, lens[r]);
+    return {r, sg, max(g < 0 ? 0 : groups[g].shared, v.first), v.end};
   };
   auto tiles_of = [&](int rows) { return (rows + kTile - 1) / kTile; };
   auto slots_of = [&](int e, int rows) {
@@ -714,12 +715,12 @@ void prefix_attn_kernel(PfParams p) {
       ml = p.own_ml + 2 * at;
       part = p.own_o + at * D;
     }
-    const bool careful = pf_walk<T, D, kCap>(p, w, hk, ends, s, lds0.buf, lds1, lds2, lds3);
+    const bool careful = pf_walk<T, D, kCap>(p, w, hk, lens, s, lds0.buf, lds1, lds2, lds3);
     if (kPfRows * wave < w.rows)
       pf_store(s, ml + 2 * kPfRows * wave, part + (int64_t)kPfRows * wave * D);
     if (careful) {
       __syncthreads();                                 // (all rows are stored)
-      pf_add_special<T, D>(p, w, hk, ends, part, tid, kThreads);
+      pf_add_special<T, D>(p, w, hk, lens, part, tid, kThreads);
     }
   }
 }

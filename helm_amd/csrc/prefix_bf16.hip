@@ -122,8 +122,7 @@ extern "C" int helm_prefix_decode_attn(const void* q, void* out, const void* k_p
   p.q_sign = scale < 0.f ? 0x80008000u : 0u;
   p.scale = std::max(scale < 0.f ? -scale : scale, FLT_MIN);
   p.softcap = softcap;
-  // (one of the whole table's length hides nothing)
-  p.window = window < (int64_t)max_pages * page_size ? window : 0;
+  p.window = window;
   char* ws = static_cast<char*>(workspace);
   auto take = [&](int64_t n) {
     char* at = ws;

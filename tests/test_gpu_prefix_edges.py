@@ -45,3 +45,38 @@ def test_weights_are_held_in_two_parts(dtype, D):
     d = 2 * (u * u + 2.0 ** -24 * (3 * largest + 16)) * (mag + want.abs())
     rounding = (want.to(dtype).double() - want).norm()
     assert (got - want).norm() <= rounding + 2 * d.norm()
+
+
+def _tolerance(q, k, v, want, mag, scale, u):
+    """Roundings of the output and the weights, of the logits' products in fp32 and of sums."""
+    size = R.logit_size(q, k, scale)
+    e = (q.size(-1) + 4) * 2.0 ** -24 * size + 2.0 ** -22 * (size + 8)
+    return u * want.abs() + 2 * u * u * (mag + want.abs()) \
+        + v.abs().max().item() * (2 * e + v.size(0) * (2.0 ** -24 + 2.0 ** -34)) + 1e-30
+
+
+@pytest.mark.parametrize("dtype,D", [(BF, 128), (HF, 64)])
+@pytest.mark.parametrize("S", [1, 4])
+@pytest.mark.parametrize("window", [0, 20, 96])
+def test_lengths_past_the_table_keep_their_rows_positions(dtype, D, S, window):
+    """Row s stands at len - S + s though the table ends before: it sees the table's tokens up
+    to there, and with a window only those that are not too far behind."""
+    page, room = 16, 96
+    c = make([(4, [150, 98, 97, 96, 96, 150]), (0, [150, 95])], 4, 2, D, page, dtype, S=S, seed=S)
+    lens = [150, 98, 97, 96, 73, 2 ** 31 - 1, 96 + 19, 95]
+    c["len_t"].copy_(torch.tensor(lens, dtype=torch.int32))
+    out = call(c, max_pages=room // page, window=window)
+    for r, t in enumerate(lens):
+        kv = c["arena"][c["table"][r, :room // page].long()]
+        pos = t - S + torch.arange(S, device=DEV)[:, None]
+        j = torch.arange(room, device=DEV)[None, :]
+        hidden = j > pos
+        if window:
+            hidden = hidden | (j <= pos - window)
+        for h in range(4):
+            k, v = (kv[:, i, h // 2].reshape(-1, D) for i in (0, 1))
+            scale = D ** -0.5
+            want, mag = (x[0] for x in R.attend(c["q"][r, h][None], k, v, scale, 0.0, hidden))
+            tol = _tolerance(c["q"][r, h], k, v, want, mag, scale, HALF[dtype])
+            assert ((out[r, h].double() - want).abs() <= tol).all(), (r, h)
+            assert (out[r, h][hidden.all(-1)] == 0).all()
