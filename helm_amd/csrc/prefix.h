@@ -554,9 +554,10 @@ void prefix_attn_kernel(PfParams p) {
     const PfView v = pf_view(p, len);
     lens[r] = len;
     const int g = group_of(r);
-    if (g >= 0) {
+    const int end = g < 0 ? 0 : min(v.end, groups[g].shared);
+    if (v.first < end) {                               // (it sees some of the shared tokens)
       atomicMin(&groups[g].lo, v.first);
-      atomicMax(&groups[g].hi, min(v.end, groups[g].shared));
+      atomicMax(&groups[g].hi, end);
     }
   }
   __syncthreads();

@@ -80,3 +80,18 @@ def test_lengths_past_the_table_keep_their_rows_positions(dtype, D, S, window):
             tol = _tolerance(c["q"][r, h], k, v, want, mag, scale, HALF[dtype])
             assert ((out[r, h].double() - want).abs() <= tol).all(), (r, h)
             assert (out[r, h][hidden.all(-1)] == 0).all()
+
+
+@pytest.mark.parametrize("window", [37, 100, 333])
+@pytest.mark.parametrize("nothing", [0, -7, 3000])
+def test_a_sequence_that_sees_nothing_leaves_its_groups_walk_alone(nothing, window):
+    """Its group's others get the same answer, bit for bit, as without it: nothing in front of
+    their windows, or behind them, is walked for its sake (its own window may lie past the table)."""
+    c = make([(60, [960 + n for n in (5, 60, 130)])], 16, 8, 128, 16, HF, seed=31)
+    c["len_t"][1:3] = torch.tensor([700, 650], dtype=torch.int32)
+    want = call(c, window=window)
+    d = dict(c, q=torch.cat([c["q"], c["q"][:1]]), table=torch.cat([c["table"], c["table"][:1]]),
+             len_t=torch.cat([c["len_t"], torch.full_like(c["len_t"][:1], nothing)]),
+             start_t=torch.tensor([0, 4], dtype=torch.int32, device=DEV))
+    got = call(d, window=window)
+    assert torch.equal(got[:3], want) and (got[3] == 0).all()
