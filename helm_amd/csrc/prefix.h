@@ -346,6 +346,7 @@ __device__ __forceinline__ bool pf_walk(const PfParams& p, const PfPiece& w, int
   constexpr int SB = PfBuf<D>::kBlocks, kSteps = SB / 2;
   constexpr int CPR = D / 8, kRow = 2 * D, kBlk = kBlockTok * kRow, kBlkLoads = kBlk / 1024;
   constexpr int kLoads = 2 * SB * kBlkLoads / NW;      // a wave's, of one block
+  constexpr int kAhead = (NB - 2) * kLoads;            // those of the stages behind the present one
   constexpr int NK = D / 16;
   const int lane = threadIdx.x & 63, hh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -429,11 +430,10 @@ __device__ __forceinline__ bool pf_walk(const PfParams& p, const PfPiece& w, int
       // it, then everyone's), and every wave is done with the buffer of the stage before,
       // which loads of a later one fill (a plain barrier would wait for all loads)
       if (careful) {
-        __builtin_amdgcn_s_waitcnt(0x0F70 | (NB - 2) * kLoads);    // vmcnt
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kAhead) : "memory");
         clean(cur);
       }
-      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NB - 2) * kLoads)
-                   : "memory");
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kAhead) : "memory");
       __builtin_amdgcn_sched_barrier(0);
       const uint32_t there = gone >> (32 - 8 * (NB - 1));          // this stage's
       dma(st + NB - 1, nxt);
