@@ -46,7 +46,7 @@ struct SelectArgs {
   const void* logits;
   int64_t b_stride, k_stride;                // elements
   const float* scores;
-  int B, K, V, n, chunks;
+  int B, K, V, n, chunks, size;              // chunks of a row, logits of one
   double* part_sum;                          // [B K][chunks]
   float* part_max;                          // [B K][chunks]
   float* cand_x;                             // [B][n][K chunks], -inf: none; a chunk's n best are
@@ -325,15 +325,16 @@ __global__ __launch_bounds__(kBeamThreads) void beam_scan_kernel(SelectArgs a) {
 }
 
 // The n best of request blockIdx.x from its rows' chunks.
+template <typename T>
 __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(SelectArgs a) {
   __shared__ double base[64];                // s_k - lse_k; -inf: the row offers nothing
   __shared__ __attribute__((aligned(16))) uint32_t sh_key[kBeamThreads];
-  __shared__ int sh_n[kBeamWaves], sh_count;
-  __shared__ double list_x[kJoinList];
+  __shared__ int sh_n[kBeamWaves], sh_count, sh_close;
+  __shared__ double list_x[kJoinList], sh_edge;
   __shared__ int64_t list_i[kJoinList];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int b = blockIdx.x, n = a.n, C = a.chunks;
-  if (tid == 0) sh_count = 0;
+  if (tid == 0) sh_count = sh_close = 0;
   // candidate i of the request: of list i % (K C), that is of a row's chunk, the (i / (K C))th.
   // The lists lie side by side, from their best on; eight a thread are on their way at once,
   // the first of them before the rows' sums.
@@ -420,6 +421,11 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(SelectArgs a) {
     for (int w = 0; w < kBeamWaves; ++w) bound = max(bound, sh_key[w]);
   }
   const double least = unordered(max((uint64_t)bound << 32, ordered(-(double)INFINITY)));
+  // whether another logit of the list's row may give the same sum
+  auto close = [&](int list, float v, double y) {
+    const double s = base[list / C];
+    return s + (double)unordered(ordered(v) + 1) == y || s + (double)unordered(ordered(v) - 1) == y;
+  };
   auto keep = [&](double y, int64_t t) {
     const int i = atomicAdd(&sh_count, 1);
     if (i < kJoinList) {
@@ -432,6 +438,7 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(SelectArgs a) {
   for (int u = 0; u < U; ++u)
     if (y0[u] >= least && y0[u] > -INFINITY) {
       any = true;
+      if (close(at[u], x[u], y0[u])) sh_close = 1;
       keep(y0[u], (int64_t)(at[u] / C) << 32 | t0[u]);
     }
   // on until none of the lists has one left (a sweep holds one of each)
@@ -456,6 +463,7 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(SelectArgs a) {
       const double y = sum(at[u], x[u]);
       if (y >= least && y > -INFINITY) {
         any = true;
+        if (close(at[u], x[u], y)) sh_close = 1;
         keep(y, index(i0 + u * kBeamThreads + tid));
       }
     }
@@ -504,6 +512,7 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(SelectArgs a) {
     rank += __shfl_xor(rank, 1, 64);
     rank += __shfl_xor(rank, 2, 64);
     if (i < count && rank < n && (tid & 3) == 0) {
+      if (rank == n - 1) sh_edge = y;
       // (never -inf, which stands for no candidate)
       a.out_scores[o + rank] = (float)fmin(fmax(y, -(double)FLT_MAX), (double)FLT_MAX);
       a.out_tokens[o + rank] = t & 0xffffffff;
@@ -515,6 +524,62 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(SelectArgs a) {
     a.out_tokens[o + i] = -1;
     a.out_parents[o + i] = -1;
   }
+
+  // A chunk's n best are its largest logits.  Where 64 bits do not tell sums of different logits
+  // apart (a score or lse past some 2^29 times the logits' spacing, logits next to zero), a chunk
+  // may have left out a lower token of the n-th best sum; all larger sums are there.  Then the
+  // lowest indexes of that sum are looked for in the logits, in the chunks that it is in.
+  if (!sh_close || count < n) return;         // (uniform: nobody writes either any more)
+  __syncthreads();
+  const double edge = sh_edge;
+  bool full = false;
+  for (int l = tid; l < lists; l += kBeamThreads) {
+    const float v = cx[(n - 1) * lists + l];
+    const double y = sum(l, v);
+    full |= v > -INFINITY && y == edge && close(l, v, y);
+  }
+  if (!__syncthreads_or(full)) return;
+  int above = 0;
+  for (int i = tid; i < count; i += kBeamThreads) above += list_x[i] > edge;
+  const int first = block_sum(above, sh_n), need = n - first;
+  int have = 0;
+  for (int l = -1; have < need;) {
+    if (tid == 0) sh_count = lists;
+    __syncthreads();
+    for (int i = tid; i < count; i += kBeamThreads) {
+      const int in = (int)(list_i[i] >> 32) * C + (int)((uint32_t)list_i[i] / (uint32_t)a.size);
+      if (list_x[i] == edge && in > l) atomicMin(&sh_count, in);
+    }
+    __syncthreads();
+    l = sh_count;                             // the next of those chunks
+    if (l >= lists) break;
+    const int k = l / C, t0 = l % C * a.size;
+    const double s = base[k];
+    const T* row = reinterpret_cast<const T*>(a.logits) + b * a.b_stride + k * a.k_stride + t0;
+    const int size = min(a.size, a.V - t0);
+    for (int v0 = 0; v0 < size && have < need; v0 += kBatch) {
+      uint64_t hits[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int t = v0 + u * kBeamThreads + tid;
+        const float v = t < size ? Elem<T>::read(row + t) : -INFINITY;
+        hits[u] = __builtin_amdgcn_ballot_w64(v > -INFINITY && s + (double)v == edge);
+        if (lane == 0) sh_key[u * kBeamWaves + wave] = __builtin_popcountll(hits[u]);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        for (int w = 0; w < kBeamWaves; ++w) {
+          const int r = have + __builtin_popcountll(hits[u] & ((1ull << lane) - 1));
+          if (w == wave && (hits[u] >> lane & 1) && r < need) {
+            a.out_tokens[o + first + r] = t0 + v0 + u * kBeamThreads + tid;
+            a.out_parents[o + first + r] = k;
+          }
+          have += sh_key[u * kBeamWaves + w];
+        }
+      __syncthreads();                        // (sh_key has been read)
+    }
+  }
 }
 
 // Chunks of a row: 64 bytes a thread (128 in fp32), so that the joining has few lists, or, where
@@ -523,7 +588,7 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(SelectArgs a) {
 // of 152,064 10.2, 10.8; 8 rows 11.3, 16.9; 64 rows and 64 beams 46, 205.  (32 and 128 bytes:
 // 256 rows of 131,072 take 22.6 and 24.7 us against 22.)
 struct SelectPlan {
-  int nv, chunks;
+  int nv, chunks, size;
   int64_t rows, bytes;
 };
 SelectPlan select_plan(int B, int K, int V, int n, int es) {
@@ -531,7 +596,8 @@ SelectPlan select_plan(int B, int K, int V, int n, int es) {
   p.rows = (int64_t)B * K;
   const int per = kBeamThreads * 16 / es;
   p.nv = es / 2 * (p.rows * ((V + 2047) / 2048) > 128 ? 4 : 1);
-  p.chunks = (V + p.nv * per - 1) / (p.nv * per);
+  p.size = p.nv * per;
+  p.chunks = (V + p.size - 1) / p.size;
   p.bytes = p.rows * p.chunks * (12 + 8 * (int64_t)n);
   return p;
 }
@@ -541,11 +607,12 @@ bool select_ok(int B, int K, int V, int n) {
          (int64_t)K * ((V + 1023) / 1024) * n <= 0x7fffffff;
 }
 
-template <typename T> void launch_scan(const SelectArgs& a, const SelectPlan& p, hipStream_t st) {
+template <typename T> void launch_select(const SelectArgs& a, const SelectPlan& p, hipStream_t st) {
   const dim3 grid(p.chunks, (uint32_t)p.rows);
   constexpr int S = sizeof(T) / 2;
   if (p.nv == S) hipLaunchKernelGGL((beam_scan_kernel<T, S>), grid, dim3(kBeamThreads), 0, st, a);
   else hipLaunchKernelGGL((beam_scan_kernel<T, 4 * S>), grid, dim3(kBeamThreads), 0, st, a);
+  hipLaunchKernelGGL((beam_join_kernel<T>), dim3(a.B), dim3(kBeamThreads), 0, st, a);
 }
 
 // ---- tables ----------------------------------------------------------------------------
@@ -776,6 +843,7 @@ extern "C" int helm_beam_select(const void* logits, int64_t b_stride, int64_t k_
   a.V = V;
   a.n = n;
   a.chunks = p.chunks;
+  a.size = p.size;
   const int64_t parts = p.rows * p.chunks;
   a.part_sum = static_cast<double*>(workspace);
   a.part_max = reinterpret_cast<float*>(a.part_sum + parts);
@@ -785,10 +853,9 @@ extern "C" int helm_beam_select(const void* logits, int64_t b_stride, int64_t k_
   a.out_tokens = out_tokens;
   a.out_parents = out_parents;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  if (dtype == HELM_F32) launch_scan<float>(a, p, st);
-  else if (dtype == HELM_BF16) launch_scan<bf16_t>(a, p, st);
-  else launch_scan<f16_t>(a, p, st);
-  hipLaunchKernelGGL(beam_join_kernel, dim3(B), dim3(kBeamThreads), 0, st, a);
+  if (dtype == HELM_F32) launch_select<float>(a, p, st);
+  else if (dtype == HELM_BF16) launch_select<bf16_t>(a, p, st);
+  else launch_select<f16_t>(a, p, st);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess)
     return report_error((int)e, std::string("beam selection launch: ") + hipGetErrorString(e));
