@@ -84,11 +84,20 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: Optional[int] = N
     return out
 
 
+def _overlap(n: int, slot: int, segments: int, step: int, part: int) -> bool:
+    """Whether any two of the parts at i * slot + j * step (i < n, j < segments) share memory."""
+    slot = slot if n > 1 else max(part, segments * step)
+    if slot < part:
+        return True
+    return any(abs(j * step - i * slot) < part for j in range(1, segments)
+               for i in (j * step // slot, j * step // slot + 1) if i < n)
+
+
 class PageStore:
     """The pools of a model's layers, whose pages ``beam_tables`` copies: ``Pool4`` objects, or
     tensors [n_slots, ..., page_size, D] whose pages are made of dense [page_size, D] rows
-    (an arena [n_slots, 2, Hkv, page_size, D], or its K and its V as two), all of one shape,
-    stride and type and of one slot numbering."""
+    (an arena [n_slots, 2, Hkv, page_size, D], or its K and its V as two; slots or heads
+    outermost), all of one shape, stride and type and of one slot numbering."""
 
     def __init__(self, pools: Sequence[Union[torch.Tensor, Pool4]]):
         pools = list(pools)
@@ -120,8 +129,8 @@ class PageStore:
             step = step if segments > 1 else s
             segments *= n
         part = t.size(-2) * t.size(-1)
-        if t.numel() and ((segments > 1 and step < part) or
-                          (t.size(0) > 1 and t.stride(0) < (segments - 1) * step + part)):
+        # (a slot's parts may lie among other slots': heads outermost)
+        if t.numel() and _overlap(t.size(0), t.stride(0), segments, step, part):
             raise ValueError("a pool's pages must not overlap")
         if part == 0 or segments == 0:
             raise ValueError("a pool's pages must hold something")

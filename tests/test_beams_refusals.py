@@ -117,6 +117,25 @@ def test_page_store_layouts():
     assert s._shape == (5, 2 * 2 * 17 * 64, 2, 2 * 17 * 64, 16, 17 * 64) and s.page_size == 32
 
 
+def test_page_store_takes_every_layout_without_overlaps():
+    """Slots, parts and strides: refused exactly where two parts share an element."""
+    heads = torch.zeros(2, 3, 5, 16, 8).half()                  # [K and V, heads, slots, page, D]
+    assert beams.PageStore([heads[0].transpose(0, 1)])._shape == (5, 256, 3, 1280, 1, 16)
+    assert beams.PageStore([heads.permute(2, 0, 1, 3, 4)])._shape == (5, 256, 6, 1280, 1, 16)
+    for n in (1, 2, 4):
+        for segs in (1, 2, 3):
+            for slot in range(0, 13):
+                for step in range(0, 13):
+                    t = torch.zeros(64).as_strided((n, segs, 1, 4), (slot, step, 4, 1))
+                    at = [i * slot + j * step + d for i in range(n) for j in range(segs)
+                          for d in range(4)]
+                    if len(set(at)) == len(at):
+                        beams.PageStore([t])
+                    else:
+                        with pytest.raises(ValueError):
+                            beams.PageStore([t])
+
+
 def _i32(n):
     a = np.zeros(max(1, n), dtype=np.int32)
     return a, a.ctypes.data

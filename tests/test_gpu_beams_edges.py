@@ -1,10 +1,14 @@
-"""Beam selection and beam tables at their edges: sums that 64 bits do not tell apart."""
+"""Beam selection and beam tables at their edges: sums that 64 bits do not tell apart; pools with
+heads outermost, pages outside the pool in every layout."""
 import math
+import random
 
 import pytest
 import torch
 
-from test_gpu_beams import DEV, check_select, randn
+from helm_amd import beams, pool4
+from oracle import beams as R
+from test_gpu_beams import DEV, I32, check_select, make_tables, randn
 
 pytestmark = pytest.mark.gpu
 DTYPES = [torch.bfloat16, torch.float16, torch.float32]
@@ -50,3 +54,49 @@ def test_select_groups_of_sums(n):
     x = 0.5 + step * 2.0 ** -22 + form * 2.0 ** -24
     scores = torch.tensor([[-2.0 ** 30, -2.0 ** 30 - 256]] * 3, device=DEV)
     check_select(x, scores, n)
+
+
+@pytest.mark.parametrize("layout", ["heads_outermost", "k_and_v_heads_outermost", "arena",
+                                    "k_and_v", "pool4", "odd_rows", "many"])
+def test_tables_pools_and_pages_outside_them(layout):
+    r = random.Random(9)
+    B, K, page, width, H, D, n = 2, 4, 32, 4, 3, 64, 40
+    lens, shared, unit = [page + 19, 2 * page + 1], [0, 1], 1
+    table, _ = make_tables(r, B, K, page, width, lens, shared)
+    parents = [[0, 0, 0, 2], [3, 3, 1, 1]]
+    rows = [t for t in lens for _ in range(K)]
+    if layout == "heads_outermost":
+        pools = [randn(i, (H, n, page, D), torch.float16).transpose(0, 1) for i in range(2)]
+    elif layout == "k_and_v_heads_outermost":
+        pools = [randn(i, (2, H, n, page, D), torch.float32).permute(2, 0, 1, 3, 4)
+                 for i in range(2)]
+    elif layout == "arena":
+        pools = [randn(i, (n, 2, H, page, D), torch.bfloat16) for i in range(3)]
+    elif layout == "k_and_v":
+        arena = randn(0, (n, 2, H, page, D), torch.float32)
+        pools = [arena[:, 0], arena[:, 1]]
+    elif layout == "pool4":
+        pools, unit = [pool4.Pool4(n, H, D, page_size=page, device=DEV) for _ in range(2)], 16
+        for p in pools:
+            p.data.copy_(torch.randint(0, 256, p.data.shape, device=DEV, dtype=torch.uint8))
+    elif layout == "odd_rows":
+        pools = [randn(i, (n, H, page, 5), torch.float16) for i in range(2)]
+    else:
+        pools = [randn(i, (n, page, 8), torch.float16) for i in range(131)]
+    data = [p.data if layout == "pool4" else p for p in pools]
+    store = beams.PageStore(pools)
+    outside = [list(x) for x in table]
+    for j, x in enumerate([5, -1, n, 2 ** 31 - 1] * B):
+        outside[j][lens[j // K] // page] = x
+    outside[6][2], outside[7][2] = 7, 8
+    for tab, sh in ((table, shared), (outside, None)):
+        new, copies, released = R.tables(parents, tab, rows, page, sh)
+        want = [R.copy_pages(x.cpu(), copies, rows, page, K, unit) for x in data]
+        got = beams.beam_tables(torch.tensor(parents, **I32), torch.tensor(tab, **I32),
+                                torch.tensor(rows, **I32), page, pages=store,
+                                shared_pages=None if sh is None else torch.tensor(sh, **I32))
+        for x, w in zip(data, want):
+            assert torch.equal(x.cpu(), w)
+        assert got.page_table.tolist() == new
+        assert [tuple(c) for c in got.copies.tolist()] == copies
+        assert got.released[:int(got.n_released)].tolist() == released
