@@ -952,6 +952,7 @@ extern "C" int helm_beam_tables(const int32_t* parents, int B, int K, const int3
   p.unit = unit_bytes;
   p.parts = (int)std::min<int64_t>(64, std::max<int64_t>(1, units * unit_bytes * segments >> 16));
   int joins = (int)std::max<int64_t>(1, std::min<int64_t>(64, (int64_t)B * a.chunks));
+  if (B == 0) n_pools = 0;
   for (int i0 = 0; i0 == 0 || i0 < n_pools; i0 += kPools) {
     p.n = std::min(kPools, n_pools - i0);
     uint64_t bits = (uint64_t)slot_bytes | (uint64_t)segment_bytes | (uint64_t)unit_bytes;

@@ -100,3 +100,14 @@ def test_tables_pools_and_pages_outside_them(layout):
         assert got.page_table.tolist() == new
         assert [tuple(c) for c in got.copies.tolist()] == copies
         assert got.released[:int(got.n_released)].tolist() == released
+
+
+@pytest.mark.parametrize("n", [1, 128, 131])
+def test_tables_of_no_request(n):
+    """With pools, too, of more than one launch."""
+    pools = [randn(i, (4, 16, 8), torch.float16) for i in range(n)]
+    t = beams.beam_tables(torch.zeros((0, 3), **I32), torch.zeros((0, 4), **I32),
+                          torch.zeros(0, **I32), 16, pages=beams.PageStore(pools))
+    assert int(t.n_released) == 0 and t.page_table.shape == (0, 4) and t.copies.shape == (0, 2)
+    for i, p in enumerate(pools):
+        assert torch.equal(p, randn(i, (4, 16, 8), torch.float16))
