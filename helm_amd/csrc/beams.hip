@@ -888,6 +888,8 @@ extern "C" int helm_beam_tables(const int32_t* parents, int B, int K, const int3
   const int64_t units = n_pools ? ((int64_t)page_size + unit_tokens - 1) / unit_tokens : 1;
   if (n_pools && (segments > 0x7fffffff / unit_bytes / units || segment_bytes < units * unit_bytes))
     return report_error(HELM_E_INVALID, "a page's segments overlap or pass 2^31 bytes");
+  for (int i = 0; i < n_pools; ++i)
+    if (!pools[i] && n_slots) return report_error(HELM_E_INVALID, "null pool");
   if (B == 0 && !n_released) return report_error(HELM_E_INVALID, "null pointer argument");
   if (B && (!parents || !seq_lens || !copies || !n_released ||
             (table_width && (!page_table || !new_table || !released))))
@@ -957,7 +959,6 @@ extern "C" int helm_beam_tables(const int32_t* parents, int B, int K, const int3
     p.n = std::min(kPools, n_pools - i0);
     uint64_t bits = (uint64_t)slot_bytes | (uint64_t)segment_bytes | (uint64_t)unit_bytes;
     for (int i = 0; i < p.n; ++i) {
-      if (!pools[i0 + i]) return report_error(HELM_E_INVALID, "null pool");
       p.at[i] = static_cast<char*>(const_cast<void*>(pools[i0 + i]));
       bits |= reinterpret_cast<uint64_t>(pools[i0 + i]);
     }

@@ -192,6 +192,30 @@ def test_c_entries_refuse_before_device_work():
         assert b"lies over" in lib.helm_last_error_string()
 
 
+def _tables_call(pools, n_slots=4, **kw):
+    """helm_beam_tables of 2 x 3 beams with 4 columns over `pools`, of 2 segments of 16 tokens of 2
+    bytes; kw: addresses to take instead of the operands' own."""
+    lib = _native.load()
+    sizes = dict(par=6, tab=24, lens=6, new=24, cop=12, rel=24, cnt=1, ws=0)
+    sizes["ws"] = lib.helm_beam_tables_workspace_bytes(2, 3, 4) // 4
+    arr = {k: np.zeros(n, dtype=np.int32) for k, n in sizes.items()}
+    p = dict({k: a.ctypes.data for k, a in arr.items()}, **kw)
+    return lib.helm_beam_tables(p["par"], 2, 3, p["tab"], 4, 4, p["lens"], 16, None, p["new"], 4,
+                                p["cop"], p["rel"], p["cnt"],
+                                (ctypes.c_void_p * len(pools))(*pools), len(pools), n_slots, 64, 2,
+                                32, 1, 2, p["ws"], 4 * sizes["ws"], None)
+
+
+def test_a_null_pool_is_refused_before_device_work():
+    """With the other arguments (the workspace is looked at last)."""
+    at = np.zeros(256, dtype=np.uint8)
+    pools = [at.ctypes.data] * 130 + [None]
+    assert _tables_call(pools, ws=None) == _native.HELM_E_INVALID
+    assert b"null pool" in _native.load().helm_last_error_string()
+    assert _tables_call(pools[:130], ws=None) == _native.HELM_E_WORKSPACE
+    assert _tables_call([None], n_slots=0, ws=None) == _native.HELM_E_WORKSPACE
+
+
 def test_the_restated_choice():
     """By hand: two beams of two tokens, and ties."""
     x = torch.tensor([[[0.0, 0.0], [0.0, 0.0]]])

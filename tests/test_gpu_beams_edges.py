@@ -1,12 +1,13 @@
 """Beam selection and beam tables at their edges: sums that 64 bits do not tell apart; pools with
 heads outermost, pages outside the pool in every layout."""
+import ctypes
 import math
 import random
 
 import pytest
 import torch
 
-from helm_amd import beams, pool4
+from helm_amd import _native, beams, pool4
 from oracle import beams as R
 from test_gpu_beams import DEV, I32, check_select, make_tables, randn
 
@@ -111,3 +112,28 @@ def test_tables_of_no_request(n):
     assert int(t.n_released) == 0 and t.page_table.shape == (0, 4) and t.copies.shape == (0, 2)
     for i, p in enumerate(pools):
         assert torch.equal(p, randn(i, (4, 16, 8), torch.float16))
+
+
+def test_a_refused_call_leaves_the_table_as_it_was():
+    """In place, with a pool that is null."""
+    lib = _native.load()
+    tab = torch.arange(24, **I32).view(6, 4)
+    before = tab.clone()
+    par, lens = torch.tensor([[1, 1, 0], [2, 0, 0]], **I32), torch.full((6,), 40, **I32)
+    cop, rel, cnt = torch.zeros(12, **I32), torch.zeros(24, **I32), torch.zeros(1, **I32)
+    pool = torch.zeros((24, 16, 8), dtype=torch.float16, device=DEV)
+    need = lib.helm_beam_tables_workspace_bytes(2, 3, 4)
+    ws = torch.empty(need, dtype=torch.uint8, device=DEV)
+    rc = lib.helm_beam_tables(par.data_ptr(), 2, 3, tab.data_ptr(), 4, 4, lens.data_ptr(), 16, None,
+                              tab.data_ptr(), 4, cop.data_ptr(), rel.data_ptr(), cnt.data_ptr(),
+                              (ctypes.c_void_p * 2)(pool.data_ptr(), None), 2, 24, 256, 1, 256, 1,
+                              16, ws.data_ptr(), need, None)
+    torch.cuda.synchronize()
+    assert rc == _native.HELM_E_INVALID and torch.equal(tab, before)
+
+
+def test_a_store_without_a_slot_copies_nothing():
+    t = beams.beam_tables(torch.tensor([[1, 1]], **I32), torch.zeros((2, 2), **I32),
+                          torch.full((2,), 5, **I32), 16,
+                          pages=beams.PageStore([torch.zeros((0, 16, 8), device=DEV)]))
+    assert t.copies.tolist() == [[0, 0], [-1, -1]]
