@@ -174,7 +174,8 @@ def beam_tables(parents: torch.Tensor, page_table: torch.Tensor, seq_lens: torch
     are row j's old ones.
 
     out: a former result of the same sizes, written instead of new tensors; its page_table
-    may be page_table itself.  No other output may share memory with an operand."""
+    may be page_table itself.  No other output may share memory with an operand, nor any
+    operand with the pools' pages."""
     i32 = torch.int32
     if parents.dtype != i32 or page_table.dtype != i32 or seq_lens.dtype != i32:
         raise TypeError("parents, page_table and seq_lens must be int32")

@@ -886,7 +886,9 @@ extern "C" int helm_beam_tables(const int32_t* parents, int B, int K, const int3
                                   unit_bytes < 1)))
     return report_error(HELM_E_INVALID, "bad pool shape");
   const int64_t units = n_pools ? ((int64_t)page_size + unit_tokens - 1) / unit_tokens : 1;
-  if (n_pools && (segments > 0x7fffffff / unit_bytes / units || segment_bytes < units * unit_bytes))
+  const int64_t part = n_pools ? units * unit_bytes : 0;     // of a segment
+  if (n_pools && (segments > 0x7fffffff / unit_bytes / units || segment_bytes < part ||
+                  (n_slots > 1 && slot_bytes < part)))
     return report_error(HELM_E_INVALID, "a page's segments overlap or pass 2^31 bytes");
   for (int i = 0; i < n_pools; ++i)
     if (!pools[i] && n_slots) return report_error(HELM_E_INVALID, "null pool");
@@ -922,6 +924,21 @@ extern "C" int helm_beam_tables(const int32_t* parents, int B, int K, const int3
         return report_error(HELM_E_INVALID, "an output lies over another operand (new_table may "
                                             "be page_table itself, nothing else)");
     }
+  // the pools are written: no operand may lie in one (its parts are looked at where its whole
+  // stretch of memory is touched)
+  for (int i = 0; i < n_pools && n_slots; ++i) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(pools[i]);
+    const int64_t all = (n_slots - 1) * slot_bytes + (segments - 1) * segment_bytes + part;
+    for (const Range& x : r) {
+      if (!x.rows || !x.bytes) continue;
+      const int64_t len = (x.rows - 1) * x.step + x.bytes;
+      if (!overlap({x.at, 1, len, len}, {at, 1, all, all})) continue;
+      for (int64_t j = 0; j < segments; ++j)
+        if (meet(x, {at + (uintptr_t)(j * segment_bytes), n_slots, part,
+                     n_slots > 1 ? slot_bytes : part}))
+          return report_error(HELM_E_INVALID, "an operand lies over a pool's pages");
+    }
+  }
   BeamTableArgs a{};
   a.parents = parents;
   a.B = B;

@@ -523,7 +523,7 @@ int helm_beam_select(const void* logits, int64_t b_stride, int64_t k_stride, int
  * released: full pages behind the shared ones that no row names any more, each once, by request,
  * column, row (negative entries are no pages); n_released: how many; behind them released (room
  * for B K table_width) is left as it is.  new_table may be page_table itself (at its stride); no
- * other output may lie over an operand.
+ * other output may lie over an operand, and no operand over a page.
  * pools: n_pools (0: none) addresses on the host, all of n_slots pages slot_bytes apart, a page
  * being `segments` segments segment_bytes apart whose every unit_tokens tokens are unit_bytes
  * bytes; pages outside [0, n_slots) are not copied.  K <= HELM_BEAMS_MAX, B K <= 65535. */

@@ -192,9 +192,9 @@ def test_c_entries_refuse_before_device_work():
         assert b"lies over" in lib.helm_last_error_string()
 
 
-def _tables_call(pools, n_slots=4, **kw):
+def _tables_call(pools, n_slots=4, slot=64, **kw):
     """helm_beam_tables of 2 x 3 beams with 4 columns over `pools`, of 2 segments of 16 tokens of 2
-    bytes; kw: addresses to take instead of the operands' own."""
+    bytes a page; kw: addresses to take instead of the operands' own."""
     lib = _native.load()
     sizes = dict(par=6, tab=24, lens=6, new=24, cop=12, rel=24, cnt=1, ws=0)
     sizes["ws"] = lib.helm_beam_tables_workspace_bytes(2, 3, 4) // 4
@@ -202,7 +202,7 @@ def _tables_call(pools, n_slots=4, **kw):
     p = dict({k: a.ctypes.data for k, a in arr.items()}, **kw)
     return lib.helm_beam_tables(p["par"], 2, 3, p["tab"], 4, 4, p["lens"], 16, None, p["new"], 4,
                                 p["cop"], p["rel"], p["cnt"],
-                                (ctypes.c_void_p * len(pools))(*pools), len(pools), n_slots, 64, 2,
+                                (ctypes.c_void_p * len(pools))(*pools), len(pools), n_slots, slot, 2,
                                 32, 1, 2, p["ws"], 4 * sizes["ws"], None)
 
 
@@ -214,6 +214,20 @@ def test_a_null_pool_is_refused_before_device_work():
     assert b"null pool" in _native.load().helm_last_error_string()
     assert _tables_call(pools[:130], ws=None) == _native.HELM_E_WORKSPACE
     assert _tables_call([None], n_slots=0, ws=None) == _native.HELM_E_WORKSPACE
+
+
+def test_operands_over_a_pool_are_refused():
+    """Read or written, in any part of any page: pages of 64 bytes, 128 apart, from byte 1024 on."""
+    buf = np.zeros(512, dtype=np.int32)
+    at = buf.ctypes.data
+    other = np.zeros(1024, dtype=np.uint8)
+    lib, pools = _native.load(), [other.ctypes.data, at + 1024]
+    for kw in (dict(new=at + 932), dict(new=at + 1024), dict(rel=at + 1264), dict(cnt=at + 1052),
+               dict(cop=at + 980), dict(cnt=at + 1440), dict(par=at + 1024), dict(lens=at + 1080),
+               dict(tab=at + 1216)):
+        assert _tables_call(pools, slot=128, **kw) == _native.HELM_E_INVALID, kw
+        assert b"lies over" in lib.helm_last_error_string()
+    assert _tables_call(pools, slot=31) == _native.HELM_E_INVALID        # pages over each other
 
 
 def test_the_restated_choice():

@@ -137,3 +137,26 @@ def test_a_store_without_a_slot_copies_nothing():
                           torch.full((2,), 5, **I32), 16,
                           pages=beams.PageStore([torch.zeros((0, 16, 8), device=DEV)]))
     assert t.copies.tolist() == [[0, 0], [-1, -1]]
+
+
+def test_operands_between_a_pools_pages():
+    """Memory between the pages is nobody's: outputs may lie there."""
+    lib = _native.load()
+    par, lens = torch.tensor([[1, 1, 0], [2, 0, 0]], **I32), torch.full((6,), 40, **I32)
+    tab = torch.arange(24, **I32).view(6, 4)
+    want, copies, released = R.tables(par.tolist(), tab.tolist(), [40] * 6, 16)
+    buf = torch.arange(24 * 32, **I32)                 # pages of 16 tokens of 4 bytes, 128 apart
+    pages = buf.view(24, 32)[:, :16].reshape(24, 16, 1).cpu()
+    rel, new = torch.zeros(24, **I32), torch.zeros((6, 4), **I32)
+    need = lib.helm_beam_tables_workspace_bytes(2, 3, 4)
+    ws = torch.empty(need, dtype=torch.uint8, device=DEV)
+    at = buf.data_ptr()
+    rc = lib.helm_beam_tables(par.data_ptr(), 2, 3, tab.data_ptr(), 4, 4, lens.data_ptr(), 16, None,
+                              new.data_ptr(), 4, at + 64, rel.data_ptr(), at + 23 * 128 + 124,
+                              (ctypes.c_void_p * 1)(at), 1, 24, 128, 1, 64, 1, 4, ws.data_ptr(),
+                              need, torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert rc == 0 and new.tolist() == want and int(buf[-1]) == len(released)
+    assert [tuple(c) for c in buf[16:28].view(6, 2).tolist()] == copies
+    assert torch.equal(buf.view(24, 32)[:, :16].reshape(24, 16, 1).cpu(),
+                       R.copy_pages(pages, copies, [40] * 6, 16, 3))
