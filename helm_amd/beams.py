@@ -58,8 +58,9 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: Optional[int] = N
     if not scores.is_contiguous():
         raise ValueError("scores must be contiguous")
     n = K if n is None else n
-    if not (1 <= K <= _MAX and 1 <= n <= _MAX and V >= 1 and B * K <= 65535):
-        raise ValueError("beam_select takes 1 to 64 beams and candidates of at most 65535 rows")
+    if not (1 <= K <= _MAX and 1 <= n <= _MAX and 1 <= V < 2 ** 31 and B * K <= 65535):
+        raise ValueError("beam_select takes 1 to 64 beams and candidates of at most 65535 rows, "
+                         "1 to 2^31 - 1 logits each")
     _engine.refuse_grad("beam_select", logits, scores)
     given = out is not None
     if not given:
@@ -86,9 +87,10 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: Optional[int] = N
 
 def _overlap(n: int, slot: int, segments: int, step: int, part: int) -> bool:
     """Whether any two of the parts at i * slot + j * step (i < n, j < segments) share memory."""
-    slot = slot if n > 1 else max(part, segments * step)
-    if slot < part:
+    if (n > 1 and slot < part) or (segments > 1 and step < part):
         return True
+    if n == 1 or slot >= (segments - 1) * step + part:
+        return False
     return any(abs(j * step - i * slot) < part for j in range(1, segments)
                for i in (j * step // slot, j * step // slot + 1) if i < n)
 
@@ -129,6 +131,8 @@ class PageStore:
             step = step if segments > 1 else s
             segments *= n
         part = t.size(-2) * t.size(-1)
+        if segments * part * es >= 2 ** 31:
+            raise ValueError("a page holds less than 2^31 bytes")
         # (a slot's parts may lie among other slots': heads outermost)
         if t.numel() and _overlap(t.size(0), t.stride(0), segments, step, part):
             raise ValueError("a pool's pages must not overlap")

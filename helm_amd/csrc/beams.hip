@@ -595,16 +595,16 @@ SelectPlan select_plan(int B, int K, int V, int n, int es) {
   SelectPlan p{};
   p.rows = (int64_t)B * K;
   const int per = kBeamThreads * 16 / es;
-  p.nv = es / 2 * (p.rows * ((V + 2047) / 2048) > 128 ? 4 : 1);
+  p.nv = es / 2 * (p.rows * ((V - 1) / 2048 + 1) > 128 ? 4 : 1);
   p.size = p.nv * per;
-  p.chunks = (V + p.size - 1) / p.size;
+  p.chunks = (V - 1) / p.size + 1;
   p.bytes = p.rows * p.chunks * (12 + 8 * (int64_t)n);
   return p;
 }
 bool select_ok(int B, int K, int V, int n) {
   return B >= 0 && K >= 1 && K <= HELM_BEAMS_MAX && V >= 1 && n >= 1 && n <= HELM_BEAMS_MAX &&
          (int64_t)B * K <= 65535 &&
-         (int64_t)K * ((V + 1023) / 1024) * n <= 0x7fffffff;
+         (int64_t)K * ((V - 1) / 1024 + 1) * n <= 0x7fffffff;
 }
 
 template <typename T> void launch_select(const SelectArgs& a, const SelectPlan& p, hipStream_t st) {

@@ -110,6 +110,8 @@ def _decode_args(q, k_pool, v_pool, page_table, seq_lens, group_starts, shared_p
         max_pages = page_table.size(1)
     if not 0 <= max_pages <= page_table.size(1):
         raise ValueError("max_pages must be 0 to the table's width")
+    if max_pages * P > 0x7ffff000:
+        raise ValueError("a table's pages hold at most 2^31 - 4096 tokens")
     if R > _MAX_SEQS or n > _MAX_GROUPS:
         raise ValueError(f"at most {_MAX_SEQS} sequences and {_MAX_GROUPS} groups")
     if window is not None and window < 0:

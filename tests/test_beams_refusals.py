@@ -216,6 +216,22 @@ def test_a_null_pool_is_refused_before_device_work():
     assert _tables_call([None], n_slots=0, ws=None) == _native.HELM_E_WORKSPACE
 
 
+def test_sizes_past_32_bits_are_refused():
+    """And not cut to what is left of them."""
+    logits = torch.zeros((1, 1, 1)).expand(1, 1, 2 ** 32 + 5)
+    for x in (logits, logits[..., :2 ** 31]):
+        with pytest.raises(ValueError, match="logits"):
+            beams.beam_select(x, torch.zeros((1, 1)))
+    for shape in ((1, 2 ** 32 + 1, 1, 1), (2, 2 ** 20, 16, 128)):
+        with pytest.raises(ValueError, match="2.31"):
+            beams.PageStore([torch.zeros(shape, dtype=torch.uint8, device="meta")])
+    lib = _native.load()
+    for V, n in ((2 ** 31 - 1, 64), (2 ** 31 - 2048, 1)):
+        chunks = -(-V // 8192)
+        assert lib.helm_beam_select_workspace_bytes(1, 1, V, n, 1) == chunks * (12 + 8 * n)
+    assert lib.helm_beam_select_workspace_bytes(1, 64, 2 ** 31 - 1, 64, 1) == 0
+
+
 def test_operands_over_a_pool_are_refused():
     """Read or written, in any part of any page: pages of 64 bytes, 128 apart, from byte 1024 on."""
     buf = np.zeros(512, dtype=np.int32)

@@ -100,6 +100,13 @@ def test_out_and_prepared_refusals(monkeypatch):
             no()
 
 
+def test_tables_past_32_bits_are_refused():
+    for width, page in ((2 ** 32 + 3, 16), (2 ** 27, 16), (2 ** 20, 2048)):
+        table = torch.zeros((2, width), dtype=I32, device="meta")
+        with pytest.raises(ValueError, match="2.31"):
+            prefix.prefix_decode_attention(**_args(page=page, page_table=table))
+
+
 def test_c_entry_refuses_before_device_work():
     lib = _native.load()
     raw = np.zeros(1 << 16, dtype=np.uint8)
