@@ -71,13 +71,13 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: Optional[int] = N
             if t.shape != (B, n) or t.dtype != dt or not t.is_contiguous():
                 raise ValueError(f"out.{name} must be contiguous {dt} [{B}, {n}]")
     idx = _engine.common_device("beam_select", logits, scores, *out)
+    if given:
+        for i, t in enumerate(out):
+            _engine.refuse_shared("beam_select", t, logits, scores, *out[:i])
     sb, sk, sv = logits.stride()
     if sv != 1 and V > 1:
         logits = logits.contiguous()
         sb, sk, _ = logits.stride()
-    if given:
-        for i, t in enumerate(out):
-            _engine.refuse_shared("beam_select", t, logits, scores, *out[:i])
     need = _native.load().helm_beam_select_workspace_bytes(B, K, V, n, code)
     ws = torch.empty(need, dtype=torch.uint8, device=logits.device)
     _engine.launch_on(idx, "helm_beam_select", logits.data_ptr(), sb, sk, code, scores.data_ptr(),

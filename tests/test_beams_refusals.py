@@ -56,6 +56,16 @@ def test_select_out_refusals(monkeypatch):
             beams.beam_select(**a, out=bad)
 
 
+def test_select_out_over_logits_that_are_copied_first(monkeypatch):
+    """Their own memory is the operand, not the copy's."""
+    monkeypatch.setattr(engine, "common_device", lambda *a: 0)
+    buf = torch.zeros(48)
+    out = beams.BeamChoice(buf[10:16].view(2, 3), torch.zeros((2, 3), dtype=I64),
+                           torch.zeros((2, 3), dtype=I32))
+    with pytest.raises(ValueError, match="lies over"):
+        beams.beam_select(buf.view(2, 8, 3).transpose(1, 2), torch.zeros((2, 3)), out=out)
+
+
 def _tables(B=2, K=3, W=4, **kw):
     return dict(dict(parents=torch.zeros((B, K), dtype=I32),
                      page_table=torch.zeros((B * K, W), dtype=I32),
