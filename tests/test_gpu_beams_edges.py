@@ -160,3 +160,39 @@ def test_operands_between_a_pools_pages():
     assert [tuple(c) for c in buf[16:28].view(6, 2).tolist()] == copies
     assert torch.equal(buf.view(24, 32)[:, :16].reshape(24, 16, 1).cpu(),
                        R.copy_pages(pages, copies, [40] * 6, 16, 3))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("make", ["equal", "few_values", "one_run"])
+@pytest.mark.parametrize("K,V,n", [(8, 20000, 64), (64, 20000, 64), (64, 2500, 40)])
+def test_select_more_ties_than_the_joining_holds(K, V, n, make, dtype):
+    """Rows alike, more of their lists' candidates at the bound than 2,048."""
+    B = 2
+    g = torch.Generator(device=DEV).manual_seed(K + V)
+    if make == "equal":
+        row = torch.full((B, 1, V), -2.5, device=DEV)
+    elif make == "few_values":
+        row = torch.randint(0, 3, (B, 1, V), generator=g, device=DEV).float()
+    else:                                              # the largest at the row's end
+        row = torch.zeros((B, 1, V), device=DEV)
+        row[..., V - 100:] = 3.0
+    x = row.expand(B, K, V).to(dtype).contiguous()
+    check_select(x, torch.zeros((B, K), device=DEV), n)
+    scores = -(torch.arange(K, device=DEV) % 3).float().expand(B, K).contiguous()
+    check_select(x, scores.flip(1).contiguous(), n)
+    x[:, K // 2] = -math.inf                           # one row offers nothing, one a single token
+    x[:, K // 3, 1:] = -math.inf
+    check_select(x, scores, n)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,K,V,n", [(1, 1, 152064, 8), (4, 4, 152064, 16), (1, 1, 200001, 64),
+                                     (1, 1, 600001, 33), (1, 2, 300001, 1), (1, 64, 300001, 64)])
+def test_select_many_chunks_a_row(B, K, V, n, dtype):
+    """More chunks a row than the joining's lanes, more lists than one of its sweeps takes."""
+    x = randn(V, (B, K, V), dtype, 3.0)
+    check_select(x, -10 * torch.rand((B, K), generator=torch.Generator(device=DEV).manual_seed(V),
+                                     device=DEV), n)
+    if K * V < 2 * 10 ** 6:
+        x = (x.float().clamp(min=4.0) * 2).round().to(dtype)        # a few values
+        check_select(x, -32.0 * torch.arange(K, device=DEV).expand(B, K).contiguous(), n)
