@@ -42,9 +42,11 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: Optional[int] = N
     logits: [B, K, V] float16, bfloat16 or float32, rows dense (others are copied first);
     scores: float32 [B, K], the beams' summed log-probabilities.  Token t of beam k scores
     scores[k] + log_softmax(logits[k])[t]; the order is of sums in 64 bits, ties go to the
-    lowest k * V + t.  A logit of -inf is no candidate, nor is anything of a beam whose
-    score is not finite or whose logits hold a NaN or +inf; where fewer than n are left,
-    score -inf, token -1 and parent -1 follow.  At most 64 beams and candidates, 65,535 rows.
+    lowest k * V + t.  (A beam's log-sum-exp is of 32-bit exponentials, off by some 1e-7, at
+    worst 2^-18: as near as that, candidates of different beams may come in either order.)
+    A logit of -inf is no candidate, nor is anything of a beam whose score is not finite or
+    whose logits hold a NaN or +inf; where fewer than n are left, score -inf, token -1 and
+    parent -1 follow.  At most 64 beams and candidates, 65,535 rows.
     out: a former result of the same sizes, written instead of new tensors (it may share no
     memory with an operand; scores may be `out.scores`' copy, not itself)."""
     if logits.dim() != 3 or scores.shape != logits.shape[:2]:

@@ -6,10 +6,12 @@
 // and the n best of the request's K V candidates are wanted, ties to the lowest k V + t.
 // Within a row the order is the logits' own, so one pass over them gives a chunk's
 // largest value, its sum and its n best, and the rows meet in a second, small kernel.
-// Bound by memory: the logits are read once.  The order between rows is of sums, which are
-// formed in 64 bits: exponentials in 32 (each off at random by some 2^-21 at most, most of it
-// its argument's rounding), their sums, logarithms and the scores in 64, so that two
-// candidates of different rows change places only where their scores are within some 1e-7.
+// Bound by memory: the logits are read once.  The order is of the 64-bit sums
+// (s_k - lse_k) + x_kt, ties to the lowest k V + t.  Exponentials are in 32 bits, and so are their
+// sums over a thread's up to 32 values and over its wave; waves, chunks, logarithms and scores
+// are added in 64.  That leaves lse off by some 1e-7 (2^-18 if every one of its 42 roundings fell
+// the same way), so candidates of one row are in order, and two of different rows change places
+// only where their scores are as near as that.
 //
 // A chunk's n best: the n-th largest of the 256 threads' maxima, which every wave finds for
 // itself by a search over the value's leading bits with ballots, is at most the n-th largest of

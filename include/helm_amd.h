@@ -499,7 +499,9 @@ int helm_prefix_decode_attn(const void* q, void* out, const void* k_pool, const 
  * Out, [B, n], best first, ties to the lowest k * V + t: the score (past fp32's range: its
  * largest or lowest number), the token, the beam (0 .. K - 1).  A logit of -inf is no
  * candidate, nor is anything of a row whose score is not finite or whose logits hold a NaN or
- * +inf; where fewer than n are left, -inf, -1, -1.  The order is of 64-bit sums.
+ * +inf; where fewer than n are left, -inf, -1, -1.  The order is of the 64-bit sums
+ * (score - lse) + logit, lse of a row from 32-bit exponentials, off by some 1e-7 (2^-18 at worst):
+ * candidates of different rows as near as that may come in either order.
  * 1 <= K, n <= HELM_BEAMS_MAX, B K <= 65535.  The workspace is 8-byte aligned and needs no
  * contents before or after a call; calls that may overlap need one each.  No output may
  * lie over the logits or scores. */
