@@ -61,8 +61,11 @@ def prefix_decode_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
     lengths and groups.
 
     The q_len rows are the sequence's last tokens: row s stands at p = len - q_len + s and
-    sees tokens up to p, with `window` only the last `window` of those.  Hidden tokens take
-    no part whatever they hold, and a row that sees nothing is zeros.  At most 4,096
+    sees tokens up to p, with `window` only the last `window` of those.  Hidden tokens (those
+    past max_pages too) take no part whatever they hold, a visible infinity or NaN in V counts
+    at any weight, and a row that sees nothing is zeros.  Weights are held to 2^-16 (bfloat16)
+    or 2^-22 of themselves, sums in 32 bits; weights reach 2^8 before the division, so that
+    bfloat16 V of about 2^120 and more over the number of tokens may overflow.  At most 4,096
     sequences and 512 groups.  out: contiguous; it may be q itself, but share memory with
     no other operand.  Returns out [R, Hq, q_len, D] in q's dtype."""
     idx, args, out, _ = _decode_args(q, k_pool, v_pool, page_table, seq_lens, group_starts,

@@ -473,9 +473,10 @@ int helm_prompt_attn(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
  * are the sequence's last tokens, row s sees tokens j <= p = seq_lens[r] - q_len + s, with
  * window > 0 only j > p - window.  Hidden tokens, those past max_pages and those of pages whose
  * slot is outside [0, n_slots) among them, take no part whatever they hold; a row that sees
- * nothing is zeros.  softcap <= 0: off.  out may be q, but lie over nothing else.  The workspace
- * (16-byte aligned) needs no contents before or after a call; calls that may overlap need one
- * each.  head_dim 64, 128 or 256. */
+ * nothing is zeros.  softcap <= 0: off.  out may be q, but lie over nothing else.  Weights keep
+ * 16 bits (bf16) or 22, sums are in fp32 with weights up to 2^8: bf16 V of about 2^120 and more over
+ * the number of tokens may overflow.  The workspace (16-byte aligned) needs no contents before
+ * or after a call; calls that may overlap need one each.  head_dim 64, 128 or 256. */
 #define HELM_PREFIX_MAX_SEQS 4096
 #define HELM_PREFIX_MAX_GROUPS 512
 size_t helm_prefix_workspace_bytes(int R, int Hq, int Hkv, int q_len, int D, int n_groups);
