@@ -215,43 +215,6 @@ template <typename T> __device__ __forceinline__ uint32_t nonfinite_halves(uint3
   return r;
 }
 
-// V's infinities and NaN taken out of the operand and added to the rows of o that see them
-// (sop: 1 where a row sees a token).
-template <typename T>
-__device__ __forceinline__ void careful_v(mf_u32x4& vop, const mf_u32x4& sop, mf_f32x16& o) {
-  using M32 = Mfma32<T>;
-  mf_u32x4 bad;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) bad[i] = nonfinite_halves<T>(vop[i]);
-  if (!__builtin_amdgcn_ballot_w64((bad[0] | bad[1] | bad[2] | bad[3]) != 0u)) return;
-  constexpr uint32_t kMant = std::is_same<T, bf16_t>::value ? 0x7fu : 0x3ffu;
-  const uint32_t one = MfmaOps<T>::ones8()[0];
-  mf_u32x4 pos, neg, nan;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint32_t is_nan = 0, is_neg = 0;
-    if (vop[i] & kMant) is_nan |= 0xffffu;
-    if (vop[i] >> 16 & kMant) is_nan |= 0xffff0000u;
-    if (vop[i] & 0x8000u) is_neg |= 0xffffu;
-    if (vop[i] & 0x80000000u) is_neg |= 0xffff0000u;
-    nan[i] = one & bad[i] & is_nan;
-    neg[i] = one & bad[i] & ~is_nan & is_neg;
-    pos[i] = one & bad[i] & ~is_nan & ~is_neg;
-    vop[i] &= ~bad[i];
-  }
-  mf_f32x16 zero;
-#pragma unroll
-  for (int r = 0; r < 16; ++r) zero[r] = 0.f;
-  const mf_f32x16 hp = M32::mma(pos, sop, zero), hn = M32::mma(neg, sop, zero),
-                  hx = M32::mma(nan, sop, zero);
-#pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    if (hp[r] != 0.f) o[r] += INFINITY;
-    if (hn[r] != 0.f) o[r] -= INFINITY;
-    if (hx[r] != 0.f) o[r] = __builtin_nanf("");
-  }
-}
-
 // x f, but an infinity or NaN (a visible one, which counts at any weight) stays what it is where
 // f is zero.
 __device__ __forceinline__ float scale_finite(float x, float f) {
@@ -538,8 +501,40 @@ __device__ __forceinline__ void prompt_body(const PromptParams& p) {
         const uint2 a1 = v_operand(vv, u, 1, e, vo);
         mf_u32x4 vop{a0.x, a0.y, a1.x, a1.y};
         if constexpr (careful.value) {
-          const mf_u32x4 sop{some[4 * u], some[4 * u + 1], some[4 * u + 2], some[4 * u + 3]};
-          careful_v<T>(vop, sop, o[e]);
+          // (written out here: in a function of its own it costs the walk that is not careful, 9
+          // prompts of up to 2.5k tokens 124 -> 130 us, one of 16k 1,950 -> 1,990)
+          mf_u32x4 bad;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) bad[i] = nonfinite_halves<T>(vop[i]);
+          if (__builtin_amdgcn_ballot_w64((bad[0] | bad[1] | bad[2] | bad[3]) != 0u)) {
+            const mf_u32x4 sop{some[4 * u], some[4 * u + 1], some[4 * u + 2], some[4 * u + 3]};
+            constexpr uint32_t kMant = std::is_same<T, bf16_t>::value ? 0x7fu : 0x3ffu;
+            const uint32_t one = Ops::ones8()[0];
+            mf_u32x4 pos, neg, nan;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t is_nan = 0, is_neg = 0;
+              if (vop[i] & kMant) is_nan |= 0xffffu;
+              if (vop[i] >> 16 & kMant) is_nan |= 0xffff0000u;
+              if (vop[i] & 0x8000u) is_neg |= 0xffffu;
+              if (vop[i] & 0x80000000u) is_neg |= 0xffff0000u;
+              nan[i] = one & bad[i] & is_nan;
+              neg[i] = one & bad[i] & ~is_nan & is_neg;
+              pos[i] = one & bad[i] & ~is_nan & ~is_neg;
+              vop[i] &= ~bad[i];
+            }
+            mf_f32x16 zero;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) zero[r] = 0.f;
+            const mf_f32x16 hp = M32::mma(pos, sop, zero), hn = M32::mma(neg, sop, zero),
+                            hx = M32::mma(nan, sop, zero);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              if (hp[r] != 0.f) o[e][r] += INFINITY;
+              if (hn[r] != 0.f) o[e][r] -= INFINITY;
+              if (hx[r] != 0.f) o[e][r] = __builtin_nanf("");
+            }
+          }
         }
         o[e] = M32::mma(vop, pop, o[e]);
         if (kAnew && e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
