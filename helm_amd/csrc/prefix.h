@@ -6,8 +6,8 @@
 // own pages for its own S G rows a KV head; every walk leaves partial sums (m, l, o) of its
 // rows over its tokens, and a second kernel joins a row's:
 //   out = sum 2^(m_i - M) o_i / sum 2^(m_i - M) l_i,  M = max m_i.
-// Bound by memory up to some 400 rows a KV head (4 D operations a row and token against
-// 4 D bytes a token), by the matrix cores beyond.
+// Bound by memory up to some 280 rows a KV head (6 D operations a row and token, the weights being
+// in two parts, against 4 D bytes a token), by the matrix cores beyond.
 //
 // Work: a KV head's walks, the groups' (128 rows each) and then the sequences',
 // lie end to end on one line of steps of 32 tokens, and each of the head's workgroups takes an
@@ -17,18 +17,18 @@
 // Walks of a group that has several come first on the line, each from a stretch's start on:
 // so the workgroups that read the same tokens for different rows do so side by side, through
 // one XCD's L2 (a KV head's workgroups are on one where 8, 16, ... heads lie round the XCDs):
-// 32k tokens under 64 sequences 93 -> 88 us.
+// 32k tokens under 64 sequences 93 -> 88 us at that step; 6% more is read than K and V hold.
 //
 // A walk is that of prompt.h: 32 x 32 matrix tiles, 32 rows a wave, K and V straight from memory
 // into LDS, one barrier a stage.  Few rows keep few of the waves busy; such a walk is bound by
 // memory.  K and V come from HBM here, not from L2: three stages are on their way.
 //
 // Bound, measured at D = 128, bf16 (walks and their joining, us a call): 4 beams of 16 prompts of
-// up to 4k tokens 48, 2.8 TB/s of K and V; 24 chats behind 8k shared tokens 33, of which the
-// joining takes 5 and the line 3.5; 32k tokens under 64 sequences 81, where the walks' arithmetic
-// alone takes 66 and their loads alone 57: two waves a SIMD hide part of the one behind the other.
-// (From 32k to 64k tokens 64 sequences take 37 us more, 32 sequences 24, which is 5.7 TB/s; some
-// 30 us of a call do not grow with the tokens, the partials' 33 MB out and back half of them.)
+// up to 4k tokens 49, 2.8 TB/s of K and V; 24 chats behind 8k shared tokens 36, of which the
+// joining takes 5 and the line 3.5; 32k tokens under 64 sequences 92, of whose walks' cycles the
+// matrix cores are busy 30% and LDS 12%.  From 32k to 64k tokens 64 sequences take 51 us more,
+// which is 1.0 PFLOP/s with both parts' products, 32 sequences 26, which is 5.2 TB/s; some 30 us
+// of a call do not grow with the tokens.
 //
 // Weights enter P . V in two 16-bit parts (2^-16 of the weight in bf16, 2^-22 in f16) and the row's
 // sum in fp32, as in the decode kernels; f16 weights are taken times 2^9, what is under 2^-34 of
@@ -52,18 +52,20 @@ namespace helm {
 
 constexpr int kPfRows = 32;          // of a wave, and of a slot of the groups' partials
 constexpr int kPfStep = 32;          // tokens of a step
-// What a walk costs before its first step and behind its last, in steps.  (32k tokens under 64
-// sequences 81.5 us, with 8 84.8, with 12 88; with 2, workgroups of several short walks end late:
-// 4 beams of 16 prompts 63 us against 58 with 4 and 55 with 6.)
+// What a walk costs before its first step and behind its last, in steps.  (4 beams of 16 prompts and
+// 32k tokens under 64 sequences, us: with 5 49.2 and 91.6, with 4 52.0 and 90.5, with 6 49.3 and
+// 92.7, with 8 51.3 and 95.1, with 12 54.1 and 99.9; with 2, where workgroups of several short walks
+// end late, 61.8 and 100.)
 constexpr int kPfFixed = 5;
-// A workgroup's least stretch (a prompt of 2k tokens, 4 beams: 17.1 us, with 2 18.4, with 8 21.9).
+// A workgroup's least stretch (a prompt of 2k tokens, 4 beams: 17.3 us, with 2 18.0, with 8 21.5).
 constexpr int kPfLeast = 4;
 constexpr int kPfJoinThreads = 256;
 constexpr int kPfWaves = 4;          // of a workgroup
 constexpr int kPfThreads = 64 * kPfWaves;
 constexpr int kPfTile = kPfRows * kPfWaves;            // rows of a walk
-// Stage buffers.  (Two, and three workgroups a CU: 24 chats 39.6 us, 4 beams of 16 prompts 55, 32k
-// tokens 88; three buffers, three workgroups 39.7, 58, 88; four and two 33.9, 48, 84.)
+// Stage buffers.  (With weights in one part; two, and three workgroups a CU: 24 chats 39.6 us, 4
+// beams of 16 prompts 55, 32k tokens 88; three buffers, three workgroups 39.7, 58, 88; four and
+// two 33.9, 48, 84.)
 constexpr int kPfBufs = 4;
 // Tokens of a stage; workgroups of a CU, which the buffers (16 KB, 32 at D = 256) leave room for.
 template <int D> struct PfShape {
@@ -466,8 +468,8 @@ __device__ __forceinline__ bool pf_walk(const PfParams& p, const PfPiece& w, int
 }
 
 // A wave's sums to their slot: row jr's dims 32 e + 8 g + 4 hh .. + 3 are register 4 g .. of o[e].
-// (Through LDS, in whole lines: 32k tokens under 64 sequences 81 -> 83 us, 4 beams of 16 prompts
-// 48 -> 52.)
+// (Through LDS, in whole lines, with weights in one part: 32k tokens under 64 sequences 81 -> 83 us,
+// 4 beams of 16 prompts 48 -> 52.)
 template <int D>
 __device__ __forceinline__ void pf_store(const PfRowsOf<D>& s, float* ml, float* part) {
   const int lane = threadIdx.x & 63, jr = lane & 31, hh = lane >> 5;

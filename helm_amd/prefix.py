@@ -1,7 +1,12 @@
 """Decode attention of sequences that share their first pages (``helm_prefix_decode_attn``):
 the beams of a prompt (``helm_amd.beams``), requests under one system prompt, questions about one
 document.  The pools, page tables and lengths are those of ``paged.paged_decode_attention``;
-the pages that a group shares are read once for all of its sequences."""
+the pages that a group shares are read once for all of its sequences.
+
+That pays where the sequences' K and V, counted one by one, are more than some 300 MB a call (64,000
+to 100,000 tokens of 8 heads of 128): 64 sequences behind 4,096 tokens 35 us for 101, 4 behind 16,384
+28 for 32.  Below that ``paged_decode_attention`` over the same tables gets the repeated pages from
+the card's last-level cache, and is up to twice as fast (4 behind 1,024: 8.6 us for 17.4)."""
 from __future__ import annotations
 
 from typing import Optional
